@@ -985,6 +985,20 @@ namespace qd {
 qd_status guard_call(void (*fn)(void *), void *ctx) {
   return guard([&] { fn(ctx); });
 }
+// For entry points that return instead of throwing: keeps the text for qd_last_error().
+qd_status report(qd_status status, const char *text) noexcept {
+  try {
+    g_error = text;
+  } catch (...) {
+    g_error.clear();
+  }
+  return status;
+}
+qd_status report_hip(hipError_t e, const char *what) noexcept {
+  char buf[256];
+  std::snprintf(buf, sizeof(buf), "%s: %s", what, hipGetErrorString(e));
+  return report(hip_status(e), buf);
+}
 }  // namespace qd
 
 extern "C" {

@@ -1,0 +1,994 @@
+// Operators on a paged key-value cache for gfx950: writing rotated rows into
+// pages, attention of one new token per row, and the fork of rows that share
+// pages. Declared in include/qd/qd_operators.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "qd_attention.hpp"
+#include "qd_device.hpp"
+#include "qd_device_math.hpp"
+#include "qd_operators.hpp"
+
+namespace qd {
+namespace {
+
+using namespace dev;
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+// Lengths, tables and positions are written before the kernel starts: they may
+// be read through the scalar cache.
+typedef const __attribute__((address_space(4))) int32_t const_i32;
+
+__device__ __forceinline__ int32_t load_uniform(const int32_t *p) { return *(const_i32 *)p; }
+
+__device__ __forceinline__ void raise_error(uint32_t *errors, uint32_t bit) {
+  if (errors) atomicOr(errors, bit);
+}
+
+// Waits until this thread's vector memory operations have completed.
+__device__ __forceinline__ void wait_vm_stores() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// The storage types' conversions; two values share a 32-bit register, low half first.
+struct Half {
+  static __device__ __forceinline__ float lo(uint32_t v) { return half_lo(v); }
+  static __device__ __forceinline__ float hi(uint32_t v) { return half_hi(v); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};  // to nearest even
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ f4v mfma(u4v a, u4v b, f4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+struct Brain {
+  static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
+  static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};  // to nearest even
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ f4v mfma(u4v a, u4v b, f4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+
+// Four consecutive elements as FP32, and back.
+template <typename E>
+__device__ __forceinline__ float4 load4(const void *base, int64_t i) {
+  if constexpr (std::is_same_v<E, float>) {
+    return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + i);
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(base) + i);
+    return make_float4(E::lo(v.x), E::hi(v.x), E::lo(v.y), E::hi(v.y));
+  }
+}
+template <typename E>
+__device__ __forceinline__ void store4(void *base, int64_t i, float4 v) {
+  if constexpr (std::is_same_v<E, float>)
+    *reinterpret_cast<float4 *>(static_cast<float *>(base) + i) = v;
+  else
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(base) + i) = make_uint2(E::pack(v.x, v.y), E::pack(v.z, v.w));
+}
+
+// ---- append -------------------------------------------------------------------
+// (a, b) -> (a c - b s, b c + a s) for the rotated pairs, a copy for the rest. A
+// thread takes eight elements of a head: four pairs, or eight that are copied.
+// Each value is read once and written once: bound by memory for prompts, by the
+// chain position -> page -> store for a few tokens.
+struct AppendLaunch {
+  qd_paged_cache c;
+  qd_append_args a;
+  uint32_t page_shift;
+  uint32_t units;  // eights of a token: (query heads, key heads, value heads) x head_dim / 8
+};
+
+template <typename E>
+__global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
+  const uint32_t id = blockIdx.x * kBlock + threadIdx.x;
+  const uint32_t token = id / p.units;
+  if (token >= p.a.tokens) return;
+  uint32_t unit = id - token * p.units;
+  const int64_t position = static_cast<int64_t>(p.a.positions[token]) + p.a.position_bias;
+  if (position < 0) return;
+  const uint32_t dim = p.c.head_dim, per_head = dim / 8;
+  const uint32_t heads = p.a.q ? p.a.heads : 0;
+  const uint32_t head = unit / per_head;  // queries, then keys, then values
+  unit -= head * per_head;
+
+  const int32_t row = p.a.rows ? p.a.rows[token] : static_cast<int32_t>(token);
+  const uint64_t column = static_cast<uint64_t>(position) >> p.page_shift;
+  uint32_t bad = 0;
+  int64_t page = 0;
+  if (row < 0 || static_cast<uint32_t>(row) >= p.c.rows) {
+    bad = QD_PAGED_BAD_ROW;
+  } else if (column >= p.c.table_width || (p.a.rotary_dim && static_cast<uint64_t>(position) >= p.a.table_positions)) {
+    bad = QD_PAGED_BAD_POSITION;
+  } else {
+    page = p.c.table[row * p.c.table_stride + static_cast<int64_t>(column)];
+    if (page < 0 || page >= p.c.pages) bad = QD_PAGED_BAD_PAGE;
+  }
+  const bool query = head < heads;
+  const bool value = head >= heads + p.c.kv_heads;
+  const uint32_t h = query ? head : value ? head - heads - p.c.kv_heads : head - heads;
+  if (bad) {
+    if (unit == 0 && h == 0) raise_error(p.c.errors, bad);
+    if (query) {
+      const float n = __uint_as_float(0x7FC00000u);
+      const int64_t to = token * p.a.q_out_stride + h * dim + unit * 8;
+      store4<E>(p.a.q_out, to, make_float4(n, n, n, n));
+      store4<E>(p.a.q_out, to + 4, make_float4(n, n, n, n));
+    }
+    return;
+  }
+  const void *src = query ? p.a.q : value ? p.a.v : p.a.k;
+  const int64_t from = token * (query ? p.a.q_stride : value ? p.a.v_stride : p.a.k_stride) + h * dim;
+  void *dst = query ? p.a.q_out : value ? p.c.v : p.c.k;
+  const int64_t to = query ? token * p.a.q_out_stride + h * dim
+                           : page * p.c.page_stride + (position & (p.c.page_size - 1)) * p.c.token_stride + h * p.c.head_stride;
+  const uint32_t turned = value ? 0u : p.a.rotary_dim;
+  if (unit * 8 >= turned) {
+    store4<E>(dst, to + unit * 8, load4<E>(src, from + unit * 8));
+    store4<E>(dst, to + unit * 8 + 4, load4<E>(src, from + unit * 8 + 4));
+    return;
+  }
+  const int64_t angle = position * (p.a.rotary_dim / 2) + unit * 4;
+  const float4 c = *reinterpret_cast<const float4 *>(p.a.cos_table + angle);
+  const float4 s = *reinterpret_cast<const float4 *>(p.a.sin_table + angle);
+  // Pairs (i, i + R/2): the first and second elements of four pairs are four
+  // consecutive elements each; (2i, 2i + 1): eight elements in turn.
+  const uint32_t first = p.a.interleaved ? unit * 8 : unit * 4;
+  const uint32_t second = p.a.interleaved ? first + 4 : first + p.a.rotary_dim / 2;
+  float4 x = load4<E>(src, from + first), y = load4<E>(src, from + second);
+  if (p.a.interleaved) {
+    const float4 a = make_float4(x.x, x.z, y.x, y.z), b = make_float4(x.y, x.w, y.y, y.w);
+    rope_rotate(a.x, b.x, c.x, s.x, x.x, x.y);
+    rope_rotate(a.y, b.y, c.y, s.y, x.z, x.w);
+    rope_rotate(a.z, b.z, c.z, s.z, y.x, y.y);
+    rope_rotate(a.w, b.w, c.w, s.w, y.z, y.w);
+  } else {
+    const float4 a = x, b = y;
+    rope_rotate(a.x, b.x, c.x, s.x, x.x, y.x);
+    rope_rotate(a.y, b.y, c.y, s.y, x.y, y.y);
+    rope_rotate(a.z, b.z, c.z, s.z, x.z, y.z);
+    rope_rotate(a.w, b.w, c.w, s.w, x.w, y.w);
+  }
+  store4<E>(dst, to + first, x);
+  store4<E>(dst, to + second, y);
+}
+
+// ---- attention ------------------------------------------------------------------
+// A workgroup takes a run of a row's tiles of 32 positions for one KV head and up
+// to 16 of its query heads; its waves take the tiles in turn, each with a running
+// maximum and sum. Everything stays in the registers of the matrix instructions:
+//   S^T = K Q^T   lane l: head l % 16, positions 4 (l / 16) + r of each half tile
+//   O^T += V^T P^T the same lane's probabilities are the operand as they are, and
+//                 its share of O is of its own head, so a new maximum rescales
+//                 with one factor per lane.
+// K is read in the operand's layout (16 bytes of a row per lane). V's operand
+// holds positions along the registers: FP32 takes one position per instruction,
+// so float4 loads along the head serve four of them; 16-bit rows are loaded 8 at
+// a time and turned with byte permutes.
+constexpr int kTile = 32, kSub = 16;
+constexpr int kAttnW = 4, kAttnT = kAttnW * kWave;
+// A maximum is only taken up when it passes the one in use by this many powers of
+// two: until then probabilities grow to at most 2^8, exact in every type's range.
+constexpr float kLazyMax = 8.f;
+
+struct AttnLaunch {
+  qd_paged_cache c;
+  qd_attention_args a;
+  float *records;       // [grid.x][grid.y][rec_floats]: acc [rec_heads][head_dim], maxima, sums
+  uint32_t *counters;   // [rows][grid.y]
+  uint32_t page_shift;
+  uint32_t group;       // query heads of a KV head
+  uint32_t blocks;      // of up to 16 of them
+  uint32_t rec_heads;   // the most of a block
+  uint32_t rec_floats;
+  uint32_t least;       // tiles of a chunk at least
+  uint32_t target;      // chunks aimed at, beyond one per row; 0: rows are not split
+};
+
+// Values of lanes l and l ^ 32 in a and b (any order).
+__device__ __forceinline__ void half_swap(float v, float &a, float &b) {
+  unsigned x = __builtin_bit_cast(unsigned, v), y = x;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+  a = __builtin_bit_cast(float, x);
+  b = __builtin_bit_cast(float, y);
+}
+// Over lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float quarters_max(float v) {
+  float a, b;
+  v = row_pair_max(v);
+  half_swap(v, a, b);
+  return fmaxf(a, b);
+}
+__device__ __forceinline__ float quarters_sum(float v) {
+  float a, b;
+  v = row_pair_sum(v);
+  half_swap(v, a, b);
+  return a + b;
+}
+
+// 16 positions of a page through a descriptor that ends with the last valid one:
+// loads past it give zeros and touch no memory.
+struct PageRows {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ u4v ld16(uint32_t byte) const {
+    return __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, 0));
+  }
+  __device__ __forceinline__ u2v ld8(uint32_t byte) const {
+    return __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(r, byte, 0, 0));
+  }
+};
+
+// Where a chunk lies: wave-uniform.
+struct Chunk {
+  int row, length;
+  int first, last;      // tiles
+  uint32_t begin;       // the row's first chunk's index
+  uint32_t index, of;   // of the row's chunks
+  bool bad;             // the row's length
+};
+
+// Chunk `x` of all rows'. A row of n tiles has max(1, ceil(n / size)) chunks,
+// where size makes about `target` of them in all.
+__device__ __forceinline__ bool find_chunk(const AttnLaunch &p, uint32_t x, Chunk &ch) {
+  const int lane = lane_id();
+  const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
+  auto length_of = [&](uint32_t r) {
+    const int32_t n = p.c.lengths[r];
+    return n < 0 || n > most ? 0 : n;
+  };
+  uint32_t size = 0x7fffffffu, row = x, before = 0;
+  if (p.target) {
+    uint32_t total = 0;
+    for (uint32_t r = lane; r < p.c.rows; r += kWave) total += (length_of(r) + kTile - 1) / kTile;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) total += __shfl_xor(total, o, kWave);
+    size = max(p.least, (total + p.target - 1) / p.target);
+    row = p.c.rows;
+    for (uint32_t base = 0; base < p.c.rows; base += kWave) {
+      const uint32_t r = base + lane;
+      const uint32_t tiles = r < p.c.rows ? (length_of(r) + kTile - 1) / kTile : 0u;
+      const uint32_t mine = r < p.c.rows ? max(1u, (tiles + size - 1) / size) : 0u;
+      uint32_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const uint32_t v = __shfl_up(upto, o, kWave);
+        if (lane >= o) upto += v;
+      }
+      const uint64_t past = __ballot(before + upto > x);
+      if (past) {
+        const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+        row = base + at;
+        before += __builtin_amdgcn_readlane(upto - mine, at);
+        break;
+      }
+      before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+  } else {
+    before = x;
+  }
+  row = __builtin_amdgcn_readfirstlane(row);
+  if (row >= p.c.rows) return false;
+  before = __builtin_amdgcn_readfirstlane(before);
+  size = __builtin_amdgcn_readfirstlane(size);
+  const int32_t n = load_uniform(p.c.lengths + row);
+  ch.bad = n < 0 || n > most;
+  ch.row = row;
+  ch.length = ch.bad ? 0 : n;
+  const uint32_t tiles = (ch.length + kTile - 1) / kTile;
+  ch.of = max(1u, tiles / size + (tiles % size != 0));
+  ch.begin = before;
+  ch.index = x - before;
+  ch.first = ch.index * size;
+  ch.last = min(tiles, ch.first + size);
+  return true;
+}
+
+template <typename E, int D>
+struct WaveTiles {
+  static constexpr bool kWide = std::is_same_v<E, float>;
+  static constexpr int kElem = kWide ? 4 : 2;
+  static constexpr int kPieces = D * kElem / 64;  // 16-byte loads of K per lane and half tile
+  static constexpr int kAcc = D / 16;
+  u4v q[kPieces];
+  u4v k[2][kPieces];
+  u4v v[2][4][kWide ? D / 64 : 1];  // rows 4 (l / 16) + j; 16-bit rows of 64 use half of a register quad
+  f4v o[kAcc];
+  float m, ms, l;
+
+  __device__ __forceinline__ void load_k(const PageRows &r, int sub, uint32_t off) {
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) k[sub][s] = r.ld16(off + 64 * s);
+  }
+  __device__ __forceinline__ void load_v(const PageRows &r, int sub, const uint32_t (&off)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kWide) {
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) v[sub][j][n] = r.ld16(off[j] + 256 * n);
+      } else if constexpr (D == 128) {
+        v[sub][j][0] = r.ld16(off[j]);
+      } else {
+        const u2v x = r.ld8(off[j]);
+        v[sub][j][0] = u4v{x[0], x[1], 0u, 0u};
+      }
+    }
+  }
+  // Scores of half tile `sub`, in units of the query's scale.
+  __device__ __forceinline__ f4v scores(int sub) const {
+    f4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kPieces; ++s) {
+      if constexpr (kWide) {
+        const f4v a = __builtin_bit_cast(f4v, k[sub][s]), b = __builtin_bit_cast(f4v, q[s]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[c], b[c], acc, 0, 0, 0);
+      } else {
+        acc = E::mfma(k[sub][s], q[s], acc);
+      }
+    }
+    return acc;
+  }
+  // o += V^T P^T; returns the sum of the probabilities as they were multiplied.
+  __device__ __forceinline__ float accumulate(const float (&pr)[2][4]) {
+    float sum = 0.f;
+    if constexpr (kWide) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sum += pr[sub][j];
+#pragma unroll
+          for (int n = 0; n < D / 64; ++n) {
+            const f4v a = __builtin_bit_cast(f4v, v[sub][j][n]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              o[4 * n + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[c], pr[sub][j], o[4 * n + c], 0, 0, 0);
+          }
+        }
+    } else {
+      // Probabilities are rounded to the cache's type for the matrix instruction:
+      // at most half a step each, no more than V's own rounding. The sum takes
+      // the rounded ones, so that the weights add up to one.
+      u4v b;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b[i] = E::pack(pr[i >> 1][2 * (i & 1)], pr[i >> 1][2 * (i & 1) + 1]);
+        sum += E::lo(b[i]) + E::hi(b[i]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAcc; ++j) {
+        u4v a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          a[i] = __builtin_amdgcn_perm(v[i >> 1][2 * (i & 1) + 1][0][j >> 1], v[i >> 1][2 * (i & 1)][0][j >> 1],
+                                       j & 1 ? 0x07060302u : 0x05040100u);
+        o[j] = E::mfma(a, b, o[j]);
+      }
+    }
+    return sum;
+  }
+  // First dimension of piece n (four dimensions) of accumulator row r.
+  static __device__ __forceinline__ int dim_of(int r, int n) {
+    const int row = 4 * (lane_id() >> 4) + r;
+    return kWide ? 64 * n + 4 * row : kAcc * row + 4 * n;
+  }
+};
+
+template <typename E, int D>
+__global__ __launch_bounds__(kAttnT) void attention_kernel(AttnLaunch p) {
+  using Tiles = WaveTiles<E, D>;
+  constexpr int kRow = D + 4;
+  __shared__ __attribute__((aligned(16))) float wo[kAttnW][16][kRow];
+  __shared__ float wm[kAttnW][16], wl[kAttnW][16];
+  __shared__ uint32_t last, spoilt;
+  Chunk ch;
+  if (!find_chunk(p, blockIdx.x, ch)) return;
+  const int w = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id();
+  const int col = lane & 15, quad = lane >> 4;
+  const int kvh = blockIdx.y / p.blocks, block = blockIdx.y % p.blocks;
+  const int h0 = kvh * p.group + 16 * block;                  // the first query head here
+  const int heads = min(16, static_cast<int>(p.group) - 16 * block);
+  if (threadIdx.x == 0) spoilt = ch.bad;
+
+  Tiles t;
+  const float scale = p.a.scale * 1.44269504088896340736f;  // scores in powers of two
+#pragma unroll
+  for (int s = 0; s < Tiles::kPieces; ++s) t.q[s] = u4v{0u, 0u, 0u, 0u};
+  if (col < heads) {
+    const char *q = static_cast<const char *>(p.a.q) +
+                    (ch.row * p.a.q_stride + (h0 + col) * p.a.q_head_stride) * Tiles::kElem + 16 * quad;
+#pragma unroll
+    for (int s = 0; s < Tiles::kPieces; ++s) t.q[s] = *reinterpret_cast<const u4v *>(q + 64 * s);
+  }
+#pragma unroll
+  for (int j = 0; j < Tiles::kAcc; ++j) t.o[j] = f4v{0.f, 0.f, 0.f, 0.f};
+  t.m = -INFINITY;
+  t.ms = 0.f;
+  t.l = 0.f;
+
+  const int32_t *table = p.c.table + ch.row * p.c.table_stride;
+  const uint32_t token_bytes = static_cast<uint32_t>(p.c.token_stride) * Tiles::kElem;
+  const uint32_t k_off = col * token_bytes + 16 * quad;
+  uint32_t v_off[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v_off[j] = (4 * quad + j) * token_bytes + col * (Tiles::kWide ? 16 : D / 16 * 2);
+  bool bad = false;
+  auto page_of = [&](int pos) { return pos < ch.length ? load_uniform(table + (pos >> p.page_shift)) : -1; };
+  // The 16 positions from `pos` on, in page `id`, of K or V.
+  auto rows_at = [&](const void *base, int pos, int id) {
+    const int n = min(max(ch.length - pos, 0), kSub);
+    const bool in = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
+    if (n > 0 && !in) bad = true;
+    const int64_t at = (in ? id * p.c.page_stride : 0) +
+                       static_cast<int64_t>(pos & (p.c.page_size - 1)) * p.c.token_stride + kvh * p.c.head_stride;
+    const uint32_t bytes = n > 0 && in ? (n - 1) * token_bytes + D * Tiles::kElem : 0u;
+    char *ptr = const_cast<char *>(static_cast<const char *>(base)) + at * Tiles::kElem;
+    return PageRows{__builtin_amdgcn_make_buffer_rsrc(ptr, 0, static_cast<int>(bytes), kRsrcWord3)};
+  };
+
+  int tile = ch.first + w;
+  int id[2], next[2];
+  id[0] = page_of(tile * kTile);
+  id[1] = page_of(tile * kTile + kSub);
+  if (tile < ch.last) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) t.load_k(rows_at(p.c.k, tile * kTile + s * kSub, id[s]), s, k_off);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) t.load_v(rows_at(p.c.v, tile * kTile + s * kSub, id[s]), s, v_off);
+  }
+  while (tile < ch.last) {
+    const int then = tile + kAttnW;
+    const bool more = then < ch.last;
+    if (more) {
+      next[0] = page_of(then * kTile);
+      next[1] = page_of(then * kTile + kSub);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const f4v x = t.scores(sub);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[sub][r] = x[r] * scale;
+    }
+    if (more)
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) t.load_k(rows_at(p.c.k, then * kTile + sub * kSub, next[sub]), sub, k_off);
+    if ((tile + 1) * kTile > ch.length)
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (tile * kTile + sub * kSub + 4 * quad + r >= ch.length) s[sub][r] = -INFINITY;
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
+    if (__any(top > t.m + kLazyMax)) {
+      const float m = fmaxf(t.m, quarters_max(top));
+      const float f = m == t.m ? 1.f : exp2_fast(t.m - m);
+      t.m = m;
+      t.ms = m == -INFINITY ? 0.f : m;
+      t.l *= f;
+#pragma unroll
+      for (int j = 0; j < Tiles::kAcc; ++j) t.o[j] *= f;
+    }
+    float pr[2][4];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) pr[sub][r] = exp2_fast(s[sub][r] - t.ms);
+    t.l += t.accumulate(pr);
+    if (more) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) t.load_v(rows_at(p.c.v, then * kTile + sub * kSub, next[sub]), sub, v_off);
+      id[0] = next[0];
+      id[1] = next[1];
+    }
+    tile = then;
+  }
+
+  // The waves' partial results, then the chunk's.
+  const float l = quarters_sum(t.l);
+  if (quad == 0) {
+    wm[w][col] = t.m;
+    wl[w][col] = l;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int n = 0; n < D / 64; ++n)
+      *reinterpret_cast<float4 *>(&wo[w][col][Tiles::dim_of(r, n)]) =
+          make_float4(t.o[4 * n][r], t.o[4 * n + 1][r], t.o[4 * n + 2][r], t.o[4 * n + 3][r]);
+  __syncthreads();
+  if (bad) spoilt = 1;
+  __syncthreads();
+  if (threadIdx.x == 0 && spoilt) raise_error(p.c.errors, ch.bad ? QD_PAGED_BAD_LENGTH : QD_PAGED_BAD_PAGE);
+  const float poison = spoilt ? __uint_as_float(0x7FC00000u) : 0.f;
+
+  constexpr int kQuads = D / 4;
+  auto emit = [&](int h, int d, float4 acc, float sum) {
+    // A row without positions: zeros.
+    const float inv = ch.length == 0 ? 0.f : 1.f / sum;
+    const int64_t at = ch.row * p.a.out_stride + (h0 + h) * p.a.out_head_stride + d;
+    store4<E>(p.a.out, at,
+              make_float4(acc.x * inv + poison, acc.y * inv + poison, acc.z * inv + poison, acc.w * inv + poison));
+  };
+  // Records of this row and these heads in one descriptor: chunk c at c * stride.
+  const uint32_t stride = gridDim.y * p.rec_floats;
+  const uint32_t rec_m = p.rec_heads * D, rec_l = rec_m + p.rec_heads;
+  const Coherent recs(p.records + (static_cast<size_t>(ch.begin) * gridDim.y + blockIdx.y) * p.rec_floats,
+                      ((ch.of - 1) * stride + p.rec_floats) * static_cast<uint32_t>(sizeof(float)));
+  for (int i = threadIdx.x; i < heads * kQuads; i += kAttnT) {
+    const int h = i / kQuads, d = 4 * (i % kQuads);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kAttnW; ++u) mx = fmaxf(mx, wm[u][h]);
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < kAttnW; ++u) {
+      const float f = wm[u][h] == -INFINITY && mx != -INFINITY ? 0.f : wm[u][h] == mx ? 1.f : exp2_fast(wm[u][h] - mx);
+      const float4 x = *reinterpret_cast<const float4 *>(&wo[u][h][d]);
+      sum = fmaf(f, wl[u][h], sum);
+      acc.x = fmaf(f, x.x, acc.x);
+      acc.y = fmaf(f, x.y, acc.y);
+      acc.z = fmaf(f, x.z, acc.z);
+      acc.w = fmaf(f, x.w, acc.w);
+    }
+    if (ch.of == 1) {
+      emit(h, d, acc, sum);
+    } else {
+      const uint32_t rec = ch.index * stride + h * D;
+      recs.st4((rec + d) / 4, make_float4(acc.x + poison, acc.y + poison, acc.z + poison, acc.w + poison));
+      if (d == 0) {
+        recs.st(ch.index * stride + rec_m + h, mx);
+        recs.st(ch.index * stride + rec_l + h, sum);
+      }
+    }
+  }
+  if (ch.of == 1) return;
+  // The last of the row's chunks to arrive joins them, in their order.
+  wait_vm_stores();
+  __syncthreads();
+  uint32_t *cnt = p.counters + ch.row * gridDim.y + blockIdx.y;
+  if (threadIdx.x == 0) last = atomicAdd(cnt, 1u) == ch.of - 1;
+  __syncthreads();
+  if (!last) return;
+  if (threadIdx.x == 0) *cnt = 0u;
+  // Threads share a head's four dimensions out by chunks, then in LDS.
+  struct Part {
+    float4 acc;
+    float m, l;
+  };
+  Part *parts = reinterpret_cast<Part *>(&wo[0][0][0]);
+  static_assert(sizeof(Part) * kAttnT <= sizeof(wo), "one part per thread");
+  const int items = heads * kQuads, shares = max(1, kAttnT / items);
+  for (int base = 0; base < items; base += kAttnT) {
+    const int i = base + static_cast<int>(threadIdx.x) % min(items, kAttnT), share = threadIdx.x / min(items, kAttnT);
+    const int h = i / kQuads, d = 4 * (i % kQuads);
+    Part x{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
+    auto join = [](Part &x, const Part &y) {
+      const float m = fmaxf(x.m, y.m);
+      const float f = x.m == m ? 1.f : exp2_fast(x.m - m), g = y.m == m ? 1.f : exp2_fast(y.m - m);
+      x.acc.x = fmaf(y.acc.x, g, x.acc.x * f);
+      x.acc.y = fmaf(y.acc.y, g, x.acc.y * f);
+      x.acc.z = fmaf(y.acc.z, g, x.acc.z * f);
+      x.acc.w = fmaf(y.acc.w, g, x.acc.w * f);
+      x.l = fmaf(y.l, g, x.l * f);
+      x.m = m;
+    };
+    if (share < shares && i < items) {
+      constexpr int kAhead = 8;
+      for (uint32_t c = share; c < ch.of; c += kAhead * shares) {
+        Part y[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          // (Past the last chunk the descriptor gives zeros; not joined.)
+          const uint32_t rec = min(c + u * shares, ch.of - 1) * stride;
+          y[u].acc = recs.ld4((rec + h * D + d) / 4);
+          y[u].m = recs.ld(rec + rec_m + h);
+          y[u].l = recs.ld(rec + rec_l + h);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (c + u * shares < ch.of) join(x, y[u]);
+      }
+    }
+    __syncthreads();
+    parts[threadIdx.x] = x;
+    __syncthreads();
+    if (share == 0 && i < items) {
+      for (int u = 1; u < shares; ++u) join(x, parts[threadIdx.x + u * items]);
+      emit(h, d, x.acc, x.l);
+    }
+  }
+}
+
+// ---- fork -----------------------------------------------------------------------
+// The first kernel, one workgroup, counts references, decides which rows copy
+// their last page and deals out free pages; the second writes the new table and
+// copies pages. Bound by latency: a few dependent passes over tables and
+// counts; the copies stream.
+constexpr int kForkT = 1024, kForkWaves = kForkT / kWave;
+constexpr int kForkScan = 8;  // counts that a thread looks at for free pages per pass
+
+struct ForkRow {
+  int32_t parent;   // -1: released
+  int32_t held;     // pages taken over
+  int32_t source;   // the page to copy, or -1
+  uint32_t begin;   // its fresh pages in the free list, the copy's first
+  int32_t fresh;
+  int32_t length;
+};
+struct ForkPlan {
+  uint32_t ok, copies;
+};
+struct ForkLaunch {
+  qd_fork_args a;        // (a.memories is not for the device)
+  qd_page_memory memory[kForkMemories];
+  uint32_t page_shift;
+  ForkPlan *plan;
+  ForkRow *row;          // [rows]
+  int32_t *copy_source;  // [rows] page pairs to copy
+  int32_t *copy_to;
+  int32_t *free_pages;   // [pages]
+  uint32_t blocks;       // 16 KiB pieces of one page in all memories and planes
+};
+
+__device__ __forceinline__ int32_t load_count(int32_t *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Sum over the lanes before this one, and over all waves before.
+__device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t *waves, uint32_t &total) {
+  uint32_t upto = v;
+  const int lane = lane_id();
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const uint32_t x = __shfl_up(upto, o, kWave);
+    if (lane >= o) upto += x;
+  }
+  __syncthreads();
+  if (lane == kWave - 1) waves[wave_id()] = upto;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int u = 0; u < kForkWaves; ++u) {
+    if (u < wave_id()) before += waves[u];
+    total += waves[u];
+  }
+  return before + upto - v;
+}
+
+// Adds `sign` times what the fork changes: a page that an old row takes over to
+// c children counts c - 1 more, one behind its length one less.
+__device__ __forceinline__ void count_references(const ForkLaunch &p, const int *children, int sign, uint32_t *bad) {
+  const int lane = lane_id();
+  for (uint32_t r = wave_id(); r < p.a.rows; r += kForkWaves) {
+    const int32_t *table = p.a.table + r * p.a.table_stride;
+    const uint32_t held = (static_cast<uint32_t>(p.a.lengths[r]) + p.a.page_size - 1) >> p.page_shift;
+    const int change = children[r] - 1;
+    for (uint32_t j = lane; j < p.a.table_width; j += kWave) {
+      // Up to the chunk in which the row ends.
+      const int32_t id = table[j];
+      const bool in = id >= 0 && static_cast<uint32_t>(id) < p.a.pages;
+      const bool over = id < 0;
+      // Entries behind the first negative one are none.
+      const uint64_t ends = __ballot(over);
+      const bool before_end = (ends & ((1ull << lane) - 1)) == 0;
+      if (before_end) {
+        if (j < held) {
+          if (!in) atomicOr(bad, QD_PAGED_BAD_PAGE);
+          if (in && change) atomicAdd(p.a.refs + id, sign * change);
+        } else if (!over) {
+          if (!in) atomicOr(bad, QD_PAGED_BAD_PAGE);
+          if (in) atomicAdd(p.a.refs + id, -sign);
+        }
+      }
+      if (ends) {
+        // A row that ends before its length lacks a page.
+        const uint32_t end = j - lane + __ffsll(static_cast<unsigned long long>(ends)) - 1;
+        if (end < held) atomicOr(bad, QD_PAGED_BAD_PAGE);
+        break;
+      }
+    }
+  }
+}
+
+__global__ __launch_bounds__(kForkT) void fork_plan_kernel(ForkLaunch p) {
+  __shared__ int children[kForkRows], last[kForkRows];
+  __shared__ uint32_t waves[kForkWaves], bad, copies;
+  const uint32_t r = threadIdx.x;  // one thread per row where rows are meant
+  const int64_t room = static_cast<int64_t>(p.a.table_width) << p.page_shift;
+  if (r < p.a.rows) children[r] = 0;
+  if (r == 0) bad = copies = 0;
+  __syncthreads();
+  ForkRow row{-1, 0, -1, 0u, 0, 0};
+  if (r < p.a.rows) {
+    const int32_t own = p.a.lengths[r];
+    if (own < 0 || own > room) atomicOr(&bad, QD_PAGED_BAD_LENGTH);
+    row.parent = p.a.parents ? p.a.parents[r] : static_cast<int32_t>(r);
+    if (row.parent < -1 || row.parent >= static_cast<int32_t>(p.a.rows)) {
+      atomicOr(&bad, QD_PAGED_BAD_ROW);
+      row.parent = -1;
+    }
+    if (row.parent >= 0) {
+      row.length = p.a.lengths[row.parent];
+      if (row.length < 0 || row.length + static_cast<int64_t>(p.a.append) > room) atomicOr(&bad, QD_PAGED_BAD_LENGTH);
+      atomicAdd(&children[row.parent], 1);
+    }
+  }
+  __syncthreads();
+  const bool fits = bad == 0;
+  __syncthreads();
+  if (fits) count_references(p, children, 1, &bad);
+  wait_vm_stores();  // the counts stand in L2 before any of them is read
+  __syncthreads();
+  uint32_t wanted = 0;
+  if (bad == 0) {
+    row.held = (row.length + p.a.page_size - 1) >> p.page_shift;
+    const bool partial = row.parent >= 0 && p.a.append && (row.length & (p.a.page_size - 1));
+    int id = -1;
+    if (r < p.a.rows && partial) id = p.a.table[row.parent * p.a.table_stride + row.held - 1];
+    if (r < p.a.rows) last[r] = id;
+    __syncthreads();
+    if (id >= 0) {
+      int holders = 0, lowest = kForkRows;
+      for (uint32_t u = 0; u < p.a.rows; ++u)
+        if (last[u] == id) {
+          ++holders;
+          lowest = min(lowest, static_cast<int>(u));
+        }
+      if (load_count(p.a.refs + id) != holders || lowest != static_cast<int>(r)) row.source = id;
+    }
+    if (row.parent >= 0) {
+      const uint32_t need = (static_cast<uint32_t>(row.length) + p.a.append + p.a.page_size - 1) >> p.page_shift;
+      row.fresh = static_cast<int>(need) - row.held + (row.source >= 0);
+    }
+    row.begin = block_before(row.fresh, waves, wanted);
+  }
+  // The free pages of the lowest ids.
+  uint32_t found = 0;
+  if (bad == 0)
+    for (uint32_t base = 0; base < p.a.pages && found < wanted; base += kForkT * kForkScan) {
+      int32_t n[kForkScan];
+      uint32_t mine = 0;
+#pragma unroll
+      for (int u = 0; u < kForkScan; ++u) {
+        const uint32_t page = base + r * kForkScan + u;
+        n[u] = page < p.a.pages ? load_count(p.a.refs + page) : 1;
+      }
+#pragma unroll
+      for (int u = 0; u < kForkScan; ++u) mine += n[u] == 0;
+      uint32_t here = 0;
+      uint32_t at = found + block_before(mine, waves, here);
+#pragma unroll
+      for (int u = 0; u < kForkScan; ++u)
+        if (n[u] == 0) {
+          if (at < wanted) p.free_pages[at] = base + r * kForkScan + u;
+          ++at;
+        }
+      found += here;
+    }
+  if (bad == 0 && found < wanted && r == 0) bad = QD_PAGED_EXHAUSTED;
+  wait_vm_stores();  // the free list is read back below
+  __syncthreads();
+  const uint32_t error = bad;
+  __syncthreads();
+  if (error) {
+    if (fits) count_references(p, children, -1, &bad);
+    if (r == 0) {
+      raise_error(p.a.errors, error);
+      p.plan->ok = 0;
+      p.plan->copies = 0;
+    }
+    return;
+  }
+  if (r < p.a.rows) {
+    for (int u = 0; u < row.fresh; ++u) {
+      const int32_t page = p.free_pages[row.begin + u];
+      p.a.refs[page] = 1;
+      if (u == 0 && row.source >= 0) {
+        atomicSub(p.a.refs + row.source, 1);
+        const uint32_t at = atomicAdd(&copies, 1u);
+        p.copy_source[at] = row.source;
+        p.copy_to[at] = page;
+      }
+    }
+    p.row[r] = row;
+  }
+  __syncthreads();
+  if (r == 0) {
+    p.plan->ok = 1;
+    p.plan->copies = copies;
+  }
+}
+
+constexpr uint32_t kCopyPiece = 16384;
+
+__global__ __launch_bounds__(kBlock) void fork_copy_kernel(ForkLaunch p) {
+  const ForkPlan plan = *p.plan;
+  if (blockIdx.x < p.a.rows) {
+    const uint32_t r = blockIdx.x;
+    const ForkRow row = plan.ok ? p.row[r] : ForkRow{};
+    const int32_t *from = p.a.table + (plan.ok ? max(row.parent, 0) : static_cast<int32_t>(r)) * p.a.table_stride;
+    int32_t *to = p.a.table_out + r * p.a.table_out_stride;
+    const int copied = row.source >= 0;
+    for (uint32_t j = threadIdx.x; j < p.a.table_width; j += kBlock) {
+      int32_t id = -1;
+      if (!plan.ok) {
+        id = from[j];
+      } else if (static_cast<int>(j) < row.held) {
+        id = copied && static_cast<int>(j) == row.held - 1 ? p.free_pages[row.begin] : from[j];
+      } else if (static_cast<int>(j) < row.held + row.fresh - copied) {
+        id = p.free_pages[row.begin + copied + j - row.held];
+      }
+      to[j] = id;
+    }
+    if (threadIdx.x == 0)
+      p.a.lengths_out[r] = !plan.ok ? p.a.lengths[r] : row.parent < 0 ? 0 : row.length + static_cast<int32_t>(p.a.append);
+  }
+  const uint64_t work = static_cast<uint64_t>(plan.copies) * p.blocks;
+  for (uint64_t unit = blockIdx.x; unit < work; unit += gridDim.x) {
+    const uint32_t copy = unit / p.blocks;
+    uint32_t piece = unit % p.blocks;
+    int64_t page_stride = 0;
+    uint64_t bytes = 0;
+    char *base = nullptr;
+    // (A loop over a constant number of memories: no indexed copy of them in scratch.)
+#pragma unroll
+    for (uint32_t m = 0; m < kForkMemories; ++m) {
+      if (m >= p.a.memory_count || base) continue;
+      const uint32_t per_plane = (p.memory[m].bytes + kCopyPiece - 1) / kCopyPiece, all = per_plane * p.memory[m].planes;
+      if (piece >= all) {
+        piece -= all;
+        continue;
+      }
+      base = static_cast<char *>(p.memory[m].base) + (piece / per_plane) * p.memory[m].plane_stride;
+      page_stride = p.memory[m].page_stride;
+      bytes = p.memory[m].bytes;
+      piece %= per_plane;
+    }
+    if (!base) continue;
+    const uint64_t begin = static_cast<uint64_t>(piece) * kCopyPiece;
+    const uint32_t n = min(static_cast<uint64_t>(kCopyPiece), bytes - begin);
+    const u4v *src = reinterpret_cast<const u4v *>(base + p.copy_source[copy] * page_stride + begin);
+    u4v *dst = reinterpret_cast<u4v *>(base + p.copy_to[copy] * page_stride + begin);
+    u4v x[kCopyPiece / 16 / kBlock];
+#pragma unroll
+    for (uint32_t u = 0; u < kCopyPiece / 16 / kBlock; ++u)
+      if ((threadIdx.x + u * kBlock) * 16 < n) x[u] = src[threadIdx.x + u * kBlock];
+#pragma unroll
+    for (uint32_t u = 0; u < kCopyPiece / 16 / kBlock; ++u)
+      if ((threadIdx.x + u * kBlock) * 16 < n) dst[threadIdx.x + u * kBlock] = x[u];
+  }
+}
+
+__global__ void clear_kernel(uint32_t *p, size_t n) {
+  for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * blockDim.x) p[i] = 0u;
+}
+
+uint32_t log2_of(uint32_t v) { return static_cast<uint32_t>(__builtin_ctz(v)); }
+
+template <typename... A>
+hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A... args) {
+  void *packed[] = {&args...};
+  return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, packed, 0, s);
+}
+
+// How attention splits rows over workgroups.
+constexpr uint32_t kAttnLeastTiles = 8, kAttnAim = 2048;
+struct AttnShape {
+  uint32_t group, blocks, y, rec_heads, rec_floats, target;
+};
+AttnShape attention_shape(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  AttnShape s{};
+  s.group = heads / kv_heads;
+  s.blocks = (s.group + 15) / 16;
+  s.y = kv_heads * s.blocks;
+  s.rec_heads = std::min(s.group, 16u);
+  s.rec_floats = (s.rec_heads * (head_dim + 2) + 3) / 4 * 4;
+  s.target = static_cast<uint64_t>(rows) * s.y > kOpCounters ? 0 : std::max(1u, kAttnAim / s.y);
+  return s;
+}
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+hipError_t launch_op_clear(hipStream_t s, uint32_t *counters, size_t n) {
+  return launch(clear_kernel, dim3(64), dim3(kBlock), s, counters, n);
+}
+
+hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_append_args &a) {
+  if (a.tokens == 0) return hipSuccess;
+  AppendLaunch p{c, a, log2_of(c.page_size), 0};
+  p.units = ((a.q ? a.heads : 0) + 2 * c.kv_heads) * (c.head_dim / 8);
+  const dim3 grid((static_cast<uint64_t>(a.tokens) * p.units + kBlock - 1) / kBlock);
+  return launch(c.dtype == QD_DTYPE_F32    ? append_kernel<float>
+                : c.dtype == QD_DTYPE_BF16 ? append_kernel<Brain>
+                                           : append_kernel<Half>,
+                grid, dim3(kBlock), s, p);
+}
+
+size_t paged_attention_scratch(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  const AttnShape sh = attention_shape(rows, heads, kv_heads, head_dim);
+  return sh.target ? static_cast<size_t>(rows + sh.target) * sh.y * sh.rec_floats * sizeof(float) : 0;
+}
+
+hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w) {
+  if (c.rows == 0) return hipSuccess;
+  const AttnShape sh = attention_shape(c.rows, a.heads, c.kv_heads, c.head_dim);
+  AttnLaunch p{};
+  p.c = c;
+  p.a = a;
+  p.records = reinterpret_cast<float *>(w.scratch);
+  p.counters = w.counters;
+  p.page_shift = log2_of(c.page_size);
+  p.group = sh.group;
+  p.blocks = sh.blocks;
+  p.rec_heads = sh.rec_heads;
+  p.rec_floats = sh.rec_floats;
+  p.least = kAttnLeastTiles;
+  p.target = sh.target;
+  const uint64_t most = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + kTile - 1) / kTile;
+  if (most <= p.least) p.target = 0;
+  uint64_t x = c.rows;
+  if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + p.least - 1) / p.least));
+  const dim3 grid(static_cast<uint32_t>(x), sh.y), block(kAttnT);
+  const bool wide = c.head_dim == 128;
+  switch (c.dtype) {
+    case QD_DTYPE_F32: return launch(wide ? attention_kernel<float, 128> : attention_kernel<float, 64>, grid, block, s, p);
+    case QD_DTYPE_BF16: return launch(wide ? attention_kernel<Brain, 128> : attention_kernel<Brain, 64>, grid, block, s, p);
+    default: return launch(wide ? attention_kernel<Half, 128> : attention_kernel<Half, 64>, grid, block, s, p);
+  }
+}
+
+size_t pages_fork_scratch(uint32_t rows, uint32_t pages) {
+  return round256(sizeof(ForkPlan)) + round256(rows * sizeof(ForkRow)) + 2 * round256(rows * sizeof(int32_t)) +
+         round256(static_cast<size_t>(pages) * sizeof(int32_t));
+}
+
+hipError_t launch_pages_fork(hipStream_t s, const qd_fork_args &a, const OpScratch &w) {
+  if (a.rows == 0) return hipSuccess;
+  ForkLaunch p{};
+  p.a = a;
+  p.a.memories = nullptr;
+  uint64_t blocks = 0;
+  for (uint32_t m = 0; m < a.memory_count; ++m) {
+    p.memory[m] = a.memories[m];
+    blocks += (p.memory[m].bytes + kCopyPiece - 1) / kCopyPiece * p.memory[m].planes;
+  }
+  p.page_shift = log2_of(a.page_size);
+  p.blocks = static_cast<uint32_t>(blocks);
+  char *at = w.scratch;
+  auto take = [&](size_t bytes) {
+    char *r = at;
+    at += round256(bytes);
+    return r;
+  };
+  p.plan = reinterpret_cast<ForkPlan *>(take(sizeof(ForkPlan)));
+  p.row = reinterpret_cast<ForkRow *>(take(a.rows * sizeof(ForkRow)));
+  p.copy_source = reinterpret_cast<int32_t *>(take(a.rows * sizeof(int32_t)));
+  p.copy_to = reinterpret_cast<int32_t *>(take(a.rows * sizeof(int32_t)));
+  p.free_pages = reinterpret_cast<int32_t *>(take(static_cast<size_t>(a.pages) * sizeof(int32_t)));
+  const hipError_t err = launch(fork_plan_kernel, dim3(1), dim3(kForkT), s, p);
+  if (err != hipSuccess) return err;
+  const uint64_t most = std::max<uint64_t>(a.rows, std::min<uint64_t>(a.rows * blocks, 2048));
+  return launch(fork_copy_kernel, dim3(static_cast<uint32_t>(most)), dim3(kBlock), s, p);
+}
+
+}  // namespace qd
