@@ -1,0 +1,4 @@
+"""torch brings a HIP runtime of its own. A process can hold one: whichever of torch
+and the engine's library is loaded first, the second has to find that one, which
+works only with torch first. Test modules load the library when they are collected."""
+import torch  # noqa: F401

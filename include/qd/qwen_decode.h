@@ -330,6 +330,29 @@ QD_API qd_status qd_generate_resident(qd_engine *engine, uint32_t seq,
                                       uint32_t *stop_reason,
                                       float *all_logits);
 
+/* Beam search from a slot: consumes first_token at the slot's position, then
+ * keeps the `beams` (1..16) best continuations of each step for up to
+ * max_tokens tokens. A beam's score is the sum of its tokens' log
+ * probabilities; one that produced eos (UINT32_MAX: none does) keeps its score
+ * and competes on. The search runs on pages of its own
+ * (include/qd/qd_operators.h): the beams share the slot's positions and each
+ * other's, copy a partly filled page when they part, and one batched step
+ * advances all of them. The slot stays as it was, position, K/V rows and state;
+ * to go on with a result, consume first_token and the tokens (qd_prefill).
+ *   out_tokens  [beams][max_tokens], the best first; past a beam's end: eos
+ *   generated   [beams] tokens of each, its eos included (nullable)
+ *   scores      [beams] score / generated^length_penalty, by which the results
+ *               are ordered (nullable); -inf for a place no continuation filled
+ * max_tokens more positions must fit the slot's capacity. FP32 decoder weights
+ * only. Synchronous; the host waits for the device every 16 steps to see
+ * whether all beams ended. The reference has no beam search
+ * (examples/qwen/README.md:431-432). */
+QD_API qd_status qd_generate_beams(qd_engine *engine, uint32_t seq,
+                                   uint32_t first_token, uint32_t beams,
+                                   uint32_t max_tokens, uint32_t eos,
+                                   float length_penalty, uint32_t *out_tokens,
+                                   uint32_t *generated, float *scores);
+
 /* Runs `tokens` greedy generate-mode steps from the slot's position with a
  * HIP event pair around every kernel launch on the engine stream, and
  * reports per-kernel totals (at most `capacity` entries). Advances the

@@ -129,6 +129,26 @@ class Engine {
     return greedy;
   }
 
+  // One result of a beam search: its tokens (an EOS included) and its score.
+  struct Beam {
+    std::vector<uint32_t> tokens;
+    float score;
+  };
+  // Beam search from slot `seq`, which stays as it was; the best beam first.
+  std::vector<Beam> generate_beams(uint32_t seq, uint32_t first_token, uint32_t beams, uint32_t max_tokens,
+                                   uint32_t eos = UINT32_MAX, float length_penalty = 0.f) {
+    std::vector<uint32_t> tokens(size_t(beams) * max_tokens), generated(beams);
+    std::vector<float> scores(beams);
+    check(qd_generate_beams(get(), seq, first_token, beams, max_tokens, eos, length_penalty, tokens.data(),
+                            generated.data(), scores.data()));
+    std::vector<Beam> r(beams);
+    for (uint32_t b = 0; b < beams; ++b) {
+      const auto first = tokens.begin() + size_t(b) * max_tokens;
+      r[b] = {std::vector<uint32_t>(first, first + generated[b]), scores[b]};
+    }
+    return r;
+  }
+
   uint32_t prefill(uint32_t seq, const std::vector<uint32_t> &tokens,
                    std::vector<float> *last_logits = nullptr,
                    float *top_logit = nullptr) {

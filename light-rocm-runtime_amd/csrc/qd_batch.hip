@@ -276,9 +276,10 @@ struct KvRows {
 // ---- kernels --------------------------------------------------------------------
 
 __global__ __launch_bounds__(kBlock) void batch_embed_kernel(BatchLaunch p, const float *__restrict__ emb,
-                                                             const float *__restrict__ gain, int vocab) {
+                                                             const float *__restrict__ gain, int vocab,
+                                                             const int32_t *__restrict__ tokens) {
   const int b = blockIdx.x;
-  const uint32_t tok = p.token[b];
+  const uint32_t tok = tokens ? static_cast<uint32_t>(tokens[b]) : p.token[b];
   if (tok >= static_cast<uint32_t>(vocab)) return;
   const float *src = emb + static_cast<size_t>(tok) * kH;
   for (int tile = threadIdx.x >> 4; tile < kH / 16; tile += kBlock / 16) {
@@ -293,10 +294,13 @@ __global__ __launch_bounds__(kBlock) void batch_embed_kernel(BatchLaunch p, cons
 // j + 8: the rotate-half partners sit in lanes l and l ^ 8. Heads [0, nq)
 // are queries, then nkv keys, then nkv values (not rotated). K = 896 is
 // split over kQkvSplit workgroups of four waves (two: 144 workgroups instead
-// of 72).
+// of 72). kRaw: the biased rows of all heads go to `raw` [rows][(nq + 2 nkv)
+// * 64] as they are, for a cache of pages.
 constexpr int kQkvSplit = 2;
+template <bool kRaw>
 __global__ __launch_bounds__(kBlock) void batch_qkv_kernel(BatchLaunch p, const float *__restrict__ wqkv,
-                                                           const float *__restrict__ bqkv, int layer) {
+                                                           const float *__restrict__ bqkv, int layer,
+                                                           float *__restrict__ raw) {
   __shared__ __attribute__((aligned(16))) float ring[kWavesPerBlock][kRingFloats];
   __shared__ float red[kWavesPerBlock][4][kWave];
   const int tile = blockIdx.x;
@@ -309,10 +313,10 @@ __global__ __launch_bounds__(kBlock) void batch_qkv_kernel(BatchLaunch p, const 
   const int jt = t & 15;
   const int i = i0 + (jt & 7);
   const int row = head * kHeadDim + (jt < 8 ? i : kRotary + i);
-  const int pos = static_cast<int>(p.pos[min(seq, p.rows - 1)]);
+  const int pos = kRaw ? 0 : static_cast<int>(p.pos[min(seq, p.rows - 1)]);
   const float bias = bqkv[row];
-  const float c = p.rope_cos[pos * kRotary + i];
-  const float s = p.rope_sin[pos * kRotary + i];
+  const float c = kRaw ? 0.f : p.rope_cos[pos * kRotary + i];
+  const float s = kRaw ? 0.f : p.rope_sin[pos * kRotary + i];
   const float inv = row_inv(p, seq);
   const f4v acc = split_product<kH, kQkvSplit>(ring, p.gained, [&](int j) {
     return wqkv + static_cast<size_t>(head * kHeadDim + (j < 8 ? i0 + j : kRotary + i0 + j - 8)) * kH;
@@ -321,6 +325,10 @@ __global__ __launch_bounds__(kBlock) void batch_qkv_kernel(BatchLaunch p, const 
   if (!split_gather<kQkvSplit>(v, p.split, p.counters + kCntQkv, tile)) return;
   // Epilogue over the 256 tile elements.
   v = v * inv + bias;
+  if constexpr (kRaw) {
+    if (seq < p.rows) raw[seq * ((p.nq + 2 * p.nkv) * kHeadDim) + row] = v;
+    return;
+  }
   const float other = __shfl_xor(v, 8, kWave);
   if (seq >= p.rows) return;
   const uint32_t slot = p.slot[seq];
@@ -892,22 +900,26 @@ hipError_t launch_batch_embed(hipStream_t s, const BatchLaunch &b, const float *
     if (b.pos[i] >= static_cast<uint32_t>(b.capacity) || b.token[i] >= static_cast<uint32_t>(vocab))
       return hipErrorInvalidValue;
   Scope scope(m, kBEmbed);
-  batch_embed_kernel<<<b.rows, kBlock, 0, s>>>(b, embed, first_gain, vocab);
+  batch_embed_kernel<<<b.rows, kBlock, 0, s>>>(b, embed, first_gain, vocab, nullptr);
   return hipGetLastError();
 }
 
-hipError_t launch_batch_layer(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, int layer,
-                              const float *next_gain, Marker *m) {
+hipError_t launch_batch_embed_tokens(hipStream_t s, const BatchLaunch &b, const int32_t *tokens, const float *embed,
+                                     const float *first_gain, int vocab) {
   if (!batch_shape_ok(b)) return hipErrorInvalidValue;
-  {
-    Scope scope(m, kBQkvRope);
-    batch_qkv_kernel<<<dim3((b.nq + 2 * b.nkv) * 4, kQkvSplit), kBlock, 0, s>>>(
-        b, w.wqkv, w.bqkv, layer);
-  }
-  {
-    Scope scope(m, kBAttn);
-    batch_attn_kernel<<<dim3(kAttnMaxChunks, b.nkv, b.rows), kAttnThreads, 0, s>>>(b, layer);
-  }
+  batch_embed_kernel<<<b.rows, kBlock, 0, s>>>(b, embed, first_gain, vocab, tokens);
+  return hipGetLastError();
+}
+
+hipError_t launch_batch_qkv_raw(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, float *raw) {
+  if (!batch_shape_ok(b)) return hipErrorInvalidValue;
+  batch_qkv_kernel<true><<<dim3((b.nq + 2 * b.nkv) * 4, kQkvSplit), kBlock, 0, s>>>(b, w.wqkv, w.bqkv, 0, raw);
+  return hipGetLastError();
+}
+
+hipError_t launch_batch_after_attention(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, const float *next_gain,
+                                        Marker *m) {
+  if (!batch_shape_ok(b)) return hipErrorInvalidValue;
   {
     Scope scope(m, kBOproj);
     batch_oproj_kernel<<<dim3(kH / 16, kOSplit), kBlock, 0, s>>>(b, w.wo, w.mlp_norm);
@@ -921,6 +933,27 @@ hipError_t launch_batch_layer(hipStream_t s, const BatchLaunch &b, const LayerPt
     batch_down_kernel<<<dim3(kH / 16, kDownSplit), kBlock, 0, s>>>(b, w.wd, next_gain);
   }
   return hipGetLastError();
+}
+
+hipError_t launch_batch_logits(hipStream_t s, const BatchLaunch &b, const BatchTail &t) {
+  if (!batch_shape_ok(b) || t.vocab <= 0) return hipErrorInvalidValue;
+  batch_lmhead_kernel<<<kBatchLmParts, kLmThreads, 0, s>>>(b, t);
+  return hipGetLastError();
+}
+
+hipError_t launch_batch_layer(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, int layer,
+                              const float *next_gain, Marker *m) {
+  if (!batch_shape_ok(b)) return hipErrorInvalidValue;
+  {
+    Scope scope(m, kBQkvRope);
+    batch_qkv_kernel<false><<<dim3((b.nq + 2 * b.nkv) * 4, kQkvSplit), kBlock, 0, s>>>(
+        b, w.wqkv, w.bqkv, layer, nullptr);
+  }
+  {
+    Scope scope(m, kBAttn);
+    batch_attn_kernel<<<dim3(kAttnMaxChunks, b.nkv, b.rows), kAttnThreads, 0, s>>>(b, layer);
+  }
+  return launch_batch_after_attention(s, b, w, next_gain, m);
 }
 
 hipError_t launch_batch_tail(hipStream_t s, const BatchLaunch &b, const BatchTail &t, Marker *m) {

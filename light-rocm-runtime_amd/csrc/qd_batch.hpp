@@ -120,6 +120,15 @@ hipError_t launch_batch_embed(hipStream_t s, const BatchLaunch &b, const float *
                               int vocab, Marker *m = nullptr);
 hipError_t launch_batch_layer(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, int layer,
                               const float *next_gain, Marker *m = nullptr);
+// The pieces of a step whose rows' K and V live in pages (a beam search): the
+// embedding of tokens on the device, the biased QKV rows [rows][(nq + 2 nkv) *
+// 64] before rotation, O to down, and the logits alone (row b to row slot[b]).
+hipError_t launch_batch_embed_tokens(hipStream_t s, const BatchLaunch &b, const int32_t *tokens, const float *embed,
+                                     const float *first_gain, int vocab);
+hipError_t launch_batch_qkv_raw(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, float *raw);
+hipError_t launch_batch_after_attention(hipStream_t s, const BatchLaunch &b, const LayerPtrs &w, const float *next_gain,
+                                        Marker *m = nullptr);
+hipError_t launch_batch_logits(hipStream_t s, const BatchLaunch &b, const BatchTail &t);
 hipError_t launch_batch_tail(hipStream_t s, const BatchLaunch &b, const BatchTail &t,
                              Marker *m = nullptr);
 

@@ -27,6 +27,7 @@
 #include "qd_device.hpp"
 #include "qd_kernels.hpp"
 #include "qd_batch.hpp"
+#include "qd_operators.hpp"
 #include "qd_prefill.hpp"
 #include "qd_resident.hpp"
 #include "qd_rng.hpp"
@@ -200,6 +201,29 @@ struct qd_engine {
   // (qd_step_batch_noalloc), looked up at creation; null if the lookup failed.
   void *batch_scratch = nullptr;
   std::string batch_scratch_error;
+
+  // A beam search's memory (qd_generate_beams), one allocation of the largest
+  // search so far: pages of all layers, two tables taken in turn, the steps'
+  // choices, and the operators' scratch.
+  static constexpr uint32_t kBeamPage = 16;  // positions: a step copies up to 15 pages of 24 layers, 6 MB at this size
+  struct BeamWorkspace {
+    char *block;
+    size_t bytes;
+    uint32_t pages, width, steps;
+    float *k, *v;               // [layers][pages][kBeamPage][kv_heads * 64]
+    int32_t *refs;              // [pages]
+    int32_t *table[2];          // [kBatchRows][width]
+    int32_t *lengths[2];        // [kBatchRows]
+    int32_t *rows, *positions;  // [capacity]: zeros and 0, 1, 2, ..., for the prompt's rows
+    int32_t *parents, *tokens;  // [steps + 1][kBatchRows]; the first row of each is what the search starts from
+    float *scores[2];           // [kBatchRows]
+    uint8_t *done[2];           // [kBatchRows]
+    uint32_t *errors;
+    float *qkv;                 // [kBatchRows][qkv rows]
+    float *logits;              // [kBatchRows][vocab]
+    qd::OpScratch scratch;
+  };
+  BeamWorkspace bm{};
 
   qd::SeqState *h_states = nullptr;  // pinned [max_batch]
   uint32_t *h_tokens = nullptr;      // pinned [capacity]
@@ -461,6 +485,205 @@ struct qd_engine {
     check(hipMemsetAsync(w.squares, 0, qd::kBatchRows * qd::kBatchTiles * sizeof(float), stream), "memset");
     check(hipMemsetAsync(w.counters, 0, qd::kBatchCounters * sizeof(uint32_t), stream), "memset");
     bt = w;
+  }
+
+  // The memory of a search of `steps` steps over `pages` pages, from `base` on
+  // (nullptr: its size only).
+  BeamWorkspace carve_beam_workspace(char *base, uint32_t pages, uint32_t steps) const {
+    BeamWorkspace w{};
+    w.block = base;
+    w.pages = pages;
+    w.steps = steps;
+    w.width = uint32_t((CAP + kBeamPage - 1) / kBeamPage);
+    auto take = [&](auto *&p, size_t count) {
+      p = base ? reinterpret_cast<std::remove_reference_t<decltype(p)>>(base + w.bytes) : nullptr;
+      w.bytes += (count * sizeof(*p) + 255) / 256 * 256;
+    };
+    const size_t r = qd::kBatchRows;
+    take(w.k, L * pages * kBeamPage * KVD);
+    take(w.v, L * pages * kBeamPage * KVD);
+    take(w.refs, pages);
+    for (int i = 0; i < 2; ++i) {
+      take(w.table[i], r * w.width);
+      take(w.lengths[i], r);
+      take(w.scores[i], r);
+      take(w.done[i], r);
+    }
+    take(w.rows, CAP);
+    take(w.positions, CAP);
+    take(w.parents, (steps + 1) * r);
+    take(w.tokens, (steps + 1) * r);
+    take(w.errors, 1);
+    take(w.qkv, r * QKV);
+    take(w.logits, r * V);
+    take(w.scratch.counters, qd::kOpCounters);
+    size_t scratch = std::max(qd::paged_attention_scratch(uint32_t(r), uint32_t(NQ), uint32_t(NKV), qd::kHeadDim),
+                              qd::pages_fork_scratch(uint32_t(r), pages));
+    for (uint32_t n = 1; n <= r; ++n) scratch = std::max(scratch, qd::beam_select_scratch(1, n, n, uint32_t(V)));
+    take(w.scratch.scratch, scratch);
+    return w;
+  }
+  void beam_workspace(uint32_t pages, uint32_t steps) {
+    if (bm.block && bm.pages >= pages && bm.steps >= steps) return;
+    pages = std::max(pages, bm.pages);
+    steps = std::max(steps, bm.steps);
+    const size_t bytes = carve_beam_workspace(nullptr, pages, steps).bytes;
+    if (bm.block) {
+      check(hipStreamSynchronize(stream), "hipStreamSynchronize");
+      release(bm.block, bm.bytes);
+      bm = BeamWorkspace{};
+    }
+    bm = carve_beam_workspace(alloc<char>(bytes), pages, steps);
+    check(qd::launch_op_clear(stream, bm.scratch.counters, qd::kOpCounters), "counter clear");
+    std::vector<int32_t> iota(CAP);
+    for (size_t i = 0; i < CAP; ++i) iota[i] = int32_t(i);
+    check(hipMemcpyAsync(bm.positions, iota.data(), CAP * 4, hipMemcpyHostToDevice, stream), "H2D");
+    check(hipMemsetAsync(bm.rows, 0, CAP * 4, stream), "memset");
+    check(hipStreamSynchronize(stream), "hipStreamSynchronize");
+  }
+  // The pages of layer l as the operators take them, with table and lengths `side`.
+  qd_paged_cache beam_cache(size_t l, int side, uint32_t beams) const {
+    qd_paged_cache c{};
+    c.k = bm.k + l * bm.pages * kBeamPage * KVD;
+    c.v = bm.v + l * bm.pages * kBeamPage * KVD;
+    c.page_stride = int64_t(kBeamPage * KVD);
+    c.token_stride = int64_t(KVD);
+    c.head_stride = qd::kHeadDim;
+    c.table = bm.table[side];
+    c.table_stride = bm.width;
+    c.lengths = bm.lengths[side];
+    c.errors = bm.errors;
+    c.rows = beams;
+    c.table_width = bm.width;
+    c.pages = bm.pages;
+    c.page_size = kBeamPage;
+    c.kv_heads = uint32_t(NKV);
+    c.head_dim = qd::kHeadDim;
+    c.dtype = QD_DTYPE_F32;
+    c.device = cfg.device;
+    return c;
+  }
+  // A search's start: all beams hold the slot's positions in the first pages,
+  // one of them has a score.
+  void begin_beams(uint32_t seq, uint32_t beams, uint32_t first_token) {
+    const uint32_t n = positions[seq], held = (n + kBeamPage - 1) / kBeamPage;
+    std::vector<int32_t> refs(bm.pages, 0), table(size_t(beams) * bm.width, -1), lengths(beams, int32_t(n)),
+        tokens(beams, int32_t(first_token)), parents(beams);
+    std::vector<float> scores(beams, -INFINITY);
+    scores[0] = 0.f;
+    for (uint32_t p = 0; p < held; ++p) {
+      refs[p] = int32_t(beams);
+      for (uint32_t b = 0; b < beams; ++b) table[size_t(b) * bm.width + p] = int32_t(p);
+    }
+    for (uint32_t b = 0; b < beams; ++b) parents[b] = int32_t(b);
+    const auto put = [&](auto *dst, const auto &v) {
+      check(hipMemcpyAsync(dst, v.data(), v.size() * sizeof(v[0]), hipMemcpyHostToDevice, stream), "H2D");
+    };
+    put(bm.refs, refs);
+    put(bm.table[0], table);
+    put(bm.lengths[0], lengths);
+    put(bm.scores[0], scores);
+    put(bm.tokens, tokens);
+    put(bm.parents, parents);
+    check(hipMemsetAsync(bm.done[0], 0, beams, stream), "memset");
+    check(hipMemsetAsync(bm.errors, 0, 4, stream), "memset");
+    check(hipStreamSynchronize(stream), "hipStreamSynchronize");  // the vectors go
+    if (n == 0) return;
+    for (size_t l = 0; l < L; ++l) {
+      qd_append_args a{};
+      a.k = kv_slice(k_cache, seq, l);
+      a.v = kv_slice(v_cache, seq, l);
+      a.k_stride = a.v_stride = int64_t(KVD);
+      a.positions = bm.positions;
+      a.rows = bm.rows;
+      a.tokens = n;
+      check(qd::launch_paged_append(stream, beam_cache(l, 0, beams), a), "append launch");
+    }
+  }
+  // Step t of a search: the beams chosen by the step before take over their
+  // parents' pages with room for one token, it goes through every layer, and the
+  // best `beams` continuations are chosen.
+  void beam_step(uint32_t t, uint32_t beams, uint32_t eos) {
+    const int from = t & 1, to = 1 - from;
+    int32_t *parents = bm.parents + size_t(t) * qd::kBatchRows, *tokens = bm.tokens + size_t(t) * qd::kBatchRows;
+    const qd_page_memory memories[2] = {
+        {bm.k, int64_t(bm.pages * kBeamPage * KVD * 4), int64_t(kBeamPage * KVD * 4), kBeamPage * KVD * 4, uint32_t(L), 0},
+        {bm.v, int64_t(bm.pages * kBeamPage * KVD * 4), int64_t(kBeamPage * KVD * 4), kBeamPage * KVD * 4, uint32_t(L), 0}};
+    qd_fork_args f{};
+    f.table = bm.table[from];
+    f.lengths = bm.lengths[from];
+    f.parents = parents;
+    f.table_out = bm.table[to];
+    f.lengths_out = bm.lengths[to];
+    f.refs = bm.refs;
+    f.table_stride = f.table_out_stride = bm.width;
+    f.errors = bm.errors;
+    f.memories = memories;
+    f.memory_count = 2;
+    f.rows = beams;
+    f.table_width = bm.width;
+    f.pages = bm.pages;
+    f.page_size = kBeamPage;
+    f.append = 1;
+    f.device = cfg.device;
+    check(qd::launch_pages_fork(stream, f, bm.scratch), "fork launch");
+
+    uint32_t rows[qd::kBatchRows] = {}, none[qd::kBatchRows] = {};
+    qd::BatchLaunch b = batch_args(bt, rows, none, int(beams));  // (slots, positions and tokens stay on the device)
+    for (uint32_t i = 0; i < beams; ++i) b.slot[i] = i;
+    check(qd::launch_batch_embed_tokens(stream, b, tokens, embed, layers[0].attn_norm, int(V)), "embed launch");
+    for (size_t l = 0; l < L; ++l) {
+      const qd_paged_cache c = beam_cache(l, to, beams);
+      check(qd::launch_batch_qkv_raw(stream, b, layers[l], bm.qkv), "qkv launch");
+      qd_append_args a{};
+      a.q = bm.qkv;
+      a.k = bm.qkv + QD;
+      a.v = bm.qkv + QD + KVD;
+      a.q_out = bt.q;
+      a.q_stride = a.k_stride = a.v_stride = int64_t(QKV);
+      a.q_out_stride = int64_t(QD);
+      a.positions = bm.lengths[to];
+      a.position_bias = -1;
+      a.tokens = beams;
+      a.heads = uint32_t(NQ);
+      a.rotary_dim = qd::kHeadDim;
+      a.table_positions = uint32_t(CAP);
+      a.cos_table = rope_cos;
+      a.sin_table = rope_sin;
+      check(qd::launch_paged_append(stream, c, a), "append launch");
+      qd_attention_args at{};
+      at.q = bt.q;
+      at.out = bt.attn;
+      at.q_stride = at.out_stride = int64_t(QD);
+      at.q_head_stride = at.out_head_stride = qd::kHeadDim;
+      at.heads = uint32_t(NQ);
+      at.scale = 0.125f;  // 1 / sqrt(64)
+      check(qd::launch_paged_attention(stream, c, at, bm.scratch), "attention launch");
+      check(qd::launch_batch_after_attention(stream, b, layers[l], l + 1 < L ? layers[l + 1].attn_norm : final_norm),
+            "layer launch");
+    }
+    qd::BatchTail tail = batch_tail(bt, 0);
+    tail.logits = bm.logits;
+    check(qd::launch_batch_logits(stream, b, tail), "logits launch");
+    qd_select_args s{};
+    s.logits = bm.logits;
+    s.group_stride = int64_t(beams * V);
+    s.beam_stride = int64_t(V);
+    s.scores = bm.scores[from];
+    s.scores_out = bm.scores[to];
+    s.parents = parents + qd::kBatchRows;
+    s.tokens = tokens + qd::kBatchRows;
+    if (eos != UINT32_MAX) {
+      s.done = bm.done[from];
+      s.done_out = bm.done[to];
+      s.eos = eos;
+    }
+    s.dtype = QD_DTYPE_F32;
+    s.groups = 1;
+    s.beams = s.k = beams;
+    s.vocab = uint32_t(V);
+    s.device = cfg.device;
+    check(qd::launch_beam_select(stream, s, bm.scratch), "select launch");
   }
 
   // Arguments of one batched launch over rows sequences: slot ids, tokens
@@ -2033,6 +2256,86 @@ qd_status qd_generate_resident(qd_engine *e, uint32_t seq, uint32_t first_token,
   });
 }
 
+
+qd_status qd_generate_beams(qd_engine *e, uint32_t seq, uint32_t first_token, uint32_t beams, uint32_t max_tokens,
+                            uint32_t eos, float length_penalty, uint32_t *out_tokens, uint32_t *generated,
+                            float *scores) {
+  return guard([&] {
+    if (!e || !out_tokens) fail(QD_ERROR_INVALID_ARGUMENT, "null argument");
+    e->check_seq(seq);
+    e->check_loaded();
+    if (e->narrow()) fail(QD_ERROR_NOT_SUPPORTED, "beam search needs FP32 decoder weights");
+    if (beams == 0 || beams > uint32_t(qd::kBatchRows))
+      fail(QD_ERROR_INVALID_ARGUMENT, "%u beams: 1 to %d", beams, qd::kBatchRows);
+    if (beams > e->V) fail(QD_ERROR_INVALID_ARGUMENT, "%u beams over a vocabulary of %zu", beams, e->V);
+    if (max_tokens == 0) fail(QD_ERROR_INVALID_ARGUMENT, "max_tokens must be positive");
+    if (first_token >= e->V) fail(QD_ERROR_INVALID_ARGUMENT, "token %u >= vocab", first_token);
+    if (eos != UINT32_MAX && eos >= e->V) fail(QD_ERROR_INVALID_ARGUMENT, "eos %u >= vocab", eos);
+    if (!std::isfinite(length_penalty)) fail(QD_ERROR_INVALID_ARGUMENT, "length_penalty must be finite");
+    if (!qd::beam_select_fits(beams, uint32_t(e->V)))
+      fail(QD_ERROR_NOT_SUPPORTED, "%u beams over a vocabulary of %zu: up to 2^24 in all", beams, e->V);
+    if (size_t(e->positions[seq]) + max_tokens > e->CAP)
+      fail(QD_ERROR_INVALID_ARGUMENT, "search of %u tokens from position %u overflows capacity %zu", max_tokens,
+           e->positions[seq], e->CAP);
+    e->set_device();
+    e->settle_layers();
+    e->batch_workspace();
+    // The slot's pages, and for each beam those it fills alone: one begun inside
+    // the last of the slot's, and a fresh copy beside it while pages change hands.
+    const uint32_t page = qd_engine::kBeamPage;
+    const uint64_t pages = (e->positions[seq] + page - 1) / page + uint64_t(beams) * (max_tokens / page + 3);
+    e->beam_workspace(uint32_t(pages), max_tokens);
+    e->begin_beams(seq, beams, first_token);
+    uint8_t done[qd::kBatchRows];
+    uint32_t steps = 0;
+    while (steps < max_tokens) {
+      e->beam_step(steps, beams, eos);
+      ++steps;
+      if (eos == UINT32_MAX || steps % 16 != 0 || steps == max_tokens) continue;
+      check(hipMemcpyAsync(done, e->bm.done[steps & 1], beams, hipMemcpyDeviceToHost, e->stream), "D2H");
+      e->sync();
+      if (std::all_of(done, done + beams, [](uint8_t d) { return d != 0; })) break;
+    }
+    const size_t r = qd::kBatchRows;
+    std::vector<int32_t> parents((steps + 1) * r), tokens((steps + 1) * r);
+    std::vector<float> sums(beams);
+    uint32_t errors = 0;
+    check(hipMemcpyAsync(parents.data(), e->bm.parents, parents.size() * 4, hipMemcpyDeviceToHost, e->stream), "D2H");
+    check(hipMemcpyAsync(tokens.data(), e->bm.tokens, tokens.size() * 4, hipMemcpyDeviceToHost, e->stream), "D2H");
+    check(hipMemcpyAsync(sums.data(), e->bm.scores[steps & 1], beams * 4, hipMemcpyDeviceToHost, e->stream), "D2H");
+    check(hipMemcpyAsync(&errors, e->bm.errors, 4, hipMemcpyDeviceToHost, e->stream), "D2H");
+    e->sync();
+    if (errors) fail(QD_ERROR_RUNTIME, "beam search: the pages do not fit (error word 0x%x)", errors);
+    // Each beam's tokens, from the last step back.
+    struct Result {
+      std::vector<uint32_t> tokens;
+      uint32_t generated;
+      float score;
+    };
+    std::vector<Result> results(beams);
+    for (uint32_t b = 0; b < beams; ++b) {
+      Result &x = results[b];
+      x.tokens.assign(max_tokens, eos == UINT32_MAX ? 0 : eos);
+      uint32_t at = b;
+      for (uint32_t t = steps; t > 0; --t) {
+        x.tokens[t - 1] = uint32_t(tokens[t * r + at]);
+        at = uint32_t(parents[t * r + at]);
+      }
+      x.generated = steps;
+      if (eos != UINT32_MAX) {
+        const auto end = std::find(x.tokens.begin(), x.tokens.begin() + steps, eos);
+        x.generated = std::min(steps, uint32_t(end - x.tokens.begin()) + 1);
+      }
+      x.score = float(double(sums[b]) / std::pow(double(x.generated), double(length_penalty)));
+    }
+    std::stable_sort(results.begin(), results.end(), [](const Result &a, const Result &b) { return a.score > b.score; });
+    for (uint32_t b = 0; b < beams; ++b) {
+      std::copy(results[b].tokens.begin(), results[b].tokens.end(), out_tokens + size_t(b) * max_tokens);
+      if (generated) generated[b] = results[b].generated;
+      if (scores) scores[b] = results[b].score;
+    }
+  });
+}
 
 qd_status qd_profile_kernels(qd_engine *e, uint32_t seq, uint32_t first_token, uint32_t tokens,
                              qd_kernel_stat *stats, uint32_t capacity, uint32_t *count) {

@@ -17,7 +17,12 @@
 // qd_prefill (dense MFMA GEMMs); generation is one qd_step per token, or
 // with --sync-stack the reference's layer-by-layer decode
 // (qd_embed_hidden, qd_layer_decode per layer with a synchronisation after
-// each, qd_tail), or with --resident one device-resident launch.
+// each, qd_tail), or with --resident one device-resident launch. With
+// --beams N it is a beam search (qd_generate_beams) from the prompt's last
+// token: one line per beam, then the best beam's tokens as above:
+//
+//   beam N score=X generated_tokens=G token_ids=[t1,t2,...]
+//
 // --e2e-check applies the reference's gate
 // (benchmarks/triton_mini_decoder_layer.cpp:1369-1391): finite logits and the
 // requested token count.
@@ -67,6 +72,8 @@ struct Options {
   bool gpu_stage_profile = false;
   bool cpu_submit_profile = false;
   bool resident = false;
+  uint32_t beams = 0;  // 0: greedy
+  float length_penalty = 0.f;
   int device = 0;
 };
 
@@ -77,7 +84,7 @@ void usage(FILE *f) {
       "[--vocab V])\n"
       "              [--valid-keys N] [--warmup-iterations N | --no-warmup] [--no-model-tail]\n"
       "              [--e2e-check] [--max-new-tokens N --prompt-token-ids a,b,c]\n"
-      "              [--sync-stack | --resident] [--layer-sweep] [--trace-setup] [--trace-run]\n"
+      "              [--sync-stack | --resident | --beams N [--length-penalty X]] [--layer-sweep] [--trace-setup] [--trace-run]\n"
       "              [--gpu-stage-profile] [--cpu-submit-profile] [--keys CAPACITY]\n"
       "              [--eos-token-id T] [--device D]\n");
 }
@@ -172,6 +179,15 @@ Options parse(int argc, char **argv) {
       o.cpu_submit_profile = true;
     } else if (!std::strcmp(a, "--resident")) {
       o.resident = true;
+    } else if (!std::strcmp(a, "--beams")) {
+      o.beams = parse_u32(a, value());
+      if (o.beams < 1 || o.beams > 16) throw std::invalid_argument("--beams takes 1 to 16");
+    } else if (!std::strcmp(a, "--length-penalty")) {
+      const char *text = value();
+      char *end = nullptr;
+      o.length_penalty = std::strtof(text, &end);
+      if (end == text || *end || !std::isfinite(o.length_penalty))
+        throw std::invalid_argument(std::string("--length-penalty requires a number, got '") + text + "'");
     } else if (!std::strcmp(a, "--device")) {
       o.device = static_cast<int>(parse_u32(a, value()));
     } else if (a[0] != '-' && !o.iterations_set) {
@@ -199,6 +215,9 @@ Options parse(int argc, char **argv) {
     throw std::invalid_argument("--warmup-iterations and --no-warmup are mutually exclusive");
   if (o.sync_stack && o.resident)
     throw std::invalid_argument("--sync-stack and --resident are mutually exclusive");
+  if (o.beams && (o.sync_stack || o.resident))
+    throw std::invalid_argument("--beams excludes --sync-stack and --resident");
+  if (o.beams && !o.max_new_tokens) throw std::invalid_argument("--beams requires --max-new-tokens");
   if (o.prompt.empty() && !o.no_model_tail) throw std::invalid_argument("--prompt-token-ids is required");
   if (o.no_model_tail) {
     // The stack alone runs on token 0's embedding at every prompt position.
@@ -404,7 +423,20 @@ int run(const Options &o) {
     bad += non_finite;
     std::printf("step %u top_token=%u logit=%g vocab=%u\n", step, tok, top, vocab);
   };
-  if (o.max_new_tokens) {
+  if (o.beams) {
+    // From the prompt's last token, so that the first choice is among the beams too.
+    engine.kv_reset(0, prompt_len - 1);
+    const auto found = engine.generate_beams(0, o.prompt.back(), o.beams, o.max_new_tokens, o.eos, o.length_penalty);
+    engine.kv_reset(0, prompt_len);
+    for (size_t b = 0; b < found.size(); ++b) {
+      std::printf("beam %zu score=%g generated_tokens=%zu token_ids=[", b + 1, found[b].score, found[b].tokens.size());
+      for (size_t i = 0; i < found[b].tokens.size(); ++i) std::printf("%s%u", i ? "," : "", found[b].tokens[i]);
+      std::printf("]\n");
+      if (!std::isfinite(found[b].score)) ++bad;
+    }
+    generated = found[0].tokens;
+    eos_hit = !generated.empty() && generated.back() == o.eos;
+  } else if (o.max_new_tokens) {
     emit(1, logits);
     generated.push_back(token);
     eos_hit = token == o.eos;
@@ -482,7 +514,7 @@ int run(const Options &o) {
   }
   std::printf("qd_run summary prompt_tokens=%u generated_tokens=%zu generation_ms=%.3f path=%s\n",
               prompt_len, generated.size(), gen_ms,
-              o.resident ? "resident" : (o.sync_stack ? "layer-by-layer" : "step"));
+              o.beams ? "beams" : o.resident ? "resident" : (o.sync_stack ? "layer-by-layer" : "step"));
   std::fflush(stdout);
   if (o.e2e_check) {
     if (bad) {

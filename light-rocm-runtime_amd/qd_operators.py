@@ -6,15 +6,24 @@ the work is queued on `stream` (a raw stream handle such as
 torch.cuda.current_stream().cuda_stream; 0 is the null stream), and errors raise
 QdError. Tensors must stay alive until the stream has run the call; a tensor of
 another stream needs the caller's wait or event, as with any kernel launch.
+
+torch brings a HIP runtime of its own, and a process can hold one: import torch, or
+this module, before the first call into the engine's library.
 """
 from __future__ import annotations
 
 import ctypes as C
+import sys
 
 import numpy as np
 
 import qwen_decode as qd
 from qwen_decode import QdError  # noqa: F401  (what the calls raise)
+
+if qd._lib is not None and "torch" not in sys.modules:
+    raise ImportError("the engine's library is loaded with another HIP runtime than torch's: "
+                      "import torch or qd_operators before the first call of qwen_decode")
+import torch  # noqa: E402
 
 BAD_LENGTH, BAD_PAGE, BAD_POSITION, BAD_ROW, EXHAUSTED = 1, 2, 4, 8, 16
 
@@ -96,18 +105,13 @@ def _check(status):
 
 # ---- what a tensor is -----------------------------------------------------------------
 
-_types = None
+_TYPES = {torch.float32: qd.DTYPE_F32, torch.bfloat16: qd.DTYPE_BF16, torch.float16: qd.DTYPE_F16,
+          torch.int32: "int32", torch.uint8: "uint8"}
 
 
 def _dtype(t):
     """qd_dtype of a tensor, or None."""
-    global _types
-    if _types is None:
-        import torch
-
-        _types = {torch.float32: qd.DTYPE_F32, torch.bfloat16: qd.DTYPE_BF16, torch.float16: qd.DTYPE_F16,
-                  torch.int32: "int32", torch.uint8: "uint8"}
-    return _types.get(t.dtype)
+    return _TYPES.get(t.dtype)
 
 
 def _refuse(text):

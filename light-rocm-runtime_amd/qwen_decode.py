@@ -97,6 +97,8 @@ _SIGNATURES = {
     "qd_step_batch_noalloc": (C.c_int, [_E, C.c_uint32, _U, _U, _F, _U]),
     "qd_generate_resident": (C.c_int, [_E, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32,
                                        _U, _U, _U, _F]),
+    "qd_generate_beams": (C.c_int, [_E, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_float,
+                                    _U, _U, _F]),
     "qd_last_timing": (C.c_int, [_E, C.POINTER(Timing)]),
     "qd_profile_kernels": (C.c_int, [_E, C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(KernelStat),
                                      C.c_uint32, _U]),
@@ -356,6 +358,17 @@ class Engine:
                                           C.byref(n), C.byref(reason), _f(logits)))
         k = int(n.value)
         return out[:k], int(reason.value), (None if logits is None else logits[:k])
+
+    def generate_beams(self, seq: int, first_token: int, beams: int, max_tokens: int, eos: int = NO_EOS,
+                       length_penalty: float = 0.0):
+        """Beam search from the slot, which stays as it was: per beam, the best first, its tokens
+        and its score."""
+        out = np.zeros((beams, max_tokens), np.uint32)
+        n = np.zeros(beams, np.uint32)
+        scores = np.zeros(beams, np.float32)
+        _check(lib().qd_generate_beams(self.handle, seq, first_token, beams, max_tokens, eos, length_penalty, _u(out),
+                                       _u(n), _f(scores)))
+        return [out[b, : n[b]] for b in range(beams)], scores
 
     @staticmethod
     def _stats(call) -> dict:
