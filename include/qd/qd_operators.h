@@ -239,8 +239,8 @@ typedef struct qd_select_args {
   uint32_t dtype;        /* of the logits */
   uint32_t groups;
   uint32_t beams;        /* up to 32 */
-  uint32_t vocab;
-  uint32_t k;            /* up to 64 and beams x vocab; k x vocab up to 2^24 */
+  uint32_t vocab;        /* up to 2^24 */
+  uint32_t k;            /* up to 64 and beams x vocab */
   uint32_t eos;          /* read with done */
   int32_t device;
 } qd_select_args;

@@ -2272,8 +2272,7 @@ qd_status qd_generate_beams(qd_engine *e, uint32_t seq, uint32_t first_token, ui
     if (first_token >= e->V) fail(QD_ERROR_INVALID_ARGUMENT, "token %u >= vocab", first_token);
     if (eos != UINT32_MAX && eos >= e->V) fail(QD_ERROR_INVALID_ARGUMENT, "eos %u >= vocab", eos);
     if (!std::isfinite(length_penalty)) fail(QD_ERROR_INVALID_ARGUMENT, "length_penalty must be finite");
-    if (!qd::beam_select_fits(beams, uint32_t(e->V)))
-      fail(QD_ERROR_NOT_SUPPORTED, "%u beams over a vocabulary of %zu: up to 2^24 in all", beams, e->V);
+    if (e->V > qd::kSelectVocab) fail(QD_ERROR_NOT_SUPPORTED, "a vocabulary of %zu: up to %u", e->V, qd::kSelectVocab);
     if (size_t(e->positions[seq]) + max_tokens > e->CAP)
       fail(QD_ERROR_INVALID_ARGUMENT, "search of %u tokens from position %u overflows capacity %zu", max_tokens,
            e->positions[seq], e->CAP);

@@ -145,7 +145,7 @@ qd_status check_select(uint32_t groups, uint32_t beams, uint32_t k, uint32_t voc
   if (beams > qd::kSelectBeams || k > qd::kSelectK)
     return refuse(QD_ERROR_NOT_SUPPORTED, "%u beams, k %u: up to %u and %u", beams, k, qd::kSelectBeams, qd::kSelectK);
   if (k > static_cast<uint64_t>(beams) * vocab) return refuse(QD_ERROR_INVALID_ARGUMENT, "k %u of %u x %u", k, beams, vocab);
-  if (!qd::beam_select_fits(k, vocab)) return refuse(QD_ERROR_NOT_SUPPORTED, "k x vocab past 2^24 (k %u, vocab %u)", k, vocab);
+  if (vocab > qd::kSelectVocab) return refuse(QD_ERROR_NOT_SUPPORTED, "vocab %u: up to %u", vocab, qd::kSelectVocab);
   if (static_cast<uint64_t>(groups) * (beams + 1) > 65535)
     return refuse(QD_ERROR_NOT_SUPPORTED, "%u groups of %u beams: up to 65535 groups and beams together", groups, beams);
   return QD_SUCCESS;

@@ -24,7 +24,7 @@ struct OpScratch {
 
 constexpr uint32_t kPageSizeLeast = 16, kPageSizeMost = 1024;
 constexpr uint32_t kForkRows = 1024, kForkMemories = 4;
-constexpr uint32_t kSelectBeams = 32, kSelectK = 64;
+constexpr uint32_t kSelectBeams = 32, kSelectK = 64, kSelectVocab = 1u << 24;
 
 hipError_t launch_op_clear(hipStream_t s, uint32_t *counters, size_t n);
 
@@ -38,8 +38,6 @@ size_t pages_fork_scratch(uint32_t rows, uint32_t pages);
 hipError_t launch_pages_fork(hipStream_t s, const qd_fork_args &a, const OpScratch &w);
 
 size_t beam_select_scratch(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab);
-// Whether one row's candidates fit the kernel's merge.
-bool beam_select_fits(uint32_t k, uint32_t vocab);
 hipError_t launch_beam_select(hipStream_t s, const qd_select_args &a, const OpScratch &w);
 
 }  // namespace qd

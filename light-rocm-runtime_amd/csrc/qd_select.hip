@@ -1,11 +1,12 @@
 // Beam selection for gfx950: the best k of beams x vocabulary. Declared in
 // include/qd/qd_operators.h.
 //
-// A workgroup takes a slice of a row's logits into registers in one pass and
-// leaves its maximum, its sum of exponentials and its best k as sorted keys; the
-// last slice of a row to arrive joins them into the row's best k with their
+// A workgroup takes a run of a row's logits, tile after tile with the next one's
+// loads under way; each wave keeps, without a barrier, a running maximum and sum
+// per lane and the keys at or above a bound that only rises, and hands over its
+// best k. The last run of a row to arrive joins the row's best k with their
 // scores; the last row of a group to arrive chooses among its beams'. Bound by
-// reading the logits for many rows, by the two hand-overs for few.
+// the logits' bandwidth for many rows, by the two hand-overs for few.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,24 +25,30 @@ namespace {
 using namespace dev;
 
 constexpr int kT = kBlock;
-constexpr int kJoin = 2048;   // keys that one row's slices, or one group's rows, hand over at most
-constexpr int kShort = 1024;  // keys that are put in order; beyond, the slower ways below
+constexpr int kEach = 16, kTile = kT * kEach;  // logits of a thread and of a workgroup at once
+constexpr int kJoin = 2048;  // keys that one row's runs, or one group's rows, hand over at most
+constexpr int kOwn = 640;    // keys of a wave: k from before, and a piece of 64 x 8
+constexpr int kOwnStride = kOwn + 8;  // and zeros behind them
 constexpr uint32_t kLowest = 0x00800000u;  // the order of the lowest finite number
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct SelectLaunch {
   qd_select_args a;
-  uint32_t slices;      // of a row
-  uint64_t *keys;       // [rows][slices][k]
-  double *sums;         // [rows][slices]
-  float *maxima;        // [rows][slices]
+  uint32_t runs;        // of a row
+  uint32_t tiles;       // of a run
+  uint64_t *keys;       // [rows][runs][k]
+  double *sums;         // [rows][runs]
+  float *maxima;        // [rows][runs]
   double *row_score;    // [rows][k]
   uint32_t *row_token;  // [rows][k]
-  uint32_t *row_count;  // arrivals [rows]
+  uint32_t *row_count;  // arrivals [rows * apart]
   uint32_t *group_count;
+  uint32_t apart;       // words between two counters
 };
 
 // A key orders a row's continuations: the higher logit first, then the lower
-// token. The high word is the logit's bits, monotone; 0 is no key.
+// token. The high word is the logit's bits, monotone (those of 0 for -0, which is
+// no lower); 0 is no key.
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t u = __float_as_uint(x);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -51,7 +58,7 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
-  return static_cast<uint64_t>(order_of(x)) << 32 | ~token;
+  return static_cast<uint64_t>(order_of(x + 0.f)) << 32 | ~token;
 }
 __device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~static_cast<uint32_t>(key); }
 
@@ -76,6 +83,7 @@ __device__ __forceinline__ float widen(uint32_t bits) {
     return half_lo(bits);
 }
 // 16 bytes at any element's address.
+// (Under-aligned types: the compiler's loads take any address.)
 typedef uint32_t Words4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t Words2 __attribute__((ext_vector_type(4), aligned(2)));
 template <typename E>
@@ -84,18 +92,44 @@ struct Piece {
   using words = std::conditional_t<sizeof(E) == 4, Words4, Words2>;
 };
 
+constexpr int kFew = 512;  // keys of a run that are ranked from one list
+
 struct Shared {
-  uint64_t list[kJoin];
-  uint64_t shorter[kShort];
+  uint64_t own[kWavesPerBlock][kOwnStride];  // the waves' keys
+  uint64_t best[kWavesPerBlock][kSelectK];
+  uint64_t few[kFew];
   double sum[kWavesPerBlock];
   float top[kWavesPerBlock];
-  uint32_t bound[kWavesPerBlock];
+  uint32_t bound[kWavesPerBlock], count[kWavesPerBlock];
   uint32_t n, last;
 };
+// The joins' keys and their places, where the waves' keys were.
+static_assert(sizeof(Shared::own) + sizeof(Shared::best) >= kJoin * (sizeof(uint64_t) + sizeof(uint16_t)), "the joins' lists");
 
-// A lower bound of the order of the workgroup's k-th best, from each thread's
-// best: the k-th best lane of a wave has k as good before or at it. (The last 12
-// bits are left zero.) Between barriers.
+// Sum over the wave in 64 bits, in wave_sum's order.
+template <int kCtrl>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint32_t lo = __float_as_uint(dpp<kCtrl>(__uint_as_float(static_cast<uint32_t>(u))));
+  const uint32_t hi = __float_as_uint(dpp<kCtrl>(__uint_as_float(static_cast<uint32_t>(u >> 32))));
+  return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+__device__ __forceinline__ double read_lane64(double v, int lane) {
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
+  const uint32_t lo = __float_as_uint(read_lane(__uint_as_float(static_cast<uint32_t>(u)), lane));
+  const uint32_t hi = __float_as_uint(read_lane(__uint_as_float(static_cast<uint32_t>(u >> 32)), lane));
+  return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(hi) << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<kDppXor1>(v);
+  v += dpp64<kDppXor2>(v);
+  v += dpp64<kDppHalfMirror>(v);
+  v += dpp64<kDppMirror>(v);
+  return (read_lane64(v, 0) + read_lane64(v, 16)) + (read_lane64(v, 32) + read_lane64(v, 48));
+}
+
+// A lower bound of the order of the wave's k-th best, from each lane's best: the
+// k-th best lane has k as good before or at it. (The last 12 bits are left zero.)
 __device__ __forceinline__ uint32_t wave_bound(uint32_t best, uint32_t k) {
   uint32_t t = 0;
 #pragma unroll
@@ -106,53 +140,150 @@ __device__ __forceinline__ uint32_t wave_bound(uint32_t best, uint32_t k) {
   return t;
 }
 
-// The best k of n keys in `from`, in order, through put(rank, key).
-template <typename Put>
-__device__ __forceinline__ void put_in_order(const uint64_t *from, uint32_t n, uint32_t k, Put put) {
-  for (uint32_t i = threadIdx.x; i < n; i += kT) {
-    const uint64_t key = from[i];
-    uint32_t rank = 0;
-    for (uint32_t j = 0; j < n; ++j) rank += from[j] > key;
-    if (rank < k) put(rank, key);
+// Sum over the four lanes of a quad.
+__device__ __forceinline__ uint32_t quad_sum_u(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kDppXor1, 0xf, 0xf, false);
+  return v + __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kDppXor2, 0xf, 0xf, false);
+}
+
+// How many of the n keys are greater. The list is read eight at a time: the
+// caller has zeroed up to seven places behind it.
+__device__ __forceinline__ uint32_t rank_of(uint64_t key, const uint64_t *list, uint32_t n) {
+  uint32_t rank = 0;
+  for (uint32_t j = 0; j < n; j += 8) {
+    ulonglong2 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = reinterpret_cast<const ulonglong2 *>(list + j)[u];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) rank += (v[u].x > key) + (v[u].y > key);
   }
+  return rank;
+}
+
+// The same, of the list's first n keys, by the four lanes of a quad together.
+__device__ __forceinline__ uint32_t quad_rank(uint64_t key, const uint64_t *list, uint32_t n) {
+  uint32_t rank = 0;
+  for (uint32_t j = 8 * (lane_id() & 3); j < n; j += 32) {
+    ulonglong2 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = reinterpret_cast<const ulonglong2 *>(list + j)[u];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) rank += (j + 2 * u < n && v[u].x > key) + (j + 2 * u + 1 < n && v[u].y > key);
+  }
+  return quad_sum_u(rank);
+}
+
+// Leaves the best k of the wave's n keys, in order, at the start of its list;
+// returns how many there are. `best` has room for k. (A wave's LDS operations take
+// place in their order; the barriers hold the compiler to it.)
+__device__ __forceinline__ uint32_t wave_best(uint64_t *list, uint32_t n, uint32_t k, uint64_t *best) {
+  const uint32_t lane = lane_id();
+  if (lane < 8) list[n + lane] = 0;
+  __builtin_amdgcn_wave_barrier();
+  for (uint32_t i = lane; i < n; i += kWave) {
+    const uint64_t key = list[i];
+    const uint32_t rank = rank_of(key, list, n);
+    if (rank < k) best[rank] = key;
+  }
+  __builtin_amdgcn_wave_barrier();
+  const uint32_t left = min(n, k);
+  if (lane < left) list[lane] = best[lane];
+  __builtin_amdgcn_wave_barrier();
+  return left;
 }
 
 // Chooses among a group's rows; called by the workgroup that arrives last.
 __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh) {
+  constexpr int kMine = kSelectBeams * kSelectK / kT;
   const uint32_t k = p.a.k, n = p.a.beams * k;
   const uint32_t row0 = group * p.a.beams;
   const Coherent scores(p.row_score + static_cast<size_t>(row0) * k, n * 8);
   const Coherent tokens(p.row_token + static_cast<size_t>(row0) * k, n * 4);
-  double *list = reinterpret_cast<double *>(sh.list);
   __shared__ uint32_t flat_beam[kSelectK], flat_token[kSelectK];
   __shared__ uint8_t taken[2 * kSelectK];
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
-  uint32_t mine = 0;
-  for (uint32_t i = threadIdx.x; i < n; i += kT) {
-    list[i] = __longlong_as_double(static_cast<long long>(load64(scores, i)));
-    mine += list[i] != -INFINITY;
+  uint64_t *list = &sh.own[0][0];
+  uint16_t *place = reinterpret_cast<uint16_t *>(list + kJoin);
+  __shared__ uint8_t was_done[kSelectBeams];
+  __shared__ uint32_t held[kSelectBeams * kSelectK];  // the entries' tokens
+  if (p.a.done && threadIdx.x < p.a.beams) was_done[threadIdx.x] = p.a.done[row0 + threadIdx.x] != 0;
+  // A score's key: its 64 bits, monotone; 0 where there is none.
+  uint64_t key[kMine];
+  uint32_t token[kMine];
+#pragma unroll
+  for (int u = 0; u < kMine; ++u) {
+    const uint32_t i = u * kT + threadIdx.x;
+    key[u] = 0;
+    token[u] = 0;
+    if (u * kT < n) {  // (past the end the descriptors give zeros)
+      key[u] = load64(scores, i);
+      token[u] = tokens.ldu(i);
+    }
   }
-  if (mine) atomicAdd(&sh.n, mine);
+#pragma unroll
+  for (int u = 0; u < kMine; ++u)
+    if (u * kT < n) held[u * kT + threadIdx.x] = token[u];
+  uint32_t best = 0;
+#pragma unroll
+  for (int u = 0; u < kMine; ++u) {
+    const double s = __longlong_as_double(static_cast<long long>(key[u]));
+    if (u * kT + threadIdx.x >= n || s == -INFINITY)
+      key[u] = 0;
+    else
+      key[u] = key[u] >> 63 ? ~key[u] : key[u] | 1ull << 63;
+    best = max(best, static_cast<uint32_t>(key[u] >> 32));
+  }
+  const uint32_t bound = wave_bound(best, k);
+  if (threadIdx.x == 0) sh.n = 0;
+  if (lane_id() == 0) sh.bound[wave_id()] = bound;
   __syncthreads();
-  const uint32_t found = min(sh.n, k);
-  auto put = [&](uint32_t i, double score, uint32_t beam, uint32_t token) {
+  uint32_t least = max(1u, sh.bound[0]);
+#pragma unroll
+  for (int w = 1; w < kWavesPerBlock; ++w) least = max(least, sh.bound[w]);
+  uint32_t mine = 0;
+#pragma unroll
+  for (int u = 0; u < kMine; ++u) mine += static_cast<uint32_t>(key[u] >> 32) >= least;
+  if (mine) {
+    uint32_t at = atomicAdd(&sh.n, mine);
+#pragma unroll
+    for (int u = 0; u < kMine; ++u)
+      if (static_cast<uint32_t>(key[u] >> 32) >= least) {
+        list[at] = key[u];
+        place[at++] = static_cast<uint16_t>(u * kT + threadIdx.x);
+      }
+  }
+  __syncthreads();
+  const uint32_t count = sh.n, found = min(count, k);
+  auto put = [&](uint32_t i, double score, uint32_t beam, uint32_t tok) {
     const size_t at = static_cast<size_t>(group) * k + i;
     p.a.scores_out[at] = static_cast<float>(score);
     p.a.parents[at] = static_cast<int32_t>(row0 + beam);
-    p.a.tokens[at] = static_cast<int32_t>(token);
-    if (p.a.done) p.a.done_out[at] = p.a.done[row0 + beam] != 0 || token == p.a.eos;
+    p.a.tokens[at] = static_cast<int32_t>(tok);
+    if (p.a.done) p.a.done_out[at] = was_done[beam] || tok == p.a.eos;
   };
-  for (uint32_t i = threadIdx.x; i < n; i += kT) {
-    const double s = list[i];
-    if (s == -INFINITY) continue;
+  // Four lanes find an entry's rank: higher scores, and equal ones of lower places.
+  for (uint32_t i = threadIdx.x / 4; i < count; i += kT / 4) {
+    const uint64_t it = list[i];
+    const uint32_t at = place[i];
     uint32_t rank = 0;
-    for (uint32_t j = 0; j < n; ++j) rank += list[j] > s || (list[j] == s && j < i);
-    if (rank >= k) continue;
-    const uint32_t token = tokens.ldu(i);
-    put(rank, s, i / k, token);
-    flat_beam[rank] = i / k;
-    flat_token[rank] = token;
+    for (uint32_t j = 8 * (threadIdx.x & 3); j < count; j += 32) {
+      ulonglong2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = reinterpret_cast<const ulonglong2 *>(list + j)[u];
+      const uint4 pl = *reinterpret_cast<const uint4 *>(place + j);
+      const uint32_t pw[4] = {pl.x, pl.y, pl.z, pl.w};
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        rank += j + 2 * u < count && (v[u].x > it || (v[u].x == it && (pw[u] & 0xFFFFu) < at));
+        rank += j + 2 * u + 1 < count && (v[u].y > it || (v[u].y == it && pw[u] >> 16 < at));
+      }
+    }
+    rank = quad_sum_u(rank);
+    if (rank >= k || (threadIdx.x & 3)) continue;
+    const uint64_t bits = it >> 63 ? it & ~(1ull << 63) : ~it;
+    const uint32_t tok = held[at];
+    put(rank, __longlong_as_double(static_cast<long long>(bits)), at / k, tok);
+    flat_beam[rank] = at / k;
+    flat_token[rank] = tok;
   }
   if (found == k) return;
   // The places left go to the lowest (beam, token) that have none.
@@ -172,65 +303,88 @@ __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh) {
   }
 }
 
-// Joins a row's slices; called by the workgroup that arrives last.
+// Joins a row's runs; called by the workgroup that arrives last.
 __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
-  const uint32_t k = p.a.k, n = p.slices * k;
-  const Coherent keys(p.keys + static_cast<size_t>(row) * n, n * 8);
-  const Coherent sums(p.sums + static_cast<size_t>(row) * p.slices, p.slices * 8);
-  const Coherent maxima(p.maxima + static_cast<size_t>(row) * p.slices, p.slices * 4);
+  constexpr int kMine = kJoin / 2 / kT;
+  const uint32_t k = p.a.k, n = p.runs * k;
+  const Coherent keys(p.keys + static_cast<size_t>(row) * (n + (n & 1)), (n + (n & 1)) * 8);
+  const Coherent sums(p.sums + static_cast<size_t>(row) * p.runs, p.runs * 8);
+  const Coherent maxima(p.maxima + static_cast<size_t>(row) * p.runs, p.runs * 4);
   const Coherent scores(p.row_score + static_cast<size_t>(row) * k, k * 8);
   const Coherent tokens(p.row_token + static_cast<size_t>(row) * k, k * 4);
+  // Two keys a load, all of them on their way before the first is used.
+  uint64_t key[2 * kMine];
+#pragma unroll
+  for (int u = 0; u < kMine; ++u) {
+    key[2 * u] = key[2 * u + 1] = 0;
+    if (2 * u * kT < n) {
+      const float4 v = keys.ld4(u * kT + threadIdx.x);
+      const uint2 a = {__float_as_uint(v.x), __float_as_uint(v.y)}, b = {__float_as_uint(v.z), __float_as_uint(v.w)};
+      key[2 * u] = a.x | static_cast<uint64_t>(a.y) << 32;
+      key[2 * u + 1] = b.x | static_cast<uint64_t>(b.y) << 32;
+    }
+  }
   float m = -INFINITY;
-  for (uint32_t s = threadIdx.x; s < p.slices; s += kT) m = fmaxf(m, maxima.ld(s));
-  m = wave_max(m);
+  double sum = 0.0;
+  for (uint32_t s = threadIdx.x; s < p.runs; s += kT) {
+    const float top = maxima.ld(s);
+    const double part = __longlong_as_double(static_cast<long long>(load64(sums, s)));
+    if (top > m) {
+      sum = m == -INFINITY ? part : part + sum * exp2_fast((m - top) * kLog2e);
+      m = top;
+    } else if (top > -INFINITY) {
+      sum += top == m ? part : part * exp2_fast((top - m) * kLog2e);
+    }
+  }
   uint32_t best = 0;
-  for (uint32_t i = threadIdx.x; i < n; i += kT) {
-    sh.list[i] = load64(keys, i);
-    best = max(best, static_cast<uint32_t>(sh.list[i] >> 32));
+#pragma unroll
+  for (int u = 0; u < 2 * kMine; ++u) {
+    // (A row of an odd number of keys ends with half of a load.)
+    if (2 * ((u >> 1) * kT + threadIdx.x) + (u & 1) >= n) key[u] = 0;
+    best = max(best, static_cast<uint32_t>(key[u] >> 32));
   }
   const uint32_t bound = wave_bound(best, k);
+  const float wave_m = wave_max(m);
   if (lane_id() == 0) {
-    sh.top[wave_id()] = m;
+    sh.top[wave_id()] = wave_m;
     sh.bound[wave_id()] = bound;
   }
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  uint32_t least = kLowest;
+  float top = sh.top[0];
+  uint32_t least = max(kLowest, sh.bound[0]);
 #pragma unroll
-  for (int w = 0; w < kWavesPerBlock; ++w) {
-    m = fmaxf(m, sh.top[w]);
+  for (int w = 1; w < kWavesPerBlock; ++w) {
+    top = fmaxf(top, sh.top[w]);
     least = max(least, sh.bound[w]);
   }
-  double sum = 0.0;
-  for (uint32_t s = threadIdx.x; s < p.slices; s += kT) {
-    const float top = maxima.ld(s);
-    const double part = __longlong_as_double(static_cast<long long>(load64(sums, s)));
-    sum += top == m ? part : top == -INFINITY ? 0.0 : part * exp(static_cast<double>(top) - m);
-  }
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+  sum = m == top ? sum : m == -INFINITY ? 0.0 : sum * exp2_fast((m - top) * kLog2e);
+  sum = wave_sum64(sum);
   if (lane_id() == 0) sh.sum[wave_id()] = sum;
-  for (uint32_t i = threadIdx.x; i < n; i += kT)
-    if (static_cast<uint32_t>(sh.list[i] >> 32) >= least) {
-      const uint32_t at = atomicAdd(&sh.n, 1u);
-      if (at < kShort) sh.shorter[at] = sh.list[i];
-    }
+  uint64_t *list = &sh.own[0][0];
+  uint32_t mine = 0;
+#pragma unroll
+  for (int u = 0; u < 2 * kMine; ++u) mine += static_cast<uint32_t>(key[u] >> 32) >= least;
+  if (mine) {
+    uint32_t at = atomicAdd(&sh.n, mine);
+#pragma unroll
+    for (int u = 0; u < 2 * kMine; ++u)
+      if (static_cast<uint32_t>(key[u] >> 32) >= least) list[at++] = key[u];
+  }
   __syncthreads();
-  const double total = (sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]);
-  const double base = static_cast<double>(p.a.scores[row]), log_total = log(total);
-  auto put = [&](uint32_t rank, uint64_t key) {
-    const float x = logit_of(key);
-    // (An infinite maximum leaves the others nothing.)
-    const double s = key == 0 ? -INFINITY : base + ((x == m ? 0.0 : static_cast<double>(x) - m) - log_total);
-    store64(scores, rank, static_cast<uint64_t>(__double_as_longlong(s)));
-    tokens.stu(rank, token_of(key));
-  };
   const uint32_t count = sh.n;
-  if (count <= static_cast<uint32_t>(kShort)) {
-    put_in_order(sh.shorter, count, k, put);
-    for (uint32_t i = count + threadIdx.x; i < k; i += kT) put(i, 0);
-  } else {
-    put_in_order(sh.list, n, k, put);  // more than k keys are there: every place is filled
+  const double log_total = log((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]));
+  const double base = static_cast<double>(p.a.scores[row]);
+  for (uint32_t i = threadIdx.x / 4; i < max(count, k); i += kT / 4) {
+    const uint64_t it = i < count ? list[i] : 0;
+    const uint32_t rank = i < count ? quad_rank(it, list, count) : i;
+    if (rank >= k || (threadIdx.x & 3)) continue;
+    const float x = logit_of(it);
+    // (An infinite maximum leaves the others nothing.)
+    const double s =
+        i >= count ? -INFINITY : base + ((x == top ? 0.0 : static_cast<double>(x) - top) - log_total);
+    store64(scores, rank, static_cast<uint64_t>(__double_as_longlong(s)));
+    tokens.stu(rank, token_of(it));
   }
 }
 
@@ -240,25 +394,43 @@ __device__ __forceinline__ void row_done(const SelectLaunch &p, uint32_t row, Sh
   wait_vm_stores();
   __syncthreads();
   if (threadIdx.x == 0) {
-    sh.last = p.a.beams == 1 || atomicAdd(p.group_count + group, 1u) == p.a.beams - 1;
-    if (sh.last && p.a.beams > 1) p.group_count[group] = 0u;
+    sh.last = p.a.beams == 1 || atomicAdd(p.group_count + group * p.apart, 1u) == p.a.beams - 1;
+    if (sh.last && p.a.beams > 1) p.group_count[group * p.apart] = 0u;
   }
   __syncthreads();
   if (sh.last) choose(p, group, sh);
 }
 
-template <typename E, int kEach>
+template <typename E>
 __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   using P = Piece<E>;
   constexpr int kPieces = kEach / P::kElems;
-  __shared__ Shared sh;
-  const uint32_t row = blockIdx.y, slice = blockIdx.x, k = p.a.k;
+  static_assert(kOwn >= static_cast<int>(kSelectK) + kWave * P::kElems, "a piece fits behind k keys");
+  __shared__ __attribute__((aligned(16))) Shared sh;
+  const uint32_t row = blockIdx.y, run = blockIdx.x, k = p.a.k;
+  const E *logits = static_cast<const E *>(p.a.logits) + static_cast<int64_t>(row / p.a.beams) * p.a.group_stride +
+                    static_cast<int64_t>(row % p.a.beams) * p.a.beam_stride;
+  const uint32_t lane = lane_id(), w = wave_id();
+  const uint32_t begin = run * p.tiles * kTile, end = min(p.a.vocab, begin + p.tiles * kTile);
+  // Piece j of a tile: P::kElems logits of each thread, one after the other.
+  typename P::words next[kPieces];
+  auto fetch = [&](uint32_t tile) {
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+      const uint32_t at = tile + (j * kT + threadIdx.x) * P::kElems;
+      if (at + P::kElems <= end)
+        next[j] = *reinterpret_cast<const typename P::words *>(logits + at);
+      else
+        next[j] = typename P::words{0u, 0u, 0u, 0u};
+    }
+  };
+  fetch(begin);  // on its way while the row's score is looked at
   const float score = p.a.scores[row];
   const bool live = fabsf(score) < INFINITY;
   const bool done = p.a.done && p.a.done[row];
   if (!live || done) {
-    // No logits are read: one continuation, or none.
-    if (slice) return;
+    // The logits do not matter: one continuation, or none.
+    if (run) return;
     const Coherent scores(p.row_score + static_cast<size_t>(row) * k, k * 8);
     const Coherent tokens(p.row_token + static_cast<size_t>(row) * k, k * 4);
     for (uint32_t i = threadIdx.x; i < k; i += kT) {
@@ -269,121 +441,146 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
     row_done(p, row, sh);
     return;
   }
-  const E *logits = static_cast<const E *>(p.a.logits) + static_cast<int64_t>(row / p.a.beams) * p.a.group_stride +
-                    static_cast<int64_t>(row % p.a.beams) * p.a.beam_stride;
-  const uint32_t first = slice * (kT * kEach) + threadIdx.x * P::kElems;
-  float x[kEach];
+  uint64_t *own = sh.own[w];
+  uint32_t count = 0;
+  float least = logit_of(static_cast<uint64_t>(kLowest) << 32);  // keys at or above it are kept
+  float m = -INFINITY, sum = 0.f;
+  for (uint32_t tile = begin; tile < end; tile += kTile) {
+    float x[kEach];
 #pragma unroll
-  for (int j = 0; j < kPieces; ++j) {
-    const uint32_t at = first + j * (kT * P::kElems);
-    typename P::words v = {0u, 0u, 0u, 0u};
-    const bool whole = at + P::kElems <= p.a.vocab;
-    if (whole) v = *reinterpret_cast<const typename P::words *>(logits + at);
+    for (int j = 0; j < kPieces; ++j) {
+      const uint32_t at = tile + (j * kT + threadIdx.x) * P::kElems;
 #pragma unroll
-    for (int c = 0; c < P::kElems; ++c) {
-      uint32_t bits;
-      if constexpr (sizeof(E) == 4)
-        bits = v[c];
-      else
-        bits = c & 1 ? v[c >> 1] >> 16 : v[c >> 1] & 0xFFFFu;
-      float y = widen<E>(bits);
-      if (!whole) {
-        y = -INFINITY;
-        if (at + c < p.a.vocab) {
-          if constexpr (sizeof(E) == 4)
-            y = reinterpret_cast<const float *>(logits)[at + c];
-          else
-            y = widen<E>(reinterpret_cast<const uint16_t *>(logits)[at + c]);
+      for (int c = 0; c < P::kElems; ++c) {
+        uint32_t bits;
+        if constexpr (sizeof(E) == 4)
+          bits = next[j][c];
+        else
+          bits = c & 1 ? next[j][c >> 1] >> 16 : next[j][c >> 1] & 0xFFFFu;
+        x[j * P::kElems + c] = widen<E>(bits);
+      }
+      if (at + P::kElems > end) {  // the row's end: one by one
+#pragma unroll
+        for (int c = 0; c < P::kElems; ++c) {
+          float y = -INFINITY;
+          if (at + c < end) {
+            if constexpr (sizeof(E) == 4)
+              y = reinterpret_cast<const float *>(logits)[at + c];
+            else
+              y = widen<E>(reinterpret_cast<const uint16_t *>(logits)[at + c]);
+          }
+          x[j * P::kElems + c] = y;
         }
       }
-      x[j * P::kElems + c] = y != y ? -INFINITY : y + 0.f;  // (+0 for -0, which is no lower)
+    }
+    if (tile + kTile < end) fetch(tile + kTile);
+    float top = -INFINITY;
+    // (NaN is no maximum and at or above no bound; of its exponential, fmaxf makes 0.)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
+    // Sum of exp(x - m), FP32 within a thread. The difference is exact to half a
+    // step, so the sum has no error common to its terms.
+    if (top > m) {
+      if (m > -INFINITY) sum *= exp2_fast((m - top) * kLog2e);
+      m = top;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    if (!__any(m == INFINITY)) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += fmaxf(exp2_fast((x[i] - base) * kLog2e), 0.f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sum += x[i] == base ? 1.f : fmaxf(exp2_fast((x[i] - base) * kLog2e), 0.f);
+    }
+    // The bound rises with the lanes' maxima, after 1, 2, 4, ... tiles, and when
+    // the wave's list is full.
+    if (const uint32_t seen = (tile - begin) / kTile + 1; (seen & (seen - 1)) == 0)
+      least = fmaxf(least, logit_of(static_cast<uint64_t>(max(kLowest, wave_bound(order_of(m), k))) << 32));
+    if (__any(top >= least)) {
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        if (count + kWave * P::kElems > kOwn) {
+          count = wave_best(own, count, k, sh.best[w]);
+          // Later tokens are higher: only greater logits count. (A bound of
+          // infinity keeps the infinite ones, of which enough are there.)
+          if (count == k) {
+            const uint32_t above = static_cast<uint32_t>(own[k - 1] >> 32) + 1;
+            least = fmaxf(least, logit_of(static_cast<uint64_t>(min(above, order_of(INFINITY))) << 32));
+          }
+        }
+        const uint32_t first = tile + (j * kT + threadIdx.x) * P::kElems;
+#pragma unroll
+        for (int c = 0; c < P::kElems; ++c) {
+          const bool in = x[j * P::kElems + c] >= least;
+          const uint64_t mask = __ballot(in);
+          if (mask == 0) continue;
+          if (in) own[count + __popcll(mask & ((1ull << lane) - 1))] = key_of(x[j * P::kElems + c], first + c);
+          count += __popcll(mask);
+        }
+      }
     }
   }
-  float top = x[0];
-#pragma unroll
-  for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
-  const uint32_t bound = wave_bound(order_of(top), k);
-  const float wave_top = wave_max(top);
-  if (lane_id() == 0) {
-    sh.top[wave_id()] = wave_top;
-    sh.bound[wave_id()] = bound;
+  const float wave_m = wave_max(m);
+  const uint32_t bound = wave_bound(order_of(m), k);
+  if (lane == 0) {
+    sh.top[w] = wave_m;
+    sh.bound[w] = bound;
+    sh.count[w] = count;
   }
   if (threadIdx.x == 0) sh.n = 0;
+  if (lane < 8) own[count + lane] = 0;
   __syncthreads();
-  float m = sh.top[0];
-  uint32_t least = max(kLowest, sh.bound[0]);
+  float top = sh.top[0];
+  uint32_t all_least = max(kLowest, sh.bound[0]);
 #pragma unroll
-  for (int w = 1; w < kWavesPerBlock; ++w) {
-    m = fmaxf(m, sh.top[w]);
-    least = max(least, sh.bound[w]);
+  for (int u = 1; u < kWavesPerBlock; ++u) {
+    top = fmaxf(top, sh.top[u]);
+    all_least = max(all_least, sh.bound[u]);
   }
-  // Sum of exp(x - m): FP32 within a thread, 64 bits beyond. The difference is
-  // exact to half a step, so the sum has no error common to its terms.
-  float part = 0.f;
-  if (fabsf(m) < INFINITY) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) part += exp2_fast((x[i] - m) * 1.44269504088896340736f);
-  } else if (m > 0) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) part += x[i] == m ? 1.f : 0.f;
+  // Its keys at or above the highest bound, mostly few, go to one list.
+  for (uint32_t i = 0; i < count; i += kWave) {
+    const uint64_t key = i + lane < count ? own[i + lane] : 0;
+    const bool in = static_cast<uint32_t>(key >> 32) >= all_least;
+    const uint64_t mask = __ballot(in);
+    uint32_t at = 0;
+    if (lane == 0) at = atomicAdd(&sh.n, static_cast<uint32_t>(__popcll(mask)));
+    at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((1ull << lane) - 1));
+    if (in && at < static_cast<uint32_t>(kFew)) sh.few[at] = key;
   }
-  double sum = part;
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
-  if (lane_id() == 0) sh.sum[wave_id()] = sum;
-  if (order_of(top) >= least) {
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (order_of(x[i]) >= least) {
-        const uint32_t at = atomicAdd(&sh.n, 1u);
-        if (at < kShort)
-          sh.shorter[at] = key_of(x[i], first + (i / P::kElems) * (kT * P::kElems) + i % P::kElems);
-      }
-  }
+  const double total = wave_sum64(m == top ? sum : m == -INFINITY ? 0.f : sum * exp2_fast((m - top) * kLog2e));
+  if (lane == 0) sh.sum[w] = total;
   __syncthreads();
-  const uint32_t n = p.slices * k;
-  const Coherent keys(p.keys + static_cast<size_t>(row) * n, n * 8);
-  const uint32_t count = sh.n;
-  auto put = [&](uint32_t rank, uint64_t key) { store64(keys, slice * k + rank, key); };
-  if (count <= static_cast<uint32_t>(kShort)) {
-    put_in_order(sh.shorter, count, k, put);
-    for (uint32_t i = count + threadIdx.x; i < k; i += kT) put(i, 0);
+  const uint32_t n = p.runs * k;
+  const Coherent keys(p.keys + static_cast<size_t>(row) * (n + (n & 1)), (n + (n & 1)) * 8);
+  uint32_t all = sh.n;
+  if (all <= static_cast<uint32_t>(kFew)) {
+    for (uint32_t i = threadIdx.x / 4; i < all; i += kT / 4) {
+      const uint64_t key = sh.few[i];
+      const uint32_t rank = quad_rank(key, sh.few, all);
+      if (rank < k && (threadIdx.x & 3) == 0) store64(keys, run * k + rank, key);
+    }
   } else {
-    // Many equal or nearly equal logits: one after the other.
-    uint64_t before = ~0ull;
-    for (uint32_t rank = 0; rank < k; ++rank) {
-      uint64_t best = 0;
+    // Crowded near the top: a key's place is the sum of its places in the four lists.
+    for (uint32_t i = lane; i < count; i += kWave) {
+      const uint64_t key = own[i];
+      uint32_t rank = 0;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const uint64_t key =
-            x[i] == -INFINITY ? 0 : key_of(x[i], first + (i / P::kElems) * (kT * P::kElems) + i % P::kElems);
-        if (key < before && key > best) best = key;
-      }
-#pragma unroll
-      for (int o = kWave / 2; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor(static_cast<unsigned long long>(best), o, kWave);
-        best = other > best ? other : best;
-      }
-      if (lane_id() == 0) sh.list[wave_id()] = best;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < kWavesPerBlock; ++w) best = sh.list[w] > best ? sh.list[w] : best;
-      __syncthreads();
-      if (threadIdx.x == 0) put(rank, best);
-      before = best;
+      for (int u = 0; u < kWavesPerBlock; ++u) rank += rank_of(key, sh.own[u], sh.count[u]);
+      if (rank < k) store64(keys, run * k + rank, key);
     }
   }
+  for (uint32_t i = all + threadIdx.x; i < k; i += kT) store64(keys, run * k + i, 0);
   if (threadIdx.x == 0) {
-    const Coherent sums(p.sums + static_cast<size_t>(row) * p.slices, p.slices * 8);
-    const Coherent maxima(p.maxima + static_cast<size_t>(row) * p.slices, p.slices * 4);
-    store64(sums, slice, static_cast<uint64_t>(__double_as_longlong((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]))));
-    maxima.st(slice, m);
+    const Coherent sums(p.sums + static_cast<size_t>(row) * p.runs, p.runs * 8);
+    const Coherent maxima(p.maxima + static_cast<size_t>(row) * p.runs, p.runs * 4);
+    store64(sums, run, static_cast<uint64_t>(__double_as_longlong((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]))));
+    maxima.st(run, top);
   }
   wait_vm_stores();
   __syncthreads();
   if (threadIdx.x == 0) {
-    sh.last = p.slices == 1 || atomicAdd(p.row_count + row, 1u) == p.slices - 1;
-    if (sh.last && p.slices > 1) p.row_count[row] = 0u;
+    sh.last = p.runs == 1 || atomicAdd(p.row_count + row * p.apart, 1u) == p.runs - 1;
+    if (sh.last && p.runs > 1) p.row_count[row * p.apart] = 0u;
   }
   __syncthreads();
   if (!sh.last) return;
@@ -391,13 +588,15 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   row_done(p, row, sh);
 }
 
-// Logits of a thread: 32 where slices of that size give every CU two or more,
-// else 8, as long as the slices' candidates fit the join.
-constexpr uint32_t kWideSlice = kT * 32, kNarrowSlice = kT * 8;
-uint32_t slices_of(uint32_t vocab, uint32_t slice) { return (vocab + slice - 1) / slice; }
-bool wide_slices(uint32_t rows, uint32_t k, uint32_t vocab) {
-  return static_cast<uint64_t>(slices_of(vocab, kWideSlice)) * rows >= 512 ||
-         static_cast<uint64_t>(slices_of(vocab, kNarrowSlice)) * k > kJoin;
+// A row's runs: as many as make kAim workgroups (four fit a CU), no more than it
+// has tiles and the join takes.
+constexpr uint32_t kAim = 1024;
+uint32_t tiles_of(uint32_t vocab) { return (vocab + kTile - 1) / kTile; }
+void split_rows(SelectLaunch &p, uint32_t rows, uint32_t k, uint32_t vocab) {
+  const uint32_t tiles = tiles_of(vocab);
+  const uint32_t runs = std::max(1u, std::min({tiles, kAim / std::max(1u, rows), kJoin / k}));
+  p.tiles = (tiles + runs - 1) / runs;
+  p.runs = (tiles + p.tiles - 1) / p.tiles;
 }
 
 template <typename... A>
@@ -416,8 +615,8 @@ size_t carve(SelectLaunch &p, char *base, uint32_t rows, uint32_t k) {
     used += round256(bytes);
     return r;
   };
-  const size_t parts = static_cast<size_t>(rows) * p.slices;
-  p.keys = reinterpret_cast<uint64_t *>(take(parts * k * 8));
+  const size_t parts = static_cast<size_t>(rows) * p.runs, keys = p.runs * k;
+  p.keys = reinterpret_cast<uint64_t *>(take(rows * (keys + (keys & 1)) * 8));
   p.sums = reinterpret_cast<double *>(take(parts * 8));
   p.maxima = reinterpret_cast<float *>(take(parts * 4));
   p.row_score = reinterpret_cast<double *>(take(static_cast<size_t>(rows) * k * 8));
@@ -427,33 +626,31 @@ size_t carve(SelectLaunch &p, char *base, uint32_t rows, uint32_t k) {
 
 }  // namespace
 
-bool beam_select_fits(uint32_t k, uint32_t vocab) {
-  return static_cast<uint64_t>(slices_of(vocab, kWideSlice)) * k <= kJoin;
-}
-
 size_t beam_select_scratch(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab) {
   const uint32_t rows = groups * beams;
   SelectLaunch p{};
-  p.slices = slices_of(vocab, wide_slices(rows, k, vocab) ? kWideSlice : kNarrowSlice);
+  split_rows(p, rows, k, vocab);
   return carve(p, nullptr, rows, k);
 }
 
 hipError_t launch_beam_select(hipStream_t s, const qd_select_args &a, const OpScratch &w) {
   const uint32_t rows = a.groups * a.beams;
   if (rows == 0) return hipSuccess;
-  const bool wide = wide_slices(rows, a.k, a.vocab);
   SelectLaunch p{};
   p.a = a;
-  p.slices = slices_of(a.vocab, wide ? kWideSlice : kNarrowSlice);
+  split_rows(p, rows, a.k, a.vocab);
   carve(p, w.scratch, rows, a.k);
+  // Counters in lines of their own where there is room: 608 arrivals at 16 counters
+  // of one line took 6 us, at lines of their own 1.1.
+  p.apart = 32;
+  while (static_cast<uint64_t>(rows + a.groups) * p.apart > kOpCounters) p.apart /= 2;
   p.row_count = w.counters;
-  p.group_count = w.counters + rows;
-  const dim3 grid(p.slices, rows), block(kT);
-  switch (a.dtype) {
-    case QD_DTYPE_F32: return launch(wide ? select_kernel<float, 32> : select_kernel<float, 8>, grid, block, s, p);
-    case QD_DTYPE_BF16: return launch(wide ? select_kernel<Bf16, 32> : select_kernel<Bf16, 8>, grid, block, s, p);
-    default: return launch(wide ? select_kernel<F16, 32> : select_kernel<F16, 8>, grid, block, s, p);
-  }
+  p.group_count = w.counters + static_cast<size_t>(rows) * p.apart;
+  const dim3 grid(p.runs, rows), block(kT);
+  return launch(a.dtype == QD_DTYPE_F32    ? select_kernel<float>
+                : a.dtype == QD_DTYPE_BF16 ? select_kernel<Bf16>
+                                           : select_kernel<F16>,
+                grid, block, s, p);
 }
 
 }  // namespace qd

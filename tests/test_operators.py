@@ -172,7 +172,7 @@ def test_fork_refusals(status, changes, memory):
     (qd.NOT_SUPPORTED, dict(beams=33)),
     (qd.NOT_SUPPORTED, dict(k=65)),
     (qd.INVALID_ARGUMENT, dict(beams=1, vocab=3, k=4)),
-    (qd.NOT_SUPPORTED, dict(vocab=1 << 24)),
+    (qd.NOT_SUPPORTED, dict(vocab=(1 << 24) + 1)),
     (qd.NOT_SUPPORTED, dict(groups=20000)),
     (qd.INVALID_ARGUMENT, dict(scores=None)),
     (qd.INVALID_ARGUMENT, dict(logits=AT + 2)),
