@@ -265,6 +265,10 @@ qd_status qd_paged_attention(const qd_paged_cache *c, const qd_attention_args *a
     QD_TRY(check_stride(a->out_stride, c->rows > 1 ? c->head_dim : 0, e, "out_stride"));
     QD_TRY(check_stride(a->out_head_stride, a->heads > 1 ? c->head_dim : 0, e, "out_head_stride"));
   }
+  const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((a->heads / c->kv_heads + 15) / 16);
+  if (c->rows * parts * (static_cast<uint64_t>(c->table_width) * c->page_size / 32 + 1) > 0x7f000000u)
+    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of up to %llu positions and %u heads are too much for one call", c->rows,
+                  static_cast<unsigned long long>(static_cast<uint64_t>(c->table_width) * c->page_size), a->heads);
   qd::OpScratch scratch{};
   QD_TRY(check_workspace(w, c->device, qd::paged_attention_scratch(c->rows, a->heads, c->kv_heads, c->head_dim), &scratch));
   Device on;

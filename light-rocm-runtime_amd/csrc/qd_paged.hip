@@ -166,9 +166,12 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 }
 
 // ---- attention ------------------------------------------------------------------
-// A workgroup takes a run of a row's tiles of 32 positions for one KV head and up
-// to 16 of its query heads; its waves take the tiles in turn, each with a running
-// maximum and sum. Everything stays in the registers of the matrix instructions:
+// The work is cut into tiles of 32 positions of one (row, KV head, up to 16 of its
+// query heads), here an item, and dealt to the workgroups in equal runs, so that
+// all are done at about the same time whatever the rows' lengths; a cut near an
+// item's ends moves there. A workgroup's waves take an item's tiles in turn, each
+// with a running maximum and sum. Everything stays in the registers of the matrix
+// instructions:
 //   S^T = K Q^T   lane l: head l % 16, positions 4 (l / 16) + r of each half tile
 //   O^T += V^T P^T the same lane's probabilities are the operand as they are, and
 //                 its share of O is of its own head, so a new maximum rescales
@@ -178,7 +181,8 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 // so float4 loads along the head serve four of them; 16-bit rows are loaded 8 at
 // a time and turned with byte permutes.
 constexpr int kTile = 32, kSub = 16;
-constexpr int kAttnW = 4, kAttnT = kAttnW * kWave;
+constexpr uint32_t kMostPieces = 256;  // of an item
+constexpr int kWaves = 4;              // of a workgroup
 // A maximum is only taken up when it passes the one in use by this many powers of
 // two: until then probabilities grow to at most 2^8, exact in every type's range.
 constexpr float kLazyMax = 8.f;
@@ -186,15 +190,17 @@ constexpr float kLazyMax = 8.f;
 struct AttnLaunch {
   qd_paged_cache c;
   qd_attention_args a;
-  float *records;       // [grid.x][grid.y][rec_floats]: acc [rec_heads][head_dim], maxima, sums
-  uint32_t *counters;   // [rows][grid.y]
+  float *records;       // [workgroups][2][rec_floats]: acc [rec_heads][head_dim], maxima, sums
+  uint32_t *counters;   // [rows][parts * apart]
+  uint32_t apart;       // words between two counters
+  uint32_t parts;       // items of a row: KV heads x blocks of query heads
   uint32_t page_shift;
   uint32_t group;       // query heads of a KV head
   uint32_t blocks;      // of up to 16 of them
   uint32_t rec_heads;   // the most of a block
   uint32_t rec_floats;
-  uint32_t least;       // tiles of a chunk at least
-  uint32_t target;      // chunks aimed at, beyond one per row; 0: rows are not split
+  uint32_t least;       // tiles on either side of a cut; 0: items are not cut
+  uint32_t target;      // pieces aimed at besides one of each item (the short kernel)
 };
 
 // Values of lanes l and l ^ 32 in a and b (any order).
@@ -220,128 +226,264 @@ __device__ __forceinline__ float quarters_sum(float v) {
 
 // 16 positions of a page through a descriptor that ends with the last valid one:
 // loads past it give zeros and touch no memory.
+template <int kPolicy>
 struct PageRows {
   __amdgpu_buffer_rsrc_t r;
   __device__ __forceinline__ u4v ld16(uint32_t byte) const {
-    return __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, 0));
+    return __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, kPolicy));
   }
   __device__ __forceinline__ u2v ld8(uint32_t byte) const {
-    return __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(r, byte, 0, 0));
+    return __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(r, byte, 0, kPolicy));
   }
 };
 
-// Where a chunk lies: wave-uniform.
-struct Chunk {
+// An item and the run of its tiles that a workgroup takes: wave-uniform.
+struct Item {
   int row, length;
-  int first, last;      // tiles
-  uint32_t begin;       // the row's first chunk's index
-  uint32_t index, of;   // of the row's chunks
-  bool bad;             // the row's length
+  uint32_t part;
+  uint32_t at, tiles;        // its first tile among all, and how many it has (one at least)
+  uint32_t first, last;      // the run
+  uint32_t home, pieces;     // the workgroup of its first piece, and how many there are
+  bool bad;                  // the row's length
 };
 
-// Chunk `x` of all rows'. A row of n tiles has max(1, ceil(n / size)) chunks,
-// where size makes about `target` of them in all.
-__device__ __forceinline__ bool find_chunk(const AttnLaunch &p, uint32_t x, Chunk &ch) {
+// The runs of all workgroups: run i is [i share, (i + 1) share) of all tiles, but
+// for the cuts that move.
+struct Deal {
+  uint32_t share, total;
+};
+
+__device__ __forceinline__ uint32_t tiles_of(const AttnLaunch &p, int32_t n, int64_t most) {
+  return n <= 0 || n > most ? 1u : (static_cast<uint32_t>(n) + kTile - 1) / kTile;
+}
+
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
+  int x = static_cast<int>(v);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 to 1, 2 to 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1 to 2 and 3
+  return static_cast<uint32_t>(x);
+}
+
+// How a cut `off` tiles into an item of n moves: 0 to its start, 1 not, 2 to its end.
+__device__ __forceinline__ int cut_of(const AttnLaunch &p, uint32_t off, uint32_t n) {
+  if (p.least && n >= 2 * p.least) return off < p.least ? 0 : n - off < p.least ? 2 : 1;
+  return 2 * off < n ? 0 : 2;
+}
+
+__device__ __forceinline__ void set_item(const AttnLaunch &p, const Deal &d, Item &it, uint32_t row, uint32_t part,
+                                         uint32_t at, int32_t n, int64_t most) {
+  it.row = static_cast<int>(row);
+  it.part = part;
+  it.at = at;
+  it.bad = n < 0 || n > most;
+  it.length = it.bad ? 0 : n;
+  it.tiles = tiles_of(p, n, most);
+  it.first = 0;
+  it.last = it.tiles;
+  it.home = 0;
+  it.pieces = 1;
+  if (p.least && it.tiles >= 2 * p.least) {
+    const uint32_t lo = (at + p.least + d.share - 1) / d.share, hi = (at + it.tiles - p.least) / d.share;
+    if (hi >= lo) {
+      it.pieces = hi - lo + 2;
+      it.home = lo - 1;
+    }
+  }
+}
+
+// Ends the run of `it` where workgroup i's does; false: the item is the next one's.
+__device__ __forceinline__ bool end_run(const AttnLaunch &p, const Deal &d, uint32_t i, Item &it) {
+  const uint32_t end = (i + 1) * d.share;
+  if (it.at + it.tiles <= end || end >= d.total) return true;
+  if (end <= it.at) return false;
+  const int cut = cut_of(p, end - it.at, it.tiles);
+  if (cut == 1) it.last = end - it.at;
+  return cut != 0;
+}
+
+// Maximum over the wave of numbers below 2^31.
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  int x = static_cast<int>(v);
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppXor1, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppXor2, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppHalfMirror, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppMirror, 0xf, 0xf, false));
+  return static_cast<uint32_t>(max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
+                                   max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48))));
+}
+
+// Workgroup i's first item; false if it has none. Lane l looks at rows l, l + 64, ...
+__device__ __forceinline__ bool first_item(const AttnLaunch &p, uint32_t i, uint32_t groups, Deal &d, Item &it) {
   const int lane = lane_id();
   const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
-  auto length_of = [&](uint32_t r) {
-    const int32_t n = p.c.lengths[r];
-    return n < 0 || n > most ? 0 : n;
-  };
-  uint32_t size = 0x7fffffffu, row = x, before = 0;
-  if (p.target) {
-    uint32_t total = 0;
-    for (uint32_t r = lane; r < p.c.rows; r += kWave) total += (length_of(r) + kTile - 1) / kTile;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) total += __shfl_xor(total, o, kWave);
-    size = max(p.least, (total + p.target - 1) / p.target);
-    row = p.c.rows;
-    for (uint32_t base = 0; base < p.c.rows; base += kWave) {
-      const uint32_t r = base + lane;
-      const uint32_t tiles = r < p.c.rows ? (length_of(r) + kTile - 1) / kTile : 0u;
-      const uint32_t mine = r < p.c.rows ? max(1u, (tiles + size - 1) / size) : 0u;
-      uint32_t upto = mine;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) {
-        const uint32_t v = __shfl_up(upto, o, kWave);
-        if (lane >= o) upto += v;
-      }
-      const uint64_t past = __ballot(before + upto > x);
-      if (past) {
-        const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-        row = base + at;
-        before += __builtin_amdgcn_readlane(upto - mine, at);
-        break;
-      }
-      before += __builtin_amdgcn_readlane(upto, kWave - 1);
-    }
-  } else {
-    before = x;
+  uint32_t total = 0, longest = 0;
+  int32_t n = 0;  // of the row looked at last
+  for (uint32_t r = lane; r < p.c.rows; r += kWave) {
+    n = p.c.lengths[r];
+    const uint32_t tiles = tiles_of(p, n, most);
+    total += tiles;
+    longest = max(longest, tiles);
   }
-  row = __builtin_amdgcn_readfirstlane(row);
-  if (row >= p.c.rows) return false;
-  before = __builtin_amdgcn_readfirstlane(before);
-  size = __builtin_amdgcn_readfirstlane(size);
-  const int32_t n = load_uniform(p.c.lengths + row);
-  ch.bad = n < 0 || n > most;
-  ch.row = row;
-  ch.length = ch.bad ? 0 : n;
-  const uint32_t tiles = (ch.length + kTile - 1) / kTile;
-  ch.of = max(1u, tiles / size + (tiles % size != 0));
-  ch.begin = before;
-  ch.index = x - before;
-  ch.first = ch.index * size;
-  ch.last = min(tiles, ch.first + size);
+  uint32_t upto = lanes_upto(total);
+  total = __builtin_amdgcn_readlane(upto, kWave - 1) * p.parts;
+  longest = lanes_max(longest);
+  d.total = total;
+  d.share = max((total + groups - 1) / groups, (longest + kMostPieces - 3) / (kMostPieces - 2));
+  const uint32_t begin = i * d.share;
+  if (static_cast<uint64_t>(i) * d.share >= total) return false;
+  // The row in which the run begins.
+  uint32_t before = 0, base = 0;
+  const bool once = p.c.rows <= kWave;
+  uint64_t past;
+  for (;;) {
+    if (!once) {
+      n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
+      upto = lanes_upto(base + lane < p.c.rows ? tiles_of(p, n, most) : 0u);
+    }
+    past = __ballot(before + upto * p.parts > begin);
+    if (past) break;
+    before += __builtin_amdgcn_readlane(upto, kWave - 1) * p.parts;
+    base += kWave;
+  }
+  const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+  const int32_t length = __builtin_amdgcn_readlane(n, at);
+  const uint32_t tiles = tiles_of(p, length, most), row = base + at;
+  before += (__builtin_amdgcn_readlane(upto, at) - tiles) * p.parts;
+  const uint32_t part = (begin - before) / tiles, off = begin - before - part * tiles;
+  const int cut = off ? cut_of(p, off, tiles) : 0;
+  if (cut < 2) {
+    set_item(p, d, it, row, part, before + part * tiles, length, most);
+    if (cut == 1) it.first = off;
+  } else if (part + 1 < p.parts) {  // from the next item on
+    set_item(p, d, it, row, part + 1, before + (part + 1) * tiles, length, most);
+  } else {
+    if (row + 1 >= p.c.rows) return false;
+    set_item(p, d, it, row + 1, 0, before + (part + 1) * tiles, load_uniform(p.c.lengths + row + 1), most);
+  }
+  return end_run(p, d, i, it);
+}
+
+// The short kernel's pieces: a row of n tiles has max(1, ceil(n / size)) of each
+// item, where size makes about `target` of them. Piece x of all rows' (counted for
+// one part); it.home is its number within the row, `begin` the number of its
+// row's first.
+__device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint32_t part, Item &it, uint32_t &begin) {
+  const int lane = lane_id();
+  const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
+  uint32_t size = 0x7fffffffu, row = x;
+  int32_t n = 0;
+  begin = x;
+  if (p.target) {
+    uint32_t total = 0, longest = 0;
+    for (uint32_t r = lane; r < p.c.rows; r += kWave) {
+      n = p.c.lengths[r];
+      const uint32_t tiles = tiles_of(p, n, most);
+      total += tiles;
+      longest = max(longest, tiles);
+    }
+    total = __builtin_amdgcn_readlane(lanes_upto(total), kWave - 1);
+    size = max(max(p.least, (total + p.target - 1) / p.target), (lanes_max(longest) + kMostPieces - 1) / kMostPieces);
+    const bool once = p.c.rows <= kWave;
+    uint32_t base = 0, upto, mine;
+    begin = 0;
+    uint64_t past;
+    for (;; base += kWave) {
+      if (base >= p.c.rows) return false;
+      if (!once) n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
+      mine = base + lane < p.c.rows ? (tiles_of(p, n, most) + size - 1) / size : 0u;
+      upto = lanes_upto(mine);
+      past = __ballot(begin + upto > x);
+      if (past) break;
+      begin += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+    row = base + at;
+    begin += __builtin_amdgcn_readlane(upto - mine, at);
+    n = __builtin_amdgcn_readlane(n, at);
+    it.pieces = __builtin_amdgcn_readlane(mine, at);
+  } else {
+    n = load_uniform(p.c.lengths + row);
+    it.pieces = 1;
+  }
+  it.row = static_cast<int>(row);
+  it.part = part;
+  it.bad = n < 0 || n > most;
+  it.length = it.bad ? 0 : n;
+  it.at = 0;
+  it.tiles = tiles_of(p, n, most);
+  it.home = x - begin;
+  it.first = it.home * size;
+  it.last = min(it.tiles, it.first + size);
   return true;
 }
 
-template <typename E, int D>
+// The item behind `it` in workgroup i's run; false at its end.
+__device__ __forceinline__ bool next_item(const AttnLaunch &p, const Deal &d, uint32_t i, const Item &it, Item &next) {
+  const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
+  const uint32_t at = it.at + it.tiles;
+  if (it.last < it.tiles || at >= d.total || at >= (i + 1) * d.share) return false;
+  if (it.part + 1 < p.parts) {
+    set_item(p, d, next, it.row, it.part + 1, at, it.bad ? -1 : it.length, most);
+  } else {
+    set_item(p, d, next, it.row + 1, 0, at, load_uniform(p.c.lengths + it.row + 1), most);
+  }
+  return end_run(p, d, i, next);
+}
+
+template <typename E, int D, int kStages>
 struct WaveTiles {
   static constexpr bool kWide = std::is_same_v<E, float>;
   static constexpr int kElem = kWide ? 4 : 2;
   static constexpr int kPieces = D * kElem / 64;  // 16-byte loads of K per lane and half tile
   static constexpr int kAcc = D / 16;
   u4v q[kPieces];
-  u4v k[2][kPieces];
-  u4v v[2][4][kWide ? D / 64 : 1];  // rows 4 (l / 16) + j; 16-bit rows of 64 use half of a register quad
+  u4v k[kStages][2][kPieces];
+  u4v v[kStages][2][4][kWide ? D / 64 : 1];  // rows 4 (l / 16) + j; 16-bit rows of 64 use half of a register quad
   f4v o[kAcc];
   float m, ms, l;
 
-  __device__ __forceinline__ void load_k(const PageRows &r, int sub, uint32_t off) {
+  template <typename R>
+  __device__ __forceinline__ void load_k(const R &r, int st, int sub, uint32_t off) {
 #pragma unroll
-    for (int s = 0; s < kPieces; ++s) k[sub][s] = r.ld16(off + 64 * s);
+    for (int s = 0; s < kPieces; ++s) k[st][sub][s] = r.ld16(off + 64 * s);
   }
-  __device__ __forceinline__ void load_v(const PageRows &r, int sub, const uint32_t (&off)[4]) {
+  template <typename R>
+  __device__ __forceinline__ void load_v(const R &r, int st, int sub, const uint32_t (&off)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (kWide) {
 #pragma unroll
-        for (int n = 0; n < D / 64; ++n) v[sub][j][n] = r.ld16(off[j] + 256 * n);
+        for (int n = 0; n < D / 64; ++n) v[st][sub][j][n] = r.ld16(off[j] + 256 * n);
       } else if constexpr (D == 128) {
-        v[sub][j][0] = r.ld16(off[j]);
+        v[st][sub][j][0] = r.ld16(off[j]);
       } else {
         const u2v x = r.ld8(off[j]);
-        v[sub][j][0] = u4v{x[0], x[1], 0u, 0u};
+        v[st][sub][j][0] = u4v{x[0], x[1], 0u, 0u};
       }
     }
   }
   // Scores of half tile `sub`, in units of the query's scale.
-  __device__ __forceinline__ f4v scores(int sub) const {
+  __device__ __forceinline__ f4v scores(int st, int sub) const {
     f4v acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < kPieces; ++s) {
       if constexpr (kWide) {
-        const f4v a = __builtin_bit_cast(f4v, k[sub][s]), b = __builtin_bit_cast(f4v, q[s]);
+        const f4v a = __builtin_bit_cast(f4v, k[st][sub][s]), b = __builtin_bit_cast(f4v, q[s]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[c], b[c], acc, 0, 0, 0);
       } else {
-        acc = E::mfma(k[sub][s], q[s], acc);
+        acc = E::mfma(k[st][sub][s], q[s], acc);
       }
     }
     return acc;
   }
   // o += V^T P^T; returns the sum of the probabilities as they were multiplied.
-  __device__ __forceinline__ float accumulate(const float (&pr)[2][4]) {
+  __device__ __forceinline__ float accumulate(int st, const float (&pr)[2][4]) {
     float sum = 0.f;
     if constexpr (kWide) {
 #pragma unroll
@@ -351,7 +493,7 @@ struct WaveTiles {
           sum += pr[sub][j];
 #pragma unroll
           for (int n = 0; n < D / 64; ++n) {
-            const f4v a = __builtin_bit_cast(f4v, v[sub][j][n]);
+            const f4v a = __builtin_bit_cast(f4v, v[st][sub][j][n]);
 #pragma unroll
             for (int c = 0; c < 4; ++c)
               o[4 * n + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[c], pr[sub][j], o[4 * n + c], 0, 0, 0);
@@ -372,7 +514,7 @@ struct WaveTiles {
         u4v a;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          a[i] = __builtin_amdgcn_perm(v[i >> 1][2 * (i & 1) + 1][0][j >> 1], v[i >> 1][2 * (i & 1)][0][j >> 1],
+          a[i] = __builtin_amdgcn_perm(v[st][i >> 1][2 * (i & 1) + 1][0][j >> 1], v[st][i >> 1][2 * (i & 1)][0][j >> 1],
                                        j & 1 ? 0x07060302u : 0x05040100u);
         o[j] = E::mfma(a, b, o[j]);
       }
@@ -386,92 +528,118 @@ struct WaveTiles {
   }
 };
 
-template <typename E, int D>
-__global__ __launch_bounds__(kAttnT) void attention_kernel(AttnLaunch p) {
-  using Tiles = WaveTiles<E, D>;
-  constexpr int kRow = D + 4;
-  __shared__ __attribute__((aligned(16))) float wo[kAttnW][16][kRow];
-  __shared__ float wm[kAttnW][16], wl[kAttnW][16];
-  __shared__ uint32_t last, spoilt;
-  Chunk ch;
-  if (!find_chunk(p, blockIdx.x, ch)) return;
-  const int w = __builtin_amdgcn_readfirstlane(wave_id()), lane = lane_id();
-  const int col = lane & 15, quad = lane >> 4;
-  const int kvh = blockIdx.y / p.blocks, block = blockIdx.y % p.blocks;
-  const int h0 = kvh * p.group + 16 * block;                  // the first query head here
-  const int heads = min(16, static_cast<int>(p.group) - 16 * block);
-  if (threadIdx.x == 0) spoilt = ch.bad;
+// What both kernels do with an item: its tiles, the waves' partial results, and
+// the join of its pieces.
+template <typename E, int D, int kStages>
+struct AttnShared {
+  __attribute__((aligned(16))) float wo[kWaves][16][D + 4];
+  float wm[kWaves][16], wl[kWaves][16];
+  uint32_t spoilt, last;
+};
 
-  Tiles t;
-  const float scale = p.a.scale * 1.44269504088896340736f;  // scores in powers of two
-#pragma unroll
-  for (int s = 0; s < Tiles::kPieces; ++s) t.q[s] = u4v{0u, 0u, 0u, 0u};
-  if (col < heads) {
-    const char *q = static_cast<const char *>(p.a.q) +
-                    (ch.row * p.a.q_stride + (h0 + col) * p.a.q_head_stride) * Tiles::kElem + 16 * quad;
-#pragma unroll
-    for (int s = 0; s < Tiles::kPieces; ++s) t.q[s] = *reinterpret_cast<const u4v *>(q + 64 * s);
-  }
-#pragma unroll
-  for (int j = 0; j < Tiles::kAcc; ++j) t.o[j] = f4v{0.f, 0.f, 0.f, 0.f};
-  t.m = -INFINITY;
-  t.ms = 0.f;
-  t.l = 0.f;
-
-  const int32_t *table = p.c.table + ch.row * p.c.table_stride;
-  const uint32_t token_bytes = static_cast<uint32_t>(p.c.token_stride) * Tiles::kElem;
-  const uint32_t k_off = col * token_bytes + 16 * quad;
+template <typename E, int D, int kStages, int kPolicy>
+struct Attention {
+  using Tiles = WaveTiles<E, D, kStages>;
+  using Shared = AttnShared<E, D, kStages>;
+  static constexpr int kT = kWaves * kWave, kQuads = D / 4;
+  const AttnLaunch &p;
+  Shared &sh;
+  const int w, lane, col, quad;
+  const float scale;  // scores in powers of two
+  const uint32_t token_bytes, k_off, rec_m, rec_l;
   uint32_t v_off[4];
+  Tiles t;
+  uint32_t tile;
+  int ahead[2];  // the pages of the tile that is loaded next
+
+  __device__ __forceinline__ Attention(const AttnLaunch &launch, Shared &shared)
+      : p(launch),
+        sh(shared),
+        w(__builtin_amdgcn_readfirstlane(wave_id())),
+        lane(lane_id()),
+        col(lane & 15),
+        quad(lane >> 4),
+        scale(p.a.scale * 1.44269504088896340736f),
+        token_bytes(static_cast<uint32_t>(p.c.token_stride) * Tiles::kElem),
+        k_off(col * token_bytes + 16 * quad),
+        rec_m(p.rec_heads * D),
+        rec_l(rec_m + p.rec_heads) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    v_off[j] = (4 * quad + j) * token_bytes + col * (Tiles::kWide ? 16 : D / 16 * 2);
-  bool bad = false;
-  auto page_of = [&](int pos) { return pos < ch.length ? load_uniform(table + (pos >> p.page_shift)) : -1; };
+    for (int j = 0; j < 4; ++j) v_off[j] = (4 * quad + j) * token_bytes + col * (Tiles::kWide ? 16 : D / 16 * 2);
+  }
+  __device__ __forceinline__ uint32_t first_head(const Item &x) const {
+    return (x.part / p.blocks) * p.group + 16 * (x.part % p.blocks);
+  }
+  __device__ __forceinline__ int heads_of(const Item &x) const {
+    return min(16, static_cast<int>(p.group - 16 * (x.part % p.blocks)));
+  }
   // The 16 positions from `pos` on, in page `id`, of K or V.
-  auto rows_at = [&](const void *base, int pos, int id) {
-    const int n = min(max(ch.length - pos, 0), kSub);
+  __device__ __forceinline__ PageRows<kPolicy> rows_at(const Item &x, const void *base, uint32_t pos, int id, bool &bad) const {
+    const int n = min(max(x.length - static_cast<int>(pos), 0), kSub);
     const bool in = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
     if (n > 0 && !in) bad = true;
-    const int64_t at = (in ? id * p.c.page_stride : 0) +
-                       static_cast<int64_t>(pos & (p.c.page_size - 1)) * p.c.token_stride + kvh * p.c.head_stride;
+    const int64_t at = (in ? id * p.c.page_stride : 0) + static_cast<int64_t>(pos & (p.c.page_size - 1)) * p.c.token_stride +
+                       static_cast<int64_t>(x.part / p.blocks) * p.c.head_stride;
     const uint32_t bytes = n > 0 && in ? (n - 1) * token_bytes + D * Tiles::kElem : 0u;
     char *ptr = const_cast<char *>(static_cast<const char *>(base)) + at * Tiles::kElem;
-    return PageRows{__builtin_amdgcn_make_buffer_rsrc(ptr, 0, static_cast<int>(bytes), kRsrcWord3)};
-  };
-
-  int tile = ch.first + w;
-  int id[2], next[2];
-  id[0] = page_of(tile * kTile);
-  id[1] = page_of(tile * kTile + kSub);
-  if (tile < ch.last) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) t.load_k(rows_at(p.c.k, tile * kTile + s * kSub, id[s]), s, k_off);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) t.load_v(rows_at(p.c.v, tile * kTile + s * kSub, id[s]), s, v_off);
+    return PageRows<kPolicy>{__builtin_amdgcn_make_buffer_rsrc(ptr, 0, static_cast<int>(bytes), kRsrcWord3)};
   }
-  while (tile < ch.last) {
-    const int then = tile + kAttnW;
-    const bool more = then < ch.last;
-    if (more) {
-      next[0] = page_of(then * kTile);
-      next[1] = page_of(then * kTile + kSub);
+  __device__ __forceinline__ void load_k(const Item &x, int st, uint32_t at, const int (&id)[2], bool &bad) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) t.load_k(rows_at(x, p.c.k, at * kTile + s * kSub, id[s], bad), st, s, k_off);
+  }
+  __device__ __forceinline__ void load_v(const Item &x, int st, uint32_t at, const int (&id)[2], bool &bad) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) t.load_v(rows_at(x, p.c.v, at * kTile + s * kSub, id[s], bad), st, s, v_off);
+  }
+  // The pages of a wave's tile `at`, -1 past its run.
+  __device__ __forceinline__ void pages_of(const Item &x, uint32_t at, int (&id)[2]) const {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint32_t pos = at * kTile + s * kSub;
+      id[s] = at < x.last && pos < static_cast<uint32_t>(x.length)
+                  ? load_uniform(p.c.table + x.row * p.c.table_stride + (pos >> p.page_shift))
+                  : -1;
     }
+  }
+  // The queries and the first tiles of a run are on their way when this returns.
+  __device__ __forceinline__ void begin(const Item &x, bool &bad) {
+    tile = x.first + w;
+    int id[kStages][2];
+#pragma unroll
+    for (int st = 0; st < kStages; ++st) pages_of(x, tile + st * kWaves, id[st]);
+#pragma unroll
+    for (int s = 0; s < Tiles::kPieces; ++s) t.q[s] = u4v{0u, 0u, 0u, 0u};
+    if (col < heads_of(x)) {
+      const char *q = static_cast<const char *>(p.a.q) +
+                      (x.row * p.a.q_stride + (first_head(x) + col) * p.a.q_head_stride) * Tiles::kElem + 16 * quad;
+#pragma unroll
+      for (int s = 0; s < Tiles::kPieces; ++s) t.q[s] = *reinterpret_cast<const u4v *>(q + 64 * s);
+    }
+#pragma unroll
+    for (int st = 0; st < kStages; ++st) {
+      if (tile + st * kWaves >= x.last) continue;
+      load_k(x, st, tile + st * kWaves, id[st], bad);
+      load_v(x, st, tile + st * kWaves, id[st], bad);
+    }
+    pages_of(x, tile + kStages * kWaves, ahead);
+  }
+  __device__ __forceinline__ void tile_through(const Item &it, int st, bool &bad) {
+    const bool more = tile + kStages * kWaves < it.last;
     float s[2][4];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub) {
-      const f4v x = t.scores(sub);
+      const f4v x = t.scores(st, sub);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[sub][r] = x[r] * scale;
     }
-    if (more)
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) t.load_k(rows_at(p.c.k, then * kTile + sub * kSub, next[sub]), sub, k_off);
-    if ((tile + 1) * kTile > ch.length)
+    if (more) load_k(it, st, tile + kStages * kWaves, ahead, bad);
+    if (static_cast<int>((tile + 1) * kTile) > it.length)
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (tile * kTile + sub * kSub + 4 * quad + r >= ch.length) s[sub][r] = -INFINITY;
+          if (static_cast<int>(tile * kTile + sub * kSub + 4 * quad + r) >= it.length) s[sub][r] = -INFINITY;
     float top = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
@@ -489,130 +657,251 @@ __global__ __launch_bounds__(kAttnT) void attention_kernel(AttnLaunch p) {
     for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
       for (int r = 0; r < 4; ++r) pr[sub][r] = exp2_fast(s[sub][r] - t.ms);
-    t.l += t.accumulate(pr);
-    if (more) {
+    t.l += t.accumulate(st, pr);
+    if (more) load_v(it, st, tile + kStages * kWaves, ahead, bad);
+    tile += kWaves;
+    pages_of(it, tile + kStages * kWaves, ahead);
+  }
+  __device__ __forceinline__ void run(const Item &it, bool &bad) {
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub) t.load_v(rows_at(p.c.v, then * kTile + sub * kSub, next[sub]), sub, v_off);
-      id[0] = next[0];
-      id[1] = next[1];
+    for (int j = 0; j < Tiles::kAcc; ++j) t.o[j] = f4v{0.f, 0.f, 0.f, 0.f};
+    t.m = -INFINITY;
+    t.ms = 0.f;
+    t.l = 0.f;
+    for (;;) {
+      if (tile >= it.last) break;
+      tile_through(it, 0, bad);
+      if constexpr (kStages > 1) {
+        if (tile >= it.last) break;
+        tile_through(it, 1, bad);
+      }
     }
-    tile = then;
   }
-
-  // The waves' partial results, then the chunk's.
-  const float l = quarters_sum(t.l);
-  if (quad == 0) {
-    wm[w][col] = t.m;
-    wl[w][col] = l;
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-#pragma unroll
-    for (int n = 0; n < D / 64; ++n)
-      *reinterpret_cast<float4 *>(&wo[w][col][Tiles::dim_of(r, n)]) =
-          make_float4(t.o[4 * n][r], t.o[4 * n + 1][r], t.o[4 * n + 2][r], t.o[4 * n + 3][r]);
-  __syncthreads();
-  if (bad) spoilt = 1;
-  __syncthreads();
-  if (threadIdx.x == 0 && spoilt) raise_error(p.c.errors, ch.bad ? QD_PAGED_BAD_LENGTH : QD_PAGED_BAD_PAGE);
-  const float poison = spoilt ? __uint_as_float(0x7FC00000u) : 0.f;
-
-  constexpr int kQuads = D / 4;
-  auto emit = [&](int h, int d, float4 acc, float sum) {
+  __device__ __forceinline__ void emit(const Item &x, int h, int d, float4 acc, float sum, float poison) const {
     // A row without positions: zeros.
-    const float inv = ch.length == 0 ? 0.f : 1.f / sum;
-    const int64_t at = ch.row * p.a.out_stride + (h0 + h) * p.a.out_head_stride + d;
+    const float inv = x.length == 0 ? 0.f : 1.f / sum;
+    const int64_t at = x.row * p.a.out_stride + (first_head(x) + h) * p.a.out_head_stride + d;
     store4<E>(p.a.out, at,
               make_float4(acc.x * inv + poison, acc.y * inv + poison, acc.z * inv + poison, acc.w * inv + poison));
-  };
-  // Records of this row and these heads in one descriptor: chunk c at c * stride.
-  const uint32_t stride = gridDim.y * p.rec_floats;
-  const uint32_t rec_m = p.rec_heads * D, rec_l = rec_m + p.rec_heads;
-  const Coherent recs(p.records + (static_cast<size_t>(ch.begin) * gridDim.y + blockIdx.y) * p.rec_floats,
-                      ((ch.of - 1) * stride + p.rec_floats) * static_cast<uint32_t>(sizeof(float)));
-  for (int i = threadIdx.x; i < heads * kQuads; i += kAttnT) {
-    const int h = i / kQuads, d = 4 * (i % kQuads);
-    float mx = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < kAttnW; ++u) mx = fmaxf(mx, wm[u][h]);
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < kAttnW; ++u) {
-      const float f = wm[u][h] == -INFINITY && mx != -INFINITY ? 0.f : wm[u][h] == mx ? 1.f : exp2_fast(wm[u][h] - mx);
-      const float4 x = *reinterpret_cast<const float4 *>(&wo[u][h][d]);
-      sum = fmaf(f, wl[u][h], sum);
-      acc.x = fmaf(f, x.x, acc.x);
-      acc.y = fmaf(f, x.y, acc.y);
-      acc.z = fmaf(f, x.z, acc.z);
-      acc.w = fmaf(f, x.w, acc.w);
+  }
+  // The waves' partial results to LDS. A barrier before the next ones.
+  __device__ __forceinline__ void put_partials() {
+    const float l = quarters_sum(t.l);
+    if (quad == 0) {
+      sh.wm[w][col] = t.m;
+      sh.wl[w][col] = l;
     }
-    if (ch.of == 1) {
-      emit(h, d, acc, sum);
-    } else {
-      const uint32_t rec = ch.index * stride + h * D;
-      recs.st4((rec + d) / 4, make_float4(acc.x + poison, acc.y + poison, acc.z + poison, acc.w + poison));
-      if (d == 0) {
-        recs.st(ch.index * stride + rec_m + h, mx);
-        recs.st(ch.index * stride + rec_l + h, sum);
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int n = 0; n < D / 64; ++n)
+        *reinterpret_cast<float4 *>(&sh.wo[w][col][Tiles::dim_of(r, n)]) =
+            make_float4(t.o[4 * n][r], t.o[4 * n + 1][r], t.o[4 * n + 2][r], t.o[4 * n + 3][r]);
+  }
+  // The piece's result, out or to its record. sh.spoilt is zero, and is again.
+  __device__ __forceinline__ void put_piece(const Item &it, bool bad, float *record) {
+    if (bad || it.bad) sh.spoilt = 1u;
+    __syncthreads();
+    const bool spoilt = sh.spoilt;
+    const float poison = spoilt ? __uint_as_float(0x7FC00000u) : 0.f;
+    const int heads = heads_of(it);
+    const bool whole = it.pieces == 1;
+    const Coherent rec(record, p.rec_floats * static_cast<uint32_t>(sizeof(float)));
+    for (int i = threadIdx.x; i < heads * kQuads; i += kT) {
+      const int h = i / kQuads, d = 4 * (i % kQuads);
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kWaves; ++u) mx = fmaxf(mx, sh.wm[u][h]);
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < kWaves; ++u) {
+        const float f = sh.wm[u][h] == mx ? 1.f : exp2_fast(sh.wm[u][h] - mx);
+        const float4 x = *reinterpret_cast<const float4 *>(&sh.wo[u][h][d]);
+        sum = fmaf(f, sh.wl[u][h], sum);
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
       }
+      if (whole) {
+        emit(it, h, d, acc, sum, poison);
+      } else {
+        rec.st4((h * D + d) / 4, make_float4(acc.x + poison, acc.y + poison, acc.z + poison, acc.w + poison));
+        if (d == 0) {
+          rec.st(rec_m + h, mx);
+          rec.st(rec_l + h, sum);
+        }
+      }
+    }
+    if (spoilt) {
+      if (threadIdx.x == 0) raise_error(p.c.errors, it.bad ? QD_PAGED_BAD_LENGTH : QD_PAGED_BAD_PAGE);
+      __syncthreads();
+      sh.spoilt = 0u;
     }
   }
-  if (ch.of == 1) return;
-  // The last of the row's chunks to arrive joins them, in their order.
-  wait_vm_stores();
-  __syncthreads();
-  uint32_t *cnt = p.counters + ch.row * gridDim.y + blockIdx.y;
-  if (threadIdx.x == 0) last = atomicAdd(cnt, 1u) == ch.of - 1;
-  __syncthreads();
-  if (!last) return;
-  if (threadIdx.x == 0) *cnt = 0u;
-  // Threads share a head's four dimensions out by chunks, then in LDS.
-  struct Part {
-    float4 acc;
-    float m, l;
-  };
-  Part *parts = reinterpret_cast<Part *>(&wo[0][0][0]);
-  static_assert(sizeof(Part) * kAttnT <= sizeof(wo), "one part per thread");
-  const int items = heads * kQuads, shares = max(1, kAttnT / items);
-  for (int base = 0; base < items; base += kAttnT) {
-    const int i = base + static_cast<int>(threadIdx.x) % min(items, kAttnT), share = threadIdx.x / min(items, kAttnT);
-    const int h = i / kQuads, d = 4 * (i % kQuads);
-    Part x{make_float4(0.f, 0.f, 0.f, 0.f), -INFINITY, 0.f};
-    auto join = [](Part &x, const Part &y) {
-      const float m = fmaxf(x.m, y.m);
-      const float f = x.m == m ? 1.f : exp2_fast(x.m - m), g = y.m == m ? 1.f : exp2_fast(y.m - m);
-      x.acc.x = fmaf(y.acc.x, g, x.acc.x * f);
-      x.acc.y = fmaf(y.acc.y, g, x.acc.y * f);
-      x.acc.z = fmaf(y.acc.z, g, x.acc.z * f);
-      x.acc.w = fmaf(y.acc.w, g, x.acc.w * f);
-      x.l = fmaf(y.l, g, x.l * f);
-      x.m = m;
+  // Counts the piece in; true in the workgroup whose piece came last.
+  __device__ __forceinline__ bool arrive(const Item &it) {
+    wait_vm_stores();
+    __syncthreads();
+    uint32_t *cnt = p.counters + (static_cast<size_t>(it.row) * p.parts + it.part) * p.apart;
+    if (threadIdx.x == 0) {
+      sh.last = atomicAdd(cnt, 1u) == it.pieces - 1;
+      if (sh.last) *cnt = 0u;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(sh.last);
+  }
+  // Joins an item's pieces in their order: each head's weights of the pieces, by a
+  // wave per head with every maximum and sum on its way at once, then the weighted
+  // sums, shared out among the threads. Piece c > 0 is `second` + (c - 1) * stride
+  // floats behind piece 0.
+  __device__ __forceinline__ void join(const Item &x, const float *records, uint32_t second, uint32_t stride) {
+    float(*weight)[kMostPieces] = reinterpret_cast<float(*)[kMostPieces]>(&sh.wo[0][0][0]);
+    static_assert(sizeof(float) * 16 * kMostPieces <= sizeof(sh.wo), "a weight per head and piece");
+    const int heads = heads_of(x);
+    const uint32_t of = x.pieces;
+    const Coherent recs(records, (second + (of - 2) * stride + p.rec_floats) * static_cast<uint32_t>(sizeof(float)));
+    auto at_piece = [&](uint32_t c) { return c == 0 ? 0u : second + (c - 1) * stride; };
+    const int items = heads * kQuads, shares = max(1, kT / items);
+    const int i0 = static_cast<int>(threadIdx.x) % min(items, kT), share = threadIdx.x / min(items, kT);
+    constexpr int kAhead = 8;
+    float4 next[kAhead];
+    auto fetch = [&](int i, uint32_t c) {
+      const int h = i / kQuads, d = 4 * (i % kQuads);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) next[u] = recs.ld4((at_piece(min(c + u * shares, of - 1)) + h * D + d) / 4);
     };
-    if (share < shares && i < items) {
-      constexpr int kAhead = 8;
-      for (uint32_t c = share; c < ch.of; c += kAhead * shares) {
-        Part y[kAhead];
+    fetch(min(i0, items - 1), min(static_cast<uint32_t>(share), of - 1));
+    __syncthreads();  // the partial results have been read
+    for (int h = w; h < heads; h += kWaves) {
+      constexpr int kPer = kMostPieces / kWave;
+      float cm[kPer], cl[kPer], m = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          // (Past the last chunk the descriptor gives zeros; not joined.)
-          const uint32_t rec = min(c + u * shares, ch.of - 1) * stride;
-          y[u].acc = recs.ld4((rec + h * D + d) / 4);
-          y[u].m = recs.ld(rec + rec_m + h);
-          y[u].l = recs.ld(rec + rec_l + h);
+      for (int u = 0; u < kPer; ++u) {
+        const uint32_t c = u * kWave + lane;
+        cm[u] = -INFINITY;
+        cl[u] = 0.f;
+        if (u * kWave < of && c < of) {
+          cm[u] = recs.ld(at_piece(c) + rec_m + h);
+          cl[u] = recs.ld(at_piece(c) + rec_l + h);
         }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-          if (c + u * shares < ch.of) join(x, y[u]);
       }
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) m = fmaxf(m, cm[u]);
+      m = wave_max(m);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        const uint32_t c = u * kWave + lane;
+        if (c >= of) continue;
+        const float f = cm[u] == m ? 1.f : exp2_fast(cm[u] - m);
+        weight[h][c] = f;
+        sum = fmaf(f, cl[u], sum);
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) sh.wl[0][h] = sum;
     }
     __syncthreads();
-    parts[threadIdx.x] = x;
-    __syncthreads();
-    if (share == 0 && i < items) {
-      for (int u = 1; u < shares; ++u) join(x, parts[threadIdx.x + u * items]);
-      emit(h, d, x.acc, x.l);
+    for (int base = 0; base < items; base += kT) {
+      const int i = base + i0, h = i / kQuads, d = 4 * (i % kQuads);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (share < shares && i < items) {
+        for (uint32_t c = share; c < of; c += kAhead * shares) {
+          if (base > 0 || c != static_cast<uint32_t>(share)) fetch(i, c);
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            if (c + u * shares >= of) continue;
+            const float f = weight[h][c + u * shares];
+            acc.x = fmaf(f, next[u].x, acc.x);
+            acc.y = fmaf(f, next[u].y, acc.y);
+            acc.z = fmaf(f, next[u].z, acc.z);
+            acc.w = fmaf(f, next[u].w, acc.w);
+          }
+        }
+      }
+      if (shares > 1) {  // (then there is one pass: the weights are read no more)
+        float4 *sums = reinterpret_cast<float4 *>(&sh.wo[0][0][0]);
+        __syncthreads();
+        sums[threadIdx.x] = acc;
+        __syncthreads();
+        if (share == 0)
+          for (int u = 1; u < shares; ++u) {
+            const float4 y = sums[threadIdx.x + u * items];
+            acc = make_float4(acc.x + y.x, acc.y + y.y, acc.z + y.z, acc.w + y.w);
+          }
+      }
+      if (share == 0 && i < items) emit(x, h, d, acc, sh.wl[0][h], 0.f);
     }
+  }
+};
+
+// Few positions in all: a workgroup per piece, no more than `target` pieces
+// besides one for each item. Short code and one dependent load less, because each
+// step of such a call waits for the one before it.
+template <typename E, int D>
+__global__ __launch_bounds__(kWaves *kWave) void attention_short_kernel(AttnLaunch p) {
+  __shared__ AttnShared<E, D, 1> sh;
+  Item it;
+  const uint32_t part = blockIdx.x % p.parts;
+  uint32_t begin;
+  if (!find_piece(p, blockIdx.x / p.parts, part, it, begin)) return;
+  if (threadIdx.x == 0) sh.spoilt = 0u;
+  Attention<E, D, 1, 0> a(p, sh);
+  bool bad = false;
+  a.begin(it, bad);
+  a.run(it, bad);
+  a.put_partials();
+  const uint32_t stride = p.parts * p.rec_floats;
+  float *first = p.records + (static_cast<size_t>(begin) * p.parts + part) * p.rec_floats;
+  __syncthreads();
+  a.put_piece(it, bad, first + static_cast<size_t>(it.home) * stride);
+  if (it.pieces == 1) return;
+  if (a.arrive(it)) a.join(it, first, stride, stride);
+}
+
+// Many: equal runs of all tiles, one for each workgroup that the card holds.
+template <typename E, int D, int kStages, int kPolicy>
+__global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunch p) {
+  __shared__ AttnShared<E, D, kStages> sh;
+  const uint32_t group_id = blockIdx.x;
+  Deal deal;
+  Item it;
+  if (!first_item(p, group_id, gridDim.x, deal, it)) return;
+  if (threadIdx.x == 0) sh.spoilt = 0u;
+  Attention<E, D, kStages, kPolicy> a(p, sh);
+  // The record of an item's piece: its workgroup's first if it begins inside the item, else the second.
+  auto record_of = [&](const Item &x, uint32_t piece) {
+    return p.records + (2 * static_cast<size_t>(x.home + piece) + (piece == 0)) * p.rec_floats;
+  };
+  // At most the first and the last item of a run have other pieces.
+  Item join[2];
+  int to_join = 0;
+  bool bad = false;
+  a.begin(it, bad);
+  for (;;) {
+    a.run(it, bad);
+    a.put_partials();
+    // The next item's loads are under way while this one's results are put together.
+    Item next;
+    const bool more = next_item(p, deal, group_id, it, next);
+    bool next_bad = false;
+    if (more) a.begin(next, next_bad);
+    __syncthreads();
+    const bool whole = it.pieces == 1;
+    a.put_piece(it, bad, record_of(it, whole ? 0 : group_id - it.home));
+    if (!whole && a.arrive(it)) {
+      join[1] = join[0];
+      join[0] = it;
+      ++to_join;
+    }
+    if (!more) break;
+    __syncthreads();  // LDS is written again
+    it = next;
+    bad = next_bad;
+  }
+  for (; to_join > 0; --to_join, join[0] = join[1]) {
+    a.join(join[0], record_of(join[0], 0), p.rec_floats, 2 * p.rec_floats);
+    __syncthreads();
   }
 }
 
@@ -889,19 +1178,29 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
   return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, packed, 0, s);
 }
 
-// How attention splits rows over workgroups.
-constexpr uint32_t kAttnLeastTiles = 8, kAttnAim = 2048;
+// How attention cuts its work. The short kernel: pieces of eight tiles or more, so
+// that they are about kShortAim. The long one: as many workgroups as CUs.
+constexpr uint32_t kAttnLeast = 8, kShortAim = 2048, kCus = 256, kMostPerCu = 2;
+constexpr uint64_t kShortBytes = 96ull << 20;
+constexpr uint64_t kCachedBytes = 256ull << 20;
 struct AttnShape {
-  uint32_t group, blocks, y, rec_heads, rec_floats, target;
+  uint32_t group, blocks, parts, rec_heads, rec_floats, apart, least, target, records;
 };
 AttnShape attention_shape(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
   AttnShape s{};
   s.group = heads / kv_heads;
   s.blocks = (s.group + 15) / 16;
-  s.y = kv_heads * s.blocks;
+  s.parts = kv_heads * s.blocks;
   s.rec_heads = std::min(s.group, 16u);
   s.rec_floats = (s.rec_heads * (head_dim + 2) + 3) / 4 * 4;
-  s.target = static_cast<uint64_t>(rows) * s.y > kOpCounters ? 0 : std::max(1u, kAttnAim / s.y);
+  const uint64_t items = static_cast<uint64_t>(rows) * s.parts;
+  if (items <= kOpCounters) {
+    s.least = kAttnLeast;
+    s.target = std::max(1u, kShortAim / s.parts);
+    s.records = std::max((rows + s.target) * s.parts, 2 * kCus * kMostPerCu);
+    // Counters in lines of their own where there is room.
+    for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
+  }
   return s;
 }
 
@@ -926,7 +1225,27 @@ hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_
 
 size_t paged_attention_scratch(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
   const AttnShape sh = attention_shape(rows, heads, kv_heads, head_dim);
-  return sh.target ? static_cast<size_t>(rows + sh.target) * sh.y * sh.rec_floats * sizeof(float) : 0;
+  return static_cast<size_t>(sh.records) * sh.rec_floats * sizeof(float);
+}
+
+// per_cu: workgroups of the long kernel on a CU, so that 64 KB are on their way there.
+template <typename E, int D, int kStages, int per_cu>
+static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
+  static_assert(per_cu <= static_cast<int>(kMostPerCu), "records");
+  const uint64_t most = ((static_cast<uint64_t>(p.c.table_width) << p.page_shift) + kTile - 1) / kTile;
+  const uint64_t position = 2ull * p.c.kv_heads * D * (std::is_same_v<E, float> ? 4 : 2);
+  const uint64_t pool = static_cast<uint64_t>(p.c.pages) * p.c.page_size;
+  const uint64_t positions = std::min<uint64_t>(static_cast<uint64_t>(p.c.rows) * p.c.table_width << p.page_shift, pool);
+  const dim3 block(kWaves * kWave);
+  if (positions * position <= kShortBytes || p.least == 0) {
+    if (most <= p.least) p.target = 0;
+    uint64_t x = p.c.rows;
+    if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + p.least - 1) / p.least));
+    return launch(attention_short_kernel<E, D>, dim3(static_cast<uint32_t>(x * p.parts)), block, s, p);
+  }
+  // Pages that cannot all stay in the last-level cache are read as a stream.
+  return launch(pool * position > kCachedBytes ? attention_long_kernel<E, D, kStages, kPolicyNt> : attention_long_kernel<E, D, kStages, 0>,
+                dim3(kCus * per_cu), block, s, p);
 }
 
 hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w) {
@@ -942,18 +1261,15 @@ hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const 
   p.blocks = sh.blocks;
   p.rec_heads = sh.rec_heads;
   p.rec_floats = sh.rec_floats;
-  p.least = kAttnLeastTiles;
+  p.apart = sh.apart;
+  p.parts = sh.parts;
+  p.least = sh.least;
   p.target = sh.target;
-  const uint64_t most = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + kTile - 1) / kTile;
-  if (most <= p.least) p.target = 0;
-  uint64_t x = c.rows;
-  if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + p.least - 1) / p.least));
-  const dim3 grid(static_cast<uint32_t>(x), sh.y), block(kAttnT);
   const bool wide = c.head_dim == 128;
   switch (c.dtype) {
-    case QD_DTYPE_F32: return launch(wide ? attention_kernel<float, 128> : attention_kernel<float, 64>, grid, block, s, p);
-    case QD_DTYPE_BF16: return launch(wide ? attention_kernel<Brain, 128> : attention_kernel<Brain, 64>, grid, block, s, p);
-    default: return launch(wide ? attention_kernel<Half, 128> : attention_kernel<Half, 64>, grid, block, s, p);
+    case QD_DTYPE_F32: return wide ? launch_attention<float, 128, 1, 1>(s, p) : launch_attention<float, 64, 2, 1>(s, p);
+    case QD_DTYPE_BF16: return wide ? launch_attention<Brain, 128, 2, 1>(s, p) : launch_attention<Brain, 64, 2, 2>(s, p);
+    default: return wide ? launch_attention<Half, 128, 2, 1>(s, p) : launch_attention<Half, 64, 2, 2>(s, p);
   }
 }
 

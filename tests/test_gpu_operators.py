@@ -222,6 +222,48 @@ def test_attention_split(dtype, heads, kv_heads, dim, page, lengths):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,lengths", [
+    (14, 2, 64, 16, EDGES), (8, 2, 128, 64, EDGES + [900, 0, 0, 1500, 513, 511]), (34, 2, 64, 32, [3000, 0, 1, 520, 0, 260]),
+    (4, 4, 128, 16, [1] * 300 + [2500] + [0] * 20 + [700] * 3), (7, 1, 64, 16, [20000]), (2, 2, 64, 16, [0] * 5 + [9000, 0])])
+def test_attention_equal_runs(dtype, heads, kv_heads, dim, page, lengths):
+    """Pools large enough for the kernel that deals equal runs of tiles: rows that begin and end
+    inside a run, rows of several runs, empty ones between and at the ends."""
+    say("attention runs", dtype, heads, kv_heads, dim, page, len(lengths))
+    g = seeded(heads + len(lengths))
+    many = (100 << 20) // (2 * page * kv_heads * dim * (4 if dtype == F32 else 2)) + 1  # pages of 100 MB
+    table, used = tables_for(g, lengths, page, max(-(-many // len(lengths)), -(-max(lengths) // page)), spare=many)
+    q = normal(g, (len(lengths), heads, dim), dtype, 1.5)
+    k, v = (torch.zeros((used, page, kv_heads, dim), dtype=dtype) for _ in range(2))
+    held = table[table >= 0].long()
+    k[held], v[held] = (normal(g, (len(held), page, kv_heads, dim), dtype) for _ in range(2))
+    n = int32(lengths)
+    hide(k, v, table, n, page)
+    out = run_attention(q, k, v, table, n, dim ** -0.5)
+    close(out, *oracle.attention(q, k, v, table, n, dim ** -0.5), "out")
+
+
+@pytest.mark.parametrize("dtype,dim", [(F32, 64), (F32, 128), (BF16, 64), (BF16, 128), (F16, 64), (F16, 128)])
+def test_attention_of_a_pool_past_the_caches(dtype, dim):
+    say("attention of a large pool", dtype, dim)
+    g, page, kv_heads = seeded(dim), 64, 2
+    pages = (288 << 20) // (2 * page * kv_heads * dim * (4 if dtype == F32 else 2))
+    lengths = [1500, 0, 77, 640]
+    table, _ = tables_for(g, lengths, page, 400)
+    table = torch.where(table >= 0, table * (pages // 48), table)
+    k, v = (torch.zeros((pages, page, kv_heads, dim), dtype=dtype, device="cuda") for _ in range(2))
+    held = table[table >= 0].long()
+    hk, hv = (normal(g, (len(held), page, kv_heads, dim), dtype) for _ in range(2))
+    k[held.cuda()], v[held.cuda()] = hk.cuda(), hv.cuda()
+    q = normal(g, (4, 6, dim), dtype, 1.5)
+    out = torch.full(q.shape, NAN, dtype=dtype, device="cuda")
+    workspace = ops.Workspace(ops.attention_workspace(4, 6, kv_heads, dim))
+    ops.paged_attention(ops.PagedCache(k, v, table.cuda(), int32(lengths).cuda()), out, q.cuda(), workspace)
+    small = torch.full_like(table, -1)
+    small[table >= 0] = torch.arange(len(held), dtype=torch.int32)
+    close(out, *oracle.attention(q, hk, hv, small, int32(lengths), dim ** -0.5), "out")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_attention_scores_of_any_size(dtype):
     """A maximum that rises and falls along the row, scores near the range's ends, one key that takes all."""
     say("attention: large scores", dtype)
