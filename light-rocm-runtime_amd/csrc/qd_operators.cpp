@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -95,10 +96,14 @@ qd_status check_cache(const qd_paged_cache *c) {
 class Device {
  public:
   qd_status enter(int32_t device) {
-    int n = 0;
-    if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) {
-      (void)hipGetLastError();
-      return refuse(QD_ERROR_NOT_SUPPORTED, "no HIP device visible");
+    static std::atomic<int> count{0};  // a process's devices do not change
+    int n = count.load(std::memory_order_relaxed);
+    if (n == 0) {
+      if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) {
+        (void)hipGetLastError();
+        return refuse(QD_ERROR_NOT_SUPPORTED, "no HIP device visible");
+      }
+      count.store(n, std::memory_order_relaxed);
     }
     if (device < 0 || device >= n) return refuse(QD_ERROR_INVALID_ARGUMENT, "device %d out of range (%d visible)", device, n);
     hipError_t e = hipGetDevice(&before_);

@@ -104,14 +104,11 @@ def _check(status):
 
 
 # ---- what a tensor is -----------------------------------------------------------------
+# A call takes a few microseconds on the device, so each tensor is looked at once, in few steps:
+# _take and _flat return its address if it is as it has to be and say what is wrong if not.
 
-_TYPES = {torch.float32: qd.DTYPE_F32, torch.bfloat16: qd.DTYPE_BF16, torch.float16: qd.DTYPE_F16,
-          torch.int32: "int32", torch.uint8: "uint8"}
-
-
-def _dtype(t):
-    """qd_dtype of a tensor, or None."""
-    return _TYPES.get(t.dtype)
+_TYPES = {torch.float32: qd.DTYPE_F32, torch.bfloat16: qd.DTYPE_BF16, torch.float16: qd.DTYPE_F16}
+_F32, _I32T, _U8T = torch.float32, torch.int32, torch.uint8
 
 
 def _refuse(text):
@@ -124,25 +121,32 @@ def _dims(name, t, n):
     return t.shape
 
 
-def _expect(name, t, dtype, shape, device):
-    """Address of a tensor of this type, shape and device, its last dimension contiguous."""
-    if t is None or t.shape != shape:
-        if t is None:
-            _refuse(f"{name} is missing")
+def _wrong(name, t, dtype, shape, device):
+    if t is None:
+        _refuse(f"{name} is missing")
+    if t.shape != shape:
         _refuse(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    if _dtype(t) != dtype:
-        _refuse(f"{name} has type {t.dtype}")
+    if t.dtype is not dtype:
+        _refuse(f"{name} has type {t.dtype}, not {dtype}")
     if t.get_device() != device:
         _refuse(f"{name} is on {t.device}, not on device {device}")
-    if shape and shape[-1] > 1 and t.stride(-1) != 1:
-        _refuse(f"the last dimension of {name} is not contiguous")
-    return t.data_ptr()
+    _refuse(f"{name} is not contiguous where it has to be (strides {t.stride()})")
 
 
-def _expect_flat(name, t, dtype, shape, device):
-    if t is not None and not t.is_contiguous():
-        _refuse(f"{name} is not contiguous")
-    return _expect(name, t, dtype, shape, device)
+def _take(name, t, dtype, shape, device):
+    """Address and strides of a tensor of this type, shape and device, its last dimension contiguous."""
+    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device:
+        s = t.stride()
+        if s[-1] == 1 or shape[-1] <= 1:
+            return t.data_ptr(), s
+    _wrong(name, t, dtype, shape, device)
+
+
+def _flat(name, t, dtype, shape, device):
+    """Address of a contiguous tensor of this type, shape and device."""
+    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    _wrong(name, t, dtype, shape, device)
 
 
 def _bytes(call, *args):
@@ -190,31 +194,33 @@ class PagedCache:
 
     def __init__(self, k, v, table, lengths, errors=None):
         self.tensors = (k, v, table, lengths, errors)
-        _dims("k", k, 4)
-        device, dtype = k.get_device(), _dtype(k)
-        if dtype not in (qd.DTYPE_F32, qd.DTYPE_BF16, qd.DTYPE_F16):
-            _refuse(f"pages of type {k.dtype}")
-        _expect("k", k, dtype, k.shape, device)
-        _expect("v", v, dtype, k.shape, device)
-        if k.stride() != v.stride():
-            _refuse("k and v have different strides")
-        pages, page_size, kv_heads, head_dim = k.shape
+        pages, page_size, kv_heads, head_dim = _dims("k", k, 4)
         rows, width = _dims("table", table, 2)
+        device, dtype = k.get_device(), k.dtype
+        if dtype not in _TYPES:
+            _refuse(f"pages of type {dtype}")
+        k_at, s = _take("k", k, dtype, k.shape, device)
+        v_at, sv = _take("v", v, dtype, k.shape, device)
+        if s != sv:
+            _refuse("k and v have different strides")
         # The stride of a dimension of one element is not used and may be anything.
-        s = [n if k.shape[i] > 1 else head_dim for i, n in enumerate(k.stride()[:3])]
+        s = [n if k.shape[i] > 1 else head_dim for i, n in enumerate(s[:3])]
+        table_at, ts = _take("table", table, _I32T, (rows, width), device)
         self.device, self.dtype, self.rows, self.kv_heads, self.head_dim = device, dtype, rows, kv_heads, head_dim
         self.c = CacheStruct(
-            k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], _expect("table", table, "int32", table.shape, device),
-            table.stride(0) if rows > 1 else width, _expect_flat("lengths", lengths, "int32", (rows,), device),
-            None if errors is None else _expect_flat("errors", errors, "int32", (1,), device), rows, width, pages,
-            page_size, kv_heads, head_dim, dtype, device)
+            k_at, v_at, s[0], s[1], s[2], table_at, ts[0] if rows > 1 else width,
+            _flat("lengths", lengths, _I32T, (rows,), device),
+            None if errors is None else _flat("errors", errors, _I32T, (1,), device), rows, width, pages, page_size,
+            kv_heads, head_dim, _TYPES[dtype], device)
 
 
-def _token_stride(name, t):
-    """Stride from token to token of [tokens, heads, head_dim] whose heads lie together."""
-    if t.shape[1] > 1 and t.stride(1) != t.shape[2]:
-        _refuse(f"the heads of a token of {name} do not lie together")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _tokens(name, t, dtype, shape, device):
+    """Address and stride from token to token of [tokens, heads, head_dim] whose heads lie together."""
+    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device:
+        s = t.stride()
+        if s[2] == 1 and (s[1] == shape[2] or shape[1] == 1):
+            return t.data_ptr(), s[0] if shape[0] > 1 else shape[1] * shape[2]
+    _wrong(name, t, dtype, shape, device)
 
 
 def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None, interleaved=False, position_bias=0,
@@ -223,43 +229,54 @@ def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None
     pages. q, q_out [tokens, heads, head_dim] (both None: keys and values only), k, v
     [tokens, kv_heads, head_dim], positions and rows [tokens] int32, cos and sin
     [positions, rotary_dim / 2] FP32 (None: no rotation)."""
-    device, dtype = cache.device, cache.dtype
-    tokens = _dims("k", k, 3)[0]
-    shape = (tokens, cache.kv_heads, cache.head_dim)
-    a = AppendStruct()
-    a.k, a.v = _expect("k", k, dtype, shape, device), _expect("v", v, dtype, shape, device)
-    a.k_stride, a.v_stride = _token_stride("k", k), _token_stride("v", v)
-    if (q is None) != (q_out is None):
-        _refuse("q and q_out go together")
-    if q is not None:
+    device, dtype, dim = cache.device, cache.dtype, cache.head_dim
+    tokens = len(k)
+    shape = (tokens, cache.kv_heads, dim)
+    k_at, k_stride = _tokens("k", k, dtype, shape, device)
+    v_at, v_stride = _tokens("v", v, dtype, shape, device)
+    q_at = out_at = None
+    q_stride = out_stride = heads = rotary = table_positions = 0
+    cos_at = sin_at = None
+    if q is not None and q_out is not None:
         heads = _dims("q", q, 3)[1]
-        shape = (tokens, heads, cache.head_dim)
-        a.q, a.q_out = _expect("q", q, dtype, shape, device), _expect("q_out", q_out, dtype, shape, device)
-        a.q_stride, a.q_out_stride, a.heads = _token_stride("q", q), _token_stride("q_out", q_out), heads
-    a.positions = _expect_flat("positions", positions, "int32", (tokens,), device)
-    if rows is not None:
-        a.rows = _expect_flat("rows", rows, "int32", (tokens,), device)
-    a.position_bias, a.tokens, a.interleaved = position_bias, tokens, 1 if interleaved else 0
-    if (cos is None) != (sin is None):
+        shape = (tokens, heads, dim)
+        q_at, q_stride = _tokens("q", q, dtype, shape, device)
+        out_at, out_stride = _tokens("q_out", q_out, dtype, shape, device)
+    elif q is not None or q_out is not None:
+        _refuse("q and q_out go together")
+    if cos is not None and sin is not None:
+        shape = _dims("cos", cos, 2)
+        cos_at, sin_at = _flat("cos", cos, _F32, shape, device), _flat("sin", sin, _F32, shape, device)
+        table_positions, rotary = shape[0], 2 * shape[1]
+    elif cos is not None or sin is not None:
         _refuse("cos and sin go together")
-    if cos is not None:
-        a.cos_table = _expect_flat("cos", cos, qd.DTYPE_F32, _dims("cos", cos, 2), device)
-        a.sin_table = _expect_flat("sin", sin, qd.DTYPE_F32, cos.shape, device)
-        a.table_positions, a.rotary_dim = cos.shape[0], 2 * cos.shape[1]
-    _check(lib().qd_paged_append(cache.c, a, stream))
+    shape = (tokens,)
+    status = lib().qd_paged_append(cache.c, AppendStruct(
+        q_at, k_at, v_at, out_at, q_stride, k_stride, v_stride, out_stride,
+        _flat("positions", positions, _I32T, shape, device),
+        None if rows is None else _flat("rows", rows, _I32T, shape, device), position_bias, tokens, heads, rotary,
+        1 if interleaved else 0, table_positions, cos_at, sin_at), stream)
+    if status:
+        _check(status)
 
 
 def paged_attention(cache, out, q, workspace, scale=None, stream=0):
     """Attention of one new token per cache row: q and out [rows, heads, head_dim]."""
-    device, dtype = cache.device, cache.dtype
+    device, dtype, dim, rows = cache.device, cache.dtype, cache.head_dim, cache.rows
     heads = _dims("q", q, 3)[1]
-    shape = (cache.rows, heads, cache.head_dim)
-    a = AttentionStruct(
-        _expect("q", q, dtype, shape, device), _expect("out", out, dtype, shape, device),
-        q.stride(0) if cache.rows > 1 else heads * cache.head_dim, q.stride(1) if heads > 1 else cache.head_dim,
-        out.stride(0) if cache.rows > 1 else heads * cache.head_dim, out.stride(1) if heads > 1 else cache.head_dim,
-        heads, cache.head_dim ** -0.5 if scale is None else scale)
-    _check(lib().qd_paged_attention(cache.c, a, workspace.handle, stream))
+    shape = (rows, heads, dim)
+    q_at, qs = _take("q", q, dtype, shape, device)
+    out_at, os = _take("out", out, dtype, shape, device)
+    # (The stride of a dimension of one element is not used and may be anything.)
+    if rows == 1:
+        qs, os = (heads * dim, qs[1]), (heads * dim, os[1])
+    if heads == 1:
+        qs, os = (qs[0], dim), (os[0], dim)
+    status = lib().qd_paged_attention(
+        cache.c, AttentionStruct(q_at, out_at, qs[0], qs[1], os[0], os[1], heads, dim ** -0.5 if scale is None else scale),
+        workspace.handle, stream)
+    if status:
+        _check(status)
 
 
 class PagePool:
@@ -269,7 +286,8 @@ class PagePool:
     def __init__(self, refs, page_size, tensors, planes=True):
         self.refs, self.page_size, self.tensors = refs, page_size, list(tensors)
         self.device, pages = refs.get_device(), _dims("refs", refs, 1)[0]
-        _expect_flat("refs", refs, "int32", (pages,), self.device)
+        self.pages = pages
+        _flat("refs", refs, _I32T, (pages,), self.device)
         self.memories = (MemoryStruct * max(1, len(self.tensors)))()
         for m, t in zip(self.memories, self.tensors):
             p = 1 if planes else 0
@@ -288,41 +306,42 @@ def pages_fork(pool, table, lengths, parents, append, table_out, lengths_out, wo
     """Row r of table_out takes over row parents[r] of table (None: its own, -1: released) with
     room for `append` more tokens; shared pages are counted and copied on write."""
     device = pool.device
-    rows, width = _dims("table", table, 2)
-    shape = (rows, width)
-    a = ForkStruct(
-        _expect("table", table, "int32", shape, device), _expect_flat("lengths", lengths, "int32", (rows,), device),
-        None if parents is None else _expect_flat("parents", parents, "int32", (rows,), device),
-        _expect("table_out", table_out, "int32", shape, device),
-        _expect_flat("lengths_out", lengths_out, "int32", (rows,), device), pool.refs.data_ptr(),
-        table.stride(0) if rows > 1 else width, table_out.stride(0) if rows > 1 else width,
-        None if errors is None else _expect_flat("errors", errors, "int32", (1,), device), pool.memories,
-        len(pool.tensors), rows, width, pool.refs.shape[0], pool.page_size, append, device)
-    _check(lib().qd_pages_fork(a, workspace.handle, stream))
+    rows, width = shape = _dims("table", table, 2)
+    table_at, ts = _take("table", table, _I32T, shape, device)
+    out_at, os = _take("table_out", table_out, _I32T, shape, device)
+    flat = (rows,)
+    status = lib().qd_pages_fork(ForkStruct(
+        table_at, _flat("lengths", lengths, _I32T, flat, device),
+        None if parents is None else _flat("parents", parents, _I32T, flat, device), out_at,
+        _flat("lengths_out", lengths_out, _I32T, flat, device), pool.refs.data_ptr(), ts[0] if rows > 1 else width,
+        os[0] if rows > 1 else width, None if errors is None else _flat("errors", errors, _I32T, (1,), device),
+        pool.memories, len(pool.tensors), rows, width, pool.pages, pool.page_size, append, device), workspace.handle, stream)
+    if status:
+        _check(status)
 
 
 def beam_select(logits, scores, scores_out, parents, tokens, workspace, done=None, done_out=None, eos=None, stream=0):
     """The best k = scores_out.shape[1] continuations of each group: logits [groups, beams, vocab],
     scores and done [groups, beams], the results [groups, k]."""
-    groups, beams, vocab = _dims("logits", logits, 3)
-    device, dtype = logits.get_device(), _dtype(logits)
-    if dtype not in (qd.DTYPE_F32, qd.DTYPE_BF16, qd.DTYPE_F16):
-        _refuse(f"logits of type {logits.dtype}")
+    groups, beams, vocab = shape = _dims("logits", logits, 3)
+    device, dtype = logits.get_device(), logits.dtype
+    if dtype not in _TYPES:
+        _refuse(f"logits of type {dtype}")
+    logits_at, s = _take("logits", logits, dtype, shape, device)
     k = _dims("scores_out", scores_out, 2)[1]
-    if (done is None) != (done_out is None) or (done is not None and eos is None):
+    given, chosen = (groups, beams), (groups, k)
+    done_at = done_out_at = None
+    if done is not None and done_out is not None and eos is not None:
+        done_at, done_out_at = _flat("done", done, _U8T, given, device), _flat("done_out", done_out, _U8T, chosen, device)
+    elif done is not None or done_out is not None:
         _refuse("done, done_out and eos go together")
-    if vocab > 1 and logits.stride(2) != 1:
-        _refuse("the last dimension of logits is not contiguous")
-    a = SelectStruct(
-        logits.data_ptr(), logits.stride(0), logits.stride(1),
-        _expect_flat("scores", scores, qd.DTYPE_F32, (groups, beams), device),
-        None if done is None else _expect_flat("done", done, "uint8", (groups, beams), device),
-        _expect_flat("scores_out", scores_out, qd.DTYPE_F32, (groups, k), device),
-        _expect_flat("parents", parents, "int32", (groups, k), device),
-        _expect_flat("tokens", tokens, "int32", (groups, k), device),
-        None if done is None else _expect_flat("done_out", done_out, "uint8", (groups, k), device), dtype, groups, beams,
-        vocab, k, 0 if eos is None else eos, device)
-    _check(lib().qd_beam_select(a, workspace.handle, stream))
+    status = lib().qd_beam_select(SelectStruct(
+        logits_at, s[0], s[1], _flat("scores", scores, _F32, given, device), done_at,
+        _flat("scores_out", scores_out, _F32, chosen, device), _flat("parents", parents, _I32T, chosen, device),
+        _flat("tokens", tokens, _I32T, chosen, device), done_out_at, _TYPES[dtype], groups, beams, vocab, k,
+        0 if eos is None else eos, device), workspace.handle, stream)
+    if status:
+        _check(status)
 
 
 def rope_table(theta, rotary_dim, positions, stretch=1.0, original=32768, fast=32.0, slow=1.0):
