@@ -230,7 +230,7 @@ def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None
     [tokens, kv_heads, head_dim], positions and rows [tokens] int32, cos and sin
     [positions, rotary_dim / 2] FP32 (None: no rotation)."""
     device, dtype, dim = cache.device, cache.dtype, cache.head_dim
-    tokens = len(k)
+    tokens = 0 if k is None else len(k)
     shape = (tokens, cache.kv_heads, dim)
     k_at, k_stride = _tokens("k", k, dtype, shape, device)
     v_at, v_stride = _tokens("v", v, dtype, shape, device)

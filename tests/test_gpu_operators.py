@@ -96,6 +96,28 @@ def test_append(dtype, heads, kv_heads, dim, rotary, interleaved, page, tokens):
     assert torch.equal(kp[untouched], filled[0][untouched]) and torch.equal(vp[untouched], filled[1][untouched])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_append_of_a_long_prompt(dtype):
+    """Enough to be written past the caches."""
+    say("append of a long prompt", dtype)
+    g, heads, kv_heads, dim, page = seeded(9), 16, 4, 128, 64
+    tokens = (40 << 20) // ((heads + 2 * kv_heads) * dim * (4 if dtype == F32 else 2))
+    table, pages = tables_for(g, [tokens], page, -(-tokens // page))
+    q, k, v = (normal(g, (tokens, n, dim), dtype) for n in (heads, kv_heads, kv_heads))
+    cos, sin = (torch.from_numpy(t) for t in ops.rope_table(1e6, 64, tokens))
+    kp, vp = (torch.zeros((pages, page, kv_heads, dim), dtype=dtype, device="cuda") for _ in range(2))
+    cache = ops.PagedCache(kp, vp, table.cuda(), int32([0]).cuda())
+    out = torch.empty((tokens, heads, dim), dtype=dtype, device="cuda")
+    at = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    ops.paged_append(cache, out, q.cuda(), k.cuda(), v.cuda(), at, rows=torch.zeros_like(at), cos=cos.cuda(), sin=sin.cuda())
+    want, size = oracle.rotate(q, cos, sin, False)
+    close(out, want, oracle.rotate_bound(want, size, dtype), "q")
+    want, size = oracle.rotate(k, cos, sin, False)
+    where = table[0].long().cuda()
+    close(kp[where].flatten(0, 1)[:tokens], want, oracle.rotate_bound(want, size, dtype), "k")
+    assert torch.equal(vp[where].flatten(0, 1)[:tokens].cpu(), v)
+
+
 def append_state(dtype=F32, rows=4, page=16, width=3, dim=64):
     g = seeded(5)
     table, pages = tables_for(g, [width * page] * rows, page, width)
