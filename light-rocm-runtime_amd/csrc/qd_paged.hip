@@ -1019,34 +1019,36 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t *waves, ui
 }
 
 // Adds `sign` times what the fork changes: a page that an old row takes over to
-// c children counts c - 1 more, one behind its length one less.
-__device__ __forceinline__ void count_references(const ForkLaunch &p, const int *children, int sign, uint32_t *bad) {
+// c children counts c - 1 more, one behind its length one less. `early` holds the
+// first columns of each wave's first row.
+__device__ __forceinline__ void count_references(const ForkLaunch &p, const int *children, const int *lengths, int sign,
+                                                 int32_t early, uint32_t *bad) {
   const int lane = lane_id();
   for (uint32_t r = wave_id(); r < p.a.rows; r += kForkWaves) {
     const int32_t *table = p.a.table + r * p.a.table_stride;
-    const uint32_t held = (static_cast<uint32_t>(p.a.lengths[r]) + p.a.page_size - 1) >> p.page_shift;
+    const uint32_t held = (static_cast<uint32_t>(lengths[r]) + p.a.page_size - 1) >> p.page_shift;
     const int change = children[r] - 1;
-    for (uint32_t j = lane; j < p.a.table_width; j += kWave) {
-      // Up to the chunk in which the row ends.
-      const int32_t id = table[j];
-      const bool in = id >= 0 && static_cast<uint32_t>(id) < p.a.pages;
-      const bool over = id < 0;
-      // Entries behind the first negative one are none.
-      const uint64_t ends = __ballot(over);
-      const bool before_end = (ends & ((1ull << lane) - 1)) == 0;
-      if (before_end) {
-        if (j < held) {
-          if (!in) atomicOr(bad, QD_PAGED_BAD_PAGE);
-          if (in && change) atomicAdd(p.a.refs + id, sign * change);
-        } else if (!over) {
-          if (!in) atomicOr(bad, QD_PAGED_BAD_PAGE);
-          if (in) atomicAdd(p.a.refs + id, -sign);
-        }
+    for (uint32_t base = 0;; base += kWave) {
+      const uint32_t j = base + lane;
+      int32_t id = -1;
+      if (base == 0 && r == static_cast<uint32_t>(wave_id()))
+        id = early;
+      else if (j < p.a.table_width)
+        id = table[j];
+      // Entries behind the first negative one, or the last column, are none.
+      const uint64_t ends = __ballot(id < 0);
+      if ((ends & ((1ull << lane) - 1)) == 0 && id >= 0) {
+        if (static_cast<uint32_t>(id) >= p.a.pages)
+          atomicOr(bad, QD_PAGED_BAD_PAGE);
+        else if (j >= held)
+          atomicAdd(p.a.refs + id, -sign);
+        else if (change)
+          atomicAdd(p.a.refs + id, sign * change);
       }
       if (ends) {
         // A row that ends before its length lacks a page.
-        const uint32_t end = j - lane + __ffsll(static_cast<unsigned long long>(ends)) - 1;
-        if (end < held) atomicOr(bad, QD_PAGED_BAD_PAGE);
+        const uint32_t end = base + __ffsll(static_cast<unsigned long long>(ends)) - 1;
+        if (end < held && lane == 0) atomicOr(bad, QD_PAGED_BAD_PAGE);
         break;
       }
     }
@@ -1054,87 +1056,107 @@ __device__ __forceinline__ void count_references(const ForkLaunch &p, const int 
 }
 
 __global__ __launch_bounds__(kForkT) void fork_plan_kernel(ForkLaunch p) {
-  __shared__ int children[kForkRows], last[kForkRows];
+  constexpr int kList = 1024;  // free pages kept in LDS too
+  __shared__ __attribute__((aligned(16))) int last[kForkRows];  // -1 behind the rows
+  __shared__ int children[kForkRows], lengths[kForkRows], list[kList];
   __shared__ uint32_t waves[kForkWaves], bad, copies;
   const uint32_t r = threadIdx.x;  // one thread per row where rows are meant
+  static_assert(kForkT == kForkRows, "a thread per row");
   const int64_t room = static_cast<int64_t>(p.a.table_width) << p.page_shift;
-  if (r < p.a.rows) children[r] = 0;
-  if (r == 0) bad = copies = 0;
-  __syncthreads();
+  // Nothing here waits for another: the wave's first row, the lengths and parents.
+  const uint32_t wave_row = wave_id(), lane = lane_id();
+  const int32_t early = wave_row < p.a.rows && lane < p.a.table_width ? p.a.table[wave_row * p.a.table_stride + lane] : -1;
   ForkRow row{-1, 0, -1, 0u, 0, 0};
   if (r < p.a.rows) {
-    const int32_t own = p.a.lengths[r];
-    if (own < 0 || own > room) atomicOr(&bad, QD_PAGED_BAD_LENGTH);
+    children[r] = 0;
+    lengths[r] = p.a.lengths[r];
     row.parent = p.a.parents ? p.a.parents[r] : static_cast<int32_t>(r);
+  }
+  if (r == 0) bad = copies = 0;
+  __syncthreads();
+  int32_t id = -1;  // the page in which the row goes on
+  if (r < p.a.rows) {
+    if (lengths[r] < 0 || lengths[r] > room) atomicOr(&bad, QD_PAGED_BAD_LENGTH);
     if (row.parent < -1 || row.parent >= static_cast<int32_t>(p.a.rows)) {
       atomicOr(&bad, QD_PAGED_BAD_ROW);
       row.parent = -1;
     }
     if (row.parent >= 0) {
-      row.length = p.a.lengths[row.parent];
-      if (row.length < 0 || row.length + static_cast<int64_t>(p.a.append) > room) atomicOr(&bad, QD_PAGED_BAD_LENGTH);
+      row.length = lengths[row.parent];
+      if (row.length < 0 || row.length + static_cast<int64_t>(p.a.append) > room) {
+        atomicOr(&bad, QD_PAGED_BAD_LENGTH);
+      } else {
+        row.held = (row.length + p.a.page_size - 1) >> p.page_shift;
+        if (p.a.append && (row.length & (p.a.page_size - 1)))
+          id = p.a.table[row.parent * p.a.table_stride + row.held - 1];
+      }
       atomicAdd(&children[row.parent], 1);
     }
   }
+  last[r] = id;
   __syncthreads();
   const bool fits = bad == 0;
   __syncthreads();
-  if (fits) count_references(p, children, 1, &bad);
+  if (fits) count_references(p, children, lengths, 1, early, &bad);
   wait_vm_stores();  // the counts stand in L2 before any of them is read
   __syncthreads();
-  uint32_t wanted = 0;
-  if (bad == 0) {
-    row.held = (row.length + p.a.page_size - 1) >> p.page_shift;
-    const bool partial = row.parent >= 0 && p.a.append && (row.length & (p.a.page_size - 1));
-    int id = -1;
-    if (r < p.a.rows && partial) id = p.a.table[row.parent * p.a.table_stride + row.held - 1];
-    if (r < p.a.rows) last[r] = id;
-    __syncthreads();
+  const bool sound = bad == 0;
+  uint32_t wanted = 0, found = 0;
+  if (sound) {
+    // The counts of the row's page and of the first pages, for the free ones.
+    const int held_by = id >= 0 ? load_count(p.a.refs + id) : 0;
+    int32_t n[kForkScan];
+    auto look = [&](uint32_t base) {
+#pragma unroll
+      for (int u = 0; u < kForkScan; ++u) {
+        const uint32_t page = base + r * kForkScan + u;
+        n[u] = page < p.a.pages ? load_count(p.a.refs + page) : 1;
+      }
+    };
+    look(0);
     if (id >= 0) {
       int holders = 0, lowest = kForkRows;
-      for (uint32_t u = 0; u < p.a.rows; ++u)
-        if (last[u] == id) {
-          ++holders;
-          lowest = min(lowest, static_cast<int>(u));
-        }
-      if (load_count(p.a.refs + id) != holders || lowest != static_cast<int>(r)) row.source = id;
+      for (int u = 0; u < static_cast<int>(p.a.rows); u += 8) {
+        const int4 a = *reinterpret_cast<const int4 *>(last + u), b = *reinterpret_cast<const int4 *>(last + u + 4);
+        const int ids[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int v = 7; v >= 0; --v)
+          if (ids[v] == id) {
+            ++holders;
+            lowest = min(lowest, u + v);
+          }
+      }
+      if (held_by != holders || lowest != static_cast<int>(r)) row.source = id;
     }
     if (row.parent >= 0) {
       const uint32_t need = (static_cast<uint32_t>(row.length) + p.a.append + p.a.page_size - 1) >> p.page_shift;
       row.fresh = static_cast<int>(need) - row.held + (row.source >= 0);
     }
     row.begin = block_before(row.fresh, waves, wanted);
-  }
-  // The free pages of the lowest ids.
-  uint32_t found = 0;
-  if (bad == 0)
+    // The free pages of the lowest ids.
     for (uint32_t base = 0; base < p.a.pages && found < wanted; base += kForkT * kForkScan) {
-      int32_t n[kForkScan];
-      uint32_t mine = 0;
-#pragma unroll
-      for (int u = 0; u < kForkScan; ++u) {
-        const uint32_t page = base + r * kForkScan + u;
-        n[u] = page < p.a.pages ? load_count(p.a.refs + page) : 1;
-      }
+      if (base) look(base);
+      uint32_t mine = 0, here = 0;
 #pragma unroll
       for (int u = 0; u < kForkScan; ++u) mine += n[u] == 0;
-      uint32_t here = 0;
       uint32_t at = found + block_before(mine, waves, here);
 #pragma unroll
       for (int u = 0; u < kForkScan; ++u)
         if (n[u] == 0) {
-          if (at < wanted) p.free_pages[at] = base + r * kForkScan + u;
+          const int32_t page = static_cast<int32_t>(base + r * kForkScan + u);
+          if (at < wanted) p.free_pages[at] = page;
+          if (at < static_cast<uint32_t>(kList)) list[at] = page;
           ++at;
         }
       found += here;
     }
-  if (bad == 0 && found < wanted && r == 0) bad = QD_PAGED_EXHAUSTED;
-  wait_vm_stores();  // the free list is read back below
+    if (wanted > kList) wait_vm_stores();  // the rest is read back below
+  }
   __syncthreads();
-  const uint32_t error = bad;
-  __syncthreads();
-  if (error) {
-    if (fits) count_references(p, children, -1, &bad);
+  if (!sound || found < wanted) {
+    const uint32_t error = sound ? static_cast<uint32_t>(QD_PAGED_EXHAUSTED) : bad;
+    __syncthreads();
+    if (fits) count_references(p, children, lengths, -1, early, &bad);
     if (r == 0) {
       raise_error(p.a.errors, error);
       p.plan->ok = 0;
@@ -1144,13 +1166,14 @@ __global__ __launch_bounds__(kForkT) void fork_plan_kernel(ForkLaunch p) {
   }
   if (r < p.a.rows) {
     for (int u = 0; u < row.fresh; ++u) {
-      const int32_t page = p.free_pages[row.begin + u];
+      const uint32_t at = row.begin + u;
+      const int32_t page = at < static_cast<uint32_t>(kList) ? list[at] : p.free_pages[at];
       p.a.refs[page] = 1;
       if (u == 0 && row.source >= 0) {
         atomicSub(p.a.refs + row.source, 1);
-        const uint32_t at = atomicAdd(&copies, 1u);
-        p.copy_source[at] = row.source;
-        p.copy_to[at] = page;
+        const uint32_t to = atomicAdd(&copies, 1u);
+        p.copy_source[to] = row.source;
+        p.copy_to[to] = page;
       }
     }
     p.row[r] = row;
@@ -1218,7 +1241,7 @@ __global__ __launch_bounds__(kBlock) void fork_copy_kernel(ForkLaunch p) {
       if ((threadIdx.x + u * kBlock) * 16 < n) x[u] = src[threadIdx.x + u * kBlock];
 #pragma unroll
     for (uint32_t u = 0; u < kCopyPiece / 16 / kBlock; ++u)
-      if ((threadIdx.x + u * kBlock) * 16 < n) dst[threadIdx.x + u * kBlock] = x[u];
+      if ((threadIdx.x + u * kBlock) * 16 < n) put<false>(dst + threadIdx.x + u * kBlock, x[u]);
   }
 }
 
