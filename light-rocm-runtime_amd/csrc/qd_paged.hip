@@ -239,6 +239,9 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 constexpr int kTile = 32, kSub = 16;
 constexpr uint32_t kMostPieces = 256;  // of an item
 constexpr int kWaves = 4;              // of a workgroup
+// The short kernel: tiles of a piece at least, of an item that stays whole, and
+// pieces of an item at most.
+constexpr uint32_t kShortLeast = 4, kShortWhole = 8, kShortPieces = 64;
 // A maximum is only taken up when it passes the one in use by this many powers of
 // two: until then probabilities grow to at most 2^8, exact in every type's range.
 constexpr float kLazyMax = 8.f;
@@ -443,7 +446,8 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint
       longest = max(longest, tiles);
     }
     total = __builtin_amdgcn_readlane(lanes_upto(total), kWave - 1);
-    size = max(max(p.least, (total + p.target - 1) / p.target), (lanes_max(longest) + kMostPieces - 1) / kMostPieces);
+    size = max(max(kShortLeast, (total + p.target - 1) / p.target), (lanes_max(longest) + kShortPieces - 1) / kShortPieces);
+    const auto pieces_of = [&](uint32_t tiles) { return tiles <= kShortWhole ? 1u : (tiles + size - 1) / size; };
     const bool once = p.c.rows <= kWave;
     uint32_t base = 0, upto, mine;
     begin = 0;
@@ -451,7 +455,7 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint
     for (;; base += kWave) {
       if (base >= p.c.rows) return false;
       if (!once) n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
-      mine = base + lane < p.c.rows ? (tiles_of(p, n, most) + size - 1) / size : 0u;
+      mine = base + lane < p.c.rows ? pieces_of(tiles_of(p, n, most)) : 0u;
       upto = lanes_upto(mine);
       past = __ballot(begin + upto > x);
       if (past) break;
@@ -473,8 +477,8 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint
   it.at = 0;
   it.tiles = tiles_of(p, n, most);
   it.home = x - begin;
-  it.first = it.home * size;
-  it.last = min(it.tiles, it.first + size);
+  it.first = it.pieces == 1 ? 0 : it.home * size;
+  it.last = it.pieces == 1 ? it.tiles : min(it.tiles, it.first + size);
   return true;
 }
 
@@ -1263,9 +1267,18 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
 
 constexpr uint64_t kAppendStream = 32ull << 20;
 
-// How attention cuts its work. The short kernel: pieces of eight tiles or more, so
-// that they are about kShortAim. The long one: as many workgroups as CUs.
-constexpr uint32_t kAttnLeast = 8, kShortAim = 2048, kCus = 256, kMostPerCu = 2;
+// How attention cuts its work. Workgroups that the card holds at once: of the short
+// kernel, by head_dim, which its pieces are made for (16 beams at 576 positions in
+// pieces of 4 tiles or more 8.9 us, of 8 10.8; 4 rows of 3,000 with 8 KV heads of 128
+// in about 512 pieces 15.5 us, in 768 18.6; 64 rows to 2,000 with 2 of 64 21.9 in
+// 512, 20.4 in 768), and of the long one. The long kernel's cuts keep eight tiles
+// from an item's ends.
+constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
+constexpr uint32_t short_aim(uint32_t head_dim) { return head_dim == 128 ? 2 * kCus : 3 * kCus; }
+// Which kernel, by the bytes of all positions that the tables, or the pool, can
+// hold (their real number is on the device): 68 MB of 2 heads of 64 short 20.4 us,
+// long 24.0; 101 MB of 8 of 128 29.1 and 27.1; 102 MB of one row 37.8 and 34.0;
+// 193 MB 57 and 48.
 constexpr uint64_t kShortBytes = 96ull << 20;
 constexpr uint64_t kCachedBytes = 256ull << 20;
 struct AttnShape {
@@ -1281,7 +1294,7 @@ AttnShape attention_shape(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint
   const uint64_t items = static_cast<uint64_t>(rows) * s.parts;
   if (items <= kOpCounters) {
     s.least = kAttnLeast;
-    s.target = std::max(1u, kShortAim / s.parts);
+    s.target = std::max(1u, short_aim(head_dim) / s.parts);
     s.records = std::max((rows + s.target) * s.parts, 2 * kCus * kMostPerCu);
     // Counters in lines of their own where there is room.
     for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
@@ -1332,9 +1345,9 @@ static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
   const uint64_t positions = std::min<uint64_t>(static_cast<uint64_t>(p.c.rows) * p.c.table_width << p.page_shift, pool);
   const dim3 block(kWaves * kWave);
   if (positions * position <= kShortBytes || p.least == 0) {
-    if (most <= p.least) p.target = 0;
+    if (most <= kShortWhole) p.target = 0;
     uint64_t x = p.c.rows;
-    if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + p.least - 1) / p.least));
+    if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + kShortLeast - 1) / kShortLeast));
     return launch(attention_short_kernel<E, D>, dim3(static_cast<uint32_t>(x * p.parts)), block, s, p);
   }
   // Pages that cannot all stay in the last-level cache are read as a stream.

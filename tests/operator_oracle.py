@@ -52,11 +52,11 @@ def attention(q, k, v, table, lengths, scale):
             out[r, h] = p @ vv[:, g]
             # Scores: at most dim FP32 additions and three roundings of sum |q k| each, and
             # twice in the ratio; exponentials 2^-22 more, sums over at most n / 4 + 64
-            # positions in turn, and (16 bits) the probabilities' rounding in both sums.
+            # positions in turn, and (16 bits) what two numbers leave of a probability.
             score = (dim + 3) * 2.0 ** -24 * float(products.abs().sum(-1).max())
             weight = 2 * score + 2.0 ** -22 + 2 * (n / 4 + 64) * 2.0 ** -24
             if q.dtype != torch.float32:
-                weight += 2 * HALF_STEP[q.dtype]
+                weight += HALF_STEP[q.dtype] ** 2
             bound[r, h] = weight * (p @ vv[:, g].abs()) + HALF_STEP[q.dtype] * out[r, h].abs() + HALF_LEAST[q.dtype]
             if q.dtype != torch.float32:
                 # Small probabilities: the largest in the sum is 1 or more, each of n is off by the least
