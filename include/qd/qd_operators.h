@@ -104,8 +104,8 @@ QD_API qd_status qd_rope_table(double theta, uint32_t rotary_dim, uint32_t posit
  * `interleaved` is nonzero: (a, b) -> (a c - b s, b c + a s) with c and s from
  * row `position` of cos_table and sin_table [table_positions][rotary_dim / 2],
  * in FP32, rounded once. rotary_dim 0: nothing is rotated and the tables may be
- * NULL. q NULL: keys and values only. q_out may be q itself (in place). A token
- * whose position is negative is skipped: nothing of it is read or written. A
+ * NULL. q NULL: keys and values only. q_out may be q itself, with its stride. A
+ * token whose position is negative is skipped: nothing of it is read or written. A
  * (row, position) given twice gets one token's row or the other's, not
  * necessarily of one whole token. cache->lengths is not read. A token whose row,
  * position or page does not exist is not written, and its q_out row is NaN. */
@@ -134,10 +134,11 @@ QD_API qd_status qd_paged_append(const qd_paged_cache *cache, const qd_append_ar
 /* Attention of one new token per cache row: query head h of row r over
  * positions 0 .. lengths[r] - 1 of KV head h / (heads / kv_heads),
  *   out[r][h] = sum_j softmax_j(scale q[r][h] . K_j) V_j,
- * statistics and sums in FP32. A row of length 0 gets zeros; what the pages
+ * statistics and sums in FP32 (products are summed before they are divided, by
+ * weights up to 2^8: finite for |V| below 2^89). A row of length 0 gets zeros; what the pages
  * hold past a row's length is not read. A row with a bad length or page gets
  * NaN. q and out are [rows][heads][head_dim] with strides that are multiples of
- * 16 bytes; out may be q itself. The result of a row does not depend on when
+ * 16 bytes; out may be q itself, with its strides. The result of a row does not depend on when
  * its parts finish (they are joined in order), but how its positions are split
  * goes by all rows' lengths. */
 typedef struct qd_attention_args {
@@ -188,7 +189,8 @@ typedef struct qd_page_memory {
  * (QD_PAGED_BAD_LENGTH) or too few free pages, an error bit is set and table,
  * lengths and refs are handed on as they were, with no page copied. table_out
  * and lengths_out must not overlap table and lengths: a program keeps two of
- * each and takes them in turn. */
+ * each and takes them in turn. Forks that share refs follow each other, as calls
+ * that share a workspace do. */
 typedef struct qd_fork_args {
   const int32_t *table;   /* [rows][table_width] */
   const int32_t *lengths;
@@ -215,7 +217,7 @@ QD_API qd_status qd_pages_fork_workspace(uint32_t rows, uint32_t pages, size_t *
  * Of each group's beams x vocab continuations the best k. Continuation (b, t)
  * scores
  *   scores[b] + log softmax(logits[b])[t],
- * sums in 64 bits (exponentials FP32), candidates compared in 64 bits. Higher
+ * sums in 64 bits (exponentials and 16 of them FP32), candidates compared in 64 bits. Higher
  * scores come first; continuations of one beam go by their logits, then by the
  * lower token; equal scores of two beams by the lower beam. NaN counts as -inf.
  * A beam whose score is not finite has no continuation; one that is done (done[b]
@@ -225,7 +227,9 @@ QD_API qd_status qd_pages_fork_workspace(uint32_t rows, uint32_t pages, size_t *
  *   scores_out[g][i]   FP32
  *   parents[g][i]      g * beams + b: the row the i-th goes on from
  *   tokens[g][i]       t
- *   done_out[g][i]     1 if that beam was done or t is eos (NULL with done NULL) */
+ *   done_out[g][i]     1 if that beam was done or t is eos (NULL with done NULL)
+ * The results must not be the tensors that are read: a program keeps two of
+ * scores and done and takes them in turn. */
 typedef struct qd_select_args {
   const void *logits;    /* [groups][beams][vocab] */
   int64_t group_stride;

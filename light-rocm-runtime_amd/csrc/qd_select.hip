@@ -444,7 +444,8 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   uint64_t *own = sh.own[w];
   uint32_t count = 0;
   float least = logit_of(static_cast<uint64_t>(kLowest) << 32);  // keys at or above it are kept
-  float m = -INFINITY, sum = 0.f;
+  float m = -INFINITY, base = -INFINITY;
+  double sum = 0.0;
   for (uint32_t tile = begin; tile < end; tile += kTile) {
     float x[kEach];
 #pragma unroll
@@ -478,20 +479,24 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
     // (NaN is no maximum and at or above no bound; of its exponential, fmaxf makes 0.)
 #pragma unroll
     for (int i = 0; i < kEach; ++i) top = fmaxf(top, x[i]);
-    // Sum of exp(x - m), FP32 within a thread. The difference is exact to half a
-    // step, so the sum has no error common to its terms.
-    if (top > m) {
-      if (m > -INFINITY) sum *= exp2_fast((m - top) * kLog2e);
-      m = top;
+    // Sum of exp(x - base), 16 terms in FP32 and 64 bits beyond. The base follows the
+    // lane's maximum by steps of 1 and more: the differences that count are exact to
+    // half a step, and a new base's factor is soon outweighed.
+    m = fmaxf(m, top);
+    if (top > base + 1.f) {
+      if (base > -INFINITY) sum *= exp2_fast((base - top) * kLog2e);
+      base = top;
     }
-    const float base = m == -INFINITY ? 0.f : m;
-    if (!__any(m == INFINITY)) {
+    const float from = base == -INFINITY ? 0.f : base;
+    float part = 0.f;
+    if (!__any(base == INFINITY)) {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) sum += fmaxf(exp2_fast((x[i] - base) * kLog2e), 0.f);
+      for (int i = 0; i < kEach; ++i) part += fmaxf(exp2_fast((x[i] - from) * kLog2e), 0.f);
     } else {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) sum += x[i] == base ? 1.f : fmaxf(exp2_fast((x[i] - base) * kLog2e), 0.f);
+      for (int i = 0; i < kEach; ++i) part += x[i] == from ? 1.f : fmaxf(exp2_fast((x[i] - from) * kLog2e), 0.f);
     }
+    sum += part;
     // The bound rises with the lanes' maxima, after 1, 2, 4, ... tiles, and when
     // the wave's list is full.
     if (const uint32_t seen = (tile - begin) / kTile + 1; (seen & (seen - 1)) == 0)
@@ -547,7 +552,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
     at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((1ull << lane) - 1));
     if (in && at < static_cast<uint32_t>(kFew)) sh.few[at] = key;
   }
-  const double total = wave_sum64(m == top ? sum : m == -INFINITY ? 0.f : sum * exp2_fast((m - top) * kLog2e));
+  const double total = wave_sum64(base == top ? sum : base == -INFINITY ? 0.0 : sum * exp2_fast((base - top) * kLog2e));
   if (lane == 0) sh.sum[w] = total;
   __syncthreads();
   const uint32_t n = p.runs * k;
