@@ -227,8 +227,9 @@ qd_status qd_paged_append(const qd_paged_cache *c, const qd_append_args *a, void
   if (a->q) QD_TRY(check_heads(a->heads, c->kv_heads));
   if (a->rotary_dim % 8 != 0 || a->rotary_dim > dim)
     return refuse(QD_ERROR_INVALID_ARGUMENT, "rotary_dim %u: a multiple of 8 up to head_dim %u is needed", a->rotary_dim, dim);
-  const uint64_t units = (static_cast<uint64_t>(a->q ? a->heads : 0) + 2 * c->kv_heads) * (dim / 8);
-  if (units * a->tokens > 0xffff0000ull) return refuse(QD_ERROR_NOT_SUPPORTED, "%u tokens are too many for one call", a->tokens);
+  // A grid has fewer than 2^32 threads: whole waves for each token, eight elements a lane.
+  const uint64_t lanes = ((static_cast<uint64_t>(a->q ? a->heads : 0) + 2 * c->kv_heads) * (dim / 8) + 63) / 64 * 64;
+  if (lanes * a->tokens > 0xffff0000ull) return refuse(QD_ERROR_NOT_SUPPORTED, "%u tokens are too many for one call", a->tokens);
   if (a->tokens) {
     if (!a->k || !a->v || !a->positions || (a->q && !a->q_out)) return invalid("null tensor");
     if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->q_out))
@@ -238,6 +239,7 @@ qd_status qd_paged_append(const qd_paged_cache *c, const qd_append_args *a, void
     if (a->q) {
       QD_TRY(check_stride(a->q_stride, 0, e, "q_stride"));
       QD_TRY(check_stride(a->q_out_stride, a->tokens > 1 ? static_cast<int64_t>(a->heads) * dim : 0, e, "q_out_stride"));
+      if (a->q_out == a->q && a->tokens > 1 && a->q_out_stride != a->q_stride) return invalid("q in place needs one stride");
     }
     QD_TRY(check_stride(a->k_stride, 0, e, "k_stride"));
     QD_TRY(check_stride(a->v_stride, 0, e, "v_stride"));
@@ -269,9 +271,14 @@ qd_status qd_paged_attention(const qd_paged_cache *c, const qd_attention_args *a
     QD_TRY(check_stride(a->q_head_stride, 0, e, "q_head_stride"));
     QD_TRY(check_stride(a->out_stride, c->rows > 1 ? c->head_dim : 0, e, "out_stride"));
     QD_TRY(check_stride(a->out_head_stride, a->heads > 1 ? c->head_dim : 0, e, "out_head_stride"));
+    if (a->out == a->q && ((c->rows > 1 && a->out_stride != a->q_stride) ||
+                           (a->heads > 1 && a->out_head_stride != a->q_head_stride)))
+      return invalid("q in place needs one stride");
   }
   const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((a->heads / c->kv_heads + 15) / 16);
-  if (c->rows * parts * (static_cast<uint64_t>(c->table_width) * c->page_size / 32 + 1) > 0x7f000000u)
+  // Tiles are counted in 31 bits, and a grid has fewer than 2^32 threads.
+  if (c->rows * parts * (static_cast<uint64_t>(c->table_width) * c->page_size / 32 + 1) > 0x7f000000u ||
+      c->rows * parts > 0xffff00u)
     return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of up to %llu positions and %u heads are too much for one call", c->rows,
                   static_cast<unsigned long long>(static_cast<uint64_t>(c->table_width) * c->page_size), a->heads);
   qd::OpScratch scratch{};
@@ -339,6 +346,8 @@ qd_status qd_beam_select(const qd_select_args *a, qd_workspace *w, void *stream)
   if (a->groups) {
     if (!a->logits || !a->scores || !a->scores_out || !a->parents || !a->tokens || (a->done && !a->done_out))
       return invalid("null tensor");
+    if (a->scores_out == a->scores || (a->done && a->done_out == a->done))
+      return invalid("scores_out and done_out must not be scores and done");
     if (reinterpret_cast<uintptr_t>(a->logits) % element_bytes(a->dtype) != 0) return invalid("misaligned logits");
     if (a->done && a->eos >= a->vocab) return refuse(QD_ERROR_INVALID_ARGUMENT, "eos %u >= vocab %u", a->eos, a->vocab);
     const int64_t most = int64_t(1) << 40;

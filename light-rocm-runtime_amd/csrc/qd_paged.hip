@@ -1249,7 +1249,7 @@ __global__ __launch_bounds__(kBlock) void fork_copy_kernel(ForkLaunch p) {
       if ((threadIdx.x + u * kBlock) * 16 < n) x[u] = src[threadIdx.x + u * kBlock];
 #pragma unroll
     for (uint32_t u = 0; u < kCopyPiece / 16 / kBlock; ++u)
-      if ((threadIdx.x + u * kBlock) * 16 < n) put<false>(dst + threadIdx.x + u * kBlock, x[u]);
+      if ((threadIdx.x + u * kBlock) * 16 < n) dst[threadIdx.x + u * kBlock] = x[u];
   }
 }
 

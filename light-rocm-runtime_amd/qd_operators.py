@@ -250,6 +250,8 @@ def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None
         table_positions, rotary = shape[0], 2 * shape[1]
     elif cos is not None or sin is not None:
         _refuse("cos and sin go together")
+    if not -2 ** 31 <= position_bias < 2 ** 31:
+        _refuse(f"position_bias {position_bias} does not fit 32 bits")
     shape = (tokens,)
     status = lib().qd_paged_append(cache.c, AppendStruct(
         q_at, k_at, v_at, out_at, q_stride, k_stride, v_stride, out_stride,
@@ -293,8 +295,10 @@ class PagePool:
             p = 1 if planes else 0
             if t.dim() <= p or t.shape[p] != pages or t.get_device() != self.device:
                 _refuse(f"a tensor of shape {tuple(t.shape)} on {t.device} does not hold {pages} pages of device {self.device}")
+            if t.numel() == 0:
+                _refuse(f"a tensor of shape {tuple(t.shape)} holds nothing")
             inner = t.select(p, 0).select(0, 0) if planes else t.select(0, 0)
-            if pages and not inner.is_contiguous():
+            if not inner.is_contiguous():
                 _refuse("a page's values do not lie together")
             size = t.element_size()
             m.base, m.bytes = t.data_ptr(), inner.numel() * size
@@ -347,6 +351,8 @@ def beam_select(logits, scores, scores_out, parents, tokens, workspace, done=Non
 def rope_table(theta, rotary_dim, positions, stretch=1.0, original=32768, fast=32.0, slow=1.0):
     """cos and sin [positions, rotary_dim / 2] for paged_append, numpy FP32 on the host."""
     f = C.POINTER(C.c_float)
+    if rotary_dim < 0 or positions < 0:
+        _refuse("rotary_dim and positions must not be negative")
     cos, sin = (np.empty((positions, rotary_dim // 2), np.float32) for _ in range(2))
     _check(lib().qd_rope_table(theta, rotary_dim, positions, stretch, original, fast, slow, cos.ctypes.data_as(f),
                                sin.ctypes.data_as(f)))

@@ -626,6 +626,162 @@ def test_select_descending_and_nearly_equal_rows(dtype):
     check_select(logits[:, 2:], torch.zeros(1, 1), 64)
 
 
+# ---- calls beside each other, and the ends of the ranges --------------------------------------
+
+
+def test_append_of_one_position_by_two_tokens():
+    say("append: a position given twice")
+    table, k, v, errors, x = append_state()
+    cache = ops.PagedCache(k, v, table.cuda(), int32([0] * 4).cuda(), errors)
+    ops.paged_append(cache, None, None, x[:, 6:8], x[:, 8:], int32([5, 5, 5, 6]).cuda(), rows=int32([1, 1, 1, 1]).cuda())
+    for pages, new in ((k, x[:3, 6:8]), (v, x[:3, 8:])):
+        got = pages[int(table[1, 0])]
+        assert bool((got[5][None] == new).any(0).all()) and int((pages != 0).any(-1).sum()) == 2 * 2
+    assert torch.equal(k[int(table[1, 0]), 6], x[3, 6:8]) and int(errors) == 0
+
+
+def test_two_calls_at_once():
+    """Two streams, a workspace each: attention, select and fork of different sizes beside each other."""
+    say("two streams with a workspace each")
+    g = seeded(21)
+    sides = []
+    for rows, most, vocab in ((9, 3000, 40000), (33, 400, 151936)):
+        lengths = torch.randint(0, most, (rows,), generator=g).tolist()
+        table, pages = tables_for(g, lengths, 16, -(-most // 16))
+        k, v = (normal(g, (pages, 16, 2, 64), F32).cuda() for _ in range(2))
+        refs = torch.bincount(table[table >= 0].long(), minlength=pages).to(torch.int32)
+        refs = torch.cat([refs, torch.zeros(3 * rows, dtype=torch.int32)]).cuda()
+        more = torch.zeros((refs.numel(), 16, 2, 64), device="cuda")
+        sides.append(dict(
+            stream=torch.cuda.Stream(), cache=ops.PagedCache(k, v, table.cuda(), int32(lengths).cuda()),
+            q=normal(g, (rows, 14, 64), F32).cuda(), out=torch.empty((rows, 14, 64), device="cuda"),
+            logits=normal(g, (1, 8, vocab), F32, 3.0).cuda(), scores=torch.zeros(1, 8, device="cuda"),
+            best=[torch.empty((1, 8), device="cuda")] + [torch.empty((1, 8), dtype=torch.int32, device="cuda") for _ in range(2)],
+            refs=refs, start=refs.clone(), pool=ops.PagePool(refs, 16, [more], planes=False),
+            parents=torch.randint(0, rows, (rows,), generator=g).to(torch.int32).cuda(),
+            table=torch.empty_like(table.cuda()), lengths=torch.empty(rows, dtype=torch.int32, device="cuda"),
+            work=ops.Workspace(max(ops.attention_workspace(rows, 14, 2, 64), ops.select_workspace(1, 8, 8, vocab),
+                                   ops.fork_workspace(rows, refs.numel())))))
+
+    def calls(s):
+        at = s["stream"].cuda_stream
+        ops.paged_attention(s["cache"], s["out"], s["q"], s["work"], stream=at)
+        ops.beam_select(s["logits"], s["scores"], *s["best"], s["work"], stream=at)
+        with torch.cuda.stream(s["stream"]):
+            s["refs"].copy_(s["start"])
+        ops.pages_fork(s["pool"], s["cache"].tensors[2], s["cache"].tensors[3], s["parents"], 1, s["table"], s["lengths"],
+                       s["work"], stream=at)
+        with torch.cuda.stream(s["stream"]):
+            return [x.clone() for x in (s["out"], *s["best"], s["table"], s["lengths"], s["refs"])]
+
+    torch.cuda.synchronize()
+    want = []
+    for s in sides:
+        want.append(calls(s))
+        torch.cuda.synchronize()
+    got = [[calls(s) for s in sides] for _ in range(20)]
+    torch.cuda.synchronize()
+    for turn in got:
+        assert all(torch.equal(a, b) for mine, right in zip(turn, want) for a, b in zip(mine, right))
+
+
+def test_two_graphs_share_a_workspace():
+    """Replayed in turn on one stream, with eager calls on the same workspace between them."""
+    say("two graphs, one workspace")
+    g = seeded(22)
+    work, graphs = ops.Workspace(max(ops.attention_workspace(40, 14, 2, 64), ops.select_workspace(2, 16, 16, 50000))), []
+    for rows, most, groups in ((40, 700, 1), (3, 6000, 2)):
+        lengths = torch.randint(0, most, (rows,), generator=g).tolist()
+        table, pages = tables_for(g, lengths, 32, -(-most // 32))
+        cache = ops.PagedCache(*(normal(g, (pages, 32, 2, 64), F32).cuda() for _ in range(2)), table.cuda(), int32(lengths).cuda())
+        q, logits = normal(g, (rows, 14, 64), F32).cuda(), normal(g, (groups, 16, 50000), F32, 3.0).cuda()
+        scores = torch.zeros(groups, 16, device="cuda")
+        results = [torch.empty_like(q), torch.empty_like(scores)] + [torch.empty((groups, 16), dtype=torch.int32, device="cuda")
+                                                                    for _ in range(2)]
+
+        def calls(stream=0, a=(cache, results, q, logits, scores)):
+            ops.paged_attention(a[0], a[1][0], a[2], work, stream=stream)
+            ops.beam_select(a[3], a[4], *a[1][1:], work, stream=stream)
+
+        calls()
+        torch.cuda.synchronize()
+        want = [x.clone() for x in results]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            calls(torch.cuda.current_stream().cuda_stream)
+        graphs.append((graph, calls, results, want))
+    for turn in range(5):
+        for graph, _, results, _ in graphs:
+            for x in results:
+                x.fill_(-1)
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, calls, results, want in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(results, want)), turn
+            calls()  # eager work between the replays
+        torch.cuda.synchronize()
+
+
+def test_attention_of_more_rows_than_counters():
+    """Past 65,536 pairs of a row and a KV head no row is cut into pieces."""
+    say("attention of 40,000 rows")
+    g, rows, page = seeded(23), 40000, 16
+    lengths = torch.randint(0, 49, (rows,), generator=g)
+    table = torch.randint(0, 64, (rows, 3), generator=g).to(torch.int32)
+    k, v = (normal(g, (64, page, 2, 64), F32) for _ in range(2))
+    q = normal(g, (rows, 2, 64), F32, 1.5)
+    cache = ops.PagedCache(k.cuda(), v.cuda(), table.cuda(), lengths.to(torch.int32).cuda())
+    out = torch.empty((rows, 2, 64), device="cuda")
+    ops.paged_attention(cache, out, q.cuda(), ops.Workspace(ops.attention_workspace(rows, 2, 2, 64)))
+    for low in range(0, rows, 5000):
+        part = slice(low, low + 5000)
+        at = table[part].long()
+        keys, values = (x.double()[at].reshape(-1, 48, 2, 64) for x in (k, v))
+        s = (q[part].double()[:, None] * keys).sum(-1) * 64 ** -0.5
+        inside = torch.arange(48)[None, :, None] < lengths[part][:, None, None]
+        p = torch.softmax(s.masked_fill(~inside, -math.inf), 1).nan_to_num(0.0)
+        want = (p[..., None] * values).sum(1)
+        # Scores below 60 in magnitude from 64 products, 2^-24 of their sum of magnitudes (at most 64 x 8 x 4 / 8):
+        # 256 x 64 x 2^-24 = 1e-3 were all roundings of one sign; a tenth of it holds with room.
+        assert float((out[part].cpu().double() - want).abs().max()) < 1e-4
+    assert not out[(lengths == 0).cuda()].any()
+
+
+def test_fork_of_the_most_rows():
+    say("fork of 1,024 rows")
+    s = Forked(1024, 6000, 5, 16, planes=1)
+    rng = random.Random(9)
+    s.step(None, 20)
+    for append in (1, 13, 0):
+        s.step([rng.randrange(-1, 1024) for _ in range(1024)], append)
+
+
+def test_fork_copies_memories_of_different_sizes():
+    """Pages of one piece and of several with a rest, in planes of different numbers."""
+    say("fork: memories of 512 bytes, 16,400 and 49,152")
+    page, pages = 16, 12
+    g = seeded(5)
+    memories = [normal(g, (n, pages, page, w), F32) for n, w in ((1, 8), (3, 256 + 4), (2, 768))]
+    memories[1] = memories[1].flatten(2)[:, :, :4100].contiguous()
+    on = [m.cuda() for m in memories]
+    table, lengths, refs = int32([[3, 5, -1], [3, 5, -1], [3, 5, -1]]).cuda(), int32([20, 20, 20]).cuda(), int32([0] * pages)
+    refs[3] = refs[5] = 3
+    refs = refs.cuda()
+    after, more = torch.empty_like(table), torch.empty_like(lengths)
+    ops.pages_fork(ops.PagePool(refs, page, on), table, lengths, None, 1, after, more, ops.Workspace(ops.fork_workspace(3, pages)))
+    assert after.tolist() == [[3, 5, -1], [3, 0, -1], [3, 1, -1]] and more.tolist() == [21] * 3
+    assert refs.tolist() == [1, 1, 0, 3, 0, 1, 0, 0, 0, 0, 0, 0]
+    for d, m in zip(on, memories):
+        m[:, 0] = m[:, 1] = m[:, 5]
+        assert torch.equal(d.cpu(), m)
+
+
+def test_select_of_the_largest_vocabulary():
+    say("select of 2^24 tokens")
+    g = seeded(24)
+    check_select(normal(g, (1, 2, 1 << 24), BF16, 3.0), torch.tensor([[-1.0, -1.5]]), 64)
+
+
 # ---- together -----------------------------------------------------------------------------
 
 

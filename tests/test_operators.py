@@ -72,7 +72,7 @@ def fork(memory=None, **changes):
 
 
 def select(**changes):
-    a = dict(logits=AT, group_stride=4000, beam_stride=1000, scores=AT, done=None, scores_out=AT, parents=AT, tokens=AT,
+    a = dict(logits=AT, group_stride=4000, beam_stride=1000, scores=AT, done=None, scores_out=2 * AT, parents=AT, tokens=AT,
              done_out=None, dtype=qd.DTYPE_F32, groups=2, beams=4, vocab=1000, k=4, eos=0, device=0)
     a.update(changes)
     return ops.SelectStruct(**a)
@@ -123,6 +123,8 @@ def test_cache_refusals(status, changes):
     (qd.INVALID_ARGUMENT, dict(q_out_stride=64)),
     (qd.INVALID_ARGUMENT, dict(v_stride=-128)),
     (qd.NOT_SUPPORTED, dict(tokens=1 << 30)),
+    (qd.NOT_SUPPORTED, dict(q=None, q_out=None, tokens=1 << 26)),  # half of each token's wave idles: 2^32 threads
+    (qd.INVALID_ARGUMENT, dict(q_out=AT, q_stride=18 * 64)),  # in place, at another stride
 ])
 def test_append_refusals(status, changes):
     refused(status, "qd_paged_append", cache(), append(**changes), None)
@@ -137,6 +139,8 @@ def test_append_refusals(status, changes):
     (qd.INVALID_ARGUMENT, dict(scale=math.inf)),
     (qd.INVALID_ARGUMENT, dict(q_head_stride=66)),
     (qd.INVALID_ARGUMENT, dict(out_head_stride=0)),
+    (qd.INVALID_ARGUMENT, dict(out_stride=18 * 64)),  # in place, at other strides
+    (qd.INVALID_ARGUMENT, dict(out_head_stride=128)),
     (qd.INVALID_ARGUMENT, dict()),  # no workspace
 ])
 def test_attention_refusals(status, changes):
@@ -177,12 +181,19 @@ def test_fork_refusals(status, changes, memory):
     (qd.INVALID_ARGUMENT, dict(scores=None)),
     (qd.INVALID_ARGUMENT, dict(logits=AT + 2)),
     (qd.INVALID_ARGUMENT, dict(done=AT)),
-    (qd.INVALID_ARGUMENT, dict(done=AT, done_out=AT, eos=1000)),
+    (qd.INVALID_ARGUMENT, dict(done=AT, done_out=2 * AT, eos=1000)),
+    (qd.INVALID_ARGUMENT, dict(done=AT, done_out=AT)),
+    (qd.INVALID_ARGUMENT, dict(scores_out=AT)),
     (qd.INVALID_ARGUMENT, dict(beam_stride=-1)),
     (qd.INVALID_ARGUMENT, dict()),  # no workspace
 ])
 def test_select_refusals(status, changes):
     refused(status, "qd_beam_select", select(**changes), None, None)
+
+
+def test_more_workgroups_than_a_grid_has_are_refused():
+    refused(qd.NOT_SUPPORTED, "qd_paged_attention", cache(rows=1 << 20, kv_heads=16, token_stride=1024, page_stride=16384),
+            attention(heads=16, q_stride=1024, out_stride=1024), None, None)
 
 
 def test_null_arguments_are_refused():
@@ -214,6 +225,23 @@ def test_without_a_gpu_calls_fail_loudly():
         ops.Workspace(1024)
     assert e.value.status == qd.NOT_SUPPORTED
     refused(qd.NOT_SUPPORTED, "qd_paged_append", cache(), append(), None)
+
+
+def test_numbers_that_the_structures_would_cut_are_refused():
+    import torch
+
+    k = torch.zeros(4, 16, 2, 64)
+    table, lengths = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    c = ops.PagedCache(k, k, table, lengths)
+    for bias in (2 ** 31, -2 ** 31 - 1, 2 ** 32):
+        with pytest.raises(qd.QdError, match="position_bias"):
+            ops.paged_append(c, None, None, k[0, :1], k[0, :1], lengths, position_bias=bias)
+    for t in (k[:, :0], k[None][:0]):
+        with pytest.raises(qd.QdError):
+            ops.PagePool(torch.zeros(4, dtype=torch.int32), 16, [t], planes=t.dim() == 5)
+    for dim, positions in ((-2, 4), (64, -1)):
+        with pytest.raises(qd.QdError):
+            ops.rope_table(1e4, dim, positions)
 
 
 def test_cpu_tensors_are_refused():
