@@ -239,6 +239,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 constexpr int kTile = 32, kSub = 16;
 constexpr uint32_t kMostPieces = 256;  // of an item
 constexpr int kWaves = 4;              // of a workgroup
+constexpr uint32_t kEdge = 2;          // tiles that an item's results cost the long kernel as much time as
 // The short kernel: tiles of a piece at least, of an item that stays whole, and
 // pieces of an item at most.
 constexpr uint32_t kShortLeast = 4, kShortWhole = 8, kShortPieces = 64;
@@ -300,14 +301,15 @@ struct PageRows {
 struct Item {
   int row, length;
   uint32_t part;
-  uint32_t at, tiles;        // its first tile among all, and how many it has (one at least)
+  uint32_t at, tiles;        // its first tile among all in the deal, and how many it has (one at least)
   uint32_t first, last;      // the run
   uint32_t home, pieces;     // the workgroup of its first piece, and how many there are
   bool bad;                  // the row's length
 };
 
 // The runs of all workgroups: run i is [i share, (i + 1) share) of all tiles, but
-// for the cuts that move.
+// for the cuts that move. Before its tiles each item has kEdge more that stand for
+// the time that its results take.
 struct Deal {
   uint32_t share, total;
 };
@@ -338,7 +340,7 @@ __device__ __forceinline__ void set_item(const AttnLaunch &p, const Deal &d, Ite
                                          uint32_t at, int32_t n, int64_t most) {
   it.row = static_cast<int>(row);
   it.part = part;
-  it.at = at;
+  it.at = at + kEdge;
   it.bad = n < 0 || n > most;
   it.length = it.bad ? 0 : n;
   it.tiles = tiles_of(p, n, most);
@@ -347,7 +349,7 @@ __device__ __forceinline__ void set_item(const AttnLaunch &p, const Deal &d, Ite
   it.home = 0;
   it.pieces = 1;
   if (p.least && it.tiles >= 2 * p.least) {
-    const uint32_t lo = (at + p.least + d.share - 1) / d.share, hi = (at + it.tiles - p.least) / d.share;
+    const uint32_t lo = (it.at + p.least + d.share - 1) / d.share, hi = (it.at + it.tiles - p.least) / d.share;
     if (hi >= lo) {
       it.pieces = hi - lo + 2;
       it.home = lo - 1;
@@ -384,7 +386,7 @@ __device__ __forceinline__ bool first_item(const AttnLaunch &p, uint32_t i, uint
   int32_t n = 0;  // of the row looked at last
   for (uint32_t r = lane; r < p.c.rows; r += kWave) {
     n = p.c.lengths[r];
-    const uint32_t tiles = tiles_of(p, n, most);
+    const uint32_t tiles = tiles_of(p, n, most) + kEdge;
     total += tiles;
     longest = max(longest, tiles);
   }
@@ -402,7 +404,7 @@ __device__ __forceinline__ bool first_item(const AttnLaunch &p, uint32_t i, uint
   for (;;) {
     if (!once) {
       n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
-      upto = lanes_upto(base + lane < p.c.rows ? tiles_of(p, n, most) : 0u);
+      upto = lanes_upto(base + lane < p.c.rows ? tiles_of(p, n, most) + kEdge : 0u);
     }
     past = __ballot(before + upto * p.parts > begin);
     if (past) break;
@@ -411,18 +413,18 @@ __device__ __forceinline__ bool first_item(const AttnLaunch &p, uint32_t i, uint
   }
   const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
   const int32_t length = __builtin_amdgcn_readlane(n, at);
-  const uint32_t tiles = tiles_of(p, length, most), row = base + at;
-  before += (__builtin_amdgcn_readlane(upto, at) - tiles) * p.parts;
-  const uint32_t part = (begin - before) / tiles, off = begin - before - part * tiles;
-  const int cut = off ? cut_of(p, off, tiles) : 0;
+  const uint32_t tiles = tiles_of(p, length, most), each = tiles + kEdge, row = base + at;
+  before += (__builtin_amdgcn_readlane(upto, at) - each) * p.parts;
+  const uint32_t part = (begin - before) / each, in = begin - before - part * each;
+  const int cut = in > kEdge ? cut_of(p, in - kEdge, tiles) : 0;
   if (cut < 2) {
-    set_item(p, d, it, row, part, before + part * tiles, length, most);
-    if (cut == 1) it.first = off;
+    set_item(p, d, it, row, part, before + part * each, length, most);
+    if (cut == 1) it.first = in - kEdge;
   } else if (part + 1 < p.parts) {  // from the next item on
-    set_item(p, d, it, row, part + 1, before + (part + 1) * tiles, length, most);
+    set_item(p, d, it, row, part + 1, before + (part + 1) * each, length, most);
   } else {
     if (row + 1 >= p.c.rows) return false;
-    set_item(p, d, it, row + 1, 0, before + (part + 1) * tiles, load_uniform(p.c.lengths + row + 1), most);
+    set_item(p, d, it, row + 1, 0, before + (part + 1) * each, load_uniform(p.c.lengths + row + 1), most);
   }
   return end_run(p, d, i, it);
 }
