@@ -101,7 +101,7 @@ struct Shared {
   double sum[kWavesPerBlock];
   float top[kWavesPerBlock];
   uint32_t bound[kWavesPerBlock], count[kWavesPerBlock];
-  uint32_t n, last;
+  uint32_t n, last, found;
 };
 // The joins' keys and their places, where the waves' keys were.
 static_assert(sizeof(Shared::own) + sizeof(Shared::best) >= kJoin * (sizeof(uint64_t) + sizeof(uint16_t)), "the joins' lists");
@@ -192,15 +192,46 @@ __device__ __forceinline__ uint32_t wave_best(uint64_t *list, uint32_t n, uint32
   return left;
 }
 
+// What a group's results say: places of its best continuations found so far, for
+// those that go to others.
+struct Places {
+  uint32_t beam[kSelectK], token[kSelectK];
+  uint8_t taken[2 * kSelectK];
+};
+__device__ __forceinline__ void put_result(const SelectLaunch &p, uint32_t group, uint32_t i, double score, uint32_t beam,
+                                           uint32_t token, bool was_done) {
+  const size_t at = static_cast<size_t>(group) * p.a.k + i;
+  p.a.scores_out[at] = static_cast<float>(score);
+  p.a.parents[at] = static_cast<int32_t>(group * p.a.beams + beam);
+  p.a.tokens[at] = static_cast<int32_t>(token);
+  if (p.a.done) p.a.done_out[at] = was_done || token == p.a.eos;
+}
+// The places behind the first `found` go to the lowest (beam, token) that have none.
+template <typename Done>
+__device__ void fill_places(const SelectLaunch &p, uint32_t group, uint32_t found, Places &sh, Done was_done) {
+  __syncthreads();
+  const uint64_t all = static_cast<uint64_t>(p.a.beams) * p.a.vocab;
+  const uint32_t t = threadIdx.x;
+  if (t < 2 * kSelectK) {
+    bool is = t >= all;
+    for (uint32_t j = 0; j < found; ++j) is |= sh.beam[j] == t / p.a.vocab && sh.token[j] == t % p.a.vocab;
+    sh.taken[t] = is;
+  }
+  __syncthreads();
+  if (t < 2 * kSelectK && !sh.taken[t]) {
+    uint32_t at = found;
+    for (uint32_t j = 0; j < t; ++j) at += !sh.taken[j];
+    if (at < p.a.k) put_result(p, group, at, -INFINITY, t / p.a.vocab, t % p.a.vocab, was_done(t / p.a.vocab));
+  }
+}
+
 // Chooses among a group's rows; called by the workgroup that arrives last.
-__device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh) {
+__device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh, Places &places) {
   constexpr int kMine = kSelectBeams * kSelectK / kT;
   const uint32_t k = p.a.k, n = p.a.beams * k;
   const uint32_t row0 = group * p.a.beams;
   const Coherent scores(p.row_score + static_cast<size_t>(row0) * k, n * 8);
   const Coherent tokens(p.row_token + static_cast<size_t>(row0) * k, n * 4);
-  __shared__ uint32_t flat_beam[kSelectK], flat_token[kSelectK];
-  __shared__ uint8_t taken[2 * kSelectK];
   uint64_t *list = &sh.own[0][0];
   uint16_t *place = reinterpret_cast<uint16_t *>(list + kJoin);
   __shared__ uint8_t was_done[kSelectBeams];
@@ -253,13 +284,6 @@ __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh) {
   }
   __syncthreads();
   const uint32_t count = sh.n, found = min(count, k);
-  auto put = [&](uint32_t i, double score, uint32_t beam, uint32_t tok) {
-    const size_t at = static_cast<size_t>(group) * k + i;
-    p.a.scores_out[at] = static_cast<float>(score);
-    p.a.parents[at] = static_cast<int32_t>(row0 + beam);
-    p.a.tokens[at] = static_cast<int32_t>(tok);
-    if (p.a.done) p.a.done_out[at] = was_done[beam] || tok == p.a.eos;
-  };
   // Four lanes find an entry's rank: higher scores, and equal ones of lower places.
   for (uint32_t i = threadIdx.x / 4; i < count; i += kT / 4) {
     const uint64_t it = list[i];
@@ -281,30 +305,16 @@ __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh) {
     if (rank >= k || (threadIdx.x & 3)) continue;
     const uint64_t bits = it >> 63 ? it & ~(1ull << 63) : ~it;
     const uint32_t tok = held[at];
-    put(rank, __longlong_as_double(static_cast<long long>(bits)), at / k, tok);
-    flat_beam[rank] = at / k;
-    flat_token[rank] = tok;
+    put_result(p, group, rank, __longlong_as_double(static_cast<long long>(bits)), at / k, tok, p.a.done && was_done[at / k]);
+    places.beam[rank] = at / k;
+    places.token[rank] = tok;
   }
-  if (found == k) return;
-  // The places left go to the lowest (beam, token) that have none.
-  __syncthreads();
-  const uint64_t all = static_cast<uint64_t>(p.a.beams) * p.a.vocab;
-  const uint32_t t = threadIdx.x;
-  if (t < 2 * kSelectK) {
-    bool is = t >= all;
-    for (uint32_t j = 0; j < found; ++j) is |= flat_beam[j] == t / p.a.vocab && flat_token[j] == t % p.a.vocab;
-    taken[t] = is;
-  }
-  __syncthreads();
-  if (t < 2 * kSelectK && !taken[t]) {
-    uint32_t at = found;
-    for (uint32_t j = 0; j < t; ++j) at += !taken[j];
-    if (at < k) put(at, -INFINITY, t / p.a.vocab, t % p.a.vocab);
-  }
+  if (found < k) fill_places(p, group, found, places, [&](uint32_t beam) { return p.a.done && was_done[beam]; });
 }
 
-// Joins a row's runs; called by the workgroup that arrives last.
-__device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
+// Joins a row's runs; called by the workgroup that arrives last. The row of a group
+// of one is the group's result.
+__device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh, Places &places) {
   constexpr int kMine = kJoin / 2 / kT;
   const uint32_t k = p.a.k, n = p.runs * k;
   const Coherent keys(p.keys + static_cast<size_t>(row) * (n + (n & 1)), (n + (n & 1)) * 8);
@@ -312,13 +322,17 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
   const Coherent maxima(p.maxima + static_cast<size_t>(row) * p.runs, p.runs * 4);
   const Coherent scores(p.row_score + static_cast<size_t>(row) * k, k * 8);
   const Coherent tokens(p.row_token + static_cast<size_t>(row) * k, k * 4);
-  // Two keys a load, all of them on their way before the first is used.
+  // Two keys a load, all of them on their way before the first is used. (An even k:
+  // the runs' best pairs first, so that the first wave's bound is a near one.)
+  const uint32_t depth = k & 1 ? 1 : k / 2, across = k & 1 ? (n + 1) / 2 : p.runs;
+  const float per = __builtin_amdgcn_rcpf(static_cast<float>(across));  // (below 1,024: exact where it is rounded down)
   uint64_t key[2 * kMine];
 #pragma unroll
   for (int u = 0; u < kMine; ++u) {
     key[2 * u] = key[2 * u + 1] = 0;
     if (2 * u * kT < n) {
-      const float4 v = keys.ld4(u * kT + threadIdx.x);
+      const uint32_t i = u * kT + threadIdx.x, down = static_cast<uint32_t>((static_cast<float>(i) + 0.5f) * per);
+      const float4 v = keys.ld4((i - down * across) * depth + down);  // (past the end: zeros)
       const uint2 a = {__float_as_uint(v.x), __float_as_uint(v.y)}, b = {__float_as_uint(v.z), __float_as_uint(v.w)};
       key[2 * u] = a.x | static_cast<uint64_t>(a.y) << 32;
       key[2 * u + 1] = b.x | static_cast<uint64_t>(b.y) << 32;
@@ -339,7 +353,8 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
   uint32_t best = 0;
 #pragma unroll
   for (int u = 0; u < 2 * kMine; ++u) {
-    // (A row of an odd number of keys ends with half of a load.)
+    // (Indexes past the end come to others' pairs, and an odd number of keys ends
+    // with half of a load.)
     if (2 * ((u >> 1) * kT + threadIdx.x) + (u & 1) >= n) key[u] = 0;
     best = max(best, static_cast<uint32_t>(key[u] >> 32));
   }
@@ -349,7 +364,7 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
     sh.top[wave_id()] = wave_m;
     sh.bound[wave_id()] = bound;
   }
-  if (threadIdx.x == 0) sh.n = 0;
+  if (threadIdx.x == 0) sh.n = sh.found = 0;
   __syncthreads();
   float top = sh.top[0];
   uint32_t least = max(kLowest, sh.bound[0]);
@@ -375,6 +390,7 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
   const uint32_t count = sh.n;
   const double log_total = log((sh.sum[0] + sh.sum[1]) + (sh.sum[2] + sh.sum[3]));
   const double base = static_cast<double>(p.a.scores[row]);
+  const bool alone = p.a.beams == 1;
   for (uint32_t i = threadIdx.x / 4; i < max(count, k); i += kT / 4) {
     const uint64_t it = i < count ? list[i] : 0;
     const uint32_t rank = i < count ? quad_rank(it, list, count) : i;
@@ -383,13 +399,23 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh) {
     // (An infinite maximum leaves the others nothing.)
     const double s =
         i >= count ? -INFINITY : base + ((x == top ? 0.0 : static_cast<double>(x) - top) - log_total);
-    store64(scores, rank, static_cast<uint64_t>(__double_as_longlong(s)));
-    tokens.stu(rank, token_of(it));
+    if (!alone) {
+      store64(scores, rank, static_cast<uint64_t>(__double_as_longlong(s)));
+      tokens.stu(rank, token_of(it));
+    } else if (s > -INFINITY) {
+      put_result(p, row, rank, s, 0, token_of(it), false);
+      places.beam[rank] = 0;
+      places.token[rank] = token_of(it);
+      atomicAdd(&sh.found, 1u);
+    }
   }
+  if (!alone) return;
+  __syncthreads();
+  if (sh.found < k) fill_places(p, row, sh.found, places, [](uint32_t) { return false; });
 }
 
 // What is left of a row's way once its scores are stored.
-__device__ __forceinline__ void row_done(const SelectLaunch &p, uint32_t row, Shared &sh) {
+__device__ __forceinline__ void row_done(const SelectLaunch &p, uint32_t row, Shared &sh, Places &places) {
   const uint32_t group = row / p.a.beams;
   wait_vm_stores();
   __syncthreads();
@@ -398,7 +424,7 @@ __device__ __forceinline__ void row_done(const SelectLaunch &p, uint32_t row, Sh
     if (sh.last && p.a.beams > 1) p.group_count[group * p.apart] = 0u;
   }
   __syncthreads();
-  if (sh.last) choose(p, group, sh);
+  if (sh.last) choose(p, group, sh, places);
 }
 
 template <typename E>
@@ -407,6 +433,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   constexpr int kPieces = kEach / P::kElems;
   static_assert(kOwn >= static_cast<int>(kSelectK) + kWave * P::kElems, "a piece fits behind k keys");
   __shared__ __attribute__((aligned(16))) Shared sh;
+  __shared__ Places places;
   const uint32_t row = blockIdx.y, run = blockIdx.x, k = p.a.k;
   const E *logits = static_cast<const E *>(p.a.logits) + static_cast<int64_t>(row / p.a.beams) * p.a.group_stride +
                     static_cast<int64_t>(row % p.a.beams) * p.a.beam_stride;
@@ -438,7 +465,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
       store64(scores, i, static_cast<uint64_t>(__double_as_longlong(s)));
       tokens.stu(i, p.a.eos);
     }
-    row_done(p, row, sh);
+    row_done(p, row, sh, places);
     return;
   }
   uint64_t *own = sh.own[w];
@@ -589,8 +616,8 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   }
   __syncthreads();
   if (!sh.last) return;
-  join_row(p, row, sh);
-  row_done(p, row, sh);
+  join_row(p, row, sh, places);
+  if (p.a.beams > 1) row_done(p, row, sh, places);
 }
 
 // A row's runs: as many as make kAim workgroups (four fit a CU), no more than it

@@ -606,6 +606,21 @@ def test_select_masks():
     check_select(logits[:, :, :2], scores, 6, done, 1)  # as many places as continuations
 
 
+@pytest.mark.parametrize("k", [1, 5, 64])
+def test_select_of_one_beam(k):
+    """A group of one beam: its row is the result, places left go to the lowest tokens."""
+    say("select: one beam,", k)
+    vocab = 9001
+    logits = normal(seeded(3), (7, 1, vocab), F32)
+    logits[1] = -math.inf                              # no token
+    logits[2, 0, 3:] = -math.inf                       # fewer than places
+    logits[3, 0, [2, 8999]] = math.inf                 # the others' share is nothing
+    logits[4, 0, 1:4500] = NAN
+    scores = torch.tensor([[0.0], [-1.0], [-2.0], [-3.0], [-4.0], [-math.inf], [-5.0]])
+    check_select(logits, scores, k)
+    check_select(logits, scores, k, torch.tensor([[0], [0], [0], [0], [0], [0], [1]]), 2)
+
+
 def test_select_infinite_logits():
     say("select: infinite logits")
     logits = torch.zeros(1, 2, 3000)
