@@ -13,6 +13,7 @@ this module, before the first call into the engine's library.
 from __future__ import annotations
 
 import ctypes as C
+import os
 import sys
 
 import numpy as np
@@ -24,6 +25,11 @@ if qd._lib is not None and "torch" not in sys.modules:
     raise ImportError("the engine's library is loaded with another HIP runtime than torch's: "
                       "import torch or qd_operators before the first call of qwen_decode")
 import torch  # noqa: E402
+
+try:
+    import _qd_tensors  # noqa: E402  (it links to torch's libraries, which are loaded now)
+except ImportError as e:
+    raise ImportError(f"the operators' binding is not built: make -C {os.path.dirname(os.path.abspath(__file__))}") from e
 
 BAD_LENGTH, BAD_PAGE, BAD_POSITION, BAD_ROW, EXHAUSTED = 1, 2, 4, 8, 16
 
@@ -37,34 +43,9 @@ class CacheStruct(C.Structure):
                 ("dtype", _U32), ("device", _I32)]
 
 
-class AppendStruct(C.Structure):
-    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_out", _P), ("q_stride", _I64), ("k_stride", _I64),
-                ("v_stride", _I64), ("q_out_stride", _I64), ("positions", _P), ("rows", _P), ("position_bias", _I32),
-                ("tokens", _U32), ("heads", _U32), ("rotary_dim", _U32), ("interleaved", _U32),
-                ("table_positions", _U32), ("cos_table", _P), ("sin_table", _P)]
-
-
-class AttentionStruct(C.Structure):
-    _fields_ = [("q", _P), ("out", _P), ("q_stride", _I64), ("q_head_stride", _I64), ("out_stride", _I64),
-                ("out_head_stride", _I64), ("heads", _U32), ("scale", C.c_float)]
-
-
 class MemoryStruct(C.Structure):
     _fields_ = [("base", _P), ("plane_stride", _I64), ("page_stride", _I64), ("bytes", C.c_uint64), ("planes", _U32),
                 ("reserved", _U32)]
-
-
-class ForkStruct(C.Structure):
-    _fields_ = [("table", _P), ("lengths", _P), ("parents", _P), ("table_out", _P), ("lengths_out", _P), ("refs", _P),
-                ("table_stride", _I64), ("table_out_stride", _I64), ("errors", _P), ("memories", C.POINTER(MemoryStruct)),
-                ("memory_count", _U32), ("rows", _U32), ("table_width", _U32), ("pages", _U32), ("page_size", _U32),
-                ("append", _U32), ("device", _I32)]
-
-
-class SelectStruct(C.Structure):
-    _fields_ = [("logits", _P), ("group_stride", _I64), ("beam_stride", _I64), ("scores", _P), ("done", _P),
-                ("scores_out", _P), ("parents", _P), ("tokens", _P), ("done_out", _P), ("dtype", _U32), ("groups", _U32),
-                ("beams", _U32), ("vocab", _U32), ("k", _U32), ("eos", _U32), ("device", _I32)]
 
 
 _SIZE = C.POINTER(C.c_size_t)
@@ -73,12 +54,12 @@ _SIGNATURES = {
     "qd_workspace_destroy": [_P],
     "qd_rope_table": [C.c_double, _U32, _U32, C.c_double, _U32, C.c_double, C.c_double, C.POINTER(C.c_float),
                       C.POINTER(C.c_float)],
-    "qd_paged_append": [C.POINTER(CacheStruct), C.POINTER(AppendStruct), _P],
-    "qd_paged_attention": [C.POINTER(CacheStruct), C.POINTER(AttentionStruct), _P, _P],
+    "qd_paged_append": [_P, _P, _P],
+    "qd_paged_attention": [_P, _P, _P, _P],
     "qd_paged_attention_workspace": [_U32, _U32, _U32, _U32, _SIZE],
-    "qd_pages_fork": [C.POINTER(ForkStruct), _P, _P],
+    "qd_pages_fork": [_P, _P, _P],
     "qd_pages_fork_workspace": [_U32, _U32, _SIZE],
-    "qd_beam_select": [C.POINTER(SelectStruct), _P, _P],
+    "qd_beam_select": [_P, _P, _P],
     "qd_beam_select_workspace": [_U32, _U32, _U32, _U32, _SIZE],
 }
 
@@ -94,6 +75,8 @@ def lib():
             fn = getattr(handle, name)
             fn.restype = C.c_int
             fn.argtypes = args
+        _qd_tensors.bind(*(C.cast(getattr(handle, name), _P).value for name in (
+            "qd_paged_append", "qd_paged_attention", "qd_pages_fork", "qd_beam_select")))
         _lib = handle
     return _lib
 
@@ -103,12 +86,17 @@ def _check(status):
         raise QdError(status, _lib.qd_last_error().decode(errors="replace"))
 
 
-# ---- what a tensor is -----------------------------------------------------------------
-# A call takes a few microseconds on the device, so each tensor is looked at once, in few steps:
-# _take and _flat return its address if it is as it has to be and say what is wrong if not.
+def _answer(r):
+    """Raises what a call of the binding returned: a status, or what is wrong with an argument."""
+    if isinstance(r, int):
+        _check(r)
+    raise QdError(qd.INVALID_ARGUMENT, r)
+
+
+# ---- what the calls take ----------------------------------------------------------------
+# A call's tensors are checked in the binding (csrc/qd_tensors.cpp); what is made once, here.
 
 _TYPES = {torch.float32: qd.DTYPE_F32, torch.bfloat16: qd.DTYPE_BF16, torch.float16: qd.DTYPE_F16}
-_F32, _I32T, _U8T = torch.float32, torch.int32, torch.uint8
 
 
 def _refuse(text):
@@ -121,7 +109,9 @@ def _dims(name, t, n):
     return t.shape
 
 
-def _wrong(name, t, dtype, shape, device):
+def _take(name, t, dtype, shape, device, together=False):
+    """Address and strides of a tensor of this type, shape and device; contiguous are its last dimension
+    or, `together`, all."""
     if t is None:
         _refuse(f"{name} is missing")
     if t.shape != shape:
@@ -130,23 +120,10 @@ def _wrong(name, t, dtype, shape, device):
         _refuse(f"{name} has type {t.dtype}, not {dtype}")
     if t.get_device() != device:
         _refuse(f"{name} is on {t.device}, not on device {device}")
-    _refuse(f"{name} is not contiguous where it has to be (strides {t.stride()})")
-
-
-def _take(name, t, dtype, shape, device):
-    """Address and strides of a tensor of this type, shape and device, its last dimension contiguous."""
-    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device:
-        s = t.stride()
-        if s[-1] == 1 or shape[-1] <= 1:
-            return t.data_ptr(), s
-    _wrong(name, t, dtype, shape, device)
-
-
-def _flat(name, t, dtype, shape, device):
-    """Address of a contiguous tensor of this type, shape and device."""
-    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device and t.is_contiguous():
-        return t.data_ptr()
-    _wrong(name, t, dtype, shape, device)
+    s = t.stride()
+    if not (t.is_contiguous() if together else s[-1] == 1 or shape[-1] <= 1):
+        _refuse(f"{name} is not contiguous where it has to be (strides {s})")
+    return t.data_ptr(), s
 
 
 def _bytes(call, *args):
@@ -172,13 +149,15 @@ class Workspace:
     same time (two streams, graphs on two streams) needs one each."""
 
     def __init__(self, nbytes, device=0):
-        self.handle = _P()
+        self.handle = 0
         self.nbytes, self.device = nbytes, device
-        _check(lib().qd_workspace_create(device, nbytes, C.byref(self.handle)))
+        handle = _P()
+        _check(lib().qd_workspace_create(device, nbytes, C.byref(handle)))
+        self.handle = handle.value
 
     def close(self):
         if self.handle:
-            handle, self.handle = self.handle, _P()
+            handle, self.handle = self.handle, 0
             _check(lib().qd_workspace_destroy(handle))
 
     def __del__(self):
@@ -205,22 +184,15 @@ class PagedCache:
             _refuse("k and v have different strides")
         # The stride of a dimension of one element is not used and may be anything.
         s = [n if k.shape[i] > 1 else head_dim for i, n in enumerate(s[:3])]
-        table_at, ts = _take("table", table, _I32T, (rows, width), device)
+        table_at, ts = _take("table", table, torch.int32, (rows, width), device)
         self.device, self.dtype, self.rows, self.kv_heads, self.head_dim = device, dtype, rows, kv_heads, head_dim
         self.c = CacheStruct(
             k_at, v_at, s[0], s[1], s[2], table_at, ts[0] if rows > 1 else width,
-            _flat("lengths", lengths, _I32T, (rows,), device),
-            None if errors is None else _flat("errors", errors, _I32T, (1,), device), rows, width, pages, page_size,
-            kv_heads, head_dim, _TYPES[dtype], device)
-
-
-def _tokens(name, t, dtype, shape, device):
-    """Address and stride from token to token of [tokens, heads, head_dim] whose heads lie together."""
-    if t is not None and t.shape == shape and t.dtype is dtype and t.get_device() == device:
-        s = t.stride()
-        if s[2] == 1 and (s[1] == shape[2] or shape[1] == 1):
-            return t.data_ptr(), s[0] if shape[0] > 1 else shape[1] * shape[2]
-    _wrong(name, t, dtype, shape, device)
+            _take("lengths", lengths, torch.int32, (rows,), device, True)[0],
+            None if errors is None else _take("errors", errors, torch.int32, (1,), device, True)[0], rows, width, pages,
+            page_size, kv_heads, head_dim, _TYPES[dtype], device)
+        self.at = C.addressof(self.c)
+        lib()
 
 
 def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None, interleaved=False, position_bias=0,
@@ -229,56 +201,17 @@ def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None
     pages. q, q_out [tokens, heads, head_dim] (both None: keys and values only), k, v
     [tokens, kv_heads, head_dim], positions and rows [tokens] int32, cos and sin
     [positions, rotary_dim / 2] FP32 (None: no rotation)."""
-    device, dtype, dim = cache.device, cache.dtype, cache.head_dim
-    tokens = 0 if k is None else len(k)
-    shape = (tokens, cache.kv_heads, dim)
-    k_at, k_stride = _tokens("k", k, dtype, shape, device)
-    v_at, v_stride = _tokens("v", v, dtype, shape, device)
-    q_at = out_at = None
-    q_stride = out_stride = heads = rotary = table_positions = 0
-    cos_at = sin_at = None
-    if q is not None and q_out is not None:
-        heads = _dims("q", q, 3)[1]
-        shape = (tokens, heads, dim)
-        q_at, q_stride = _tokens("q", q, dtype, shape, device)
-        out_at, out_stride = _tokens("q_out", q_out, dtype, shape, device)
-    elif q is not None or q_out is not None:
-        _refuse("q and q_out go together")
-    if cos is not None and sin is not None:
-        shape = _dims("cos", cos, 2)
-        cos_at, sin_at = _flat("cos", cos, _F32, shape, device), _flat("sin", sin, _F32, shape, device)
-        table_positions, rotary = shape[0], 2 * shape[1]
-    elif cos is not None or sin is not None:
-        _refuse("cos and sin go together")
-    if not -2 ** 31 <= position_bias < 2 ** 31:
-        _refuse(f"position_bias {position_bias} does not fit 32 bits")
-    shape = (tokens,)
-    status = lib().qd_paged_append(cache.c, AppendStruct(
-        q_at, k_at, v_at, out_at, q_stride, k_stride, v_stride, out_stride,
-        _flat("positions", positions, _I32T, shape, device),
-        None if rows is None else _flat("rows", rows, _I32T, shape, device), position_bias, tokens, heads, rotary,
-        1 if interleaved else 0, table_positions, cos_at, sin_at), stream)
-    if status:
-        _check(status)
+    r = _qd_tensors.append(cache.at, q_out, q, k, v, positions, rows, cos, sin, interleaved, position_bias, stream)
+    if r is not None:
+        _answer(r)
 
 
 def paged_attention(cache, out, q, workspace, scale=None, stream=0):
-    """Attention of one new token per cache row: q and out [rows, heads, head_dim]."""
-    device, dtype, dim, rows = cache.device, cache.dtype, cache.head_dim, cache.rows
-    heads = _dims("q", q, 3)[1]
-    shape = (rows, heads, dim)
-    q_at, qs = _take("q", q, dtype, shape, device)
-    out_at, os = _take("out", out, dtype, shape, device)
-    # (The stride of a dimension of one element is not used and may be anything.)
-    if rows == 1:
-        qs, os = (heads * dim, qs[1]), (heads * dim, os[1])
-    if heads == 1:
-        qs, os = (qs[0], dim), (os[0], dim)
-    status = lib().qd_paged_attention(
-        cache.c, AttentionStruct(q_at, out_at, qs[0], qs[1], os[0], os[1], heads, dim ** -0.5 if scale is None else scale),
-        workspace.handle, stream)
-    if status:
-        _check(status)
+    """Attention of one new token per cache row: q and out [rows, heads, head_dim]; scale None:
+    1 / sqrt(head_dim)."""
+    r = _qd_tensors.attention(cache.at, out, q, workspace.handle, scale, stream)
+    if r is not None:
+        _answer(r)
 
 
 class PagePool:
@@ -289,7 +222,7 @@ class PagePool:
         self.refs, self.page_size, self.tensors = refs, page_size, list(tensors)
         self.device, pages = refs.get_device(), _dims("refs", refs, 1)[0]
         self.pages = pages
-        _flat("refs", refs, _I32T, (pages,), self.device)
+        _take("refs", refs, torch.int32, (pages,), self.device, True)
         self.memories = (MemoryStruct * max(1, len(self.tensors)))()
         for m, t in zip(self.memories, self.tensors):
             p = 1 if planes else 0
@@ -304,48 +237,25 @@ class PagePool:
             m.base, m.bytes = t.data_ptr(), inner.numel() * size
             m.planes, m.plane_stride = (t.shape[0], t.stride(0) * size) if planes else (1, 0)
             m.page_stride = t.stride(p) * size if pages > 1 else m.bytes
+        self.at = C.addressof(self.memories)
+        lib()
 
 
 def pages_fork(pool, table, lengths, parents, append, table_out, lengths_out, workspace, errors=None, stream=0):
     """Row r of table_out takes over row parents[r] of table (None: its own, -1: released) with
     room for `append` more tokens; shared pages are counted and copied on write."""
-    device = pool.device
-    rows, width = shape = _dims("table", table, 2)
-    table_at, ts = _take("table", table, _I32T, shape, device)
-    out_at, os = _take("table_out", table_out, _I32T, shape, device)
-    flat = (rows,)
-    status = lib().qd_pages_fork(ForkStruct(
-        table_at, _flat("lengths", lengths, _I32T, flat, device),
-        None if parents is None else _flat("parents", parents, _I32T, flat, device), out_at,
-        _flat("lengths_out", lengths_out, _I32T, flat, device), pool.refs.data_ptr(), ts[0] if rows > 1 else width,
-        os[0] if rows > 1 else width, None if errors is None else _flat("errors", errors, _I32T, (1,), device),
-        pool.memories, len(pool.tensors), rows, width, pool.pages, pool.page_size, append, device), workspace.handle, stream)
-    if status:
-        _check(status)
+    r = _qd_tensors.fork(pool.refs, pool.page_size, pool.at, len(pool.tensors), table, lengths, parents, append, table_out,
+                         lengths_out, workspace.handle, errors, stream)
+    if r is not None:
+        _answer(r)
 
 
 def beam_select(logits, scores, scores_out, parents, tokens, workspace, done=None, done_out=None, eos=None, stream=0):
     """The best k = scores_out.shape[1] continuations of each group: logits [groups, beams, vocab],
     scores and done [groups, beams], the results [groups, k]."""
-    groups, beams, vocab = shape = _dims("logits", logits, 3)
-    device, dtype = logits.get_device(), logits.dtype
-    if dtype not in _TYPES:
-        _refuse(f"logits of type {dtype}")
-    logits_at, s = _take("logits", logits, dtype, shape, device)
-    k = _dims("scores_out", scores_out, 2)[1]
-    given, chosen = (groups, beams), (groups, k)
-    done_at = done_out_at = None
-    if done is not None and done_out is not None and eos is not None:
-        done_at, done_out_at = _flat("done", done, _U8T, given, device), _flat("done_out", done_out, _U8T, chosen, device)
-    elif done is not None or done_out is not None:
-        _refuse("done, done_out and eos go together")
-    status = lib().qd_beam_select(SelectStruct(
-        logits_at, s[0], s[1], _flat("scores", scores, _F32, given, device), done_at,
-        _flat("scores_out", scores_out, _F32, chosen, device), _flat("parents", parents, _I32T, chosen, device),
-        _flat("tokens", tokens, _I32T, chosen, device), done_out_at, _TYPES[dtype], groups, beams, vocab, k,
-        0 if eos is None else eos, device), workspace.handle, stream)
-    if status:
-        _check(status)
+    r = _qd_tensors.select(logits, scores, scores_out, parents, tokens, workspace.handle, done, done_out, eos, stream)
+    if r is not None:
+        _answer(r)
 
 
 def rope_table(theta, rotary_dim, positions, stretch=1.0, original=32768, fast=32.0, slow=1.0):

@@ -14,6 +14,36 @@ import operator_oracle as oracle
 import qd_operators as ops
 import qwen_decode as qd
 
+_P, _I64, _U32, _I32 = C.c_void_p, C.c_int64, C.c_uint32, C.c_int32
+
+
+# The calls' arguments as a ctypes program writes them.
+
+class AppendStruct(C.Structure):
+    _fields_ = [("q", _P), ("k", _P), ("v", _P), ("q_out", _P), ("q_stride", _I64), ("k_stride", _I64),
+                ("v_stride", _I64), ("q_out_stride", _I64), ("positions", _P), ("rows", _P), ("position_bias", _I32),
+                ("tokens", _U32), ("heads", _U32), ("rotary_dim", _U32), ("interleaved", _U32),
+                ("table_positions", _U32), ("cos_table", _P), ("sin_table", _P)]
+
+
+class AttentionStruct(C.Structure):
+    _fields_ = [("q", _P), ("out", _P), ("q_stride", _I64), ("q_head_stride", _I64), ("out_stride", _I64),
+                ("out_head_stride", _I64), ("heads", _U32), ("scale", C.c_float)]
+
+
+class ForkStruct(C.Structure):
+    _fields_ = [("table", _P), ("lengths", _P), ("parents", _P), ("table_out", _P), ("lengths_out", _P), ("refs", _P),
+                ("table_stride", _I64), ("table_out_stride", _I64), ("errors", _P), ("memories", C.POINTER(ops.MemoryStruct)),
+                ("memory_count", _U32), ("rows", _U32), ("table_width", _U32), ("pages", _U32), ("page_size", _U32),
+                ("append", _U32), ("device", _I32)]
+
+
+class SelectStruct(C.Structure):
+    _fields_ = [("logits", _P), ("group_stride", _I64), ("beam_stride", _I64), ("scores", _P), ("done", _P),
+                ("scores_out", _P), ("parents", _P), ("tokens", _P), ("done_out", _P), ("dtype", _U32), ("groups", _U32),
+                ("beams", _U32), ("vocab", _U32), ("k", _U32), ("eos", _U32), ("device", _I32)]
+
+
 HEADER = os.path.join(os.path.dirname(__file__), "..", "include", "qd", "qd_operators.h")
 AT = 4096  # an aligned address that no refused call reads
 
@@ -28,9 +58,9 @@ def test_every_declared_entry_point_is_bound():
 
 def test_structures_have_the_declared_fields():
     text = open(HEADER).read()
-    for struct, cls in (("qd_paged_cache", ops.CacheStruct), ("qd_append_args", ops.AppendStruct),
-                        ("qd_attention_args", ops.AttentionStruct), ("qd_page_memory", ops.MemoryStruct),
-                        ("qd_fork_args", ops.ForkStruct), ("qd_select_args", ops.SelectStruct)):
+    for struct, cls in (("qd_paged_cache", ops.CacheStruct), ("qd_append_args", AppendStruct),
+                        ("qd_attention_args", AttentionStruct), ("qd_page_memory", ops.MemoryStruct),
+                        ("qd_fork_args", ForkStruct), ("qd_select_args", SelectStruct)):
         body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (struct, struct), text, re.S).group(1)
         body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
         fields = [(m.group(1), "*" in line) for line in body.split(";") for m in [re.search(r"(\w+)\s*$", line.strip())] if m]
@@ -51,13 +81,13 @@ def append(**changes):
              rows=None, position_bias=0, tokens=3, heads=14, rotary_dim=64, interleaved=0, table_positions=100, cos_table=AT,
              sin_table=AT)
     a.update(changes)
-    return ops.AppendStruct(**a)
+    return AppendStruct(**a)
 
 
 def attention(**changes):
     a = dict(q=AT, out=AT, q_stride=14 * 64, q_head_stride=64, out_stride=14 * 64, out_head_stride=64, heads=14, scale=0.125)
     a.update(changes)
-    return ops.AttentionStruct(**a)
+    return AttentionStruct(**a)
 
 
 def fork(memory=None, **changes):
@@ -68,18 +98,18 @@ def fork(memory=None, **changes):
              table_out_stride=8, errors=None, memories=memories, memory_count=1, rows=3, table_width=8, pages=10,
              page_size=16, append=1, device=0)
     a.update(changes)
-    return ops.ForkStruct(**a)
+    return ForkStruct(**a)
 
 
 def select(**changes):
     a = dict(logits=AT, group_stride=4000, beam_stride=1000, scores=AT, done=None, scores_out=2 * AT, parents=AT, tokens=AT,
              done_out=None, dtype=qd.DTYPE_F32, groups=2, beams=4, vocab=1000, k=4, eos=0, device=0)
     a.update(changes)
-    return ops.SelectStruct(**a)
+    return SelectStruct(**a)
 
 
 def refused(status, call, *args):
-    got = getattr(ops.lib(), call)(*args)
+    got = getattr(ops.lib(), call)(*(C.byref(a) if isinstance(a, C.Structure) else a for a in args))
     text = ops.lib().qd_last_error().decode()
     assert got == status, (got, text)
     assert text
