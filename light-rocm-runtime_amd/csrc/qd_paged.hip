@@ -83,8 +83,9 @@ __device__ __forceinline__ void store4(void *base, int64_t i, float4 v) {
 // (a, b) -> (a c - b s, b c + a s) for the rotated pairs, a copy for the rest. A
 // wave takes rows of one token, so that its position, page and angles are looked up
 // once and through the scalar cache; each group of head_dim / 8 lanes takes a head,
-// eight elements a lane. Bound by memory for prompts, by the chain position -> page
-// -> store for a few tokens.
+// eight elements a lane. Bound by memory for prompts (6,000 tokens of 48 heads of 128
+// in BF16, 149 MB, 28.7 us: 5.2 TB/s, what a copy reaches), by the chain position ->
+// page -> store for a few tokens (16 of 18 heads of 64 in FP32 3.0 us).
 struct AppendLaunch {
   qd_paged_cache c;
   qd_append_args a;
@@ -108,23 +109,19 @@ __device__ __forceinline__ Eight<E> load8(const void *base, int64_t i) {
             make_float4(E::lo(v.z), E::hi(v.z), E::lo(v.w), E::hi(v.w))};
   }
 }
-// kStream: not to be kept in the caches.
-template <bool kStream, typename V>
-__device__ __forceinline__ void put(V *to, V v) {
-  if constexpr (kStream)
-    __builtin_nontemporal_store(v, to);
-  else
-    *to = v;
-}
-template <typename E, bool kStream>
+// Past the caches: what is appended is read by other kernels, mostly on other XCDs.
+// (6,000 tokens of 48 heads of 128 in BF16 28.7 us, with ordinary stores 34.1; 500 4.5
+// and 5.2, 16 of 18 heads of 64 in FP32 3.05 and 3.03.)
+template <typename E>
 __device__ __forceinline__ void store8(void *base, int64_t i, const Eight<E> &v) {
   if constexpr (std::is_same_v<E, float>) {
     f4v *to = reinterpret_cast<f4v *>(static_cast<float *>(base) + i);
-    put<kStream>(to, f4v{v.lo.x, v.lo.y, v.lo.z, v.lo.w});
-    put<kStream>(to + 1, f4v{v.hi.x, v.hi.y, v.hi.z, v.hi.w});
+    __builtin_nontemporal_store(f4v{v.lo.x, v.lo.y, v.lo.z, v.lo.w}, to);
+    __builtin_nontemporal_store(f4v{v.hi.x, v.hi.y, v.hi.z, v.hi.w}, to + 1);
   } else {
-    put<kStream>(reinterpret_cast<u4v *>(static_cast<uint16_t *>(base) + i),
-                 u4v{E::pack(v.lo.x, v.lo.y), E::pack(v.lo.z, v.lo.w), E::pack(v.hi.x, v.hi.y), E::pack(v.hi.z, v.hi.w)});
+    __builtin_nontemporal_store(
+        u4v{E::pack(v.lo.x, v.lo.y), E::pack(v.lo.z, v.lo.w), E::pack(v.hi.x, v.hi.y), E::pack(v.hi.z, v.hi.w)},
+        reinterpret_cast<u4v *>(static_cast<uint16_t *>(base) + i));
   }
 }
 
@@ -145,7 +142,7 @@ __device__ __forceinline__ float4 turn4(float4 x, float4 y, float4 c, float4 s, 
   return a;
 }
 
-template <typename E, bool kStream>
+template <typename E>
 __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   const uint32_t id = blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(wave_id());
   const uint32_t token = id / p.waves;
@@ -174,7 +171,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   if (bad) {
     const float n = __uint_as_float(0x7FC00000u);
     const float4 nans = make_float4(n, n, n, n);
-    if (j < heads) store8<E, kStream>(p.a.q_out, token * p.a.q_out_stride + j * dim + e, {nans, nans});
+    if (j < heads) store8<E>(p.a.q_out, token * p.a.q_out_stride + j * dim + e, {nans, nans});
     if (id == token * p.waves && lane == 0) raise_error(p.c.errors, bad);
     return;
   }
@@ -218,7 +215,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   void *dst = query ? p.a.q_out : value ? p.c.v : p.c.k;
   const int64_t to = query ? token * p.a.q_out_stride + h * dim
                            : page * p.c.page_stride + (position & (p.c.page_size - 1)) * p.c.token_stride + h * p.c.head_stride;
-  store8<E, kStream>(dst, to + e, x);
+  store8<E>(dst, to + e, x);
 }
 
 // ---- attention ------------------------------------------------------------------
@@ -236,15 +233,25 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 // holds positions along the registers: FP32 takes one position per instruction,
 // so float4 loads along the head serve four of them; 16-bit rows are loaded 8 at
 // a time and turned with byte permutes.
+// Bound by the memory for long rows: 64 rows of 0 to 8,192 with 8 KV heads of 128 in
+// BF16, 1,086 MB, 192 us (5.7 TB/s; a streaming read reaches 6.6), two of about
+// 105,000 with 4 in FP16, 431 MB, 88 us. Short ones wait: for the launch, length,
+// page, K, the other waves, the other pieces, each near 1 us (one row of 129 7.4 us,
+// 16 beams at 576 8.9).
 constexpr int kTile = 32, kSub = 16;
 constexpr uint32_t kMostPieces = 256;  // of an item
 constexpr int kWaves = 4;              // of a workgroup
-constexpr uint32_t kEdge = 2;          // tiles that an item's results cost the long kernel as much time as
-// The short kernel: tiles of a piece at least, of an item that stays whole, and
-// pieces of an item at most.
+// Tiles that an item's results cost the long kernel as much time as: 128 rows of 0 to
+// 4,000 took 171 us, counted as none 177, as one 176, as four 173.
+constexpr uint32_t kEdge = 2;
+// The short kernel: tiles of a piece at least, of an item that stays whole (one row of
+// 129 positions 7.4 us, with items of 5 tiles cut 8.6; 8 rows of 448 8.8, with items
+// of 14 whole 11.6), and pieces of an item at most (one row of 30,000 18.9 us, in up
+// to 256 pieces 25.3).
 constexpr uint32_t kShortLeast = 4, kShortWhole = 8, kShortPieces = 64;
 // A maximum is only taken up when it passes the one in use by this many powers of
-// two: until then probabilities grow to at most 2^8, exact in every type's range.
+// two: until then probabilities grow to at most 2^8, in every type's range. (Taken up
+// at once, 64 rows of 0 to 8,192 took 193 us instead of 192.)
 constexpr float kLazyMax = 8.f;
 
 struct AttnLaunch {
@@ -974,8 +981,9 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
 // ---- fork -----------------------------------------------------------------------
 // The first kernel, one workgroup, counts references, decides which rows copy
 // their last page and deals out free pages; the second writes the new table and
-// copies pages. Bound by latency: a few dependent passes over tables and
-// counts; the copies stream.
+// copies pages. The first is bound by latency, a few dependent passes over tables
+// and counts (16 beams over pages of 24 layers: 5 of 9.2 us); the copies stream (64
+// rows that copy about 22 pages of 2 x 8 layers x 128 KB, 91 MB, 24 us in all).
 constexpr int kForkT = 1024, kForkWaves = kForkT / kWave;
 constexpr int kForkScan = 8;  // counts that a thread looks at for free pages per pass
 
@@ -1267,14 +1275,12 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
   return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, packed, 0, s);
 }
 
-constexpr uint64_t kAppendStream = 32ull << 20;
-
 // How attention cuts its work. Workgroups that the card holds at once: of the short
 // kernel, by head_dim, which its pieces are made for (16 beams at 576 positions in
 // pieces of 4 tiles or more 8.9 us, of 8 10.8; 4 rows of 3,000 with 8 KV heads of 128
 // in about 512 pieces 15.5 us, in 768 18.6; 64 rows to 2,000 with 2 of 64 21.9 in
 // 512, 20.4 in 768), and of the long one. The long kernel's cuts keep eight tiles
-// from an item's ends.
+// from an item's ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
 constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
 constexpr uint32_t short_aim(uint32_t head_dim) { return head_dim == 128 ? 2 * kCus : 3 * kCus; }
 // Which kernel, by the bytes of all positions that the tables, or the pool, can
@@ -1282,6 +1288,9 @@ constexpr uint32_t short_aim(uint32_t head_dim) { return head_dim == 128 ? 2 * k
 // long 24.0; 101 MB of 8 of 128 29.1 and 27.1; 102 MB of one row 37.8 and 34.0;
 // 193 MB 57 and 48.
 constexpr uint64_t kShortBytes = 96ull << 20;
+// Pages that cannot all stay in the last-level cache (256 MB) are read as a stream:
+// 431 MB 88 us, else 93. 208 MB read again and again the other way 38.7 us, as a
+// stream 45.8.
 constexpr uint64_t kCachedBytes = 256ull << 20;
 struct AttnShape {
   uint32_t group, blocks, parts, rec_heads, rec_floats, apart, least, target, records;
@@ -1321,14 +1330,10 @@ hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_
   p.waves = (rows + at_once - 1) / at_once;
   const dim3 grid((static_cast<uint64_t>(a.tokens) * p.waves + kWavesPerBlock - 1) / kWavesPerBlock);
   const dim3 block(kBlock);
-  // What a prompt writes does not stay in the L2s (4 MB on each of eight XCDs)
-  // until it is read; written past them, 6,000 tokens take 28.6 us instead of 36.
-  const uint64_t bytes = static_cast<uint64_t>(a.tokens) * rows * c.head_dim * (c.dtype == QD_DTYPE_F32 ? 4 : 2);
-  const bool stream = bytes > kAppendStream;
   switch (c.dtype) {
-    case QD_DTYPE_F32: return launch(stream ? append_kernel<float, true> : append_kernel<float, false>, grid, block, s, p);
-    case QD_DTYPE_BF16: return launch(stream ? append_kernel<Brain, true> : append_kernel<Brain, false>, grid, block, s, p);
-    default: return launch(stream ? append_kernel<Half, true> : append_kernel<Half, false>, grid, block, s, p);
+    case QD_DTYPE_F32: return launch(append_kernel<float>, grid, block, s, p);
+    case QD_DTYPE_BF16: return launch(append_kernel<Brain>, grid, block, s, p);
+    default: return launch(append_kernel<Half>, grid, block, s, p);
   }
 }
 
@@ -1352,7 +1357,6 @@ static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
     if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + kShortLeast - 1) / kShortLeast));
     return launch(attention_short_kernel<E, D>, dim3(static_cast<uint32_t>(x * p.parts)), block, s, p);
   }
-  // Pages that cannot all stay in the last-level cache are read as a stream.
   return launch(pool * position > kCachedBytes ? attention_long_kernel<E, D, kStages, kPolicyNt> : attention_long_kernel<E, D, kStages, 0>,
                 dim3(kCus * per_cu), block, s, p);
 }
