@@ -504,7 +504,13 @@ __device__ __forceinline__ bool next_item(const AttnLaunch &p, const Deal &d, ui
   return end_run(p, d, i, next);
 }
 
-template <typename E, int D, int kStages>
+// kStages tiles are loaded ahead. kEarly (one stage): the next tile's V comes with its
+// K, into registers of its own. In the short kernel, heads of 64: one row of 129
+// positions 6.7 us instead of 7.2, one of 30,000 17.6 instead of 18.4. Heads of 128 do
+// without (8 rows of 1,000 to 2,000, 8 KV heads, BF16 16.8 us, with it 17.2; FP32 has
+// not the registers), and so does the long kernel, which has loads enough (64 rows of
+// 1,000 to 4,000, 8 KV heads of 128, FP32 217 us, with it 248).
+template <typename E, int D, int kStages, bool kEarly>
 struct WaveTiles {
   static constexpr bool kWide = std::is_same_v<E, float>;
   static constexpr int kElem = kWide ? 4 : 2;
@@ -513,6 +519,7 @@ struct WaveTiles {
   u4v q[kPieces];
   u4v k[kStages][2][kPieces];
   u4v v[kStages][2][4][kWide ? D / 64 : 1];  // rows 4 (l / 16) + j; 16-bit rows of 64 use half of a register quad
+  u4v v_next[2][4][kWide ? D / 64 : 1];      // (kEarly)
   f4v o[kAcc];
   float m, ms, l;
 
@@ -522,17 +529,17 @@ struct WaveTiles {
     for (int s = 0; s < kPieces; ++s) k[st][sub][s] = r.ld16(off + 64 * s);
   }
   template <typename R>
-  __device__ __forceinline__ void load_v(const R &r, int st, int sub, const uint32_t (&off)[4]) {
+  static __device__ __forceinline__ void load_v(const R &r, u4v (&to)[4][kWide ? D / 64 : 1], const uint32_t (&off)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (kWide) {
 #pragma unroll
-        for (int n = 0; n < D / 64; ++n) v[st][sub][j][n] = r.ld16(off[j] + 256 * n);
+        for (int n = 0; n < D / 64; ++n) to[j][n] = r.ld16(off[j] + 256 * n);
       } else if constexpr (D == 128) {
-        v[st][sub][j][0] = r.ld16(off[j]);
+        to[j][0] = r.ld16(off[j]);
       } else {
         const u2v x = r.ld8(off[j]);
-        v[st][sub][j][0] = u4v{x[0], x[1], 0u, 0u};
+        to[j][0] = u4v{x[0], x[1], 0u, 0u};
       }
     }
   }
@@ -610,9 +617,10 @@ struct AttnShared {
   uint32_t spoilt, last;
 };
 
-template <typename E, int D, int kStages, int kPolicy>
+template <typename E, int D, int kStages, int kPolicy, bool kEarly>
 struct Attention {
-  using Tiles = WaveTiles<E, D, kStages>;
+  static_assert(!kEarly || kStages == 1, "one stage");
+  using Tiles = WaveTiles<E, D, kStages, kEarly>;
   using Shared = AttnShared<E, D, kStages>;
   static constexpr int kT = kWaves * kWave, kQuads = D / 4;
   const AttnLaunch &p;
@@ -661,9 +669,10 @@ struct Attention {
 #pragma unroll
     for (int s = 0; s < 2; ++s) t.load_k(rows_at(x, p.c.k, at * kTile + s * kSub, id[s], bad), st, s, k_off);
   }
-  __device__ __forceinline__ void load_v(const Item &x, int st, uint32_t at, const int (&id)[2], bool &bad) {
+  __device__ __forceinline__ void load_v(const Item &x, u4v (&to)[2][4][Tiles::kWide ? D / 64 : 1], uint32_t at,
+                                         const int (&id)[2], bool &bad) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) t.load_v(rows_at(x, p.c.v, at * kTile + s * kSub, id[s], bad), st, s, v_off);
+    for (int s = 0; s < 2; ++s) Tiles::load_v(rows_at(x, p.c.v, at * kTile + s * kSub, id[s], bad), to[s], v_off);
   }
   // The pages of a wave's tile `at`, -1 past its run.
   __device__ __forceinline__ void pages_of(const Item &x, uint32_t at, int (&id)[2]) const {
@@ -693,7 +702,7 @@ struct Attention {
     for (int st = 0; st < kStages; ++st) {
       if (tile + st * kWaves >= x.last) continue;
       load_k(x, st, tile + st * kWaves, id[st], bad);
-      load_v(x, st, tile + st * kWaves, id[st], bad);
+      load_v(x, t.v[st], tile + st * kWaves, id[st], bad);
     }
     pages_of(x, tile + kStages * kWaves, ahead);
   }
@@ -706,7 +715,10 @@ struct Attention {
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[sub][r] = x[r] * scale;
     }
-    if (more) load_k(it, st, tile + kStages * kWaves, ahead, bad);
+    if (more) {
+      load_k(it, st, tile + kStages * kWaves, ahead, bad);
+      if constexpr (kEarly) load_v(it, t.v_next, tile + kWaves, ahead, bad);
+    }
     if (static_cast<int>((tile + 1) * kTile) > it.length)
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
@@ -731,7 +743,18 @@ struct Attention {
 #pragma unroll
       for (int r = 0; r < 4; ++r) pr[sub][r] = exp2_fast(s[sub][r] - t.ms);
     t.l += t.accumulate(st, pr);
-    if (more) load_v(it, st, tile + kStages * kWaves, ahead, bad);
+    if (more) {
+      if constexpr (kEarly) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int n = 0; n < (Tiles::kWide ? D / 64 : 1); ++n) t.v[0][sub][j][n] = t.v_next[sub][j][n];
+      } else {
+        load_v(it, t.v[st], tile + kStages * kWaves, ahead, bad);
+      }
+    }
     tile += kWaves;
     pages_of(it, tile + kStages * kWaves, ahead);
   }
@@ -908,18 +931,26 @@ struct Attention {
   }
 };
 
+// Workgroups of the short kernel that a CU holds, which its pieces are made for (16
+// beams at 576 positions in pieces of 4 tiles or more 8.9 us, of 8 10.8; 4 rows of
+// 3,000 with 8 KV heads of 128 in about 512 pieces 15.5 us, in 768 18.6; 64 rows to
+// 2,000 with 2 of 64 21.9 in 512, 20.4 in 768) and its registers: FP32 heads of 128 in
+// as many as they like, one a CU, 4 rows of 2,000 to 4,000 with 4 heads 23.8 us, in
+// those of two 20.3.
+constexpr uint32_t short_per_cu(uint32_t head_dim) { return head_dim == 128 ? 2 : 3; }
+
 // Few positions in all: a workgroup per piece, no more than `target` pieces
 // besides one for each item. Short code and one dependent load less, because each
 // step of such a call waits for the one before it.
 template <typename E, int D>
-__global__ __launch_bounds__(kWaves *kWave) void attention_short_kernel(AttnLaunch p) {
+__global__ __launch_bounds__(kWaves *kWave, short_per_cu(D)) void attention_short_kernel(AttnLaunch p) {
   __shared__ AttnShared<E, D, 1> sh;
   Item it;
   const uint32_t part = blockIdx.x % p.parts;
   uint32_t begin;
   if (!find_piece(p, blockIdx.x / p.parts, part, it, begin)) return;
   if (threadIdx.x == 0) sh.spoilt = 0u;
-  Attention<E, D, 1, 0> a(p, sh);
+  Attention<E, D, 1, 0, D == 64> a(p, sh);
   bool bad = false;
   a.begin(it, bad);
   a.run(it, bad);
@@ -941,7 +972,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
   Item it;
   if (!first_item(p, group_id, gridDim.x, deal, it)) return;
   if (threadIdx.x == 0) sh.spoilt = 0u;
-  Attention<E, D, kStages, kPolicy> a(p, sh);
+  Attention<E, D, kStages, kPolicy, false> a(p, sh);
   // The record of an item's piece: its workgroup's first if it begins inside the item, else the second.
   auto record_of = [&](const Item &x, uint32_t piece) {
     return p.records + (2 * static_cast<size_t>(x.home + piece) + (piece == 0)) * p.rec_floats;
@@ -1275,14 +1306,9 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
   return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, packed, 0, s);
 }
 
-// How attention cuts its work. Workgroups that the card holds at once: of the short
-// kernel, by head_dim, which its pieces are made for (16 beams at 576 positions in
-// pieces of 4 tiles or more 8.9 us, of 8 10.8; 4 rows of 3,000 with 8 KV heads of 128
-// in about 512 pieces 15.5 us, in 768 18.6; 64 rows to 2,000 with 2 of 64 21.9 in
-// 512, 20.4 in 768), and of the long one. The long kernel's cuts keep eight tiles
-// from an item's ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
+// How attention cuts its work. The long kernel's cuts keep eight tiles from an item's
+// ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
 constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
-constexpr uint32_t short_aim(uint32_t head_dim) { return head_dim == 128 ? 2 * kCus : 3 * kCus; }
 // Which kernel, by the bytes of all positions that the tables, or the pool, can
 // hold (their real number is on the device): 68 MB of 2 heads of 64 short 20.4 us,
 // long 24.0; 101 MB of 8 of 128 29.1 and 27.1; 102 MB of one row 37.8 and 34.0;
@@ -1305,7 +1331,7 @@ AttnShape attention_shape(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint
   const uint64_t items = static_cast<uint64_t>(rows) * s.parts;
   if (items <= kOpCounters) {
     s.least = kAttnLeast;
-    s.target = std::max(1u, short_aim(head_dim) / s.parts);
+    s.target = std::max(1u, kCus * short_per_cu(head_dim) / s.parts);
     s.records = std::max((rows + s.target) * s.parts, 2 * kCus * kMostPerCu);
     // Counters in lines of their own where there is room.
     for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
