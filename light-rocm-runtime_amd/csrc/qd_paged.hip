@@ -1310,9 +1310,9 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
 // ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
 constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
 // Which kernel, by the bytes of all positions that the tables, or the pool, can
-// hold (their real number is on the device): 68 MB of 2 heads of 64 short 20.4 us,
-// long 24.0; 101 MB of 8 of 128 29.1 and 27.1; 102 MB of one row 37.8 and 34.0;
-// 193 MB 57 and 48.
+// hold (their real number is on the device): 74 MB of 8 heads of 128 short 20.4 us,
+// long 21.7, 101 MB 30.2 and 27.6; 61 MB of one row of 2 heads of 64 24.2 and 27.1, 102
+// MB 34.3 and 35.2; 130 MB of 4 of 64 40.3 and 37.8.
 constexpr uint64_t kShortBytes = 96ull << 20;
 // Pages that cannot all stay in the last-level cache (256 MB) are read as a stream:
 // 431 MB 88 us, else 93. 208 MB read again and again the other way 38.7 us, as a
