@@ -236,7 +236,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 // Bound by the memory for long rows: 64 rows of 0 to 8,192 with 8 KV heads of 128 in
 // BF16, 1,086 MB, 192 us (5.7 TB/s; a streaming read reaches 6.6), two of about
 // 105,000 with 4 in FP16, 431 MB, 88 us. Short ones wait: for the launch, length,
-// page, K, the other waves, the other pieces, each near 1 us (one row of 129 7.4 us,
+// page, K, the other waves, the other pieces, each near 1 us (one row of 129 6.75 us,
 // 16 beams at 576 8.9).
 constexpr int kTile = 32, kSub = 16;
 constexpr uint32_t kMostPieces = 256;  // of an item
@@ -247,7 +247,7 @@ constexpr uint32_t kEdge = 2;
 // The short kernel: tiles of a piece at least, of an item that stays whole (one row of
 // 129 positions 7.4 us, with items of 5 tiles cut 8.6; 8 rows of 448 8.8, with items
 // of 14 whole 11.6), and pieces of an item at most (one row of 30,000 18.9 us, in up
-// to 256 pieces 25.3).
+// to 256 pieces 25.3; all before V was loaded with K).
 constexpr uint32_t kShortLeast = 4, kShortWhole = 8, kShortPieces = 64;
 // A maximum is only taken up when it passes the one in use by this many powers of
 // two: until then probabilities grow to at most 2^8, in every type's range. (Taken up

@@ -274,6 +274,39 @@ def test_numbers_that_the_structures_would_cut_are_refused():
             ops.rope_table(1e4, dim, positions)
 
 
+def test_arguments_that_are_something_else_are_refused():
+    import types
+
+    import torch
+
+    k = torch.zeros(4, 16, 2, 64)
+    table, lengths = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    c, q, new = ops.PagedCache(k, k, table, lengths), torch.zeros(1, 4, 64), k[0, :1]
+    closed = types.SimpleNamespace(handle=0)
+    pool = ops.PagePool(torch.zeros(4, dtype=torch.int32), 16, [k], planes=False)
+    logits, best, ids = torch.zeros(1, 2, 50), torch.zeros(1, 4), torch.zeros(1, 4, dtype=torch.int32)
+    for call, text in (
+            (lambda: ops.paged_append(c, None, None, [1], new, lengths), "k is no tensor"),
+            (lambda: ops.paged_append(c, None, None, None, new, lengths), "k is missing"),
+            (lambda: ops.paged_append(c, None, None, new, new, lengths, position_bias=1.5), "position_bias"),
+            (lambda: ops.paged_append(c, None, None, new, new, lengths, stream="s"), "stream"),
+            (lambda: ops.paged_append(c, q, q, new, new, lengths, cos=new[0, 0]), "cos and sin"),
+            (lambda: ops.paged_append(c, q, q[:, :3], new, new, lengths), "q_out has shape"),
+            (lambda: ops.paged_attention(c, q, q, closed), "null workspace"),
+            (lambda: ops.paged_attention(c, q, q, closed, scale="x"), "scale"),
+            (lambda: ops.paged_attention(c, q, q.transpose(1, 2), closed), "q has shape"),
+            (lambda: ops.pages_fork(pool, table, lengths, None, -1, table.clone(), lengths.clone(), closed), "append"),
+            (lambda: ops.pages_fork(pool, table, lengths, None, 1, table.clone(), lengths.clone(), closed), "null workspace"),
+            (lambda: ops.pages_fork(pool, table, lengths, None, 1, table, lengths.clone(), closed), "must not be"),
+            (lambda: ops.pages_fork(pool, table, lengths, lengths.long(), 1, table.clone(), lengths.clone(), closed), "parents has type"),
+            (lambda: ops.beam_select(logits.double(), best, best, ids, ids, closed), "logits of type"),
+            (lambda: ops.beam_select(logits, best[:, :2], best, ids, ids.clone(), closed), "must not be"),
+            (lambda: ops.beam_select(logits, torch.zeros(1, 2), best, ids, ids, closed, done=ids), "go together"),
+            (lambda: ops.beam_select(logits.to_sparse(), torch.zeros(1, 2), best, ids, ids, closed), "")):
+        with pytest.raises(qd.QdError, match=text):
+            call()
+
+
 def test_cpu_tensors_are_refused():
     import torch
 
