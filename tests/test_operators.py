@@ -302,7 +302,7 @@ def test_arguments_that_are_something_else_are_refused():
             (lambda: ops.beam_select(logits.double(), best, best, ids, ids, closed), "logits of type"),
             (lambda: ops.beam_select(logits, best[:, :2], best, ids, ids.clone(), closed), "must not be"),
             (lambda: ops.beam_select(logits, torch.zeros(1, 2), best, ids, ids, closed, done=ids), "go together"),
-            (lambda: ops.beam_select(logits.to_sparse(), torch.zeros(1, 2), best, ids, ids, closed), "")):
+            (lambda: ops.beam_select(logits.to_sparse(), torch.zeros(1, 2), best, ids, ids, closed), None)):
         with pytest.raises(qd.QdError, match=text):
             call()
 
