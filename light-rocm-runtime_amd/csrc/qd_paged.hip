@@ -234,8 +234,8 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 // so float4 loads along the head serve four of them; 16-bit rows are loaded 8 at
 // a time and turned with byte permutes.
 // Bound by the memory for long rows: 64 rows of 0 to 8,192 with 8 KV heads of 128 in
-// BF16, 1,086 MB, 192 us (5.7 TB/s; a streaming read reaches 6.6), two of about
-// 105,000 with 4 in FP16, 431 MB, 88 us. Short ones wait: for the launch, length,
+// BF16, 1,086 MB, 182 us (6.0 TB/s; a streaming read reaches 6.6), two of about
+// 105,000 with 4 in FP16, 431 MB, 85 us. Short ones wait: for the launch, length,
 // page, K, the other waves, the other pieces, each near 1 us (one row of 129 6.75 us,
 // 16 beams at 576 8.9).
 constexpr int kTile = 32, kSub = 16;
@@ -655,7 +655,8 @@ struct Attention {
     return min(16, static_cast<int>(p.group - 16 * (x.part % p.blocks)));
   }
   // The 16 positions from `pos` on, in page `id`, of K or V.
-  __device__ __forceinline__ PageRows<kPolicy> rows_at(const Item &x, const void *base, uint32_t pos, int id, bool &bad) const {
+  template <int kOf>
+  __device__ __forceinline__ PageRows<kOf> rows_at(const Item &x, const void *base, uint32_t pos, int id, bool &bad) const {
     const int n = min(max(x.length - static_cast<int>(pos), 0), kSub);
     const bool in = id >= 0 && static_cast<uint32_t>(id) < p.c.pages;
     if (n > 0 && !in) bad = true;
@@ -663,16 +664,18 @@ struct Attention {
                        static_cast<int64_t>(x.part / p.blocks) * p.c.head_stride;
     const uint32_t bytes = n > 0 && in ? (n - 1) * token_bytes + D * Tiles::kElem : 0u;
     char *ptr = const_cast<char *>(static_cast<const char *>(base)) + at * Tiles::kElem;
-    return PageRows<kPolicy>{__builtin_amdgcn_make_buffer_rsrc(ptr, 0, static_cast<int>(bytes), kRsrcWord3)};
+    return PageRows<kOf>{__builtin_amdgcn_make_buffer_rsrc(ptr, 0, static_cast<int>(bytes), kRsrcWord3)};
   }
+  // K stays in the caches, a stream or not: a load takes half of each line, and the
+  // next one, the other half, found it gone (64 rows of 0 to 8,192 192 us, so 182).
   __device__ __forceinline__ void load_k(const Item &x, int st, uint32_t at, const int (&id)[2], bool &bad) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) t.load_k(rows_at(x, p.c.k, at * kTile + s * kSub, id[s], bad), st, s, k_off);
+    for (int s = 0; s < 2; ++s) t.load_k(rows_at<0>(x, p.c.k, at * kTile + s * kSub, id[s], bad), st, s, k_off);
   }
   __device__ __forceinline__ void load_v(const Item &x, u4v (&to)[2][4][Tiles::kWide ? D / 64 : 1], uint32_t at,
                                          const int (&id)[2], bool &bad) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) Tiles::load_v(rows_at(x, p.c.v, at * kTile + s * kSub, id[s], bad), to[s], v_off);
+    for (int s = 0; s < 2; ++s) Tiles::load_v(rows_at<kPolicy>(x, p.c.v, at * kTile + s * kSub, id[s], bad), to[s], v_off);
   }
   // The pages of a wave's tile `at`, -1 past its run.
   __device__ __forceinline__ void pages_of(const Item &x, uint32_t at, int (&id)[2]) const {
@@ -963,8 +966,11 @@ __global__ __launch_bounds__(kWaves *kWave, short_per_cu(D)) void attention_shor
   if (a.arrive(it)) a.join(it, first, stride, stride);
 }
 
-// Many: equal runs of all tiles, one for each workgroup that the card holds.
-template <typename E, int D, int kStages, int kPolicy>
+// Many: equal runs of all tiles, one for each workgroup that the card holds. V is read
+// as a stream, as so much is not read again before others have taken its place: 16 rows
+// of 2,000 to 4,000 of one layer after the other 45.6 us, by the caches 48.6 (of one
+// layer again and again, 208 MB, 40.0 and 38.6), 64 of 0 to 8,192 182 and 202.
+template <typename E, int D, int kStages>
 __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunch p) {
   __shared__ AttnShared<E, D, kStages> sh;
   const uint32_t group_id = blockIdx.x;
@@ -972,7 +978,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
   Item it;
   if (!first_item(p, group_id, gridDim.x, deal, it)) return;
   if (threadIdx.x == 0) sh.spoilt = 0u;
-  Attention<E, D, kStages, kPolicy, false> a(p, sh);
+  Attention<E, D, kStages, kPolicyNt, false> a(p, sh);
   // The record of an item's piece: its workgroup's first if it begins inside the item, else the second.
   auto record_of = [&](const Item &x, uint32_t piece) {
     return p.records + (2 * static_cast<size_t>(x.home + piece) + (piece == 0)) * p.rec_floats;
@@ -1310,14 +1316,11 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
 // ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
 constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
 // Which kernel, by the bytes of all positions that the tables, or the pool, can
-// hold (their real number is on the device): 74 MB of 8 heads of 128 short 20.4 us,
-// long 21.7, 101 MB 30.2 and 27.6; 61 MB of one row of 2 heads of 64 24.2 and 27.1, 102
-// MB 34.3 and 35.2; 130 MB of 4 of 64 40.3 and 37.8.
+// hold (their real number is on the device). They cross between 65 and 120 MB: 65 MB
+// of 8 heads of 128 in BF16 short 24.8 us, long 22.5; 74 of 4 in FP32 26.7 and 29.1; 98
+// of 8 in BF16, rows of one length, 25.7 and 28.3; 99 of 4 in FP16 32.7 and 30.4; 123
+// of 2 of 64 in FP32 42.7 and 39.3.
 constexpr uint64_t kShortBytes = 96ull << 20;
-// Pages that cannot all stay in the last-level cache (256 MB) are read as a stream:
-// 431 MB 88 us, else 93. 208 MB read again and again the other way 38.7 us, as a
-// stream 45.8.
-constexpr uint64_t kCachedBytes = 256ull << 20;
 struct AttnShape {
   uint32_t group, blocks, parts, rec_heads, rec_floats, apart, least, target, records;
 };
@@ -1383,8 +1386,7 @@ static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
     if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + kShortLeast - 1) / kShortLeast));
     return launch(attention_short_kernel<E, D>, dim3(static_cast<uint32_t>(x * p.parts)), block, s, p);
   }
-  return launch(pool * position > kCachedBytes ? attention_long_kernel<E, D, kStages, kPolicyNt> : attention_long_kernel<E, D, kStages, 0>,
-                dim3(kCus * per_cu), block, s, p);
+  return launch(attention_long_kernel<E, D, kStages>, dim3(kCus * per_cu), block, s, p);
 }
 
 hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w) {
