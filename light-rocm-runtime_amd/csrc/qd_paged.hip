@@ -768,11 +768,10 @@ struct Attention {
     t.ms = 0.f;
     t.l = 0.f;
     for (;;) {
-      if (tile >= it.last) break;
-      tile_through(it, 0, bad);
-      if constexpr (kStages > 1) {
-        if (tile >= it.last) break;
-        tile_through(it, 1, bad);
+#pragma unroll
+      for (int st = 0; st < kStages; ++st) {
+        if (tile >= it.last) return;
+        tile_through(it, st, bad);
       }
     }
   }
@@ -1371,7 +1370,11 @@ size_t paged_attention_scratch(uint32_t rows, uint32_t heads, uint32_t kv_heads,
   return static_cast<size_t>(sh.records) * sh.rec_floats * sizeof(float);
 }
 
-// per_cu: workgroups of the long kernel on a CU, so that 64 KB are on their way there.
+// The long kernel's tiles ahead and workgroups on a CU, by type and head_dim: with 64
+// to 128 KB on their way to each CU, more only queue. Measured on 430 to 680 MB, tiles
+// x workgroups: FP32 of 128 1 x 1 66.9 us, 2 x 1 68.6, 1 x 2 71.6; FP32 of 64 2 x 1 47.8,
+// 1 x 2 48.4, 3 x 1 48.9; 16 bits of 128 2 x 1 66.1, 3 x 1 67.1, 1 x 2 69.2; 16 bits of
+// 64 1 x 2 61.4, 1 x 3 65.7, 2 x 2 64.6, 2 x 1 66.5.
 template <typename E, int D, int kStages, int per_cu>
 static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
   static_assert(per_cu <= static_cast<int>(kMostPerCu), "records");
@@ -1409,8 +1412,8 @@ hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const 
   const bool wide = c.head_dim == 128;
   switch (c.dtype) {
     case QD_DTYPE_F32: return wide ? launch_attention<float, 128, 1, 1>(s, p) : launch_attention<float, 64, 2, 1>(s, p);
-    case QD_DTYPE_BF16: return wide ? launch_attention<Brain, 128, 2, 1>(s, p) : launch_attention<Brain, 64, 2, 2>(s, p);
-    default: return wide ? launch_attention<Half, 128, 2, 1>(s, p) : launch_attention<Half, 64, 2, 2>(s, p);
+    case QD_DTYPE_BF16: return wide ? launch_attention<Brain, 128, 2, 1>(s, p) : launch_attention<Brain, 64, 1, 2>(s, p);
+    default: return wide ? launch_attention<Half, 128, 2, 1>(s, p) : launch_attention<Half, 64, 1, 2>(s, p);
   }
 }
 
