@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 // BF16, 1,086 MB, 182 us (6.0 TB/s; a streaming read reaches 6.6), two of about
 // 105,000 with 4 in FP16, 431 MB, 85 us. Short ones wait: for the launch, length,
 // page, K, the other waves, the other pieces, each near 1 us (one row of 129 6.75 us,
-// 16 beams at 576 8.9).
+// 16 beams at 576 8.5).
 constexpr int kTile = 32, kSub = 16;
 constexpr uint32_t kMostPieces = 256;  // of an item
 constexpr int kWaves = 4;              // of a workgroup
@@ -767,11 +767,13 @@ struct Attention {
     t.m = -INFINITY;
     t.ms = 0.f;
     t.l = 0.f;
+    static_assert(kStages <= 2, "the loop's two steps");
     for (;;) {
-#pragma unroll
-      for (int st = 0; st < kStages; ++st) {
-        if (tile >= it.last) return;
-        tile_through(it, st, bad);
+      if (tile >= it.last) break;
+      tile_through(it, 0, bad);
+      if constexpr (kStages > 1) {
+        if (tile >= it.last) break;
+        tile_through(it, 1, bad);
       }
     }
   }
@@ -854,9 +856,10 @@ struct Attention {
   // wave per head with every maximum and sum on its way at once, then the weighted
   // sums, shared out among the threads. Piece c > 0 is `second` + (c - 1) * stride
   // floats behind piece 0.
+  template <uint32_t kMost>  // pieces
   __device__ __forceinline__ void join(const Item &x, const float *records, uint32_t second, uint32_t stride) {
-    float(*weight)[kMostPieces] = reinterpret_cast<float(*)[kMostPieces]>(&sh.wo[0][0][0]);
-    static_assert(sizeof(float) * 16 * kMostPieces <= sizeof(sh.wo), "a weight per head and piece");
+    float(*weight)[kMost] = reinterpret_cast<float(*)[kMost]>(&sh.wo[0][0][0]);
+    static_assert(sizeof(float) * 16 * kMost <= sizeof(sh.wo), "a weight per head and piece");
     const int heads = heads_of(x);
     const uint32_t of = x.pieces;
     const Coherent recs(records, (second + (of - 2) * stride + p.rec_floats) * static_cast<uint32_t>(sizeof(float)));
@@ -870,34 +873,53 @@ struct Attention {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) next[u] = recs.ld4((at_piece(min(c + u * shares, of - 1)) + h * D + d) / 4);
     };
-    fetch(min(i0, items - 1), min(static_cast<uint32_t>(share), of - 1));
-    __syncthreads();  // the partial results have been read
-    for (int h = w; h < heads; h += kWaves) {
-      constexpr int kPer = kMostPieces / kWave;
-      float cm[kPer], cl[kPer], m = -INFINITY, sum = 0.f;
+    // A wave's heads' maxima and sums: all on their way at once in the short kernel (16
+    // beams at 576 8.5 us, head after head 8.95).
+    constexpr int kPer = kMost / kWave, kSlots = kPer == 1 ? 16 / kWaves : 1;
+    float cm[kSlots][kPer], cl[kSlots][kPer];
+    auto load_head = [&](int h, int slot) {
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
         const uint32_t c = u * kWave + lane;
-        cm[u] = -INFINITY;
-        cl[u] = 0.f;
-        if (u * kWave < of && c < of) {
-          cm[u] = recs.ld(at_piece(c) + rec_m + h);
-          cl[u] = recs.ld(at_piece(c) + rec_l + h);
+        cm[slot][u] = -INFINITY;
+        cl[slot][u] = 0.f;
+        if (h < heads && u * kWave < of && c < of) {
+          cm[slot][u] = recs.ld(at_piece(c) + rec_m + h);
+          cl[slot][u] = recs.ld(at_piece(c) + rec_l + h);
         }
       }
+    };
+    auto weigh_head = [&](int h, int slot) {
+      if (h >= heads) return;
+      float m = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < kPer; ++u) m = fmaxf(m, cm[u]);
+      for (int u = 0; u < kPer; ++u) m = fmaxf(m, cm[slot][u]);
       m = wave_max(m);
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
         const uint32_t c = u * kWave + lane;
         if (c >= of) continue;
-        const float f = cm[u] == m ? 1.f : exp2_fast(cm[u] - m);
+        const float f = cm[slot][u] == m ? 1.f : exp2_fast(cm[slot][u] - m);
         weight[h][c] = f;
-        sum = fmaf(f, cl[u], sum);
+        sum = fmaf(f, cl[slot][u], sum);
       }
       sum = wave_sum(sum);
       if (lane == 0) sh.wl[0][h] = sum;
+    };
+    if constexpr (kSlots > 1) {
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) load_head(w + i * kWaves, i);
+    }
+    fetch(min(i0, items - 1), min(static_cast<uint32_t>(share), of - 1));
+    __syncthreads();  // the partial results have been read
+    if constexpr (kSlots > 1) {
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) weigh_head(w + i * kWaves, i);
+    } else {
+      for (int h = w; h < heads; h += kWaves) {
+        load_head(h, 0);
+        weigh_head(h, 0);
+      }
     }
     __syncthreads();
     for (int base = 0; base < items; base += kT) {
@@ -934,11 +956,11 @@ struct Attention {
 };
 
 // Workgroups of the short kernel that a CU holds, which its pieces are made for (16
-// beams at 576 positions in pieces of 4 tiles or more 8.9 us, of 8 10.8; 4 rows of
-// 3,000 with 8 KV heads of 128 in about 512 pieces 15.5 us, in 768 18.6; 64 rows to
-// 2,000 with 2 of 64 21.9 in 512, 20.4 in 768) and its registers: FP32 heads of 128 in
-// as many as they like, one a CU, 4 rows of 2,000 to 4,000 with 4 heads 23.8 us, in
-// those of two 20.3.
+// beams at 576 positions in pieces of 4 tiles or more 8.9 us, of 8 10.8, before the
+// join took its loads at once; 4 rows of 3,000 with 8 KV heads of 128 in about 512
+// pieces 15.5 us, in 768 18.6; 64 rows to 2,000 with 2 of 64 21.9 in 512, 20.4 in 768)
+// and its registers: FP32 heads of 128 in as many as they like, one a CU, 4 rows of
+// 2,000 to 4,000 with 4 heads 23.8 us, in those of two 20.3.
 constexpr uint32_t short_per_cu(uint32_t head_dim) { return head_dim == 128 ? 2 : 3; }
 
 // Few positions in all: a workgroup per piece, no more than `target` pieces
@@ -962,7 +984,7 @@ __global__ __launch_bounds__(kWaves *kWave, short_per_cu(D)) void attention_shor
   __syncthreads();
   a.put_piece(it, bad, first + static_cast<size_t>(it.home) * stride);
   if (it.pieces == 1) return;
-  if (a.arrive(it)) a.join(it, first, stride, stride);
+  if (a.arrive(it)) a.template join<kShortPieces>(it, first, stride, stride);
 }
 
 // Many: equal runs of all tiles, one for each workgroup that the card holds. V is read
@@ -1009,7 +1031,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
     bad = next_bad;
   }
   for (; to_join > 0; --to_join, join[0] = join[1]) {
-    a.join(join[0], record_of(join[0], 0), p.rec_floats, 2 * p.rec_floats);
+    a.template join<kMostPieces>(join[0], record_of(join[0], 0), p.rec_floats, 2 * p.rec_floats);
     __syncthreads();
   }
 }
