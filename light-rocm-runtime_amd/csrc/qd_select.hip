@@ -227,6 +227,17 @@ __device__ void fill_places(const SelectLaunch &p, uint32_t group, uint32_t foun
   }
 }
 
+// f(u) for the N shares of n things that a thread has, `step` of them in each: most
+// calls have no more than the first, and code that is not run is not fetched either.
+template <int N, typename F>
+__device__ __forceinline__ void for_shares(uint32_t n, uint32_t step, F &&f) {
+  f(0);
+  if (n > step) {
+#pragma unroll
+    for (int u = 1; u < N; ++u) f(u);
+  }
+}
+
 // Chooses among a group's rows; called by the workgroup that arrives last.
 __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh, Places &places) {
   constexpr int kMine = kSelectBeams * kSelectK / kT;
@@ -242,29 +253,20 @@ __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh, Places
   // A score's key: its 64 bits, monotone; 0 where there is none.
   uint64_t key[kMine];
   uint32_t token[kMine];
-#pragma unroll
-  for (int u = 0; u < kMine; ++u) {
-    const uint32_t i = u * kT + threadIdx.x;
-    key[u] = 0;
-    token[u] = 0;
-    if (u * kT < n) {  // (past the end the descriptors give zeros)
-      key[u] = load64(scores, i);
-      token[u] = tokens.ldu(i);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < kMine; ++u)
-    if (u * kT < n) held[u * kT + threadIdx.x] = token[u];
+  for_shares<kMine>(n, kT, [&](int u) {  // (past the end the descriptors give zeros)
+    key[u] = load64(scores, u * kT + threadIdx.x);
+    token[u] = tokens.ldu(u * kT + threadIdx.x);
+  });
   uint32_t best = 0;
-#pragma unroll
-  for (int u = 0; u < kMine; ++u) {
+  for_shares<kMine>(n, kT, [&](int u) {
+    held[u * kT + threadIdx.x] = token[u];
     const double s = __longlong_as_double(static_cast<long long>(key[u]));
     if (u * kT + threadIdx.x >= n || s == -INFINITY)
       key[u] = 0;
     else
       key[u] = key[u] >> 63 ? ~key[u] : key[u] | 1ull << 63;
     best = max(best, static_cast<uint32_t>(key[u] >> 32));
-  }
+  });
   const uint32_t bound = wave_bound(best, k);
   if (threadIdx.x == 0) sh.n = 0;
   if (lane_id() == 0) sh.bound[wave_id()] = bound;
@@ -273,16 +275,15 @@ __device__ void choose(const SelectLaunch &p, uint32_t group, Shared &sh, Places
 #pragma unroll
   for (int w = 1; w < kWavesPerBlock; ++w) least = max(least, sh.bound[w]);
   uint32_t mine = 0;
-#pragma unroll
-  for (int u = 0; u < kMine; ++u) mine += static_cast<uint32_t>(key[u] >> 32) >= least;
+  for_shares<kMine>(n, kT, [&](int u) { mine += static_cast<uint32_t>(key[u] >> 32) >= least; });
   if (mine) {
     uint32_t at = atomicAdd(&sh.n, mine);
-#pragma unroll
-    for (int u = 0; u < kMine; ++u)
+    for_shares<kMine>(n, kT, [&](int u) {
       if (static_cast<uint32_t>(key[u] >> 32) >= least) {
         list[at] = key[u];
         place[at++] = static_cast<uint16_t>(u * kT + threadIdx.x);
       }
+    });
   }
   __syncthreads();
   const uint32_t count = sh.n, found = min(count, k);
@@ -329,17 +330,13 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh, Places
   const uint32_t depth = k & 1 ? 1 : k / 2, across = k & 1 ? (n + 1) / 2 : p.runs;
   const float per = __builtin_amdgcn_rcpf(static_cast<float>(across));  // (below 1,024: exact where it is rounded down)
   uint64_t key[2 * kMine];
-#pragma unroll
-  for (int u = 0; u < kMine; ++u) {
-    key[2 * u] = key[2 * u + 1] = 0;
-    if (2 * u * kT < n) {
-      const uint32_t i = u * kT + threadIdx.x, down = static_cast<uint32_t>((static_cast<float>(i) + 0.5f) * per);
-      const float4 v = keys.ld4((i - down * across) * depth + down);  // (past the end: zeros)
-      const uint2 a = {__float_as_uint(v.x), __float_as_uint(v.y)}, b = {__float_as_uint(v.z), __float_as_uint(v.w)};
-      key[2 * u] = a.x | static_cast<uint64_t>(a.y) << 32;
-      key[2 * u + 1] = b.x | static_cast<uint64_t>(b.y) << 32;
-    }
-  }
+  for_shares<kMine>(n, 2 * kT, [&](int u) {
+    const uint32_t i = u * kT + threadIdx.x, down = static_cast<uint32_t>((static_cast<float>(i) + 0.5f) * per);
+    const float4 v = keys.ld4((i - down * across) * depth + down);  // (past the end: zeros)
+    const uint2 a = {__float_as_uint(v.x), __float_as_uint(v.y)}, b = {__float_as_uint(v.z), __float_as_uint(v.w)};
+    key[2 * u] = a.x | static_cast<uint64_t>(a.y) << 32;
+    key[2 * u + 1] = b.x | static_cast<uint64_t>(b.y) << 32;
+  });
   float m = -INFINITY;
   double sum = 0.0;
   for (uint32_t s = threadIdx.x; s < p.runs; s += kT) {
@@ -353,13 +350,15 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh, Places
     }
   }
   uint32_t best = 0;
+  for_shares<kMine>(n, 2 * kT, [&](int u) {
 #pragma unroll
-  for (int u = 0; u < 2 * kMine; ++u) {
-    // (Indexes past the end come to others' pairs, and an odd number of keys ends
-    // with half of a load.)
-    if (2 * ((u >> 1) * kT + threadIdx.x) + (u & 1) >= n) key[u] = 0;
-    best = max(best, static_cast<uint32_t>(key[u] >> 32));
-  }
+    for (int v = 2 * u; v < 2 * u + 2; ++v) {
+      // (Indexes past the end come to others' pairs, and an odd number of keys ends
+      // with half of a load.)
+      if (2 * (u * kT + threadIdx.x) + (v & 1) >= n) key[v] = 0;
+      best = max(best, static_cast<uint32_t>(key[v] >> 32));
+    }
+  });
   const uint32_t bound = wave_bound(best, k);
   const float wave_m = wave_max(m);
   if (lane_id() == 0) {
@@ -380,13 +379,16 @@ __device__ void join_row(const SelectLaunch &p, uint32_t row, Shared &sh, Places
   if (lane_id() == 0) sh.sum[wave_id()] = sum;
   uint64_t *list = &sh.own[0][0];
   uint32_t mine = 0;
-#pragma unroll
-  for (int u = 0; u < 2 * kMine; ++u) mine += static_cast<uint32_t>(key[u] >> 32) >= least;
+  for_shares<kMine>(n, 2 * kT, [&](int u) {
+    mine += (static_cast<uint32_t>(key[2 * u] >> 32) >= least) + (static_cast<uint32_t>(key[2 * u + 1] >> 32) >= least);
+  });
   if (mine) {
     uint32_t at = atomicAdd(&sh.n, mine);
+    for_shares<kMine>(n, 2 * kT, [&](int u) {
 #pragma unroll
-    for (int u = 0; u < 2 * kMine; ++u)
-      if (static_cast<uint32_t>(key[u] >> 32) >= least) list[at++] = key[u];
+      for (int v = 2 * u; v < 2 * u + 2; ++v)
+        if (static_cast<uint32_t>(key[v] >> 32) >= least) list[at++] = key[v];
+    });
   }
   __syncthreads();
   const uint32_t count = sh.n;
