@@ -231,10 +231,10 @@ __device__ void fill_places(const SelectLaunch &p, uint32_t group, uint32_t foun
 // calls have no more than the first, and code that is not run is not fetched either.
 template <int N, typename F>
 __device__ __forceinline__ void for_shares(uint32_t n, uint32_t step, F &&f) {
-  f(0);
-  if (n > step) {
 #pragma unroll
-    for (int u = 1; u < N; ++u) f(u);
+  for (int u = 0; u < N; ++u) {
+    if (u && n <= u * step) return;
+    f(u);
   }
 }
 
