@@ -459,7 +459,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   const float score = p.a.scores[row];
   const bool live = fabsf(score) < INFINITY;
   const bool done = p.a.done && p.a.done[row];
-  if (!live || done) {
+  if (__builtin_expect(!live || done, 0)) {
     // The logits do not matter: one continuation, or none.
     if (run) return;
     const Coherent scores(p.row_score + static_cast<size_t>(row) * k, k * 8);
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
           bits = c & 1 ? next[j][c >> 1] >> 16 : next[j][c >> 1] & 0xFFFFu;
         x[j * P::kElems + c] = widen<E>(bits);
       }
-      if (at + P::kElems > end) {  // the row's end: one by one
+      if (__builtin_expect(at + P::kElems > end, 0)) {  // the row's end: one by one
 #pragma unroll
         for (int c = 0; c < P::kElems; ++c) {
           float y = -INFINITY;
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
     }
     const float from = base == -INFINITY ? 0.f : base;
     float part = 0.f;
-    if (!__any(base == INFINITY)) {
+    if (__builtin_expect(!__any(base == INFINITY), 1)) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) part += fmaxf(exp2_fast((x[i] - from) * kLog2e), 0.f);
     } else {
@@ -535,7 +535,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
     if (__any(top >= least)) {
 #pragma unroll
       for (int j = 0; j < kPieces; ++j) {
-        if (count + kWave * P::kElems > kOwn) {
+        if (__builtin_expect(count + kWave * P::kElems > kOwn, 0)) {
           count = wave_best(own, count, k, sh.best[w]);
           // Later tokens are higher: only greater logits count. (A bound of
           // infinity keeps the infinite ones, of which enough are there.)
@@ -589,7 +589,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
   const uint32_t n = p.runs * k;
   const Coherent keys(p.keys + static_cast<size_t>(row) * (n + (n & 1)), (n + (n & 1)) * 8);
   uint32_t all = sh.n;
-  if (all <= static_cast<uint32_t>(kFew)) {
+  if (__builtin_expect(all <= static_cast<uint32_t>(kFew), 1)) {
     for (uint32_t i = threadIdx.x / 4; i < all; i += kT / 4) {
       const uint64_t key = sh.few[i];
       const uint32_t rank = quad_rank(key, sh.few, all);
