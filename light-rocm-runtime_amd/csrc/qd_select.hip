@@ -7,8 +7,8 @@
 // best k. The last run of a row to arrive joins the row's best k with their
 // scores; the last row of a group to arrive chooses among its beams'. Bound by
 // the logits' bandwidth for many rows (32 groups of 8 beams x 151,936 in FP32, 156 MB,
-// 40.8 us, of which 26 stream at 6.0 TB/s), by the hand-overs for few: 16 beams 14.8
-// us, one 8.7, of which the logits take 3.
+// 40 us, of which 26 stream at 6.0 TB/s), by the hand-overs for few: 16 beams 14.4
+// us, one 8.5, of which the logits take 3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
