@@ -1043,7 +1043,8 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
 // and counts (16 beams over pages of 24 layers: 5 of 9.2 us); the copies stream (64
 // rows that copy about 22 pages of 2 x 8 layers x 128 KB, 91 MB, 24 us in all).
 constexpr int kForkT = 1024, kForkWaves = kForkT / kWave;
-constexpr int kForkScan = 8;  // counts that a thread looks at for free pages per pass
+constexpr int kForkScan = 8;   // counts that a thread looks at for free pages per pass
+constexpr int kForkEarly = 4;  // rows of a wave that are on their way
 
 struct ForkRow {
   int32_t parent;   // -1: released
@@ -1094,23 +1095,33 @@ __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t *waves, ui
   return before + upto - v;
 }
 
+// The first columns of a row, a lane each.
+__device__ __forceinline__ int32_t first_columns(const ForkLaunch &p, uint32_t r) {
+  const uint32_t lane = lane_id();
+  return r < p.a.rows && lane < p.a.table_width ? p.a.table[r * p.a.table_stride + lane] : -1;
+}
+
 // Adds `sign` times what the fork changes: a page that an old row takes over to
 // c children counts c - 1 more, one behind its length one less. `early` holds the
-// first columns of each wave's first row.
+// first columns of each wave's first rows; those of later ones are asked for as many
+// rows ahead.
 __device__ __forceinline__ void count_references(const ForkLaunch &p, const int *children, const int *lengths, int sign,
-                                                 int32_t early, uint32_t *bad) {
+                                                 const int32_t (&early)[kForkEarly], uint32_t *bad) {
   const int lane = lane_id();
+  int32_t columns[kForkEarly];
+#pragma unroll
+  for (int u = 0; u < kForkEarly; ++u) columns[u] = early[u];
   for (uint32_t r = wave_id(); r < p.a.rows; r += kForkWaves) {
+    const int32_t first = columns[0];
+#pragma unroll
+    for (int u = 0; u + 1 < kForkEarly; ++u) columns[u] = columns[u + 1];
+    columns[kForkEarly - 1] = first_columns(p, r + kForkEarly * kForkWaves);
     const int32_t *table = p.a.table + r * p.a.table_stride;
     const uint32_t held = (static_cast<uint32_t>(lengths[r]) + p.a.page_size - 1) >> p.page_shift;
     const int change = children[r] - 1;
     for (uint32_t base = 0;; base += kWave) {
       const uint32_t j = base + lane;
-      int32_t id = -1;
-      if (base == 0 && r == static_cast<uint32_t>(wave_id()))
-        id = early;
-      else if (j < p.a.table_width)
-        id = table[j];
+      const int32_t id = base == 0 ? first : j < p.a.table_width ? table[j] : -1;
       // Entries behind the first negative one, or the last column, are none.
       const uint64_t ends = __ballot(id < 0);
       if ((ends & ((1ull << lane) - 1)) == 0 && id >= 0) {
@@ -1139,9 +1150,10 @@ __global__ __launch_bounds__(kForkT) void fork_plan_kernel(ForkLaunch p) {
   const uint32_t r = threadIdx.x;  // one thread per row where rows are meant
   static_assert(kForkT == kForkRows, "a thread per row");
   const int64_t room = static_cast<int64_t>(p.a.table_width) << p.page_shift;
-  // Nothing here waits for another: the wave's first row, the lengths and parents.
-  const uint32_t wave_row = wave_id(), lane = lane_id();
-  const int32_t early = wave_row < p.a.rows && lane < p.a.table_width ? p.a.table[wave_row * p.a.table_stride + lane] : -1;
+  // Nothing here waits for another: the wave's first rows, the lengths and parents.
+  int32_t early[kForkEarly];
+#pragma unroll
+  for (int u = 0; u < kForkEarly; ++u) early[u] = first_columns(p, wave_id() + u * kForkWaves);
   ForkRow row{-1, 0, -1, 0u, 0, 0};
   if (r < p.a.rows) {
     children[r] = 0;
