@@ -1075,15 +1075,9 @@ __device__ __forceinline__ int32_t load_count(int32_t *p) {
 
 // Sum over the lanes before this one, and over all waves before.
 __device__ __forceinline__ uint32_t block_before(uint32_t v, uint32_t *waves, uint32_t &total) {
-  uint32_t upto = v;
-  const int lane = lane_id();
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const uint32_t x = __shfl_up(upto, o, kWave);
-    if (lane >= o) upto += x;
-  }
+  const uint32_t upto = lanes_upto(v);
   __syncthreads();
-  if (lane == kWave - 1) waves[wave_id()] = upto;
+  if (lane_id() == kWave - 1) waves[wave_id()] = upto;
   __syncthreads();
   uint32_t before = 0;
   total = 0;
