@@ -1040,11 +1040,13 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
 // The first kernel, one workgroup, counts references, decides which rows copy
 // their last page and deals out free pages; the second writes the new table and
 // copies pages. The first is bound by latency, a few dependent passes over tables
-// and counts (16 beams over pages of 24 layers: 5 of 9.2 us); the copies stream (64
-// rows that copy about 22 pages of 2 x 8 layers x 128 KB, 91 MB, 24 us in all).
+// and counts (16 beams over pages of 24 layers: 4.5 of 8.8 us); the copies stream (64
+// rows that copy about 22 pages of 2 x 8 layers x 128 KB, 91 MB, 23.5 us in all).
 constexpr int kForkT = 1024, kForkWaves = kForkT / kWave;
 constexpr int kForkScan = 8;   // counts that a thread looks at for free pages per pass
-constexpr int kForkEarly = 4;  // rows of a wave that are on their way
+// Rows of a wave that are on their way (256 rows of 4 beams 24.0 us, two at a time
+// 24.6, eight 23.4, but then 8 x 8 beams 23.8 instead of 23.5).
+constexpr int kForkEarly = 4;
 
 struct ForkRow {
   int32_t parent;   // -1: released
