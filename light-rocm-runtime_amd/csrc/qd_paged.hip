@@ -873,8 +873,8 @@ struct Attention {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) next[u] = recs.ld4((at_piece(min(c + u * shares, of - 1)) + h * D + d) / 4);
     };
-    // A wave's heads' maxima and sums: all on their way at once in the short kernel (16
-    // beams at 576 8.5 us, head after head 8.95).
+    // A wave's heads' maxima and sums: all on their way at once where the pieces are no
+    // more than lanes (16 beams at 576 8.5 us, head after head 8.95).
     constexpr int kPer = kMost / kWave, kSlots = kPer == 1 ? 16 / kWaves : 1;
     float cm[kSlots][kPer], cl[kSlots][kPer];
     auto load_head = [&](int h, int slot) {
@@ -1031,7 +1031,10 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
     bad = next_bad;
   }
   for (; to_join > 0; --to_join, join[0] = join[1]) {
-    a.template join<kMostPieces>(join[0], record_of(join[0], 0), p.rec_floats, 2 * p.rec_floats);
+    if (join[0].pieces <= kShortPieces)
+      a.template join<kShortPieces>(join[0], record_of(join[0], 0), p.rec_floats, 2 * p.rec_floats);
+    else
+      a.template join<kMostPieces>(join[0], record_of(join[0], 0), p.rec_floats, 2 * p.rec_floats);
     __syncthreads();
   }
 }
