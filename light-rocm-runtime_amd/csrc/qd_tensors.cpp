@@ -173,7 +173,12 @@ PyObject *call_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     g.positions = flat<const int32_t>("positions", a[5], at::kInt, {tokens}, device);
     g.rows = flat_or_null<const int32_t>("rows", a[6], at::kInt, {tokens}, device);
-    g.interleaved = PyObject_IsTrue(a[9]) == 1;
+    const int interleaved = PyObject_IsTrue(a[9]);
+    if (interleaved < 0) {
+      PyErr_Clear();
+      refuse("interleaved is neither true nor false");
+    }
+    g.interleaved = static_cast<uint32_t>(interleaved);
     g.position_bias = static_cast<int32_t>(whole("position_bias", a[10], INT32_MIN, INT32_MAX));
     g.tokens = static_cast<uint32_t>(tokens);
     return queue<const qd_paged_cache *, const qd_append_args *, void *>(g_calls.append, c, &g, address("stream", a[11]));

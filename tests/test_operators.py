@@ -290,6 +290,7 @@ def test_arguments_that_are_something_else_are_refused():
             (lambda: ops.paged_append(c, None, None, None, new, lengths), "k is missing"),
             (lambda: ops.paged_append(c, None, None, new, new, lengths, position_bias=1.5), "position_bias"),
             (lambda: ops.paged_append(c, None, None, new, new, lengths, stream="s"), "stream"),
+            (lambda: ops.paged_append(c, None, None, new, new, lengths, interleaved=q), "interleaved"),
             (lambda: ops.paged_append(c, q, q, new, new, lengths, cos=new[0, 0]), "cos and sin"),
             (lambda: ops.paged_append(c, q, q[:, :3], new, new, lengths), "q_out has shape"),
             (lambda: ops.paged_attention(c, q, q, closed), "null workspace"),
