@@ -1220,6 +1220,15 @@ __global__ __launch_bounds__(kForkT) void fork_plan_kernel(ForkLaunch p) {
       row.fresh = static_cast<int>(need) - row.held + (row.source >= 0);
     }
     row.begin = block_before(row.fresh, waves, wanted);
+    // A row takes no more pages than the table has columns. Where all rows' may pass 32
+    // bits, they are counted by 256 first: more of those than the pool has are too many,
+    // and with no more the sum is below 2^31 + 2^18. (A table of 16 GB or more: the
+    // others do without the second sum.)
+    if (static_cast<uint64_t>(p.a.rows) * p.a.table_width >> 32) {
+      uint32_t parts;
+      block_before(static_cast<uint32_t>(row.fresh) >> 8, waves, parts);
+      if (parts > p.a.pages >> 8) wanted = UINT32_MAX;
+    }
     // The free pages of the lowest ids.
     for (uint32_t base = 0; base < p.a.pages && found < wanted; base += kForkT * kForkScan) {
       if (base) look(base);

@@ -512,6 +512,37 @@ def test_fork_changes_nothing_where_it_fails(what):
     s.compare()
 
 
+@pytest.mark.parametrize("each", [1 << 22, (1 << 22) + 1])
+def test_fork_that_wants_more_pages_than_32_bits_count(each):
+    """1,024 rows that want 2^22 pages each, 2^32 in all, and one more each: too many, whatever is left of
+    their sum in 32 bits."""
+    rows, width, pages, page = 1024, (1 << 22) + 1, 2000, 16
+    say("fork of more than 2^32 pages", each)
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("two tables of 17 GB")
+    table = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+    table_out = torch.zeros_like(table)
+    lengths = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    lengths_out = torch.full_like(lengths, 7)
+    refs, errors = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (pages, 1))
+    refs[::3] = 1
+    before = refs.clone()
+    ops.pages_fork(ops.PagePool(refs, page, []), table, lengths, None, each * page, table_out, lengths_out,
+                   ops.Workspace(ops.fork_workspace(rows, pages)), errors=errors)
+    assert int(errors) == ops.EXHAUSTED
+    assert torch.equal(refs, before) and not lengths_out.any()
+    assert all(bool((part == -1).all()) for part in table_out.split(64))
+    # A few rows of the same table that fit.
+    errors.zero_()
+    few = torch.full((rows,), -1, dtype=torch.int32)
+    few[[3, 1000]] = int32([5, 5])
+    ops.pages_fork(ops.PagePool(refs, page, []), table, lengths, few.cuda(), 20, table_out, lengths_out,
+                   ops.Workspace(ops.fork_workspace(rows, pages)), errors=errors)
+    assert int(errors) == 0 and refs.sum().item() == before.sum().item() + 4
+    assert table_out[3, :3].tolist() == [1, 2, -1] and table_out[1000, :3].tolist() == [4, 5, -1]
+    assert lengths_out.sum().item() == 40
+
+
 # ---- select -------------------------------------------------------------------------------
 
 
