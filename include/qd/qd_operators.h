@@ -135,8 +135,10 @@ QD_API qd_status qd_paged_append(const qd_paged_cache *cache, const qd_append_ar
  * positions 0 .. lengths[r] - 1 of KV head h / (heads / kv_heads),
  *   out[r][h] = sum_j softmax_j(scale q[r][h] . K_j) V_j,
  * statistics and sums in FP32 (products are summed before they are divided, by
- * weights up to 2^8: finite for |V| below 2^89). A row of length 0 gets zeros; what the pages
- * hold past a row's length is not read. A row with a bad length or page gets
+ * weights up to 2^8: finite for |V| below 2^89). 16-bit types multiply a weight as two numbers,
+ * off by at most 2^-16 of it in BF16 and in FP16 by 2^-22 of it or 2^-51 of the row's largest,
+ * whichever is more; an infinite V makes the outputs that it reaches infinite or NaN. A row of
+ * length 0 gets zeros; what the pages hold past a row's length is not read. A row with a bad length or page gets
  * NaN. q and out are [rows][heads][head_dim] with strides that are multiples of
  * 16 bytes; out may be q itself, with its strides. The result of a row does not depend on when
  * its parts finish (they are joined in order), but how its positions are split

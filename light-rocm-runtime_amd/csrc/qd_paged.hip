@@ -250,9 +250,17 @@ constexpr uint32_t kEdge = 2;
 // to 256 pieces 25.3; all before V was loaded with K).
 constexpr uint32_t kShortLeast = 4, kShortWhole = 8, kShortPieces = 64;
 // A maximum is only taken up when it passes the one in use by this many powers of
-// two: until then probabilities grow to at most 2^8, in every type's range. (Taken up
-// at once, 64 rows of 0 to 8,192 took 193 us instead of 192.)
+// two: until then probabilities grow to at most 2^8. (Taken up at once, 64 rows of 0 to
+// 8,192 took 193 us instead of 192.) FP16's range is needed at the other end.
+template <typename E>
 constexpr float kLazyMax = 8.f;
+template <>
+constexpr float kLazyMax<Half> = 1.f;
+// What FP16 takes of a probability p, at most 2 before it is rounded: kWeight p, up to
+// 2^15, and kRest times the remainder, up to 2^3. Half of the least step, 2^-25, is then
+// 2^-51 of the largest probability (as they are, without these factors, 2^-25: all
+// that lay more than 17 below the largest score counted in the sum, but in no output).
+constexpr float kWeight = 0x1p14f, kRest = 0x1p12f;
 
 struct AttnLaunch {
   qd_paged_cache c;
@@ -516,6 +524,7 @@ struct WaveTiles {
   static constexpr int kElem = kWide ? 4 : 2;
   static constexpr int kPieces = D * kElem / 64;  // 16-byte loads of K per lane and half tile
   static constexpr int kAcc = D / 16;
+  static constexpr bool kScaled = std::is_same_v<E, Half>;  // o holds kWeight times the sum
   u4v q[kPieces];
   u4v k[kStages][2][kPieces];
   u4v v[kStages][2][4][kWide ? D / 64 : 1];  // rows 4 (l / 16) + j; 16-bit rows of 64 use half of a register quad
@@ -577,26 +586,44 @@ struct WaveTiles {
         }
     } else {
       // A probability goes to the matrix instruction as two numbers of the cache's
-      // type, rounded and what that left, so that its rounding adds nothing to the
-      // output's own (alone it made that 1.4 times as large); the second product
-      // costs no time that the loads do not take.
+      // type, rounded and what that left, so that its rounding adds little to the
+      // output's own (alone it made that 1.4 times as large): 2^-16 of it in BF16, whose
+      // range is FP32's, in FP16 2^-22 of it or 2^-51 of the largest. The second
+      // product costs no time that the loads do not take.
       u4v b, rest;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float x = pr[i >> 1][2 * (i & 1)], y = pr[i >> 1][2 * (i & 1) + 1];
-        b[i] = E::pack(x, y);
-        rest[i] = E::pack(x - E::lo(b[i]), y - E::hi(b[i]));
+        if constexpr (kScaled) {
+          b[i] = E::pack(x * kWeight, y * kWeight);
+          rest[i] = E::pack(fmaf(x, kWeight, -E::lo(b[i])) * kRest, fmaf(y, kWeight, -E::hi(b[i])) * kRest);
+        } else {
+          b[i] = E::pack(x, y);
+          rest[i] = E::pack(x - E::lo(b[i]), y - E::hi(b[i]));
+        }
         sum += x + y;
       }
+      uint32_t low = 0x05040100u, high = 0x07060302u;  // the pairs' halves
 #pragma unroll
       for (int j = 0; j < kAcc; ++j) {
         u4v a;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           a[i] = __builtin_amdgcn_perm(v[st][i >> 1][2 * (i & 1) + 1][0][j >> 1], v[st][i >> 1][2 * (i & 1)][0][j >> 1],
-                                       j & 1 ? 0x07060302u : 0x05040100u);
-        o[j] = E::mfma(a, rest, o[j]);
-        o[j] = E::mfma(a, b, o[j]);
+                                       j & 1 ? high : low);
+        if constexpr (kScaled) {
+          const f4v r = E::mfma(a, rest, f4v{0.f, 0.f, 0.f, 0.f});
+          o[j] = E::mfma(a, b, o[j]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[j][c] = fmaf(r[c], 1.f / kRest, o[j][c]);
+          // Four at a time: with all eight on their way FP16 heads of 128 take the registers
+          // of two workgroups a CU, not three (8 rows of 1,000 to 2,000 with 8 KV heads 17.6
+          // us, so 16.6; two of 90,001 to 120,001 with 4 85.4 and 85.3).
+          if ((j & 3) == 3) asm volatile("" : "+s"(low), "+s"(high), "+v"(o[j - 3]), "+v"(o[j - 2]), "+v"(o[j - 1]), "+v"(o[j]));
+        } else {
+          o[j] = E::mfma(a, rest, o[j]);
+          o[j] = E::mfma(a, b, o[j]);
+        }
       }
     }
     return sum;
@@ -731,7 +758,7 @@ struct Attention {
     float top = s[0][0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i >> 2][i & 3]);
-    if (__any(top > t.m + kLazyMax)) {
+    if (__any(top > t.m + kLazyMax<E>)) {
       const float m = fmaxf(t.m, quarters_max(top));
       const float f = m == t.m ? 1.f : exp2_fast(t.m - m);
       t.m = m;
@@ -786,6 +813,7 @@ struct Attention {
   }
   // The waves' partial results to LDS. A barrier before the next ones.
   __device__ __forceinline__ void put_partials() {
+    constexpr float unit = Tiles::kScaled ? 1.f / kWeight : 1.f;
     const float l = quarters_sum(t.l);
     if (quad == 0) {
       sh.wm[w][col] = t.m;
@@ -796,7 +824,7 @@ struct Attention {
 #pragma unroll
       for (int n = 0; n < D / 64; ++n)
         *reinterpret_cast<float4 *>(&sh.wo[w][col][Tiles::dim_of(r, n)]) =
-            make_float4(t.o[4 * n][r], t.o[4 * n + 1][r], t.o[4 * n + 2][r], t.o[4 * n + 3][r]);
+            make_float4(t.o[4 * n][r] * unit, t.o[4 * n + 1][r] * unit, t.o[4 * n + 2][r] * unit, t.o[4 * n + 3][r] * unit);
   }
   // The piece's result, out or to its record. sh.spoilt is zero, and is again.
   __device__ __forceinline__ void put_piece(const Item &it, bool bad, float *record) {

@@ -324,6 +324,41 @@ def test_attention_infinities_follow_the_formula():
     assert torch.isnan(run_attention(q, k, v, table, int32([64]), 1.0)).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim,length,pool_mb", [(64, 60, 0), (128, 4000, 0), (64, 4000, 100), (128, 8192, 100), (64, 30001, 100)])
+def test_attention_of_one_large_score_and_many_small_ones(dtype, dim, length, pool_mb):
+    """A position that takes nearly all of the weight and whose V is zero: the output is what the many
+    others, of equal scores 11 to 27 below, add up to."""
+    say("attention: a large score, many small ones", dtype, dim, length, pool_mb)
+    gaps = [11.0, 14.0, 16.0, 17.5, 20.0, 24.0, 27.0]
+    g, page, kv_heads, group = seeded(dim + length), 64, 2, 3
+    spare = (pool_mb << 20) // (2 * page * kv_heads * dim * (4 if dtype == F32 else 2)) + 1
+    lengths = [length] * len(gaps)
+    table, pages = tables_for(g, lengths, page, max(-(-length // page), -(-spare // len(gaps))), spare=spare)
+    q = torch.zeros((len(gaps), group * kv_heads, dim), dtype=dtype)
+    q[:, :, 0] = 1.0
+    k = torch.zeros((pages, page, kv_heads, dim), dtype=dtype)
+    v = torch.zeros_like(k)
+    for r, gap in enumerate(gaps):
+        held = table[r, : -(-length // page)].long()
+        v[held] = normal(g, (len(held), page, kv_heads, dim), dtype) + 1.0
+        at = (r * 997) % length
+        k[table[r, at // page].long(), at % page, :, 0] = gap
+        v[table[r, at // page].long(), at % page] = 0.0
+    n = int32(lengths)
+    out = run_attention(q, k, v, table, n, 1.0)
+    want, bound = oracle.attention(q, k, v, table, n, 1.0)
+    if dtype != F32:
+        # The oracle allows each weight half of the type's least step, which is all of the small ones. They
+        # keep their relative precision (in its bound already) down to 2^-51 of the largest, half a step of
+        # the remainder that FP16 keeps of a weight: 2^14 times the weight, and 2^12 times what is left of it,
+        # in steps of 2^-24. (BF16's least step is 2^-133.)
+        most = torch.stack([v[table[r, : -(-length // page)].long()].flatten(0, 1)[:length].double().abs().amax(0) for r in range(len(gaps))])
+        bound -= 2 * length * oracle.HALF_LEAST[dtype] * most.repeat_interleave(group, 1)
+        bound += length * 2.0 ** -51 * most.repeat_interleave(group, 1)
+    close(out, want, bound, "out")
+
+
 @pytest.mark.parametrize("length", [40, 3000])
 def test_attention_marks_bad_rows_and_no_others(length):
     say("attention: bad lengths and pages", length)
