@@ -465,7 +465,7 @@ __global__ __launch_bounds__(kT) void select_kernel(SelectLaunch p) {
     const Coherent scores(p.row_score + static_cast<size_t>(row) * k, k * 8);
     const Coherent tokens(p.row_token + static_cast<size_t>(row) * k, k * 4);
     for (uint32_t i = threadIdx.x; i < k; i += kT) {
-      const double s = live && i == 0 ? static_cast<double>(score) : -INFINITY;
+      const double s = live && i == 0 ? static_cast<double>(score) + 0.0 : -INFINITY;  // (-0 is no lower than 0)
       store64(scores, i, static_cast<uint64_t>(__double_as_longlong(s)));
       tokens.stu(i, p.a.eos);
     }

@@ -654,6 +654,19 @@ def test_select_ties_go_to_the_lower_token_and_beam():
     assert got[1].tolist() == [[0] * 64] and got[2].tolist() == [list(range(64))]
 
 
+def test_select_scores_of_zero_are_equal():
+    say("select: finished beams of scores -0 and 0")
+    got = run_select(torch.zeros(2, 3, 100), torch.tensor([[-0.0, 0.0, -0.0], [-1.0, 0.0, -0.0]]), 2,
+                     torch.ones(2, 3, dtype=torch.uint8), 7)
+    assert got[1].tolist() == [[0, 1], [4, 5]] and got[2].tolist() == [[7, 7], [7, 7]]
+    assert got[0].tolist() == [[0.0, 0.0], [0.0, 0.0]] and got[3].tolist() == [[1, 1], [1, 1]]
+    # A finished one at -0 beside one whose only token costs nothing.
+    logits = torch.full((1, 2, 100), -math.inf)
+    logits[0, 1, 5] = 3.0
+    got = run_select(logits, torch.tensor([[-0.0, 0.0]]), 1, torch.tensor([[1, 0]], dtype=torch.uint8), 7)
+    assert got[1].tolist() == [[0]] and got[2].tolist() == [[7]]
+
+
 def test_select_masks():
     say("select: masks, dead and finished beams, NaN")
     g = seeded(2)
