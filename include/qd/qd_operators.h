@@ -251,6 +251,7 @@ typedef struct qd_select_args {
   int32_t device;
 } qd_select_args;
 QD_API qd_status qd_beam_select(const qd_select_args *args, qd_workspace *workspace, void *stream);
+/* Bytes of workspace that calls of up to so many groups, beams, places and tokens need. */
 QD_API qd_status qd_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab, size_t *bytes);
 
 #ifdef __cplusplus

@@ -517,10 +517,9 @@ struct qd_engine {
     take(w.qkv, r * QKV);
     take(w.logits, r * V);
     take(w.scratch.counters, qd::kOpCounters);
-    size_t scratch = std::max(qd::paged_attention_scratch(uint32_t(r), uint32_t(NQ), uint32_t(NKV), qd::kHeadDim),
-                              qd::pages_fork_scratch(uint32_t(r), pages));
-    for (uint32_t n = 1; n <= r; ++n) scratch = std::max(scratch, qd::beam_select_scratch(1, n, n, uint32_t(V)));
-    take(w.scratch.scratch, scratch);
+    take(w.scratch.scratch, std::max({qd::paged_attention_scratch(uint32_t(r), uint32_t(NQ), uint32_t(NKV), qd::kHeadDim),
+                                      qd::pages_fork_scratch(uint32_t(r), pages),
+                                      qd::beam_select_scratch_most(1, uint32_t(r), uint32_t(r), uint32_t(V))}));
     return w;
   }
   void beam_workspace(uint32_t pages, uint32_t steps) {

@@ -335,7 +335,7 @@ qd_status qd_pages_fork(const qd_fork_args *a, qd_workspace *w, void *stream) {
 qd_status qd_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab, size_t *bytes) {
   if (!bytes) return invalid("null argument");
   QD_TRY(check_select(groups, beams, k, vocab));
-  *bytes = qd::beam_select_scratch(groups, beams, k, vocab);
+  *bytes = qd::beam_select_scratch_most(groups, beams, k, vocab);
   return QD_SUCCESS;
 }
 

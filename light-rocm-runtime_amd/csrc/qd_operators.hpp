@@ -37,7 +37,9 @@ hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const 
 size_t pages_fork_scratch(uint32_t rows, uint32_t pages);
 hipError_t launch_pages_fork(hipStream_t s, const qd_fork_args &a, const OpScratch &w);
 
+// What one call needs, and the most that any call of up to these sizes does.
 size_t beam_select_scratch(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab);
+size_t beam_select_scratch_most(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab);
 hipError_t launch_beam_select(hipStream_t s, const qd_select_args &a, const OpScratch &w);
 
 }  // namespace qd

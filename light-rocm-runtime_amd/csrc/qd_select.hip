@@ -670,6 +670,15 @@ size_t beam_select_scratch(uint32_t groups, uint32_t beams, uint32_t k, uint32_t
   return carve(p, nullptr, rows, k);
 }
 
+// Whatever the rows, they are in no more parts than tiles, and than kAim or one each;
+// fewer rows, places or tokens can be in more parts than more of them.
+size_t beam_select_scratch_most(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab) {
+  const size_t rows = static_cast<size_t>(groups) * beams;
+  const size_t parts = std::min<size_t>(rows * tiles_of(vocab), std::max<size_t>(rows, kAim));
+  const size_t keys = std::min(parts * k, rows * kJoin) + rows;  // (an odd row's rest of a pair)
+  return round256(keys * 8) + round256(parts * 8) + round256(parts * 4) + round256(rows * k * 8) + round256(rows * k * 4);
+}
+
 hipError_t launch_beam_select(hipStream_t s, const qd_select_args &a, const OpScratch &w) {
   const uint32_t rows = a.groups * a.beams;
   if (rows == 0) return hipSuccess;

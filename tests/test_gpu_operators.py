@@ -870,6 +870,21 @@ def test_fork_copies_memories_of_different_sizes():
         assert torch.equal(d.cpu(), m)
 
 
+def test_select_in_a_workspace_of_more_rows():
+    """A workspace of the largest batch serves every smaller one."""
+    say("select: a workspace of more groups, beams, places and tokens")
+    g, vocab = seeded(31), 30011
+    workspace = ops.Workspace(ops.select_workspace(75, 8, 46, vocab))
+    for groups, beams, k, tokens in ((75, 8, 46, vocab), (64, 8, 46, vocab), (1, 8, 46, vocab), (64, 8, 8, vocab),
+                                     (3, 1, 45, vocab), (74, 7, 1, 28000)):
+        logits, scores = normal(g, (groups, beams, tokens), F32, 3.0), torch.zeros(groups, beams)
+        out = [torch.empty((groups, k), device="cuda")] + [torch.empty((groups, k), dtype=torch.int32, device="cuda") for _ in range(2)]
+        ops.beam_select(logits.cuda(), scores.cuda(), *out, workspace)
+        picked, _ = oracle.select(logits, scores, None, None, 1)
+        for i in range(groups):
+            assert abs(float(out[0][i, 0]) - picked[i][0][0]) <= oracle.select_bound(picked[i][0][0])
+
+
 def test_select_of_the_largest_vocabulary():
     say("select of 2^24 tokens")
     g = seeded(24)

@@ -249,6 +249,18 @@ def test_workspace_sizes():
         ops.select_workspace(1, 16, 65, 1000)
 
 
+def test_a_selection_never_needs_more_than_a_larger_one():
+    rng = random.Random(7)
+    for _ in range(3000):
+        beams, vocab = rng.randint(1, 32), int(10 ** rng.uniform(0, 7.2))
+        sizes = [rng.randint(1, 65535 // (beams + 1)), beams, rng.randint(1, min(64, beams * vocab)), vocab]
+        least = [rng.randint(1, n) for n in sizes]
+        fewer = [rng.choice(pair) for pair in zip(sizes, least)]
+        if fewer[2] <= fewer[1] * fewer[3]:
+            assert ops.select_workspace(*fewer) <= ops.select_workspace(*sizes), (fewer, sizes)
+    assert ops.select_workspace(64, 8, 8, 151936) <= ops.select_workspace(75, 8, 8, 151936)
+
+
 @pytest.mark.skipif(qd.device_count() > 0, reason="host-without-GPU behaviour")
 def test_without_a_gpu_calls_fail_loudly():
     with pytest.raises(qd.QdError) as e:
