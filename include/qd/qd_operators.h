@@ -155,7 +155,7 @@ typedef struct qd_attention_args {
 } qd_attention_args;
 QD_API qd_status qd_paged_attention(const qd_paged_cache *cache, const qd_attention_args *args, qd_workspace *workspace,
                                     void *stream);
-/* Bytes of workspace that a cache of `rows` rows needs at most. */
+/* Bytes of workspace that caches of up to `rows` rows need with these heads. */
 QD_API qd_status qd_paged_attention_workspace(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                                               size_t *bytes);
 

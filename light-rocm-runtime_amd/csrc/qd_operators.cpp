@@ -254,7 +254,7 @@ qd_status qd_paged_attention_workspace(uint32_t rows, uint32_t heads, uint32_t k
   QD_TRY(check_heads(heads, kv_heads));
   if (head_dim != 64 && head_dim != 128) return refuse(QD_ERROR_NOT_SUPPORTED, "head_dim %u: the kernels take 64 and 128", head_dim);
   if (rows > (1u << 20)) return invalid("too many rows");
-  *bytes = qd::paged_attention_scratch(rows, heads, kv_heads, head_dim);
+  *bytes = qd::paged_attention_scratch_most(rows, heads, kv_heads, head_dim);
   return QD_SUCCESS;
 }
 

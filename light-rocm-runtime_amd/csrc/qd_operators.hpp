@@ -30,8 +30,9 @@ hipError_t launch_op_clear(hipStream_t s, uint32_t *counters, size_t n);
 
 hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_append_args &a);
 
-// Scratch bytes of an attention over `rows` rows.
+// Scratch bytes of an attention over `rows` rows, and the most of one over up to so many.
 size_t paged_attention_scratch(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
+size_t paged_attention_scratch_most(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w);
 
 size_t pages_fork_scratch(uint32_t rows, uint32_t pages);

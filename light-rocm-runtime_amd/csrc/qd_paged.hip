@@ -1440,6 +1440,12 @@ size_t paged_attention_scratch(uint32_t rows, uint32_t heads, uint32_t kv_heads,
   return static_cast<size_t>(sh.records) * sh.rec_floats * sizeof(float);
 }
 
+// (More rows than there are counters for are not cut and keep nothing; fewer are.)
+size_t paged_attention_scratch_most(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  const uint32_t parts = attention_shape(0, heads, kv_heads, head_dim).parts;
+  return paged_attention_scratch(std::min(rows, static_cast<uint32_t>(kOpCounters / parts)), heads, kv_heads, head_dim);
+}
+
 // The long kernel's tiles ahead and workgroups on a CU, by type and head_dim: with 64
 // to 128 KB on their way to each CU, more only queue. Measured on 430 to 680 MB, tiles
 // x workgroups: FP32 of 128 1 x 1 66.9 us, 2 x 1 68.6, 1 x 2 71.6; FP32 of 64 2 x 1 47.8,

@@ -841,6 +841,20 @@ def test_attention_of_more_rows_than_counters():
     assert not out[(lengths == 0).cuda()].any()
 
 
+def test_attention_in_a_workspace_of_more_rows():
+    """Past 65,536 pairs of a row and a KV head nothing is kept; fewer rows keep records."""
+    say("attention: a workspace of more rows")
+    g, page = seeded(32), 16
+    workspace = ops.Workspace(ops.attention_workspace(40000, 2, 2, 64))
+    for lengths in ([3000], [3000, 0, 700]):
+        table, pages = tables_for(g, lengths, page, -(-3000 // page))
+        q = normal(g, (len(lengths), 2, 64), F32, 1.5)
+        k, v = (normal(g, (pages, page, 2, 64), F32) for _ in range(2))
+        out = torch.full(q.shape, NAN, device="cuda")
+        ops.paged_attention(ops.PagedCache(k.cuda(), v.cuda(), table.cuda(), int32(lengths).cuda()), out, q.cuda(), workspace)
+        close(out, *oracle.attention(q, k, v, table, int32(lengths), 0.125), "out")
+
+
 def test_fork_of_the_most_rows():
     say("fork of 1,024 rows")
     s = Forked(1024, 6000, 5, 16, planes=1)

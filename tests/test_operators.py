@@ -249,6 +249,13 @@ def test_workspace_sizes():
         ops.select_workspace(1, 16, 65, 1000)
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (14, 2), (16, 1), (48, 3), (128, 8), (65536, 4096), (63000, 3000)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_never_needs_more_than_of_more_rows(heads, kv_heads, dim):
+    sizes = [ops.attention_workspace(rows, heads, kv_heads, dim) for rows in [*range(40), *range(40, 1 << 17, 997), 1 << 20]]
+    assert sizes == sorted(sizes)
+
+
 def test_a_selection_never_needs_more_than_a_larger_one():
     rng = random.Random(7)
     for _ in range(3000):
