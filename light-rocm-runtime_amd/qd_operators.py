@@ -201,7 +201,8 @@ def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None
     pages. q, q_out [tokens, heads, head_dim] (both None: keys and values only), k, v
     [tokens, kv_heads, head_dim], positions and rows [tokens] int32, cos and sin
     [positions, rotary_dim / 2] FP32 (None: no rotation)."""
-    r = _qd_tensors.append(cache.at, q_out, q, k, v, positions, rows, cos, sin, interleaved, position_bias, stream)
+    r = _qd_tensors.append(cache.at, q_out, q, k, v, positions, rows, cos, sin, interleaved, position_bias, stream,
+                           cache.tensors)
     if r is not None:
         _answer(r)
 
@@ -209,7 +210,7 @@ def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None
 def paged_attention(cache, out, q, workspace, scale=None, stream=0):
     """Attention of one new token per cache row: q and out [rows, heads, head_dim]; scale None:
     1 / sqrt(head_dim)."""
-    r = _qd_tensors.attention(cache.at, out, q, workspace.handle, scale, stream)
+    r = _qd_tensors.attention(cache.at, out, q, workspace.handle, scale, stream, cache.tensors)
     if r is not None:
         _answer(r)
 
@@ -219,7 +220,7 @@ class PagePool:
     [planes, pages, ...] with a page's values together."""
 
     def __init__(self, refs, page_size, tensors, planes=True):
-        self.refs, self.page_size, self.tensors = refs, page_size, list(tensors)
+        self.refs, self.page_size, self.tensors = refs, page_size, tuple(tensors)
         self.device, pages = refs.get_device(), _dims("refs", refs, 1)[0]
         self.pages = pages
         _take("refs", refs, torch.int32, (pages,), self.device, True)
@@ -245,7 +246,7 @@ def pages_fork(pool, table, lengths, parents, append, table_out, lengths_out, wo
     """Row r of table_out takes over row parents[r] of table (None: its own, -1: released) with
     room for `append` more tokens; shared pages are counted and copied on write."""
     r = _qd_tensors.fork(pool.refs, pool.page_size, pool.at, len(pool.tensors), table, lengths, parents, append, table_out,
-                         lengths_out, workspace.handle, errors, stream)
+                         lengths_out, workspace.handle, errors, stream, pool.tensors)
     if r is not None:
         _answer(r)
 

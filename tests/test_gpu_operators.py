@@ -905,6 +905,46 @@ def test_select_of_the_largest_vocabulary():
     check_select(normal(g, (1, 2, 1 << 24), BF16, 3.0), torch.tensor([[-1.0, -1.5]]), 64)
 
 
+def test_results_are_written_as_torch_writes_them():
+    """A tensor whose storage waits to be copied is copied first, and torch knows that results changed."""
+    say("results: lazily copied storage, version counters")
+    table, k, v, errors, x = append_state()
+    cache = ops.PagedCache(k, v, table.cuda(), int32([17] * 4).cuda(), errors)
+    pool = ops.PagePool(torch.zeros(40, dtype=torch.int32, device="cuda"), 16, [])
+    workspace = ops.Workspace(max(ops.attention_workspace(4, 6, 2, 64), ops.fork_workspace(4, 40), ops.select_workspace(4, 6, 6, 64)))
+    base = torch.full((4, 6, 64), 7.0, device="cuda")
+    whole = {n: torch.full((4, 6), 7, dtype=t, device="cuda")
+             for n, t in (("table", torch.int32), ("scores", F32), ("parents", torch.int32), ("tokens", torch.int32), ("done", torch.uint8))}
+    lengths = torch.full((4,), 7, dtype=torch.int32, device="cuda")
+    q, scores, done = x[:, :6].contiguous(), torch.zeros((4, 6), device="cuda"), torch.zeros((4, 6), dtype=torch.uint8, device="cuda")
+
+    def calls(q_out, out, t, n, s, p, tok, d):
+        ops.paged_append(cache, q_out, q, x[:, 6:8], x[:, 8:], int32([1] * 4).cuda())
+        ops.paged_attention(cache, out, q, workspace)
+        ops.pages_fork(pool, torch.full_like(t, -1), torch.zeros_like(n), None, 0, t, n, workspace, errors=errors)
+        ops.beam_select(q, scores, s, p, tok, workspace, done, d, 3)
+
+    originals = [base, base, whole["table"], lengths, whole["scores"], whole["parents"], whole["tokens"], whole["done"]]
+    lazy = [torch._lazy_clone(t) for t in originals]
+    written = lazy + [k, v, errors, pool.refs]
+    versions = [t._version for t in written]
+    calls(*lazy)
+    assert all(bool((t == 7).all()) for t in originals)
+    assert all(not bool((t == 7).all()) for t in lazy)
+    assert all(t._version > n for t, n in zip(written, versions))
+    # What autograd keeps is not changed behind its back.
+    w = torch.ones((4, 6, 64), device="cuda", requires_grad=True)
+    y = torch.zeros((4, 6, 64), device="cuda")
+    loss = (w * y).sum()
+    ops.paged_attention(cache, y, q, workspace)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        z = torch.empty((4, 6, 64), device="cuda")
+    ops.paged_attention(cache, z, q, workspace)  # a tensor without a version counter
+    assert torch.equal(z, y)
+
+
 # ---- together -----------------------------------------------------------------------------
 
 
