@@ -1,3 +1,4 @@
+import importlib.util
 import os
 import sys
 
@@ -8,6 +9,16 @@ for sub in ("oracle", "light-rocm-runtime_amd"):
     path = os.path.join(ROOT, sub)
     if path not in sys.path:
         sys.path.insert(0, path)
+
+
+# The operators' binding is built for torch, and the converter's tests compare with its
+# conversions: without it these are left out.
+NEED_TORCH = ["test_operators.py", "test_gpu_operators.py", "test_converter.py", "test_gpu_converter.py"]
+collect_ignore = [] if importlib.util.find_spec("torch") else NEED_TORCH
+
+
+def pytest_report_header(config):
+    return f"torch is not installed, left out: {', '.join(NEED_TORCH)}" if collect_ignore else None
 
 
 def pytest_configure(config):
