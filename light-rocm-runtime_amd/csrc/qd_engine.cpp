@@ -532,13 +532,19 @@ struct qd_engine {
       release(bm.block, bm.bytes);
       bm = BeamWorkspace{};
     }
-    bm = carve_beam_workspace(alloc<char>(bytes), pages, steps);
-    check(qd::launch_op_clear(stream, bm.scratch.counters, qd::kOpCounters), "counter clear");
     std::vector<int32_t> iota(CAP);
     for (size_t i = 0; i < CAP; ++i) iota[i] = int32_t(i);
-    check(hipMemcpyAsync(bm.positions, iota.data(), CAP * 4, hipMemcpyHostToDevice, stream), "H2D");
-    check(hipMemsetAsync(bm.rows, 0, CAP * 4, stream), "memset");
-    check(hipStreamSynchronize(stream), "hipStreamSynchronize");
+    const BeamWorkspace w = carve_beam_workspace(alloc<char>(bytes), pages, steps);
+    try {  // it is the searches' once all of it is there
+      check(qd::launch_op_clear(stream, w.scratch.counters, qd::kOpCounters), "counter clear");
+      check(hipMemcpyAsync(w.positions, iota.data(), CAP * 4, hipMemcpyHostToDevice, stream), "H2D");
+      check(hipMemsetAsync(w.rows, 0, CAP * 4, stream), "memset");
+      check(hipStreamSynchronize(stream), "hipStreamSynchronize");
+    } catch (...) {
+      release(w.block, bytes);
+      throw;
+    }
+    bm = w;
   }
   // The pages of layer l as the operators take them, with table and lengths `side`.
   qd_paged_cache beam_cache(size_t l, int side, uint32_t beams) const {

@@ -189,6 +189,29 @@ def test_refusals(engine):
 
 
 @pytest.mark.gpu
+def test_a_search_without_room_for_its_memory(monkeypatch):
+    """Its memory is the searches' once all of it is there: one that finds no room leaves nothing half made."""
+    say("beam memory refused by QD_DEVICE_BYTES_LIMIT")
+    config = dict(layers=LAYERS, vocab=VOCAB, capacity=4000, max_batch=1)
+    with qd.Engine(**config) as ref:
+        ref.load_synthetic(SEED)
+        before = ref.device_bytes()
+        want = ref.generate_beams(0, 7, 4, 20)
+        small = ref.device_bytes()
+        monkeypatch.setenv("QD_DEVICE_BYTES_LIMIT", str(small))
+        with qd.Engine(**config) as eng:
+            monkeypatch.delenv("QD_DEVICE_BYTES_LIMIT")
+            eng.load_synthetic(SEED)
+            for _ in range(2):
+                with pytest.raises(qd.QdError) as err:
+                    eng.generate_beams(0, 7, 16, 3000)
+                assert err.value.status == qd.RUNTIME and before < eng.device_bytes() < small
+                got = eng.generate_beams(0, 7, 4, 20)
+                assert all(np.array_equal(a, b) for a, b in zip(got[0], want[0])) and np.array_equal(got[1], want[1])
+                assert eng.device_bytes() == small
+
+
+@pytest.mark.gpu
 def test_24_layers_at_a_long_context():
     """The whole model deep in a context: each beam's score equals the sum of its log
     probabilities when its tokens are consumed one by one."""
