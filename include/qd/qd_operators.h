@@ -54,8 +54,9 @@ enum {
  * owner allocates one of the largest size its calls ask for and may pass it to
  * any of them, but to one call at a time: calls on the same stream, or graphs
  * replayed on the same stream, follow each other; work that may run at the same
- * time (two streams, two graphs on two streams) needs a workspace each.
- * Destroying one waits for the device. */
+ * time (two streams, two graphs on two streams) needs a workspace each. The sizes
+ * that are asked for serve smaller calls too, as each says. Destroying one waits
+ * for the device. */
 typedef struct qd_workspace qd_workspace;
 QD_API qd_status qd_workspace_create(int32_t device, size_t bytes, qd_workspace **workspace);
 QD_API qd_status qd_workspace_destroy(qd_workspace *workspace);
@@ -91,8 +92,9 @@ typedef struct qd_paged_cache {
  * context that many times longer than `original` positions: frequencies that
  * turn more than `fast` times (32) within `original` positions stay, those that
  * turn less than `slow` times (1) are divided by stretch, those between are
- * mixed by the logarithm of their turns; both tables are multiplied by
- * 0.1 ln(stretch) + 1. Host only. */
+ * mixed by the logarithm of their turns (which are not rounded to whole dimensions
+ * first); both tables are multiplied by 0.1 ln(stretch) + 1. qd_paged_append takes
+ * any tables: a checkpoint trained with other angles brings its own. Host only. */
 QD_API qd_status qd_rope_table(double theta, uint32_t rotary_dim, uint32_t positions, double stretch,
                                uint32_t original, double fast, double slow, float *cos_table, float *sin_table);
 
@@ -135,14 +137,17 @@ QD_API qd_status qd_paged_append(const qd_paged_cache *cache, const qd_append_ar
  * positions 0 .. lengths[r] - 1 of KV head h / (heads / kv_heads),
  *   out[r][h] = sum_j softmax_j(scale q[r][h] . K_j) V_j,
  * statistics and sums in FP32 (products are summed before they are divided, by
- * weights up to 2^8: finite for |V| below 2^89). 16-bit types multiply a weight as two numbers,
- * off by at most 2^-16 of it in BF16 and in FP16 by 2^-22 of it or 2^-51 of the row's largest,
- * whichever is more; an infinite V makes the outputs that it reaches infinite or NaN. A row of
- * length 0 gets zeros; what the pages hold past a row's length is not read. A row with a bad length or page gets
- * NaN. q and out are [rows][heads][head_dim] with strides that are multiples of
- * 16 bytes; out may be q itself, with its strides. The result of a row does not depend on when
- * its parts finish (they are joined in order), but how its positions are split
- * goes by all rows' lengths. */
+ * weights up to 2^8: finite for |V| below 2^89). 16-bit types multiply a weight
+ * as two numbers, off by at most 2^-16 of it in BF16, and in FP16 by 2^-22 of it
+ * or 2^-51 of the row's largest, whichever is more; an infinite V makes the
+ * outputs that it reaches infinite or NaN. A row of length 0 gets zeros; what the
+ * pages hold past a row's length is not read. A row with a bad length or page
+ * gets NaN. q and out are [rows][heads][head_dim] with strides that are multiples
+ * of 16 bytes; out may be q itself, with its strides. The result of a row does not
+ * depend on when its parts finish (they are joined in order), but how its
+ * positions are split goes by all rows' lengths and by how many positions tables
+ * and pages can hold, as the lengths are not known when the call queues. A page
+ * that several rows list is read for each of them. */
 typedef struct qd_attention_args {
   const void *q;
   void *out;
@@ -189,9 +194,11 @@ typedef struct qd_page_memory {
  * first negative entry or at the last column. Nothing happens by halves: with a
  * bad length, parent or page, a row that grows past the table's columns
  * (QD_PAGED_BAD_LENGTH) or too few free pages, an error bit is set and table,
- * lengths and refs are handed on as they were, with no page copied. table_out
- * and lengths_out must not overlap table and lengths: a program keeps two of
- * each and takes them in turn. Forks that share refs follow each other, as calls
+ * lengths and refs are handed on as they were, with no page copied. (The rows then
+ * have no room for new tokens: an append that is queued behind such a fork, at the
+ * last positions of lengths_out, writes over what stands there.) table_out and
+ * lengths_out must not overlap table and lengths: a program keeps two of each and
+ * takes them in turn. Forks that share refs follow each other, as calls
  * that share a workspace do. */
 typedef struct qd_fork_args {
   const int32_t *table;   /* [rows][table_width] */
@@ -213,6 +220,7 @@ typedef struct qd_fork_args {
   int32_t device;
 } qd_fork_args;
 QD_API qd_status qd_pages_fork(const qd_fork_args *args, qd_workspace *workspace, void *stream);
+/* Bytes of workspace that forks of up to so many rows and pages need. */
 QD_API qd_status qd_pages_fork_workspace(uint32_t rows, uint32_t pages, size_t *bytes);
 
 /* ---- beam selection --------------------------------------------------------------

@@ -1385,10 +1385,14 @@ hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A.
 // ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
 constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
 // Which kernel, by the bytes of all positions that the tables, or the pool, can
-// hold (their real number is on the device). They cross between 65 and 120 MB: 65 MB
-// of 8 heads of 128 in BF16 short 24.8 us, long 22.5; 74 of 4 in FP32 26.7 and 29.1; 98
-// of 8 in BF16, rows of one length, 25.7 and 28.3; 99 of 4 in FP16 32.7 and 30.4; 123
-// of 2 of 64 in FP32 42.7 and 39.3.
+// hold: their real number is on the device. Where rows fill what they can hold, the
+// kernels cross between 65 and 120 MB, by type, heads and raggedness: 65 MB of 8 heads of
+// 128 in BF16 short 24.8 us, long 22.5; 74 of 4 in FP32 26.7 and 29.1; 98 of 8 in BF16, rows
+// of one length, 25.7 and 28.3; 99 of 4 in FP16 32.7 and 30.4; 123 of 2 of 64 in FP32 42.7
+// and 39.3. Short rows in a large pool get the long kernel all the same (in pages of 2 GB
+// and tables of 32,768 positions, and in a pool of their size: 16 rows of 576 with 2 heads
+// of 64 in FP32 13.5 us and 8.5, 8 of 448 with 8 of 128 in BF16 12.2 and 8.0, one of 129 7.1
+// and 6.7, one of 3,000 9.2 and 9.2).
 constexpr uint64_t kShortBytes = 96ull << 20;
 struct AttnShape {
   uint32_t group, blocks, parts, rec_heads, rec_floats, apart, least, target, records;
