@@ -46,7 +46,9 @@ enum {
   QD_PAGED_BAD_PAGE = 2,    /* a page id that is needed and not in [0, pages) */
   QD_PAGED_BAD_POSITION = 4,/* a position past the table's columns or the rotary tables */
   QD_PAGED_BAD_ROW = 8,     /* a row or parent that does not exist */
-  QD_PAGED_EXHAUSTED = 16   /* fewer free pages than a fork needs */
+  QD_PAGED_EXHAUSTED = 16,  /* fewer free pages than a fork needs */
+  QD_TREE_BAD_PARENT = 32,  /* a node's parent that is not an earlier node */
+  QD_TREE_BAD_PATH = 64     /* a path that is not of ascending nodes, or a count past them */
 };
 
 /* ---- workspace --------------------------------------------------------------
@@ -261,6 +263,173 @@ typedef struct qd_select_args {
 QD_API qd_status qd_beam_select(const qd_select_args *args, qd_workspace *workspace, void *stream);
 /* Bytes of workspace that calls of up to so many groups, beams, places and tokens need. */
 QD_API qd_status qd_beam_select_workspace(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab, size_t *bytes);
+
+/* ---- trees of drafted tokens ---------------------------------------------------------
+ * A cheap model proposes several continuations of each row at once, as a tree of up to
+ * 64 nodes: node 0 is the row's newest token, which stands; the others are proposals,
+ * each the continuation of its parent. parents[r][i] is the node before node i, below i,
+ * or -1: only what the cache holds comes before it. Less than -1: there is no node i
+ * (rows with fewer nodes than the call; node 0 too in rows that only fill the batch).
+ * The nodes' keys and values stand in the cache at the last `nodes` positions of the row,
+ * in their order: node i at length - nodes + i (qd_paged_append_at). */
+
+/* qd_paged_append with a place of its own for each token: token t is rotated for
+ * positions[t] and written to position slots[t] of its row (both plus position_bias;
+ * slots NULL: qd_paged_append). A drafted token is rotated for its depth in the tree and
+ * stands at its node's place. A token is skipped if either is negative. */
+QD_API qd_status qd_paged_append_at(const qd_paged_cache *cache, const qd_append_args *args, const int32_t *slots,
+                                    void *stream);
+
+/* Attention of the nodes of a tree in each row of the cache, cache->lengths counting
+ * them: node i attends to the positions before the tree, to the nodes above it and to
+ * itself,
+ *   out[r][i][h] = sum_j softmax_j(scale q[r][i][h] . K_j) V_j,
+ * each position read once for all nodes where up to 128 pairs of a node and a query head
+ * of one KV head allow it. Precision is qd_paged_attention's. Nodes that are not there
+ * and rows of length 0 get zeros; K and V of nodes that are not seen may hold anything,
+ * also values that are not finite: outputs that see such a V become NaN or infinite. A row with
+ * a bad page, a bad parent, or a length that is not 0 and below `nodes` or past its
+ * table gets NaN. q and out are [rows][nodes][heads][head_dim] with strides that are
+ * multiples of 16 bytes; out may be q itself, with its strides. */
+typedef struct qd_tree_attention_args {
+  const void *q;
+  void *out;
+  int64_t q_stride;      /* from row to row */
+  int64_t q_node_stride;
+  int64_t q_head_stride;
+  int64_t out_stride;
+  int64_t out_node_stride;
+  int64_t out_head_stride;
+  const int32_t *parents; /* [rows][nodes] */
+  uint32_t nodes;        /* up to 64 */
+  uint32_t heads;        /* a multiple of kv_heads */
+  float scale;
+} qd_tree_attention_args;
+QD_API qd_status qd_tree_attention(const qd_paged_cache *cache, const qd_tree_attention_args *args,
+                                   qd_workspace *workspace, void *stream);
+/* Bytes of workspace that caches of up to `rows` rows and trees of up to `nodes` need. */
+QD_API qd_status qd_tree_attention_workspace(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads,
+                                             uint32_t head_dim, size_t *bytes);
+
+/* Which drafted tokens stand: from node 0 on, the token that follows a node is picked from
+ * its logits, and if a child of the node carries it (the lowest such child), the walk goes
+ * on there. The token picked at the walk's last node is new.
+ *   path[r][..]     the walk's nodes, -1 behind them
+ *   counts[r]       how many they are, node 0 among them
+ *   next_tokens[r]  the new token
+ * Picked is the token of the largest logit, the lowest of equal ones; NaN counts as -inf.
+ * With draws (numbers u from 0 up to 1), the least token t with
+ *   sum_{i <= t} p_i > u sum_i p_i,  p_i = exp(logits[i] / temperature)
+ * (p_i in FP32, off by about 2^-23 of it; sums in 64 bits), so that the tokens that come
+ * out are distributed as the model's own; where the largest logit is past 1e30 either
+ * way, the token of the largest logit. A row whose node 0 is not there gets count 0 and
+ * -1, and so does one with a bad parent. */
+typedef struct qd_accept_args {
+  const void *logits;      /* [rows][nodes][vocab] */
+  int64_t row_stride;
+  int64_t node_stride;
+  const int32_t *tokens;   /* [rows][nodes] what each node carries */
+  const int32_t *parents;  /* [rows][nodes] */
+  const float *draws;      /* [rows][nodes], or NULL */
+  int32_t *path;           /* [rows][nodes] */
+  int32_t *counts;         /* [rows] */
+  int32_t *next_tokens;    /* [rows] */
+  uint32_t *errors;        /* one word, or NULL */
+  float temperature;       /* read with draws: from 1e-6 to 1e6 */
+  uint32_t dtype;          /* of the logits */
+  uint32_t rows;
+  uint32_t nodes;          /* up to 64 */
+  uint32_t vocab;          /* up to 2^24 */
+  int32_t device;
+} qd_accept_args;
+QD_API qd_status qd_tree_accept(const qd_accept_args *args, qd_workspace *workspace, void *stream);
+/* Bytes of workspace that calls of up to so many rows and nodes need. */
+QD_API qd_status qd_tree_accept_workspace(uint32_t rows, uint32_t nodes, uint32_t vocab, size_t *bytes);
+
+/* One memory that holds something of each position: `pieces` pieces (heads) of
+ * piece_bytes bytes, piece n of position j of page p at
+ * base + plane * plane_stride + p * page_stride + j * token_stride + n * piece_stride
+ * in each of `planes` planes (layers). All in bytes. */
+typedef struct qd_token_memory {
+  void *base;
+  int64_t plane_stride;
+  int64_t page_stride;
+  int64_t token_stride;
+  int64_t piece_stride;
+  uint32_t piece_bytes;  /* a multiple of 16, as the address and the strides are */
+  uint32_t pieces;
+  uint32_t planes;
+  uint32_t reserved;
+} qd_token_memory;
+
+/* Moves what stands of each row's tree together: what the memories hold at node
+ * path[r][i]'s position goes to position length - nodes + i, i < counts[r], as if all
+ * were read before any is written. lengths_out[r] = lengths[r] - nodes + counts[r]; 0 for
+ * a row of length 0, whose path is not read. Positions behind are left as they are. A row
+ * with a bad length (not 0 and below `nodes`, or past the table), count, path (its nodes
+ * ascend) or page moves nothing and hands its length on. Rows whose trees lie in the same
+ * pages must not be committed in one call; lengths_out must not be lengths. */
+typedef struct qd_commit_args {
+  const int32_t *table;
+  const int32_t *lengths;
+  const int32_t *path;     /* [rows][nodes] */
+  const int32_t *counts;
+  int32_t *lengths_out;
+  int64_t table_stride;
+  uint32_t *errors;        /* one word, or NULL */
+  const qd_token_memory *memories; /* host array, up to 4 */
+  uint32_t memory_count;
+  uint32_t rows;           /* up to 65535 */
+  uint32_t nodes;          /* up to 64 */
+  uint32_t table_width;
+  uint32_t pages;
+  uint32_t page_size;      /* positions; a power of two from 16 to 1024 */
+  int32_t device;
+} qd_commit_args;
+QD_API qd_status qd_tree_commit(const qd_commit_args *args, void *stream);
+
+/* ---- attention over chosen pages --------------------------------------------------------
+ * A row's query reads the pages whose keys may matter most to it, by bounds that are kept
+ * of each page's keys: bounds[page][kv_head][0][d] is the least and [1][d] the largest value
+ * of element d of the keys in the page (cache dtype, contiguous). */
+
+/* The bounds of every page that holds one of a row's last `recent` positions, over all of
+ * the row's positions in it. NaN counts as neither; a page of NaN alone gets +inf and -inf.
+ * Rows that share a page write the same bounds if they hold equally much of it, else one of
+ * them does. A row with a bad length or page sets an error bit; its other pages are done. */
+QD_API qd_status qd_page_bounds(const qd_paged_cache *cache, void *bounds, uint32_t recent, void *stream);
+
+/* qd_paged_attention over up to `budget` pages of each row and KV head. Of a row of n
+ * pages, the first `first` and the last `last` are always read; if n > budget, of those
+ * between the ones that score highest, the lower of equal ones:
+ *   score(page) = sum over the KV head's query heads and d of
+ *                 max(q_d low_d, q_d high_d),
+ * as much as the products of the page's keys can sum to, in 64 bits; a score that is
+ * NaN counts as +inf.
+ *   chosen[r][kv_head][..]  the columns of the table that were read, ascending, -1 behind
+ *                           them (NULL: not told)
+ * A row of n <= budget pages reads all of them. A row with a bad length gets NaN, one
+ * with a bad page at least where its page is chosen, as it then is. */
+typedef struct qd_sparse_args {
+  const void *q;
+  void *out;
+  int64_t q_stride;
+  int64_t q_head_stride;
+  int64_t out_stride;
+  int64_t out_head_stride;
+  const void *bounds;  /* [pages][kv_heads][2][head_dim] */
+  int32_t *chosen;     /* [rows][kv_heads][budget], or NULL */
+  uint32_t heads;
+  uint32_t budget;     /* at least first + last, and 1 */
+  uint32_t first;
+  uint32_t last;       /* at least 1 */
+  float scale;
+} qd_sparse_args;
+QD_API qd_status qd_sparse_attention(const qd_paged_cache *cache, const qd_sparse_args *args, qd_workspace *workspace,
+                                     void *stream);
+/* Bytes of workspace that calls of up to so many rows, columns of the table and pages need. */
+QD_API qd_status qd_sparse_attention_workspace(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                               uint32_t table_width, uint32_t budget, size_t *bytes);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstdarg>
@@ -156,6 +157,60 @@ qd_status check_select(uint32_t groups, uint32_t beams, uint32_t k, uint32_t voc
   return QD_SUCCESS;
 }
 
+qd_status check_nodes(uint32_t nodes) {
+  if (nodes == 0 || nodes > qd::kTreeNodes) return refuse(QD_ERROR_NOT_SUPPORTED, "%u nodes: from 1 to %u", nodes, qd::kTreeNodes);
+  return QD_SUCCESS;
+}
+
+// (An arrival counter for every node and every row; a grid's second dimension.)
+qd_status check_accept(uint32_t rows, uint32_t nodes, uint32_t vocab) {
+  QD_TRY(check_nodes(nodes));
+  if (vocab == 0) return invalid("vocab must be positive");
+  if (vocab > qd::kSelectVocab) return refuse(QD_ERROR_NOT_SUPPORTED, "vocab %u: up to %u", vocab, qd::kSelectVocab);
+  if (static_cast<uint64_t>(rows) * (nodes + 1) > 65535)
+    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of %u nodes: up to 65535 rows and nodes together", rows, nodes);
+  return QD_SUCCESS;
+}
+
+qd_status check_head_dim(uint32_t head_dim) {
+  if (head_dim != 64 && head_dim != 128) return refuse(QD_ERROR_NOT_SUPPORTED, "head_dim %u: the kernels take 64 and 128", head_dim);
+  return QD_SUCCESS;
+}
+
+// Queries and outputs of `rows` rows of heads.
+qd_status check_rows_of_heads(const qd_paged_cache *c, const void *q, const void *out, int64_t q_stride, int64_t q_head_stride,
+                              int64_t out_stride, int64_t out_head_stride, uint32_t heads) {
+  const uint32_t e = element_bytes(c->dtype);
+  if (!q || !out) return invalid("null tensor");
+  if (!aligned16(q) || !aligned16(out)) return invalid("q and out need 16-byte aligned addresses");
+  QD_TRY(check_stride(q_stride, 0, e, "q_stride"));
+  QD_TRY(check_stride(q_head_stride, 0, e, "q_head_stride"));
+  QD_TRY(check_stride(out_stride, c->rows > 1 ? c->head_dim : 0, e, "out_stride"));
+  QD_TRY(check_stride(out_head_stride, heads > 1 ? c->head_dim : 0, e, "out_head_stride"));
+  if (out == q && ((c->rows > 1 && out_stride != q_stride) || (heads > 1 && out_head_stride != q_head_stride)))
+    return invalid("q in place needs one stride");
+  return QD_SUCCESS;
+}
+
+qd_status check_attention_size(const qd_paged_cache *c, uint32_t heads, uint64_t positions) {
+  const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((heads / c->kv_heads + 15) / 16);
+  // Tiles are counted in 31 bits, and a grid has fewer than 2^32 threads.
+  if (c->rows * parts * (positions / 32 + 1) > 0x7f000000u || c->rows * parts > 0xffff00u)
+    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of up to %llu positions and %u heads are too much for one call", c->rows,
+                  static_cast<unsigned long long>(positions), heads);
+  return QD_SUCCESS;
+}
+
+// (An arrival counter for every row and KV head; a grid's second dimension.)
+qd_status check_sparse(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t budget) {
+  QD_TRY(check_heads(heads, kv_heads));
+  QD_TRY(check_head_dim(head_dim));
+  if (static_cast<uint64_t>(rows) * kv_heads > 65535)
+    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of %u KV heads: up to 65535 together", rows, kv_heads);
+  if (budget == 0 || budget > (1u << 20)) return refuse(QD_ERROR_INVALID_ARGUMENT, "budget %u: from 1 to 2^20 pages", budget);
+  return QD_SUCCESS;
+}
+
 }  // namespace
 
 extern "C" {
@@ -221,6 +276,10 @@ qd_status qd_rope_table(double theta, uint32_t rotary_dim, uint32_t positions, d
 }
 
 qd_status qd_paged_append(const qd_paged_cache *c, const qd_append_args *a, void *stream) {
+  return qd_paged_append_at(c, a, nullptr, stream);
+}
+
+qd_status qd_paged_append_at(const qd_paged_cache *c, const qd_append_args *a, const int32_t *slots, void *stream) {
   QD_TRY(check_cache(c));
   if (!a) return invalid("null argument");
   const uint32_t e = element_bytes(c->dtype), dim = c->head_dim;
@@ -246,7 +305,7 @@ qd_status qd_paged_append(const qd_paged_cache *c, const qd_append_args *a, void
   }
   Device on;
   QD_TRY(on.enter(c->device));
-  return launched(qd::launch_paged_append(static_cast<hipStream_t>(stream), *c, *a), "append launch");
+  return launched(qd::launch_paged_append(static_cast<hipStream_t>(stream), *c, *a, slots), "append launch");
 }
 
 qd_status qd_paged_attention_workspace(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, size_t *bytes) {
@@ -263,24 +322,9 @@ qd_status qd_paged_attention(const qd_paged_cache *c, const qd_attention_args *a
   if (!a) return invalid("null argument");
   QD_TRY(check_heads(a->heads, c->kv_heads));
   if (!std::isfinite(a->scale)) return invalid("scale must be finite");
-  const uint32_t e = element_bytes(c->dtype);
-  if (c->rows) {
-    if (!a->q || !a->out) return invalid("null tensor");
-    if (!aligned16(a->q) || !aligned16(a->out)) return invalid("q and out need 16-byte aligned addresses");
-    QD_TRY(check_stride(a->q_stride, 0, e, "q_stride"));
-    QD_TRY(check_stride(a->q_head_stride, 0, e, "q_head_stride"));
-    QD_TRY(check_stride(a->out_stride, c->rows > 1 ? c->head_dim : 0, e, "out_stride"));
-    QD_TRY(check_stride(a->out_head_stride, a->heads > 1 ? c->head_dim : 0, e, "out_head_stride"));
-    if (a->out == a->q && ((c->rows > 1 && a->out_stride != a->q_stride) ||
-                           (a->heads > 1 && a->out_head_stride != a->q_head_stride)))
-      return invalid("q in place needs one stride");
-  }
-  const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((a->heads / c->kv_heads + 15) / 16);
-  // Tiles are counted in 31 bits, and a grid has fewer than 2^32 threads.
-  if (c->rows * parts * (static_cast<uint64_t>(c->table_width) * c->page_size / 32 + 1) > 0x7f000000u ||
-      c->rows * parts > 0xffff00u)
-    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of up to %llu positions and %u heads are too much for one call", c->rows,
-                  static_cast<unsigned long long>(static_cast<uint64_t>(c->table_width) * c->page_size), a->heads);
+  if (c->rows)
+    QD_TRY(check_rows_of_heads(c, a->q, a->out, a->q_stride, a->q_head_stride, a->out_stride, a->out_head_stride, a->heads));
+  QD_TRY(check_attention_size(c, a->heads, static_cast<uint64_t>(c->table_width) * c->page_size));
   qd::OpScratch scratch{};
   QD_TRY(check_workspace(w, c->device, qd::paged_attention_scratch(c->rows, a->heads, c->kv_heads, c->head_dim), &scratch));
   Device on;
@@ -359,6 +403,151 @@ qd_status qd_beam_select(const qd_select_args *a, qd_workspace *w, void *stream)
   Device on;
   QD_TRY(on.enter(a->device));
   return launched(qd::launch_beam_select(static_cast<hipStream_t>(stream), *a, scratch), "select launch");
+}
+
+qd_status qd_tree_attention_workspace(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
+                                      size_t *bytes) {
+  if (!bytes) return invalid("null argument");
+  QD_TRY(check_nodes(nodes));
+  QD_TRY(check_heads(heads, kv_heads));
+  QD_TRY(check_head_dim(head_dim));
+  if (rows > (1u << 20)) return invalid("too many rows");
+  *bytes = qd::tree_attention_scratch_most(rows, nodes, heads, kv_heads, head_dim);
+  return QD_SUCCESS;
+}
+
+qd_status qd_tree_attention(const qd_paged_cache *c, const qd_tree_attention_args *a, qd_workspace *w, void *stream) {
+  QD_TRY(check_cache(c));
+  if (!a) return invalid("null argument");
+  QD_TRY(check_nodes(a->nodes));
+  QD_TRY(check_heads(a->heads, c->kv_heads));
+  if (!std::isfinite(a->scale)) return invalid("scale must be finite");
+  if (c->rows) {
+    QD_TRY(check_rows_of_heads(c, a->q, a->out, a->q_stride, a->q_head_stride, a->out_stride, a->out_head_stride, a->heads));
+    const uint32_t e = element_bytes(c->dtype);
+    QD_TRY(check_stride(a->q_node_stride, 0, e, "q_node_stride"));
+    QD_TRY(check_stride(a->out_node_stride, a->nodes > 1 ? c->head_dim : 0, e, "out_node_stride"));
+    if (a->out == a->q && a->nodes > 1 && a->out_node_stride != a->q_node_stride) return invalid("q in place needs one stride");
+    if (!a->parents) return invalid("null parents");
+  }
+  // A grid has fewer than 2^32 threads, 512 of a workgroup; a block has 16 columns or more.
+  const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((static_cast<uint64_t>(a->heads / c->kv_heads) * a->nodes + 127) / 128);
+  if (c->rows * parts > 0x3f0000u)
+    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of %u nodes and %u heads are too much for one call", c->rows, a->nodes, a->heads);
+  qd::OpScratch scratch{};
+  QD_TRY(check_workspace(w, c->device, qd::tree_attention_scratch(c->rows, a->nodes, a->heads, c->kv_heads, c->head_dim), &scratch));
+  Device on;
+  QD_TRY(on.enter(c->device));
+  return launched(qd::launch_tree_attention(static_cast<hipStream_t>(stream), *c, *a, scratch), "tree attention launch");
+}
+
+qd_status qd_tree_accept_workspace(uint32_t rows, uint32_t nodes, uint32_t vocab, size_t *bytes) {
+  if (!bytes) return invalid("null argument");
+  QD_TRY(check_accept(rows, nodes, vocab));
+  *bytes = qd::tree_accept_scratch(rows, nodes);
+  return QD_SUCCESS;
+}
+
+qd_status qd_tree_accept(const qd_accept_args *a, qd_workspace *w, void *stream) {
+  if (!a) return invalid("null argument");
+  QD_TRY(check_dtype(a->dtype));
+  QD_TRY(check_accept(a->rows, a->nodes, a->vocab));
+  if (a->rows) {
+    if (!a->logits || !a->tokens || !a->parents || !a->path || !a->counts || !a->next_tokens) return invalid("null tensor");
+    if (a->path == a->tokens || a->path == a->parents) return invalid("path must not be tokens or parents");
+    if (reinterpret_cast<uintptr_t>(a->logits) % element_bytes(a->dtype) != 0) return invalid("misaligned logits");
+    const int64_t most = int64_t(1) << 40;
+    if (a->row_stride < 0 || a->node_stride < 0 || a->row_stride > most || a->node_stride > most)
+      return invalid("the logits' strides must not be negative");
+    if (a->draws && !(a->temperature >= 1e-6f && a->temperature <= 1e6f)) return invalid("a temperature from 1e-6 to 1e6 is needed");
+  }
+  qd::OpScratch scratch{};
+  QD_TRY(check_workspace(w, a->device, qd::tree_accept_scratch(a->rows, a->nodes), &scratch));
+  Device on;
+  QD_TRY(on.enter(a->device));
+  return launched(qd::launch_tree_accept(static_cast<hipStream_t>(stream), *a, scratch), "accept launch");
+}
+
+qd_status qd_tree_commit(const qd_commit_args *a, void *stream) {
+  if (!a) return invalid("null argument");
+  QD_TRY(check_page_size(a->page_size));
+  QD_TRY(check_nodes(a->nodes));
+  if (a->rows > 65535) return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows: up to 65535", a->rows);
+  if (a->pages > 0x7fffffffu) return invalid("too many pages");
+  if (static_cast<uint64_t>(a->table_width) * a->page_size > (1u << 30))
+    return refuse(QD_ERROR_NOT_SUPPORTED, "rows of more than 2^30 positions");
+  if (a->rows) {
+    if (!a->table || !a->lengths || !a->path || !a->counts || !a->lengths_out) return invalid("null tensor");
+    if (a->lengths == a->lengths_out) return invalid("lengths_out must not be lengths");
+    if (a->table_stride < static_cast<int64_t>(a->table_width) || a->table_stride > (int64_t(1) << 40))
+      return invalid("table_stride is less than table_width");
+  }
+  if (a->memory_count > qd::kForkMemories || (a->memory_count && !a->memories))
+    return refuse(QD_ERROR_INVALID_ARGUMENT, "up to %u memories", qd::kForkMemories);
+  uint64_t columns = 0;
+  for (uint32_t m = 0; m < a->memory_count; ++m) {
+    const qd_token_memory &p = a->memories[m];
+    const int64_t most = int64_t(1) << 45;
+    if (p.planes == 0 || p.pieces == 0 || p.piece_bytes == 0) return invalid("a memory without planes, pieces or bytes");
+    if (!p.base || !aligned16(p.base)) return invalid("a memory needs a 16-byte aligned address");
+    if (p.piece_bytes % 16 != 0 || p.plane_stride % 16 != 0 || p.page_stride % 16 != 0 || p.token_stride % 16 != 0 ||
+        p.piece_stride % 16 != 0 || p.plane_stride < 0 || p.plane_stride > most || p.page_stride < 0 || p.page_stride > most ||
+        p.token_stride < static_cast<int64_t>(p.piece_bytes) || p.token_stride > most || p.piece_stride < 0 || p.piece_stride > most ||
+        (p.pieces > 1 && p.piece_stride < static_cast<int64_t>(p.piece_bytes)) ||
+        (p.planes > 1 && p.plane_stride < static_cast<int64_t>(p.piece_bytes)))
+      return invalid("a memory's bytes and strides: multiples of 16, strides of at least the bytes");
+    const uint64_t row = static_cast<uint64_t>(p.piece_bytes / 16) * p.pieces;
+    if (row > 0x7fffffffu || row * p.planes > 0x7fffffffu) return refuse(QD_ERROR_NOT_SUPPORTED, "positions of more than 2^35 bytes");
+    columns += row * p.planes;
+  }
+  // A grid has fewer than 2^32 threads, 256 for 64 columns.
+  if ((columns / 64 + 1) * a->rows > 0xff0000u) return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows are too much for one call", a->rows);
+  Device on;
+  QD_TRY(on.enter(a->device));
+  return launched(qd::launch_tree_commit(static_cast<hipStream_t>(stream), *a), "commit launch");
+}
+
+qd_status qd_page_bounds(const qd_paged_cache *c, void *bounds, uint32_t recent, void *stream) {
+  QD_TRY(check_cache(c));
+  if (c->rows && c->pages && (!bounds || !aligned16(bounds))) return invalid("bounds need a 16-byte aligned address");
+  const uint64_t each = std::min<uint64_t>(c->table_width, (static_cast<uint64_t>(recent) + c->page_size - 2) / c->page_size + 1);
+  // A grid has fewer than 2^32 threads, 256 for a page.
+  if (each * c->rows > 0xff0000u || each * c->rows * c->kv_heads > 0xff0000u)
+    return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of %llu pages are too much for one call", c->rows, static_cast<unsigned long long>(each));
+  Device on;
+  QD_TRY(on.enter(c->device));
+  return launched(qd::launch_page_bounds(static_cast<hipStream_t>(stream), *c, bounds, recent), "bounds launch");
+}
+
+qd_status qd_sparse_attention_workspace(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t table_width,
+                                        uint32_t budget, size_t *bytes) {
+  if (!bytes) return invalid("null argument");
+  QD_TRY(check_sparse(rows, heads, kv_heads, head_dim, budget));
+  if (table_width > (1u << 26)) return invalid("too wide a table");
+  *bytes = qd::sparse_attention_scratch_most(rows, heads, kv_heads, head_dim, table_width, budget);
+  return QD_SUCCESS;
+}
+
+qd_status qd_sparse_attention(const qd_paged_cache *c, const qd_sparse_args *a, qd_workspace *w, void *stream) {
+  QD_TRY(check_cache(c));
+  if (!a) return invalid("null argument");
+  QD_TRY(check_sparse(c->rows, a->heads, c->kv_heads, c->head_dim, a->budget));
+  if (a->last == 0 || a->first > a->budget || a->last > a->budget - a->first)
+    return refuse(QD_ERROR_INVALID_ARGUMENT, "first %u and last %u (1 at least): up to the budget, %u", a->first, a->last, a->budget);
+  if (!std::isfinite(a->scale)) return invalid("scale must be finite");
+  if (c->rows) {
+    QD_TRY(check_rows_of_heads(c, a->q, a->out, a->q_stride, a->q_head_stride, a->out_stride, a->out_head_stride, a->heads));
+    if (c->pages && (!a->bounds || !aligned16(a->bounds))) return invalid("bounds need a 16-byte aligned address");
+  }
+  const uint64_t positions = static_cast<uint64_t>(a->budget) * c->page_size;
+  if (positions > (1u << 30)) return refuse(QD_ERROR_NOT_SUPPORTED, "a budget of more than 2^30 positions");
+  QD_TRY(check_attention_size(c, a->heads, positions));
+  qd::OpScratch scratch{};
+  QD_TRY(check_workspace(w, c->device, qd::sparse_attention_scratch(c->rows, a->heads, c->kv_heads, c->head_dim, c->table_width, a->budget),
+                         &scratch));
+  Device on;
+  QD_TRY(on.enter(c->device));
+  return launched(qd::launch_sparse_attention(static_cast<hipStream_t>(stream), *c, *a, scratch), "sparse attention launch");
 }
 
 }  // extern "C"

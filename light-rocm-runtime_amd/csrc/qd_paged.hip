@@ -11,73 +11,12 @@
 #include "qd_device.hpp"
 #include "qd_device_math.hpp"
 #include "qd_operators.hpp"
+#include "qd_paged.hpp"
 
 namespace qd {
 namespace {
 
 using namespace dev;
-
-typedef float f4v __attribute__((ext_vector_type(4)));
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-typedef uint32_t u2v __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-// Lengths, tables and positions are written before the kernel starts: they may
-// be read through the scalar cache.
-typedef const __attribute__((address_space(4))) int32_t const_i32;
-
-__device__ __forceinline__ int32_t load_uniform(const int32_t *p) { return *(const_i32 *)p; }
-
-__device__ __forceinline__ void raise_error(uint32_t *errors, uint32_t bit) {
-  if (errors) atomicOr(errors, bit);
-}
-
-// Waits until this thread's vector memory operations have completed.
-__device__ __forceinline__ void wait_vm_stores() { __builtin_amdgcn_s_waitcnt(0x0F70); }
-
-// The storage types' conversions; two values share a 32-bit register, low half first.
-struct Half {
-  static __device__ __forceinline__ float lo(uint32_t v) { return half_lo(v); }
-  static __device__ __forceinline__ float hi(uint32_t v) { return half_hi(v); }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};  // to nearest even
-    return __builtin_bit_cast(uint32_t, v);
-  }
-  static __device__ __forceinline__ f4v mfma(u4v a, u4v b, f4v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-};
-struct Brain {
-  static __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
-  static __device__ __forceinline__ float hi(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
-  static __device__ __forceinline__ uint32_t pack(float a, float b) {
-    const bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};  // to nearest even
-    return __builtin_bit_cast(uint32_t, v);
-  }
-  static __device__ __forceinline__ f4v mfma(u4v a, u4v b, f4v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
-};
-
-// Four consecutive elements as FP32, and back.
-template <typename E>
-__device__ __forceinline__ float4 load4(const void *base, int64_t i) {
-  if constexpr (std::is_same_v<E, float>) {
-    return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + i);
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(base) + i);
-    return make_float4(E::lo(v.x), E::hi(v.x), E::lo(v.y), E::hi(v.y));
-  }
-}
-template <typename E>
-__device__ __forceinline__ void store4(void *base, int64_t i, float4 v) {
-  if constexpr (std::is_same_v<E, float>)
-    *reinterpret_cast<float4 *>(static_cast<float *>(base) + i) = v;
-  else
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(base) + i) = make_uint2(E::pack(v.x, v.y), E::pack(v.z, v.w));
-}
 
 // ---- append -------------------------------------------------------------------
 // (a, b) -> (a c - b s, b c + a s) for the rotated pairs, a copy for the rest. A
@@ -92,6 +31,7 @@ struct AppendLaunch {
   uint32_t page_shift;
   uint32_t lanes_shift;  // of a head: log2(head_dim / 8)
   uint32_t waves;        // of a token
+  const int32_t *slots;  // where each token goes, or null: its position
 };
 
 // Eight consecutive elements.
@@ -149,6 +89,8 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   if (token >= p.a.tokens) return;
   const int64_t position = static_cast<int64_t>(load_uniform(p.a.positions + token)) + p.a.position_bias;
   if (position < 0) return;
+  const int64_t place = p.slots ? static_cast<int64_t>(load_uniform(p.slots + token)) + p.a.position_bias : position;
+  if (place < 0) return;
   const uint32_t dim = p.c.head_dim, lane = lane_id();
   const uint32_t heads = p.a.q ? p.a.heads : 0, all = heads + 2 * p.c.kv_heads;  // queries, then keys, then values
   const uint32_t j = (id - token * p.waves) * (kWave >> p.lanes_shift) + (lane >> p.lanes_shift);  // this lane's row
@@ -157,7 +99,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   const uint32_t rotary = p.a.rotary_dim, half = rotary / 2;
 
   const int32_t row = p.a.rows ? load_uniform(p.a.rows + token) : static_cast<int32_t>(token);
-  const uint64_t column = static_cast<uint64_t>(position) >> p.page_shift;
+  const uint64_t column = static_cast<uint64_t>(place) >> p.page_shift;
   uint32_t bad = 0;
   int64_t page = 0;
   if (row < 0 || static_cast<uint32_t>(row) >= p.c.rows) {
@@ -214,7 +156,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   }
   void *dst = query ? p.a.q_out : value ? p.c.v : p.c.k;
   const int64_t to = query ? token * p.a.q_out_stride + h * dim
-                           : page * p.c.page_stride + (position & (p.c.page_size - 1)) * p.c.token_stride + h * p.c.head_stride;
+                           : page * p.c.page_stride + (place & (p.c.page_size - 1)) * p.c.token_stride + h * p.c.head_stride;
   store8<E>(dst, to + e, x);
 }
 
@@ -276,28 +218,8 @@ struct AttnLaunch {
   uint32_t rec_floats;
   uint32_t least;       // tiles on either side of a cut; 0: items are not cut
   uint32_t target;      // pieces aimed at besides one of each item (the short kernel)
+  int64_t head_table;   // from a KV head's table of a row to the next one's; 0: they share one
 };
-
-// Values of lanes l and l ^ 32 in a and b (any order).
-__device__ __forceinline__ void half_swap(float v, float &a, float &b) {
-  unsigned x = __builtin_bit_cast(unsigned, v), y = x;
-  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
-  a = __builtin_bit_cast(float, x);
-  b = __builtin_bit_cast(float, y);
-}
-// Over lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ float quarters_max(float v) {
-  float a, b;
-  v = row_pair_max(v);
-  half_swap(v, a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float quarters_sum(float v) {
-  float a, b;
-  v = row_pair_sum(v);
-  half_swap(v, a, b);
-  return a + b;
-}
 
 // 16 positions of a page through a descriptor that ends with the last valid one:
 // loads past it give zeros and touch no memory.
@@ -331,18 +253,6 @@ struct Deal {
 
 __device__ __forceinline__ uint32_t tiles_of(const AttnLaunch &p, int32_t n, int64_t most) {
   return n <= 0 || n > most ? 1u : (static_cast<uint32_t>(n) + kTile - 1) / kTile;
-}
-
-// Inclusive sum over the lanes up to this one.
-__device__ __forceinline__ uint32_t lanes_upto(uint32_t v) {
-  int x = static_cast<int>(v);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 to 1, 2 to 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row 1 to 2 and 3
-  return static_cast<uint32_t>(x);
 }
 
 // How a cut `off` tiles into an item of n moves: 0 to its start, 1 not, 2 to its end.
@@ -380,17 +290,6 @@ __device__ __forceinline__ bool end_run(const AttnLaunch &p, const Deal &d, uint
   const int cut = cut_of(p, end - it.at, it.tiles);
   if (cut == 1) it.last = end - it.at;
   return cut != 0;
-}
-
-// Maximum over the wave of numbers below 2^31.
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-  int x = static_cast<int>(v);
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppXor1, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppXor2, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppHalfMirror, 0xf, 0xf, false));
-  x = max(x, __builtin_amdgcn_update_dpp(0, x, kDppMirror, 0xf, 0xf, false));
-  return static_cast<uint32_t>(max(max(__builtin_amdgcn_readlane(x, 0), __builtin_amdgcn_readlane(x, 16)),
-                                   max(__builtin_amdgcn_readlane(x, 32), __builtin_amdgcn_readlane(x, 48))));
 }
 
 // Workgroup i's first item; false if it has none. Lane l looks at rows l, l + 64, ...
@@ -710,7 +609,7 @@ struct Attention {
     for (int s = 0; s < 2; ++s) {
       const uint32_t pos = at * kTile + s * kSub;
       id[s] = at < x.last && pos < static_cast<uint32_t>(x.length)
-                  ? load_uniform(p.c.table + x.row * p.c.table_stride + (pos >> p.page_shift))
+                  ? load_uniform(p.c.table + x.row * p.c.table_stride + x.part / p.blocks * p.head_table + (pos >> p.page_shift))
                   : -1;
     }
   }
@@ -1373,14 +1272,6 @@ __global__ void clear_kernel(uint32_t *p, size_t n) {
   for (size_t i = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; i < n; i += static_cast<size_t>(gridDim.x) * blockDim.x) p[i] = 0u;
 }
 
-uint32_t log2_of(uint32_t v) { return static_cast<uint32_t>(__builtin_ctz(v)); }
-
-template <typename... A>
-hipError_t launch(void (*kernel)(A...), dim3 grid, dim3 block, hipStream_t s, A... args) {
-  void *packed[] = {&args...};
-  return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, packed, 0, s);
-}
-
 // How attention cuts its work. The long kernel's cuts keep eight tiles from an item's
 // ends (as many as two 128 rows of 0 to 4,000 171 us too, 32 183).
 constexpr uint32_t kAttnLeast = 8, kCus = 256, kMostPerCu = 2;
@@ -1415,17 +1306,15 @@ AttnShape attention_shape(uint32_t rows, uint32_t heads, uint32_t kv_heads, uint
   return s;
 }
 
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-
 }  // namespace
 
 hipError_t launch_op_clear(hipStream_t s, uint32_t *counters, size_t n) {
   return launch(clear_kernel, dim3(64), dim3(kBlock), s, counters, n);
 }
 
-hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_append_args &a) {
+hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_append_args &a, const int32_t *slots) {
   if (a.tokens == 0) return hipSuccess;
-  AppendLaunch p{c, a, log2_of(c.page_size), c.head_dim == 128 ? 4u : 3u, 0};
+  AppendLaunch p{c, a, log2_of(c.page_size), c.head_dim == 128 ? 4u : 3u, 0, slots};
   // (A wave that holds four rows of a token at a time was no faster: 6,000 tokens of
   // 48 heads of 128 in BF16 36.4 us against 35.3.)
   const uint32_t rows = (a.q ? a.heads : 0) + 2 * c.kv_heads, at_once = kWave >> p.lanes_shift;
@@ -1472,7 +1361,8 @@ static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
   return launch(attention_long_kernel<E, D, kStages>, dim3(kCus * per_cu), block, s, p);
 }
 
-hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w) {
+hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w,
+                                  int64_t head_table) {
   if (c.rows == 0) return hipSuccess;
   const AttnShape sh = attention_shape(c.rows, a.heads, c.kv_heads, c.head_dim);
   AttnLaunch p{};
@@ -1489,6 +1379,7 @@ hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const 
   p.parts = sh.parts;
   p.least = sh.least;
   p.target = sh.target;
+  p.head_table = head_table;
   const bool wide = c.head_dim == 128;
   switch (c.dtype) {
     case QD_DTYPE_F32: return wide ? launch_attention<float, 128, 1, 1>(s, p) : launch_attention<float, 64, 2, 1>(s, p);

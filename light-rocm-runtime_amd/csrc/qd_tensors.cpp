@@ -18,10 +18,15 @@ namespace {
 
 // The library's entry points, which Python hands over once.
 struct {
-  decltype(&qd_paged_append) append;
+  decltype(&qd_paged_append_at) append;
   decltype(&qd_paged_attention) attention;
   decltype(&qd_pages_fork) fork;
   decltype(&qd_beam_select) select;
+  decltype(&qd_tree_attention) tree_attention;
+  decltype(&qd_tree_accept) tree_accept;
+  decltype(&qd_tree_commit) tree_commit;
+  decltype(&qd_page_bounds) page_bounds;
+  decltype(&qd_sparse_attention) sparse_attention;
 } g_calls;
 
 struct Refusal {
@@ -134,6 +139,17 @@ void *address(const char *name, PyObject *o) {
   return p;
 }
 
+float number(const char *name, PyObject *o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse(std::string(name) + " is no number");
+  }
+  return static_cast<float>(v);
+}
+// None: 1 / sqrt(head_dim)
+float scale_of(PyObject *o, int64_t dim) { return !missing(o) ? number("scale", o) : dim == 64 ? 0.125f : 0.08838834764831845f; }
+
 at::ScalarType type_of(uint32_t dtype) {
   return dtype == QD_DTYPE_F32 ? at::kFloat : dtype == QD_DTYPE_BF16 ? at::kBFloat16 : at::kHalf;
 }
@@ -164,20 +180,26 @@ PyObject *answer(Py_ssize_t given, Py_ssize_t wanted, F &&call) noexcept {
   }
 }
 
-// (append, attention, fork, select): the entry points' addresses
+// (append, attention, fork, select, tree_attention, tree_accept, tree_commit, page_bounds, sparse_attention):
+// the entry points' addresses
 PyObject *call_bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  return answer(n, 4, [&] {
+  return answer(n, 9, [&] {
     g_calls.append = reinterpret_cast<decltype(g_calls.append)>(address("append", a[0]));
     g_calls.attention = reinterpret_cast<decltype(g_calls.attention)>(address("attention", a[1]));
     g_calls.fork = reinterpret_cast<decltype(g_calls.fork)>(address("fork", a[2]));
     g_calls.select = reinterpret_cast<decltype(g_calls.select)>(address("select", a[3]));
+    g_calls.tree_attention = reinterpret_cast<decltype(g_calls.tree_attention)>(address("tree_attention", a[4]));
+    g_calls.tree_accept = reinterpret_cast<decltype(g_calls.tree_accept)>(address("tree_accept", a[5]));
+    g_calls.tree_commit = reinterpret_cast<decltype(g_calls.tree_commit)>(address("tree_commit", a[6]));
+    g_calls.page_bounds = reinterpret_cast<decltype(g_calls.page_bounds)>(address("page_bounds", a[7]));
+    g_calls.sparse_attention = reinterpret_cast<decltype(g_calls.sparse_attention)>(address("sparse_attention", a[8]));
     return QD_SUCCESS;
   });
 }
 
-// (cache, q_out, q, k, v, positions, rows, cos, sin, interleaved, position_bias, stream, the cache's tensors)
+// (cache, q_out, q, k, v, positions, rows, cos, sin, interleaved, position_bias, stream, the cache's tensors, slots)
 PyObject *call_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  return answer(n, 13, [&] {
+  return answer(n, 14, [&] {
     const auto *c = static_cast<const qd_paged_cache *>(address("cache", a[0]));
     const int device = c->device;
     const at::ScalarType type = type_of(c->dtype);
@@ -214,6 +236,7 @@ PyObject *call_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     g.positions = flat<const int32_t>("positions", a[5], at::kInt, {tokens}, device);
     g.rows = flat_or_null<const int32_t>("rows", a[6], at::kInt, {tokens}, device);
+    const int32_t *const slots = flat_or_null<const int32_t>("slots", a[13], at::kInt, {tokens}, device);
     const int interleaved = PyObject_IsTrue(a[9]);
     if (interleaved < 0) {
       PyErr_Clear();
@@ -222,7 +245,8 @@ PyObject *call_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     g.interleaved = static_cast<uint32_t>(interleaved);
     g.position_bias = static_cast<int32_t>(whole("position_bias", a[10], INT32_MIN, INT32_MAX));
     g.tokens = static_cast<uint32_t>(tokens);
-    return queue<const qd_paged_cache *, const qd_append_args *, void *>(written, g_calls.append, c, &g, address("stream", a[11]));
+    return queue<const qd_paged_cache *, const qd_append_args *, const int32_t *, void *>(written, g_calls.append, c, &g, slots,
+                                                                                          address("stream", a[11]));
   });
 }
 
@@ -246,15 +270,7 @@ PyObject *call_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     g.q_head_stride = heads > 1 ? q.strides[1] : dim;
     g.out_head_stride = heads > 1 ? out.strides[1] : dim;
     g.heads = static_cast<uint32_t>(heads);
-    g.scale = dim == 64 ? 0.125f : 0.08838834764831845f;
-    if (!missing(a[4])) {
-      const double scale = PyFloat_AsDouble(a[4]);
-      if (scale == -1.0 && PyErr_Occurred()) {
-        PyErr_Clear();
-        refuse("scale is no number");
-      }
-      g.scale = static_cast<float>(scale);
-    }
+    g.scale = scale_of(a[4], dim);
     return queue<const qd_paged_cache *, const qd_attention_args *, qd_workspace *, void *>(
         written, g_calls.attention, c, &g, static_cast<qd_workspace *>(address("workspace", a[3])), address("stream", a[5]));
   });
@@ -333,9 +349,148 @@ PyObject *call_select(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+// (cache, out, q, parents, workspace, scale or None, stream, the cache's tensors)
+PyObject *call_tree_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return answer(n, 8, [&] {
+    const auto *c = static_cast<const qd_paged_cache *>(address("cache", a[0]));
+    const at::ScalarType type = type_of(c->dtype);
+    const at::Tensor &first = tensor("q", a[2], 4);
+    const int64_t rows = c->rows, nodes = first.size(1), heads = first.size(2), dim = c->head_dim;
+    if (heads > INT_MAX || nodes > INT_MAX) refuse("too many heads or nodes");
+    Written written;
+    add_some(written, "cache", a[7], 4, 4);  // errors
+    const View out = view("out", a[1], type, {rows, nodes, heads, dim}, c->device, Lies::kRows, &written);
+    const View q = view("q", a[2], type, {rows, nodes, heads, dim}, c->device, Lies::kRows);
+    qd_tree_attention_args g{};
+    g.q = q.at;
+    g.out = out.at;
+    // (The stride of a dimension of one element is not used and may be anything.)
+    g.q_stride = rows > 1 ? q.strides[0] : nodes * heads * dim;
+    g.out_stride = rows > 1 ? out.strides[0] : nodes * heads * dim;
+    g.q_node_stride = nodes > 1 ? q.strides[1] : heads * dim;
+    g.out_node_stride = nodes > 1 ? out.strides[1] : heads * dim;
+    g.q_head_stride = heads > 1 ? q.strides[2] : dim;
+    g.out_head_stride = heads > 1 ? out.strides[2] : dim;
+    g.parents = flat<const int32_t>("parents", a[3], at::kInt, {rows, nodes}, c->device);
+    g.nodes = static_cast<uint32_t>(nodes);
+    g.heads = static_cast<uint32_t>(heads);
+    g.scale = scale_of(a[5], dim);
+    return queue<const qd_paged_cache *, const qd_tree_attention_args *, qd_workspace *, void *>(
+        written, g_calls.tree_attention, c, &g, static_cast<qd_workspace *>(address("workspace", a[4])), address("stream", a[6]));
+  });
+}
+
+// (logits, tokens, parents, path, counts, next_tokens, workspace, draws or None, temperature, errors or None, stream)
+PyObject *call_tree_accept(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return answer(n, 11, [&] {
+    const at::Tensor &logits = tensor("logits", a[0], 3);
+    const at::ScalarType type = logits.scalar_type();
+    if (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf)
+      refuse(std::string("logits of type ") + c10::toString(type));
+    const int device = static_cast<int>(logits.get_device());
+    const int64_t rows = logits.size(0), nodes = logits.size(1), vocab = logits.size(2);
+    if (rows > INT_MAX || nodes > INT_MAX || vocab > INT_MAX) refuse("logits are too large");
+    qd_accept_args g{};
+    Written written;
+    g.path = flat<int32_t>("path", a[3], at::kInt, {rows, nodes}, device, written);
+    g.counts = flat<int32_t>("counts", a[4], at::kInt, {rows}, device, written);
+    g.next_tokens = flat<int32_t>("next_tokens", a[5], at::kInt, {rows}, device, written);
+    if (!missing(a[9])) g.errors = flat<uint32_t>("errors", a[9], at::kInt, {1}, device, written);
+    const View x = view("logits", a[0], type, {rows, nodes, vocab}, device, Lies::kRows);
+    g.logits = x.at;
+    g.row_stride = rows > 1 ? x.strides[0] : 0;
+    g.node_stride = nodes > 1 ? x.strides[1] : 0;
+    g.tokens = flat<const int32_t>("tokens", a[1], at::kInt, {rows, nodes}, device);
+    g.parents = flat<const int32_t>("parents", a[2], at::kInt, {rows, nodes}, device);
+    g.draws = flat_or_null<const float>("draws", a[7], at::kFloat, {rows, nodes}, device);
+    g.temperature = number("temperature", a[8]);
+    g.dtype = type == at::kFloat ? QD_DTYPE_F32 : type == at::kBFloat16 ? QD_DTYPE_BF16 : QD_DTYPE_F16;
+    g.rows = static_cast<uint32_t>(rows);
+    g.nodes = static_cast<uint32_t>(nodes);
+    g.vocab = static_cast<uint32_t>(vocab);
+    g.device = device;
+    return queue<const qd_accept_args *, qd_workspace *, void *>(
+        written, g_calls.tree_accept, &g, static_cast<qd_workspace *>(address("workspace", a[6])), address("stream", a[10]));
+  });
+}
+
+// (page_size, pages, device, memories, memory_count, table, lengths, path, counts, lengths_out, errors or None, stream,
+// the memories' tensors)
+PyObject *call_tree_commit(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return answer(n, 13, [&] {
+    const at::Tensor &table = tensor("table", a[5], 2), &path = tensor("path", a[7], 2);
+    const int device = static_cast<int>(whole("device", a[2], -1, INT_MAX));
+    const int64_t rows = table.size(0), width = table.size(1), nodes = path.size(1);
+    if (rows > INT_MAX || width > INT_MAX || nodes > INT_MAX) refuse("the table or the tree is too large");
+    qd_commit_args g{};
+    Written written;
+    add_some(written, "memory", a[12], 0, kMostTensors);
+    g.lengths_out = flat<int32_t>("lengths_out", a[9], at::kInt, {rows}, device, written);
+    if (!missing(a[10])) g.errors = flat<uint32_t>("errors", a[10], at::kInt, {1}, device, written);
+    const View t = view("table", a[5], at::kInt, {rows, width}, device, Lies::kRows);
+    g.table = static_cast<const int32_t *>(t.at);
+    g.table_stride = rows > 1 ? t.strides[0] : width;
+    g.lengths = flat<const int32_t>("lengths", a[6], at::kInt, {rows}, device);
+    g.path = flat<const int32_t>("path", a[7], at::kInt, {rows, nodes}, device);
+    g.counts = flat<const int32_t>("counts", a[8], at::kInt, {rows}, device);
+    g.memories = static_cast<const qd_token_memory *>(address("memories", a[3]));
+    g.memory_count = static_cast<uint32_t>(whole("memories", a[4], 0, UINT32_MAX));
+    g.rows = static_cast<uint32_t>(rows);
+    g.nodes = static_cast<uint32_t>(nodes);
+    g.table_width = static_cast<uint32_t>(width);
+    g.pages = static_cast<uint32_t>(whole("pages", a[1], 0, UINT32_MAX));
+    g.page_size = static_cast<uint32_t>(whole("page_size", a[0], 0, UINT32_MAX));
+    g.device = device;
+    return queue<const qd_commit_args *, void *>(written, g_calls.tree_commit, &g, address("stream", a[11]));
+  });
+}
+
+// (cache, bounds, recent, stream, the cache's tensors)
+PyObject *call_page_bounds(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return answer(n, 5, [&] {
+    const auto *c = static_cast<const qd_paged_cache *>(address("cache", a[0]));
+    Written written;
+    add_some(written, "cache", a[4], 4, 4);  // errors
+    const View bounds = view("bounds", a[1], type_of(c->dtype), {c->pages, c->kv_heads, 2, c->head_dim}, c->device, Lies::kTogether, &written);
+    return queue<const qd_paged_cache *, void *, uint32_t, void *>(
+        written, g_calls.page_bounds, c, bounds.at, static_cast<uint32_t>(whole("recent", a[2], 0, UINT32_MAX)), address("stream", a[3]));
+  });
+}
+
+// (cache, bounds, out, q, workspace, budget, first, last, chosen or None, scale or None, stream, the cache's tensors)
+PyObject *call_sparse_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return answer(n, 12, [&] {
+    const auto *c = static_cast<const qd_paged_cache *>(address("cache", a[0]));
+    const at::ScalarType type = type_of(c->dtype);
+    const int64_t rows = c->rows, heads = tensor("q", a[3], 3).size(1), dim = c->head_dim;
+    if (heads > INT_MAX) refuse("too many heads");
+    qd_sparse_args g{};
+    Written written;
+    add_some(written, "cache", a[11], 4, 4);  // errors
+    g.budget = static_cast<uint32_t>(whole("budget", a[5], 0, UINT32_MAX));
+    g.first = static_cast<uint32_t>(whole("first", a[6], 0, UINT32_MAX));
+    g.last = static_cast<uint32_t>(whole("last", a[7], 0, UINT32_MAX));
+    const View out = view("out", a[2], type, {rows, heads, dim}, c->device, Lies::kRows, &written);
+    if (!missing(a[8])) g.chosen = flat<int32_t>("chosen", a[8], at::kInt, {rows, c->kv_heads, g.budget}, c->device, written);
+    const View q = view("q", a[3], type, {rows, heads, dim}, c->device, Lies::kRows);
+    g.bounds = view("bounds", a[1], type, {c->pages, c->kv_heads, 2, dim}, c->device, Lies::kTogether).at;
+    g.q = q.at;
+    g.out = out.at;
+    g.q_stride = rows > 1 ? q.strides[0] : heads * dim;
+    g.out_stride = rows > 1 ? out.strides[0] : heads * dim;
+    g.q_head_stride = heads > 1 ? q.strides[1] : dim;
+    g.out_head_stride = heads > 1 ? out.strides[1] : dim;
+    g.heads = static_cast<uint32_t>(heads);
+    g.scale = scale_of(a[9], dim);
+    return queue<const qd_paged_cache *, const qd_sparse_args *, qd_workspace *, void *>(
+        written, g_calls.sparse_attention, c, &g, static_cast<qd_workspace *>(address("workspace", a[4])), address("stream", a[10]));
+  });
+}
+
 #define QD_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(call_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {QD_METHOD(bind), QD_METHOD(append), QD_METHOD(attention), QD_METHOD(fork), QD_METHOD(select),
-                           {nullptr, nullptr, 0, nullptr}};
+                           QD_METHOD(tree_attention), QD_METHOD(tree_accept), QD_METHOD(tree_commit), QD_METHOD(page_bounds),
+                           QD_METHOD(sparse_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_qd_tensors", nullptr, -1, g_methods};
 
 }  // namespace

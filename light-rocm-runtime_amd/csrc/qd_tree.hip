@@ -1,0 +1,1255 @@
+// Operators on trees of drafted tokens for gfx950: their attention over a paged
+// cache, the answer to them, and the move of what stands. Declared in
+// include/qd/qd_operators.h.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "qd_attention.hpp"
+#include "qd_device.hpp"
+#include "qd_device_math.hpp"
+#include "qd_operators.hpp"
+#include "qd_paged.hpp"
+
+namespace qd {
+namespace {
+
+using namespace dev;
+
+constexpr uint32_t kNan = 0x7FC00000u;
+
+// ---- the tree -------------------------------------------------------------------
+// A node's mask: itself and the nodes above it, each lane its own node's, by
+// doubling (after s steps a lane knows 2^s nodes of its chain). 0: not there.
+__device__ __forceinline__ uint64_t ancestors(const int32_t *parents, uint32_t nodes, bool &bad) {
+  const int lane = lane_id();
+  int up = static_cast<uint32_t>(lane) < nodes ? parents[lane] : -2;
+  const uint64_t there = __ballot(up >= -1);
+  // A parent comes before its child, and is there.
+  const bool wrong = up >= lane || (up >= 0 && !(there >> up & 1));
+  bad = __any(wrong);
+  if (wrong) up = -2;
+  uint64_t mask = up >= -1 ? 1ull << lane : 0ull;
+#pragma unroll
+  for (int s = 0; s < 6; ++s) {
+    const int from = up < 0 ? lane : up;
+    const uint64_t more = lane_of(mask, from);
+    const int next = __builtin_amdgcn_ds_bpermute(from << 2, up);
+    if (up >= 0) {
+      mask |= more;
+      up = next;
+    }
+  }
+  return mask;
+}
+
+// ---- attention --------------------------------------------------------------------
+// A row's queries of one KV head, its columns, are all pairs of a node and one of the
+// head's query heads. A workgroup takes a block of 16 NB WC columns over a run of the
+// row's positions, in stages of 32 WP: K and V of a stage go to LDS without passing
+// registers, the next stages' on their way, and are read from there by WC x WP waves,
+// each for 16 NB columns and 32 positions of the stage:
+//   S^T = K Q^T   lane l: column l % 16, positions 4 (l / 16) + r of each half
+//   O^T += V^T P^T with the lane's own probabilities as the operand; V is read in the
+//                 operand's layout, 16-bit types by transposing reads.
+// Positions before the tree are seen by every node; in the tree a bit of the node's
+// mask says so. What does not is hidden from the sum by its score, and by zeros in V's
+// place where V is not finite: the outputs that do see such a value become NaN.
+// Few rows are cut into runs that fill the card, which the last one joins in order.
+constexpr int kStep = 32;                // positions of a wave's step
+constexpr uint32_t kTreePieces = 64;     // of an item at most
+constexpr uint32_t kTreeLeast = 256;     // positions of a piece at least
+constexpr uint32_t kTreeCus = 256, kXcds = 8;
+constexpr uint32_t kLds = 160 * 1024;
+// As in the attention of one token (qd_paged.hip): a maximum is taken up once it passes
+// the one in use by so many powers of two, and FP16's scaled weights.
+template <typename E>
+constexpr float kLazy = 8.f;
+template <>
+constexpr float kLazy<Half> = 1.f;
+constexpr float kTreeWeight = 0x1p14f, kTreeRest = 0x1p12f;
+
+struct TreeLaunch {
+  qd_paged_cache c;
+  qd_tree_attention_args a;
+  float *records;      // [pieces][kv_heads * blocks][rec_floats]: acc [rec_columns][head_dim], maxima, sums
+  uint32_t *counters;  // [rows][kv_heads * blocks]
+  uint32_t apart;      // words between two counters
+  uint32_t group;      // query heads of a KV head
+  uint32_t columns;    // nodes * group
+  uint32_t blocks;     // of columns
+  uint32_t rec_columns, rec_floats;
+  uint32_t page_shift;
+  uint32_t target;     // pieces aimed at besides one of each row; 0: rows are not cut
+  uint32_t units;      // pieces x KV heads in the grid
+};
+
+// One 16-byte global -> LDS DMA per lane (lane l's bytes land at lds + 16 l), from
+// inline assembly: the compiler would guard every later LDS read with a wait for it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: set before each use, never saved
+__device__ __forceinline__ void dma_to_lds(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+template <int kLeft>
+__device__ __forceinline__ void dma_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4v lds_s4v;
+
+// A piece of an item: wave-uniform.
+struct Piece {
+  uint32_t row, kv, block;
+  int length, start;      // of the row, and where its tree begins
+  uint32_t first, last;   // stages
+  uint32_t index, pieces; // of the row
+  uint32_t number;        // of the row's first among all
+  bool bad;               // the length
+};
+
+template <typename E, int D, int NB, int WC, int WP>
+struct TreeShape {
+  static constexpr bool kWide = std::is_same_v<E, float>;
+  static constexpr int kElem = kWide ? 4 : 2;
+  static constexpr int kWaves = WC * WP, kThreads = kWaves * kWave;
+  static constexpr int kRowBytes = D * kElem, kPositions = kStep * WP;
+  static constexpr int kHalf = kPositions * kRowBytes;  // K or V of a stage
+  static constexpr int kStages = 2;
+  static constexpr int kColumns = 16 * NB * WC;
+  static constexpr int kRowsPerDma = 1024 / kRowBytes, kLanesPerRow = kRowBytes / 16;
+  static constexpr int kDmas = kPositions / kRowsPerDma / kWaves;  // of K, and of V, per wave and stage
+  static constexpr int kAcc = D / 16;
+  static constexpr int kMerge = (WP - 1) * WC * (NB * kAcc * 1024 + NB * 512);
+  static constexpr int kJoin = kColumns * (static_cast<int>(kTreePieces) + 1) * 4;
+  static constexpr int kBytes = std::max(kStages * 2 * kHalf, std::max(kMerge, kJoin));
+  static constexpr int kPerCu = 2 * (kBytes + 2048) <= static_cast<int>(kLds) ? 2 : 1;
+  static_assert(kDmas >= 1 && kDmas * kRowsPerDma * kWaves == kPositions, "whole transfers");
+  static_assert(kBytes + 2048 <= static_cast<int>(kLds), "LDS");
+};
+
+template <typename S>
+struct TreeShared {
+  __attribute__((aligned(1024))) char stage[S::kBytes];
+  uint64_t mask[64];     // of each node
+  uint64_t poison[128];  // nodes that see a value that is not finite, by dimension
+  uint32_t errors, last;
+};
+
+// Where 16-byte chunk c of row r of a stage lies in its row: so that neither rows
+// at one chunk (K) nor 4 x 4 rows at one pair of chunks (V) share banks.
+template <int kRowBytes, bool kWide>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
+  if constexpr (kWide) return r & 7;
+  return kRowBytes == 256 ? 2 * (r & 7) : 2 * (r >> 1 & 3);
+}
+
+template <typename E, int D, int NB, int WC, int WP>
+struct TreeAttention {
+  using S = TreeShape<E, D, NB, WC, WP>;
+  using Shared = TreeShared<S>;
+  static constexpr bool kWide = S::kWide;
+  static constexpr bool kScaled = std::is_same_v<E, Half>;
+  static constexpr int kQ = D * S::kElem / 64;  // 16-byte pieces of a query per lane
+
+  const TreeLaunch &p;
+  Shared &sh;
+  const Piece &it;
+  const int w, lane, col, quad, wc, wp;
+  const float scale;
+  const uint32_t token_bytes;
+  u4v q[NB][kQ];
+  f4v o[NB][S::kAcc];
+  float m[NB], ms[NB], l[NB];
+  int32_t ids[S::kDmas];  // the pages of the stage that is loaded next
+  uint32_t errors = 0;
+
+  __device__ __forceinline__ TreeAttention(const TreeLaunch &launch, Shared &shared, const Piece &piece)
+      : p(launch),
+        sh(shared),
+        it(piece),
+        w(__builtin_amdgcn_readfirstlane(wave_id())),
+        lane(lane_id()),
+        col(lane & 15),
+        quad(lane >> 4),
+        wc(w % WC),
+        wp(w / WC),
+        scale(p.a.scale * 1.44269504088896340736f),
+        token_bytes(static_cast<uint32_t>(p.c.token_stride) * S::kElem) {}
+
+  // This wave's n-th transfer of a stage begins at this row of it.
+  __device__ __forceinline__ uint32_t dma_row(int n) const { return (n * S::kWaves + w) * S::kRowsPerDma; }
+  __device__ __forceinline__ void pages_of(uint32_t stage) {
+    if (stage >= it.last) return;
+#pragma unroll
+    for (int n = 0; n < S::kDmas; ++n) {
+      const uint32_t pos = min(stage * S::kPositions + dma_row(n), static_cast<uint32_t>(it.length - 1));
+      ids[n] = load_uniform(p.c.table + it.row * p.c.table_stride + (pos >> p.page_shift));
+    }
+  }
+  // Positions past the length read the last one: nothing behind it is touched.
+  __device__ __forceinline__ void load(uint32_t stage) {
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)sh.stage)) +
+                         (stage - it.first) % S::kStages * (2 * S::kHalf);
+    const int64_t head = static_cast<int64_t>(it.kv) * p.c.head_stride;
+#pragma unroll
+    for (int n = 0; n < S::kDmas; ++n) {
+      const uint32_t row = dma_row(n), mine = row + lane / S::kLanesPerRow;
+      if (ids[n] < 0 || static_cast<uint32_t>(ids[n]) >= p.c.pages) {
+        errors |= QD_PAGED_BAD_PAGE;
+        continue;
+      }
+      const uint32_t pos = min(stage * S::kPositions + mine, static_cast<uint32_t>(it.length - 1)) & (p.c.page_size - 1);
+      const uint32_t chunk = (lane % S::kLanesPerRow) ^ swizzle<S::kRowBytes, kWide>(mine);
+      const int64_t base = (ids[n] * p.c.page_stride + head) * S::kElem;
+      const uint64_t off = static_cast<uint64_t>(pos) * token_bytes + 16 * chunk;
+      dma_to_lds(static_cast<const char *>(p.c.k) + base + off, lds + row * S::kRowBytes);
+      dma_to_lds(static_cast<const char *>(p.c.v) + base + off, lds + S::kHalf + row * S::kRowBytes);
+    }
+  }
+  __device__ __forceinline__ uint32_t column(int nb) const { return it.block * S::kColumns + (wc * NB + nb) * 16 + col; }
+  __device__ __forceinline__ void load_queries() {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t c = column(nb);
+      if (c < p.columns) {
+        const uint32_t node = c / p.group, head = it.kv * p.group + c % p.group;
+        const char *at = static_cast<const char *>(p.a.q) +
+                         (it.row * p.a.q_stride + node * p.a.q_node_stride + head * p.a.q_head_stride) * S::kElem + 16 * quad;
+#pragma unroll
+        for (int s = 0; s < kQ; ++s) q[nb][s] = *reinterpret_cast<const u4v *>(at + 64 * s);
+      } else {
+#pragma unroll
+        for (int s = 0; s < kQ; ++s) q[nb][s] = u4v{0u, 0u, 0u, 0u};
+      }
+    }
+  }
+  __device__ __forceinline__ const char *slot(uint32_t stage) const {
+    return sh.stage + (stage - it.first) % S::kStages * (2 * S::kHalf);
+  }
+  // Positions of the tree in a stage, and those past it: V's values that are not finite
+  // make way for zeros, and the nodes that see them are marked.
+  __device__ __forceinline__ void clean(uint32_t stage) {
+    char *v = const_cast<char *>(slot(stage)) + S::kHalf;
+    const int base = stage * S::kPositions;
+    for (int i = threadIdx.x; i < S::kPositions * S::kLanesPerRow; i += S::kThreads) {
+      const int row = i / S::kLanesPerRow, node = base + row - it.start;
+      if (node < 0) continue;
+      u4v *at = reinterpret_cast<u4v *>(v + i * 16);
+      u4v x = *at;
+      bool found = false;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (kWide) {
+          found |= (x[c] & 0x7F800000u) == 0x7F800000u;
+        } else {
+          constexpr uint32_t e = std::is_same_v<E, Half> ? 0x7C00u : 0x7F80u;
+          found |= (x[c] & e) == e || (x[c] >> 16 & e) == e;
+        }
+      }
+      if (!found) continue;
+      if (node >= static_cast<int>(p.a.nodes)) {
+        *at = u4v{0u, 0u, 0u, 0u};
+        continue;
+      }
+      uint64_t seen = 0;  // by these nodes
+      for (uint32_t n = 0; n < p.a.nodes; ++n) seen |= (sh.mask[n] >> node & 1) << n;
+      const uint32_t chunk = i % S::kLanesPerRow ^ swizzle<S::kRowBytes, kWide>(row);
+      uint32_t y[4] = {x[0], x[1], x[2], x[3]};
+      for (int d = 0; d < 16 / S::kElem; ++d) {
+        if constexpr (kWide) {
+          if ((y[d] & 0x7F800000u) != 0x7F800000u) continue;
+          y[d] = 0u;
+        } else {
+          constexpr uint32_t e = std::is_same_v<E, Half> ? 0x7C00u : 0x7F80u;
+          if ((y[d / 2] >> 16 * (d & 1) & e) != e) continue;
+          y[d / 2] &= d & 1 ? 0xFFFFu : 0xFFFF0000u;
+        }
+        atomicOr(reinterpret_cast<unsigned long long *>(&sh.poison[chunk * (16 / S::kElem) + d]), static_cast<unsigned long long>(seen));
+      }
+      *at = u4v{y[0], y[1], y[2], y[3]};
+    }
+  }
+  template <bool kTree>
+  __device__ __forceinline__ void step(uint32_t stage) {
+    const char *k = slot(stage) + wp * kStep * S::kRowBytes, *v = k + S::kHalf;
+    const int base = stage * S::kPositions + wp * kStep;
+    f4v s[2][NB];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) s[sub][nb] = f4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int t = 0; t < kQ; ++t) {
+        const uint32_t chunk = (4 * t + quad) ^ swizzle<S::kRowBytes, kWide>(col);
+        const u4v a = *reinterpret_cast<const u4v *>(k + (16 * sub + col) * S::kRowBytes + 16 * chunk);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if constexpr (kWide) {
+            const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, q[nb][t]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[sub][nb] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[c], y[c], s[sub][nb], 0, 0, 0);
+          } else {
+            s[sub][nb] = E::mfma(a, q[nb][t], s[sub][nb]);
+          }
+        }
+      }
+    float pr[NB][2][4], top[NB];
+    bool rises = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      uint64_t mask = 0;
+      if constexpr (kTree) {
+        const uint32_t c = column(nb);
+        mask = c < p.columns ? sh.mask[c / p.group] : 0ull;
+      }
+      top[nb] = -INFINITY;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = s[sub][nb][r] * scale;
+          if constexpr (kTree) {
+            const int node = base + 16 * sub + 4 * quad + r - it.start;
+            if (node >= 0 && (node >= static_cast<int>(p.a.nodes) || !(mask >> node & 1))) x = -INFINITY;
+          }
+          pr[nb][sub][r] = x;
+          top[nb] = fmaxf(top[nb], x);
+        }
+      rises |= top[nb] > m[nb] + kLazy<E>;
+    }
+    if (__any(rises)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float n = fmaxf(m[nb], quarters_max(top[nb]));
+        const float f = n == m[nb] ? 1.f : exp2_fast(m[nb] - n);
+        m[nb] = n;
+        ms[nb] = n == -INFINITY ? 0.f : n;
+        l[nb] *= f;
+#pragma unroll
+        for (int j = 0; j < S::kAcc; ++j) o[nb][j] *= f;
+      }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float sum = 0.f;
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          pr[nb][sub][r] = exp2_fast(pr[nb][sub][r] - ms[nb]);
+          sum += pr[nb][sub][r];
+        }
+      l[nb] += sum;
+    }
+    if constexpr (kWide) {
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t row = 16 * sub + 4 * quad + r;
+#pragma unroll
+          for (int n = 0; n < D / 64; ++n) {
+            const uint32_t chunk = (16 * n + col) ^ swizzle<S::kRowBytes, kWide>(row);
+            const f4v a = *reinterpret_cast<const f4v *>(v + row * S::kRowBytes + 16 * chunk);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                o[nb][4 * n + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[c], pr[nb][sub][r], o[nb][4 * n + c], 0, 0, 0);
+          }
+        }
+    } else {
+      // Probabilities as two numbers of the type, as in the attention of one token.
+      u4v b[NB], rest[NB];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = pr[nb][i >> 1][2 * (i & 1)], y = pr[nb][i >> 1][2 * (i & 1) + 1];
+          if constexpr (kScaled) {
+            b[nb][i] = E::pack(x * kTreeWeight, y * kTreeWeight);
+            rest[nb][i] = E::pack(fmaf(x, kTreeWeight, -E::lo(b[nb][i])) * kTreeRest, fmaf(y, kTreeWeight, -E::hi(b[nb][i])) * kTreeRest);
+          } else {
+            b[nb][i] = E::pack(x, y);
+            rest[nb][i] = E::pack(x - E::lo(b[nb][i]), y - E::hi(b[nb][i]));
+          }
+        }
+#pragma unroll
+      for (int j = 0; j < S::kAcc; ++j) {
+        u4v a;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          const uint32_t row = 16 * sub + 4 * quad + (col >> 2);
+          const uint32_t chunk = (2 * j + (col >> 1 & 1)) ^ swizzle<S::kRowBytes, kWide>(row);
+          const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4v *)(v + row * S::kRowBytes + 16 * chunk + 8 * (col & 1)));
+          const u2v y = __builtin_bit_cast(u2v, x);
+          a[2 * sub] = y[0];
+          a[2 * sub + 1] = y[1];
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if constexpr (kScaled) {
+            const f4v r = E::mfma(a, rest[nb], f4v{0.f, 0.f, 0.f, 0.f});
+            o[nb][j] = E::mfma(a, b[nb], o[nb][j]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[nb][j][c] = fmaf(r[c], 1.f / kTreeRest, o[nb][j][c]);
+          } else {
+            o[nb][j] = E::mfma(a, rest[nb], o[nb][j]);
+            o[nb][j] = E::mfma(a, b[nb], o[nb][j]);
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void run() {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      m[nb] = -INFINITY;
+      ms[nb] = l[nb] = 0.f;
+#pragma unroll
+      for (int j = 0; j < S::kAcc; ++j) o[nb][j] = f4v{0.f, 0.f, 0.f, 0.f};
+    }
+    if (it.length == 0) {
+      __syncthreads();
+      return;
+    }
+    for (uint32_t stage = it.first; stage < it.last; ++stage) {
+      dma_wait<0>();
+      lds_barrier();
+      if (stage + 1 < it.last) {
+        load(stage + 1);
+        pages_of(stage + 2);
+      }
+      if (static_cast<int>((stage + 1) * S::kPositions) > it.start) {
+        clean(stage);
+        lds_barrier();
+        if (static_cast<int>(stage * S::kPositions + wp * kStep) < it.length) step<true>(stage);
+      } else {
+        step<false>(stage);
+      }
+    }
+    lds_barrier();
+  }
+  // First dimension of this lane's i-th four of an accumulator.
+  static __device__ __forceinline__ int dim_of(int i) {
+    const int quad = lane_id() >> 4;
+    return kWide ? 64 * (i >> 2) + 4 * (4 * quad + (i & 3)) : 16 * i + 4 * quad;
+  }
+  __device__ __forceinline__ float4 four(int nb, int i) const {
+    if constexpr (kWide)
+      return make_float4(o[nb][i & ~3][i & 3], o[nb][(i & ~3) + 1][i & 3], o[nb][(i & ~3) + 2][i & 3], o[nb][(i & ~3) + 3][i & 3]);
+    else
+      return make_float4(o[nb][i][0], o[nb][i][1], o[nb][i][2], o[nb][i][3]);
+  }
+  // The waves' shares of the positions together, in the first WC waves.
+  __device__ __forceinline__ void merge() {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) l[nb] = quarters_sum(l[nb]);
+    if constexpr (WP > 1) {
+      constexpr int kShare = NB * S::kAcc * 1024 + NB * 512;
+      if (wp > 0) {
+        char *to = sh.stage + ((wp - 1) * WC + wc) * kShare;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+          for (int j = 0; j < S::kAcc; ++j) *reinterpret_cast<f4v *>(to + (nb * S::kAcc + j) * 1024 + lane * 16) = o[nb][j];
+          *reinterpret_cast<float2 *>(to + NB * S::kAcc * 1024 + nb * 512 + lane * 8) = make_float2(m[nb], l[nb]);
+        }
+      }
+      __syncthreads();
+      if (wp == 0) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float2 x[WP - 1];
+          float top = m[nb];
+#pragma unroll
+          for (int u = 0; u < WP - 1; ++u) {
+            x[u] = *reinterpret_cast<const float2 *>(sh.stage + (u * WC + wc) * kShare + NB * S::kAcc * 1024 + nb * 512 + lane * 8);
+            top = fmaxf(top, x[u].x);
+          }
+          const float f = m[nb] == top ? 1.f : exp2_fast(m[nb] - top);
+          l[nb] *= f;
+#pragma unroll
+          for (int j = 0; j < S::kAcc; ++j) o[nb][j] *= f;
+#pragma unroll
+          for (int u = 0; u < WP - 1; ++u) {
+            const float g = x[u].x == top ? 1.f : exp2_fast(x[u].x - top);
+            l[nb] = fmaf(g, x[u].y, l[nb]);
+#pragma unroll
+            for (int j = 0; j < S::kAcc; ++j) {
+              const f4v y = *reinterpret_cast<const f4v *>(sh.stage + (u * WC + wc) * kShare + (nb * S::kAcc + j) * 1024 + lane * 16);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nb][j][c] = fmaf(g, y[c], o[nb][j][c]);
+            }
+          }
+          m[nb] = top;
+        }
+      }
+    }
+  }
+  // Column c's four outputs from dimension d on.
+  __device__ __forceinline__ void emit(uint32_t c, int d, float4 acc, float sum, float poison) const {
+    const uint32_t node = c / p.group, head = it.kv * p.group + c % p.group;
+    const bool there = !it.bad && it.length > 0 && sh.mask[node] != 0;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (there) {
+      const float inv = 1.f / sum;
+      x = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+    if (poison != 0.f) x = make_float4(poison, poison, poison, poison);  // NaN
+    store4<E>(p.a.out, it.row * p.a.out_stride + node * p.a.out_node_stride + head * p.a.out_head_stride + d, x);
+  }
+  // The piece's result, out or to its record.
+  __device__ __forceinline__ void put(float *record) {
+    const float nan = __uint_as_float(kNan);
+    const bool spoilt = sh.errors != 0, whole = it.pieces == 1;
+    const bool tree = static_cast<int>(it.last * S::kPositions) > it.start && it.length > 0;
+    if (threadIdx.x == 0 && spoilt) raise_error(p.c.errors, sh.errors);
+    if (wp > 0) return;
+    constexpr float unit = kScaled ? 1.f / kTreeWeight : 1.f;
+    const Coherent rec(record, p.rec_floats * static_cast<uint32_t>(sizeof(float)));
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t c = column(nb), mine = c - it.block * S::kColumns;
+      if (c >= p.columns) continue;
+      const uint32_t node = c / p.group;
+#pragma unroll
+      for (int i = 0; i < S::kAcc; ++i) {
+        const int d = dim_of(i);
+        float4 x = four(nb, i);
+        x = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
+        if (tree) {
+          if (sh.poison[d] >> node & 1) x.x = nan;
+          if (sh.poison[d + 1] >> node & 1) x.y = nan;
+          if (sh.poison[d + 2] >> node & 1) x.z = nan;
+          if (sh.poison[d + 3] >> node & 1) x.w = nan;
+        }
+        if (whole) {
+          emit(c, d, x, l[nb], spoilt ? nan : 0.f);
+        } else {
+          if (spoilt) x = make_float4(nan, nan, nan, nan);
+          rec.st4((mine * D + d) / 4, x);
+        }
+      }
+      if (!whole && quad == 0) {
+        rec.st(p.rec_columns * D + mine, spoilt ? nan : m[nb]);
+        rec.st(p.rec_columns * (D + 1) + mine, l[nb]);
+      }
+    }
+  }
+  // Counts the piece in; true in the workgroup whose piece came last.
+  __device__ __forceinline__ bool arrive() {
+    wait_vm_stores();
+    __syncthreads();
+    uint32_t *cnt = p.counters + (static_cast<size_t>(it.row) * p.c.kv_heads * p.blocks + it.kv * p.blocks + it.block) * p.apart;
+    if (threadIdx.x == 0) {
+      sh.last = atomicAdd(cnt, 1u) == it.pieces - 1;
+      if (sh.last) *cnt = 0u;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(sh.last);
+  }
+  // Joins the pieces in their order. Piece u's record is u * stride floats behind the first.
+  __device__ __forceinline__ void join(const float *first, uint32_t stride) {
+    float *weight = reinterpret_cast<float *>(sh.stage);  // [columns][pieces]
+    float *sums = weight + S::kColumns * kTreePieces;
+    const uint32_t n = it.pieces, columns = min(static_cast<uint32_t>(S::kColumns), p.columns - it.block * S::kColumns);
+    const Coherent rec(first, ((n - 1) * stride + p.rec_floats) * static_cast<uint32_t>(sizeof(float)));
+    for (uint32_t c = threadIdx.x; c < columns; c += S::kThreads) {
+      float top = -INFINITY, sum = 0.f;
+      bool spoilt = false;
+      for (uint32_t u = 0; u < n; ++u) {
+        const float x = rec.ld(u * stride + p.rec_columns * D + c);
+        spoilt |= x != x;
+        top = fmaxf(top, x);
+      }
+      for (uint32_t u = 0; u < n; ++u) {
+        const float x = rec.ld(u * stride + p.rec_columns * D + c);
+        const float f = spoilt ? __uint_as_float(kNan) : x == top ? 1.f : exp2_fast(x - top);
+        weight[c * kTreePieces + u] = f;
+        sum = fmaf(f, rec.ld(u * stride + p.rec_columns * (D + 1) + c), sum);
+      }
+      sums[c] = sum;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < columns * (D / 4); i += S::kThreads) {
+      const uint32_t c = i / (D / 4), d = 4 * (i % (D / 4));
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t u = 0; u < n; ++u) {
+        const float f = weight[c * kTreePieces + u];
+        const float4 x = rec.ld4((u * stride + c * D + d) / 4);
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+      }
+      const float sum = sums[c];
+      emit(it.block * S::kColumns + c, d, acc, sum, weight[c * kTreePieces] != weight[c * kTreePieces] ? __uint_as_float(kNan) : 0.f);
+    }
+  }
+};
+
+// The piece that a workgroup takes: rows are cut into pieces of `size` stages, so
+// that there are about `target` of them besides one of each row.
+template <int kPositions>
+__device__ __forceinline__ bool find_piece(const TreeLaunch &p, Piece &it) {
+  // Consecutive workgroups go to consecutive XCDs: the blocks of a piece, which read
+  // the same positions, come to one.
+  const uint32_t xcd = blockIdx.x % kXcds, idx = blockIdx.x / kXcds;
+  const uint32_t unit = idx / p.blocks * kXcds + xcd;
+  if (unit >= p.units) return false;
+  it.block = idx % p.blocks;
+  it.kv = unit % p.c.kv_heads;
+  const uint32_t x = unit / p.c.kv_heads;
+  const int lane = lane_id();
+  const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
+  const auto wrong = [&](int32_t n) { return n != 0 && (n < static_cast<int32_t>(p.a.nodes) || n > most); };
+  const auto stages_of = [&](int32_t n) { return wrong(n) || n == 0 ? 1u : (static_cast<uint32_t>(n) + kPositions - 1) / kPositions; };
+  uint32_t size = 0x7fffffffu, row = x;
+  int32_t n = 0;
+  it.number = x;
+  it.pieces = 1;
+  if (p.target) {
+    uint32_t total = 0, longest = 0;
+    for (uint32_t r = lane; r < p.c.rows; r += kWave) {
+      n = p.c.lengths[r];
+      total += stages_of(n);
+      longest = max(longest, stages_of(n));
+    }
+    total = __builtin_amdgcn_readlane(lanes_upto(total), kWave - 1);
+    size = max(max((kTreeLeast + kPositions - 1) / kPositions, (total + p.target - 1) / p.target), (lanes_max(longest) + kTreePieces - 1) / kTreePieces);
+    const bool once = p.c.rows <= kWave;
+    uint32_t base = 0, upto, mine;
+    it.number = 0;
+    uint64_t past;
+    for (;; base += kWave) {
+      if (base >= p.c.rows) return false;
+      if (!once) n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
+      mine = base + lane < p.c.rows ? (stages_of(n) + size - 1) / size : 0u;
+      upto = lanes_upto(mine);
+      past = __ballot(it.number + upto > x);
+      if (past) break;
+      it.number += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
+    row = base + at;
+    it.number += __builtin_amdgcn_readlane(upto - mine, at);
+    n = __builtin_amdgcn_readlane(n, at);
+    it.pieces = __builtin_amdgcn_readlane(mine, at);
+  } else {
+    n = load_uniform(p.c.lengths + row);
+  }
+  it.row = row;
+  it.bad = wrong(n);
+  it.length = it.bad ? 0 : n;
+  it.start = it.length - static_cast<int>(p.a.nodes);
+  it.index = x - it.number;
+  const uint32_t stages = stages_of(n);
+  it.first = it.pieces == 1 ? 0 : it.index * size;
+  it.last = it.pieces == 1 ? stages : min(stages, it.first + size);
+  return true;
+}
+
+template <typename E, int D, int NB, int WC, int WP>
+__global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunch p) {
+  using S = TreeShape<E, D, NB, WC, WP>;
+  __shared__ TreeShared<S> sh;
+  Piece it;
+  if (!find_piece<S::kPositions>(p, it)) return;
+  TreeAttention<E, D, NB, WC, WP> a(p, sh, it);
+  if (it.length) {
+    a.pages_of(it.first);
+    a.load(it.first);
+    a.pages_of(it.first + 1);
+  }
+  if (threadIdx.x == 0) sh.errors = 0;
+  for (int i = threadIdx.x; i < 128; i += S::kThreads) sh.poison[i] = 0;
+  if (a.w == 0) {
+    bool bad;
+    const uint64_t mask = ancestors(p.a.parents + static_cast<size_t>(it.row) * p.a.nodes, p.a.nodes, bad);
+    sh.mask[a.lane] = mask;
+    if (bad) a.errors |= QD_TREE_BAD_PARENT;
+  }
+  if (it.bad) a.errors |= QD_PAGED_BAD_LENGTH;
+  a.load_queries();
+  a.run();
+  if (a.errors && a.lane == 0) atomicOr(&sh.errors, a.errors);
+  a.merge();
+  if constexpr (WP == 1) __syncthreads();
+  // (Without columns of its own a block has none to put together.)
+  const uint32_t stride = p.c.kv_heads * p.blocks * p.rec_floats;
+  float *first = p.records + (static_cast<size_t>(it.number) * p.c.kv_heads * p.blocks + it.kv * p.blocks + it.block) * p.rec_floats;
+  a.put(first + static_cast<size_t>(it.index) * stride);
+  if (it.pieces == 1) return;
+  if (a.arrive()) a.join(first, stride);
+}
+
+struct TreePlan {
+  uint32_t group, columns, block_columns, blocks, rec_columns, rec_floats, apart, target, positions, records;
+};
+// The columns of a workgroup: as many as there are, by steps that the kernels come in.
+constexpr uint32_t block_columns_of(uint32_t columns) { return columns <= 16 ? 16 : columns <= 32 ? 32 : columns <= 64 ? 64 : 128; }
+
+// Calls f with the kernel's shape for so many columns.
+template <typename E, int D, typename F>
+auto with_shape(uint32_t block_columns, F &&f) {
+  // FP32 heads of 128: half as many positions a stage.
+  constexpr int kFew = std::is_same_v<E, float> && D == 128 ? 2 : 4;
+  switch (block_columns) {
+    case 16: return f(TreeShape<E, D, 1, 1, kFew>{}, tree_attention_kernel<E, D, 1, 1, kFew>);
+    case 32:
+      if constexpr (std::is_same_v<E, float>)
+        return f(TreeShape<E, D, 1, 2, kFew>{}, tree_attention_kernel<E, D, 1, 2, kFew>);
+      else
+        return f(TreeShape<E, D, 2, 1, kFew>{}, tree_attention_kernel<E, D, 2, 1, kFew>);
+    case 64:
+      if constexpr (std::is_same_v<E, float>)
+        return f(TreeShape<E, D, 1, 4, 2>{}, tree_attention_kernel<E, D, 1, 4, 2>);
+      else
+        return f(TreeShape<E, D, 2, 2, 4>{}, tree_attention_kernel<E, D, 2, 2, 4>);
+    default: return f(TreeShape<E, D, 2, 4, 2>{}, tree_attention_kernel<E, D, 2, 4, 2>);
+  }
+}
+template <typename F>
+auto with_type(uint32_t dtype, uint32_t head_dim, uint32_t block_columns, F &&f) {
+  const bool wide = head_dim == 128;
+  switch (dtype) {
+    case QD_DTYPE_F32: return wide ? with_shape<float, 128>(block_columns, f) : with_shape<float, 64>(block_columns, f);
+    case QD_DTYPE_BF16: return wide ? with_shape<Brain, 128>(block_columns, f) : with_shape<Brain, 64>(block_columns, f);
+    default: return wide ? with_shape<Half, 128>(block_columns, f) : with_shape<Half, 64>(block_columns, f);
+  }
+}
+
+TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  TreePlan s{};
+  s.group = heads / kv_heads;
+  s.columns = nodes * s.group;
+  s.block_columns = block_columns_of(s.columns);
+  s.blocks = (s.columns + s.block_columns - 1) / s.block_columns;
+  s.rec_columns = std::min(s.columns, s.block_columns);
+  s.rec_floats = (s.rec_columns * (head_dim + 2) + 3) / 4 * 4;
+  const uint64_t items = static_cast<uint64_t>(rows) * kv_heads * s.blocks;
+  if (items <= kOpCounters) {
+    s.target = std::max(1u, 2 * kTreeCus / (kv_heads * s.blocks));
+    s.records = (rows + s.target) * kv_heads * s.blocks;
+    for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
+  }
+  return s;
+}
+
+// ---- accept ------------------------------------------------------------------------
+// A workgroup takes a share of one node's logits: its largest, or (draws) the sum of
+// exp(x / T) in 64 bits relative to a power of two. Greedy, the last share of a row to
+// arrive walks the tree; with draws the last share of a node finds the share in which the
+// running sum passes the draw, reads it again and picks the token, and the last node of a
+// row walks. Bound by memory for large batches, by the chain of hand-overs for small ones.
+constexpr int kAcceptT = 256;
+constexpr uint32_t kAcceptShares = 64;    // of a node at most: a lane each
+constexpr uint32_t kAcceptAim = 1024;     // shares in all
+constexpr uint32_t kAcceptLeast = 4096;   // logits of a share at least
+constexpr float kHuge = 1e30f;            // logits past it are not exponentiated
+
+struct AcceptShare {
+  double sum;    // of 2^(x c - r), or the largest logit and its token
+  float r;
+  uint32_t pad;
+};
+struct AcceptLaunch {
+  qd_accept_args a;
+  AcceptShare *share;   // [rows * nodes][shares]
+  int32_t *picks;       // [rows * nodes]
+  uint32_t *counters;   // [rows * nodes] nodes, then [rows] rows
+  uint32_t shares;
+  float c_hi, c_lo;     // log2(e) / temperature
+};
+
+// Logits `at` .. of a row that may start anywhere: as FP32.
+template <typename E>
+__device__ __forceinline__ float logit(const void *row, uint32_t i) {
+  if constexpr (std::is_same_v<E, float>) {
+    return static_cast<const float *>(row)[i];
+  } else {
+    const uint32_t v = static_cast<const uint16_t *>(row)[i];
+    return E::lo(v);
+  }
+}
+// 2^(x c - r), where x c is computed to about 2^-46 of it. NaN and what is below -1e30 give 0.
+__device__ __forceinline__ float power(float x, float c_hi, float c_lo, float r) {
+  x = fmaxf(x, -kHuge);
+  const float hi = x * c_hi, lo = fmaf(x, c_lo, fmaf(x, c_hi, -hi));
+  return exp2_fast((hi - r) + lo);
+}
+__device__ __forceinline__ double scaled(double s, float by) { return ldexp(s, static_cast<int>(fmaxf(by, -4000.f))); }
+
+template <typename E, bool kSampled>
+__global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
+  constexpr int kW = kAcceptT / kWave, kPer = std::is_same_v<E, float> ? 4 : 8, kAhead = 4;
+  __shared__ double sums[kAcceptT];
+  __shared__ float tops[kW];
+  __shared__ uint32_t ids[kW], last;
+  __shared__ int32_t picked;
+  const uint32_t node = blockIdx.y % p.a.nodes, row = blockIdx.y / p.a.nodes, share = blockIdx.x;
+  const int lane = lane_id(), w = wave_id();
+  const size_t at = static_cast<size_t>(row) * p.a.nodes;
+  const int32_t parent = static_cast<uint32_t>(lane) < p.a.nodes ? p.a.parents[at + lane] : -2;
+  const uint64_t there = __ballot(parent >= -1);
+  const bool bad = __any(parent >= lane || (parent >= 0 && !(there >> parent & 1)));
+  if (bad || !(there & 1)) {
+    if (node == 0 && share == 0) {
+      if (bad && threadIdx.x == 0) raise_error(p.a.errors, QD_TREE_BAD_PARENT);
+      if (threadIdx.x < p.a.nodes) p.a.path[at + threadIdx.x] = -1;
+      if (threadIdx.x == 0) {
+        p.a.counts[row] = 0;
+        p.a.next_tokens[row] = -1;
+      }
+    }
+    return;
+  }
+  if (!(there >> node & 1)) return;
+  const uint32_t present = __popcll(there);
+  const char *x = static_cast<const char *>(p.a.logits) + (row * p.a.row_stride + node * p.a.node_stride) * static_cast<int64_t>(16 / kPer);
+  // The row's 16-byte pieces, and what lies before the first of them.
+  const uint32_t skew = static_cast<uint32_t>(-(reinterpret_cast<uintptr_t>(x) / (16 / kPer))) % kPer;
+  const uint32_t head = min(skew, p.a.vocab), pieces = (p.a.vocab - head) / kPer;
+  // Piece j of share s: [s * each, (s + 1) * each); the first has the head, the last the tail too.
+  const uint32_t each = (pieces + p.shares - 1) / p.shares;
+  const auto begin_of = [&](uint32_t s) { return s == 0 ? 0u : min(pieces, s * each) * kPer + head; };
+  const auto end_of = [&](uint32_t s) { return s + 1 == p.shares ? p.a.vocab : min(pieces, (s + 1) * each) * kPer + head; };
+  const uint32_t from = min(pieces, share * each), to = min(pieces, (share + 1) * each);
+  float top = -INFINITY;
+  uint32_t best = UINT32_MAX;
+  double sum = 0.0;
+  float r = -INFINITY;  // (a whole number)
+  const auto take = [&](float v, uint32_t i) {
+    if (v > top) {
+      top = v;
+      best = i;
+    }
+  };
+  // Raises r to the largest logit so far.
+  const auto raise = [&](float most) {
+    if (most > top) {
+      top = most;
+      const float up = ceilf(fminf(most, kHuge) * p.c_hi);
+      if (up > r) {
+        sum = r == -INFINITY ? 0.0 : scaled(sum, r - up);
+        r = up;
+      }
+    }
+  };
+  const auto values = [&](const u4v &v, float (&y)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t word = v[i];
+      if constexpr (std::is_same_v<E, float>) {
+        y[i] = __uint_as_float(word);
+      } else {
+        y[2 * i] = E::lo(word);
+        y[2 * i + 1] = E::hi(word);
+      }
+    }
+  };
+  const auto single = [&](uint32_t i) {
+    const float v = logit<E>(x, i);
+    if constexpr (kSampled) {
+      raise(fmaxf(v, -kHuge));
+      sum += power(v, p.c_hi, p.c_lo, r);
+    } else {
+      take(v, i);
+    }
+  };
+  if (share == 0 && threadIdx.x < head) single(threadIdx.x);
+  const u4v *body = reinterpret_cast<const u4v *>(x + head * (16 / kPer));
+  for (uint32_t j = from + threadIdx.x; j < to; j += kAhead * kAcceptT) {
+    u4v v[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = body[min(j + u * kAcceptT, to - 1)];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const uint32_t k = j + u * kAcceptT;
+      if (k >= to) break;
+      float y[kPer];
+      values(v[u], y);
+      if constexpr (kSampled) {
+        float most = -kHuge;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) most = fmaxf(most, y[i]);
+        raise(most);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += power(y[i], p.c_hi, p.c_lo, r);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) take(y[i], head + k * kPer + i);
+      }
+    }
+  }
+  if (share + 1 == p.shares && head + pieces * kPer + threadIdx.x < p.a.vocab) single(head + pieces * kPer + threadIdx.x);
+  // The workgroup's share.
+  AcceptShare mine{0.0, 0.f, 0u};
+  if constexpr (kSampled) {
+    const float wave_top = wave_max(top);
+    if (lane == 0) tops[w] = wave_top;
+    __syncthreads();
+    float all = tops[0];
+#pragma unroll
+    for (int u = 1; u < kW; ++u) all = fmaxf(all, tops[u]);
+    mine.r = all;  // the largest logit; sums relative to the whole number above it
+    const float up = ceilf(fminf(all, kHuge) * p.c_hi);
+    double s = r == -INFINITY ? 0.0 : scaled(sum, r - up);
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) s += lane_of(s, lane ^ step);
+    if (lane == 0) sums[w] = s;
+    __syncthreads();
+    mine.sum = sums[0];
+#pragma unroll
+    for (int u = 1; u < kW; ++u) mine.sum += sums[u];
+  } else {
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) {
+      const float v = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane ^ step) << 2, __builtin_bit_cast(int, top)));
+      const uint32_t i = __builtin_amdgcn_ds_bpermute((lane ^ step) << 2, static_cast<int>(best));
+      if (better(v, i, top, best)) {
+        top = v;
+        best = i;
+      }
+    }
+    if (lane == 0) {
+      tops[w] = top;
+      ids[w] = best;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int u = 1; u < kW; ++u)
+        if (better(tops[u], ids[u], top, best)) {
+          top = tops[u];
+          best = ids[u];
+        }
+      mine.r = top;
+      mine.pad = best;
+    }
+  }
+  const size_t shares_of_node = (at + node) * p.shares;
+  const Coherent shares(p.share + at * p.shares, static_cast<uint32_t>(p.a.nodes * p.shares * sizeof(AcceptShare)));
+  const auto word = [&](uint32_t n, uint32_t s) { return (n * p.shares + s) * 4; };
+  (void)shares_of_node;
+  if (threadIdx.x == 0) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, mine.sum);
+    shares.stu(word(node, share), static_cast<uint32_t>(bits));
+    shares.stu(word(node, share) + 1, static_cast<uint32_t>(bits >> 32));
+    shares.st(word(node, share) + 2, mine.r);
+    shares.stu(word(node, share) + 3, mine.pad);
+  }
+  const auto arrive = [&](uint32_t *counter, uint32_t of) {
+    wait_vm_stores();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      last = atomicAdd(counter, 1u) == of - 1;
+      if (last) *counter = 0u;
+    }
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(last) != 0;
+  };
+  uint32_t *row_counter = p.counters + static_cast<size_t>(p.a.rows) * p.a.nodes + row;
+  int32_t pick = 0;  // lane n's: node n's
+  if constexpr (!kSampled) {
+    if (!arrive(row_counter, present * p.shares)) return;
+    if (w != 0) return;
+    float v = -INFINITY;
+    uint32_t id = UINT32_MAX;
+    if (there >> lane & 1)
+      for (uint32_t s = 0; s < p.shares; ++s) {
+        const float y = shares.ld(word(lane, s) + 2);
+        const uint32_t i = shares.ldu(word(lane, s) + 3);
+        if (better(y, i, v, id)) {
+          v = y;
+          id = i;
+        }
+      }
+    pick = id == UINT32_MAX ? 0 : static_cast<int32_t>(id);  // (nothing above -inf)
+  } else {
+    if (!arrive(p.counters + at + node, p.shares)) return;
+    // Every wave: all shares, a lane each.
+    float most = -INFINITY;
+    double s = 0.0;
+    if (static_cast<uint32_t>(lane) < p.shares) {
+      most = shares.ld(word(node, lane) + 2);
+      const uint64_t lo = shares.ldu(word(node, lane)), hi = shares.ldu(word(node, lane) + 1);
+      s = __builtin_bit_cast(double, hi << 32 | lo);
+    }
+    const float all = wave_max(most);
+    if (threadIdx.x == 0) picked = -1;
+    __syncthreads();
+    if (!(all > -kHuge && all < kHuge)) {
+      // The largest logit, read again by the whole workgroup.
+      top = -INFINITY;
+      best = UINT32_MAX;
+      for (uint32_t i = threadIdx.x; i < p.a.vocab; i += kAcceptT) take(logit<E>(x, i), i);
+      const float wave_top = wave_max(top);
+      if (lane == 0) tops[w] = wave_top;
+      if (threadIdx.x == 0) ids[0] = UINT32_MAX;
+      __syncthreads();
+      const float m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      if (top == m && best != UINT32_MAX) atomicMin(&ids[0], best);
+      __syncthreads();
+      if (threadIdx.x == 0) picked = ids[0] == UINT32_MAX ? 0 : static_cast<int32_t>(ids[0]);
+    } else {
+      const float up = ceilf(all * p.c_hi);
+      s = scaled(s, ceilf(fminf(most, kHuge) * p.c_hi) - up);
+      double upto = s;
+#pragma unroll
+      for (int step = 1; step < kWave; step <<= 1) {
+        const double v = lane_of(upto, max(lane - step, 0));
+        if (lane >= step) upto += v;
+      }
+      const double total = lane_of(upto, kWave - 1), aim = static_cast<double>(p.a.draws[at + node]) * total;
+      const uint64_t past = __ballot(upto > aim), some = __ballot(s > 0.0);
+      // (A draw of 1 or more passes nothing: the last share with a token.)
+      const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<unsigned long long>(some));
+      const double before = lane_of(upto - s, in);
+      const uint32_t begin = begin_of(in), end = end_of(in), n = (end - begin + kAcceptT - 1) / kAcceptT;
+      const uint32_t a = min(end, begin + threadIdx.x * n), b = min(end, a + n);
+      double run = 0.0;
+      for (uint32_t i = a; i < b; ++i) run += power(logit<E>(x, i), p.c_hi, p.c_lo, up);
+      sums[threadIdx.x] = run;
+      __syncthreads();
+      // The first thread whose run passes the draw, or the last with a token.
+      double mine_before = before;
+      for (int u = 0; u < static_cast<int>(threadIdx.x); ++u) mine_before += sums[u];
+      const uint64_t passes = __ballot(run > 0.0 && mine_before + run > aim), any = __ballot(run > 0.0);
+      if (lane == 0) {
+        ids[w] = passes ? w * kWave + __ffsll(static_cast<unsigned long long>(passes)) - 1 : UINT32_MAX;
+        tops[w] = any ? static_cast<float>(w * kWave + 63 - __clzll(static_cast<unsigned long long>(any))) : -1.f;
+      }
+      __syncthreads();
+      uint32_t who = min(min(ids[0], ids[1]), min(ids[2], ids[3]));
+      if (who == UINT32_MAX) who = static_cast<uint32_t>(fmaxf(0.f, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))));
+      if (threadIdx.x == who) {
+        uint32_t found = a;
+        for (uint32_t i = a; i < b; ++i) {
+          const float y = power(logit<E>(x, i), p.c_hi, p.c_lo, up);
+          if (y > 0.f) found = i;
+          mine_before += y;
+          if (y > 0.f && mine_before > aim) break;
+        }
+        picked = static_cast<int32_t>(found);
+      }
+    }
+    __syncthreads();
+    const Coherent picks(p.picks + at, static_cast<uint32_t>(p.a.nodes * sizeof(int32_t)));
+    if (threadIdx.x == 0) picks.stu(node, static_cast<uint32_t>(picked));
+    if (!arrive(row_counter, present)) return;
+    if (w != 0) return;
+    if (there >> lane & 1) pick = static_cast<int32_t>(picks.ldu(lane));
+  }
+  // The walk: lane n is node n.
+  const int32_t token = static_cast<uint32_t>(lane) < p.a.nodes ? p.a.tokens[at + lane] : -1;
+  const int32_t wanted = __builtin_amdgcn_ds_bpermute(max(parent, 0) << 2, pick);
+  const bool fits = parent >= 0 && token == wanted;
+  int32_t here = 0, path = -1;
+  uint32_t count = 0;
+  for (;;) {
+    if (static_cast<uint32_t>(lane) == count) path = here;
+    ++count;
+    const uint64_t next = __ballot(fits && parent == here);
+    if (!next) break;
+    here = __ffsll(static_cast<unsigned long long>(next)) - 1;
+  }
+  if (static_cast<uint32_t>(lane) < p.a.nodes) p.a.path[at + lane] = path;
+  const int32_t following = __builtin_amdgcn_readlane(pick, here);
+  if (lane == 0) {
+    p.a.counts[row] = static_cast<int32_t>(count);
+    p.a.next_tokens[row] = following;
+  }
+}
+
+// ---- commit --------------------------------------------------------------------------
+// Lane n of every wave looks up node n's move; a workgroup takes 64 columns of 16 bytes of
+// one row, its waves every fourth move, and stores when all of them are loaded: a move's
+// target is an earlier move's source. Bound by memory for large trees, else by the chain
+// length, path, page, load, store.
+constexpr int kCommitT = 256;
+constexpr int kMovesPerWave = 64 / (kCommitT / kWave);
+struct CommitLaunch {
+  qd_commit_args a;         // (a.memories is not for the device)
+  qd_token_memory memory[kForkMemories];
+  uint32_t columns[kForkMemories];  // of 16 bytes in all planes
+  uint32_t page_shift;
+};
+
+__global__ __launch_bounds__(kCommitT) void commit_kernel(CommitLaunch p) {
+  const uint32_t row = blockIdx.y, lane = lane_id(), w = wave_id();
+  const int32_t length = p.a.lengths[row], nodes = static_cast<int32_t>(p.a.nodes);
+  const bool first = blockIdx.x == 0 && threadIdx.x == 0;
+  if (length == 0) {
+    if (first) p.a.lengths_out[row] = 0;
+    return;
+  }
+  const int64_t room = static_cast<int64_t>(p.a.table_width) << p.page_shift;
+  uint32_t bad = length < nodes || length > room ? QD_PAGED_BAD_LENGTH : 0;
+  const int32_t count = p.a.counts[row], start = length - nodes;
+  if (count < 0 || count > nodes) bad |= QD_TREE_BAD_PATH;
+  int32_t from = -1, from_page = -1, to_page = -1;
+  const bool mine = !bad && static_cast<int32_t>(lane) < count;
+  if (mine) from = p.a.path[static_cast<size_t>(row) * p.a.nodes + lane];
+  const int32_t before = __builtin_amdgcn_ds_bpermute((static_cast<int>(lane) - 1) << 2, from);
+  if (__any(mine && (from < 0 || from >= nodes || (lane > 0 && from <= before)))) bad |= QD_TREE_BAD_PATH;
+  const bool moves = mine && !bad && from != static_cast<int32_t>(lane);
+  if (moves) {
+    const int32_t *table = p.a.table + row * p.a.table_stride;
+    from_page = table[(start + from) >> p.page_shift];
+    to_page = table[(start + static_cast<int32_t>(lane)) >> p.page_shift];
+  }
+  if (__any(moves && (from_page < 0 || static_cast<uint32_t>(from_page) >= p.a.pages || to_page < 0 ||
+                      static_cast<uint32_t>(to_page) >= p.a.pages)))
+    bad |= QD_PAGED_BAD_PAGE;
+  if (first) {
+    p.a.lengths_out[row] = bad ? length : start + count;
+    if (bad) raise_error(p.a.errors, bad);
+  }
+  if (bad) return;
+  const uint64_t moving = __ballot(moves);
+  if (!moving) return;
+  // This lane's column.
+  uint32_t column = blockIdx.x * kWave + lane;
+  char *base = nullptr;
+  int64_t page_stride = 0, token_stride = 0;
+#pragma unroll
+  for (uint32_t m = 0; m < kForkMemories; ++m) {
+    if (m >= p.a.memory_count || base) continue;
+    if (column >= p.columns[m]) {
+      column -= p.columns[m];
+      continue;
+    }
+    const uint32_t per_piece = p.memory[m].piece_bytes / 16, piece = column / per_piece;
+    base = static_cast<char *>(p.memory[m].base) + piece / p.memory[m].pieces * p.memory[m].plane_stride +
+           piece % p.memory[m].pieces * p.memory[m].piece_stride + column % per_piece * 16;
+    page_stride = p.memory[m].page_stride;
+    token_stride = p.memory[m].token_stride;
+  }
+  const int32_t mask = static_cast<int32_t>(p.a.page_size) - 1;
+  u4v x[kMovesPerWave];
+#pragma unroll
+  for (int u = 0; u < kMovesPerWave; ++u) {
+    const int i = __builtin_amdgcn_readfirstlane(w) + u * (kCommitT / kWave);
+    if (!(moving >> i & 1)) continue;
+    const int32_t pos = start + __builtin_amdgcn_readlane(from, i), page = __builtin_amdgcn_readlane(from_page, i);
+    if (base) x[u] = *reinterpret_cast<const u4v *>(base + page * page_stride + (pos & mask) * token_stride);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kMovesPerWave; ++u) {
+    const int i = __builtin_amdgcn_readfirstlane(w) + u * (kCommitT / kWave);
+    if (!(moving >> i & 1)) continue;
+    const int32_t pos = start + i, page = __builtin_amdgcn_readlane(to_page, i);
+    if (base) *reinterpret_cast<u4v *>(base + page * page_stride + (pos & mask) * token_stride) = x[u];
+  }
+}
+
+uint32_t accept_shares(uint32_t rows, uint32_t nodes, uint32_t vocab) {
+  const uint64_t all = static_cast<uint64_t>(rows) * nodes;
+  const uint64_t want = (kAcceptAim + all - 1) / std::max<uint64_t>(all, 1);
+  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min({want, static_cast<uint64_t>(kAcceptShares),
+                                                                static_cast<uint64_t>((vocab + kAcceptLeast - 1) / kAcceptLeast)})));
+}
+
+}  // namespace
+
+size_t tree_attention_scratch(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  const TreePlan s = tree_plan(rows, nodes, heads, kv_heads, head_dim);
+  return static_cast<size_t>(s.records) * s.rec_floats * sizeof(float);
+}
+
+size_t tree_attention_scratch_most(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  size_t most = 0;
+  // (More rows than there are counters for are not cut and keep nothing; fewer are. A
+  // few nodes less may take narrower blocks.)
+  for (uint32_t n = 1; n <= nodes; ++n) {
+    const uint32_t parts = kv_heads * tree_plan(0, n, heads, kv_heads, head_dim).blocks;
+    most = std::max(most, tree_attention_scratch(std::min(rows, static_cast<uint32_t>(kOpCounters / parts)), n, heads, kv_heads, head_dim));
+  }
+  return most;
+}
+
+hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const qd_tree_attention_args &a, const OpScratch &w) {
+  if (c.rows == 0 || a.nodes == 0) return hipSuccess;
+  const TreePlan plan = tree_plan(c.rows, a.nodes, a.heads, c.kv_heads, c.head_dim);
+  TreeLaunch p{};
+  p.c = c;
+  p.a = a;
+  p.records = reinterpret_cast<float *>(w.scratch);
+  p.counters = w.counters;
+  p.apart = plan.apart;
+  p.group = plan.group;
+  p.columns = plan.columns;
+  p.blocks = plan.blocks;
+  p.rec_columns = plan.rec_columns;
+  p.rec_floats = plan.rec_floats;
+  p.page_shift = log2_of(c.page_size);
+  return with_type(c.dtype, c.head_dim, plan.block_columns, [&](auto shape, auto kernel) {
+    using S = decltype(shape);
+    const uint64_t most = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + kTreeLeast - 1) / kTreeLeast;
+    p.target = plan.target == 0 || most <= 1 ? 0 : std::max(1u, plan.target * S::kPerCu / 2);
+    uint64_t x = c.rows;
+    if (p.target) x = std::min<uint64_t>(x + p.target, x * most);
+    p.units = static_cast<uint32_t>(x * c.kv_heads);
+    const uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.blocks;
+    return launch(kernel, dim3(grid), dim3(S::kThreads), s, p);
+  });
+}
+
+// (As many shares of a node as kAcceptAim asks for: all of them are fewer than that and
+// one more of each node.)
+size_t tree_accept_scratch(uint32_t rows, uint32_t nodes) {
+  const size_t all = static_cast<size_t>(rows) * nodes;
+  return round256(std::min(all * kAcceptShares, all + kAcceptAim) * sizeof(AcceptShare)) + round256(all * sizeof(int32_t));
+}
+
+hipError_t launch_tree_accept(hipStream_t s, const qd_accept_args &a, const OpScratch &w) {
+  if (a.rows == 0 || a.nodes == 0) return hipSuccess;
+  AcceptLaunch p{};
+  p.a = a;
+  p.shares = accept_shares(a.rows, a.nodes, a.vocab);
+  const size_t all = static_cast<size_t>(a.rows) * a.nodes;
+  p.share = reinterpret_cast<AcceptShare *>(w.scratch);
+  p.picks = reinterpret_cast<int32_t *>(w.scratch + round256(std::min(all * kAcceptShares, all + kAcceptAim) * sizeof(AcceptShare)));
+  p.counters = w.counters;
+  if (a.draws) {
+    const double c = 1.4426950408889634074 / a.temperature;
+    p.c_hi = static_cast<float>(c);
+    p.c_lo = static_cast<float>(c - p.c_hi);
+  }
+  const dim3 grid(p.shares, static_cast<uint32_t>(all)), block(kAcceptT);
+  const auto run = [&](auto greedy, auto sampled) { return launch(a.draws ? sampled : greedy, grid, block, s, p); };
+  switch (a.dtype) {
+    case QD_DTYPE_F32: return run(accept_kernel<float, false>, accept_kernel<float, true>);
+    case QD_DTYPE_BF16: return run(accept_kernel<Brain, false>, accept_kernel<Brain, true>);
+    default: return run(accept_kernel<Half, false>, accept_kernel<Half, true>);
+  }
+}
+
+hipError_t launch_tree_commit(hipStream_t s, const qd_commit_args &a) {
+  if (a.rows == 0) return hipSuccess;
+  CommitLaunch p{};
+  p.a = a;
+  p.a.memories = nullptr;
+  uint64_t columns = 0;
+  for (uint32_t m = 0; m < a.memory_count; ++m) {
+    p.memory[m] = a.memories[m];
+    p.columns[m] = a.memories[m].piece_bytes / 16 * a.memories[m].pieces * a.memories[m].planes;
+    columns += p.columns[m];
+  }
+  p.page_shift = log2_of(a.page_size);
+  const uint32_t x = static_cast<uint32_t>(std::max<uint64_t>(1, (columns + kWave - 1) / kWave));
+  return launch(commit_kernel, dim3(x, a.rows), dim3(kCommitT), s, p);
+}
+
+}  // namespace qd

@@ -31,7 +31,7 @@ try:
 except ImportError as e:
     raise ImportError(f"the operators' binding is not built: make -C {os.path.dirname(os.path.abspath(__file__))}") from e
 
-BAD_LENGTH, BAD_PAGE, BAD_POSITION, BAD_ROW, EXHAUSTED = 1, 2, 4, 8, 16
+BAD_LENGTH, BAD_PAGE, BAD_POSITION, BAD_ROW, EXHAUSTED, BAD_PARENT, BAD_PATH = 1, 2, 4, 8, 16, 32, 64
 
 _P, _I64, _U32, _I32 = C.c_void_p, C.c_int64, C.c_uint32, C.c_int32
 
@@ -48,6 +48,11 @@ class MemoryStruct(C.Structure):
                 ("reserved", _U32)]
 
 
+class TokenStruct(C.Structure):
+    _fields_ = [("base", _P), ("plane_stride", _I64), ("page_stride", _I64), ("token_stride", _I64), ("piece_stride", _I64),
+                ("piece_bytes", _U32), ("pieces", _U32), ("planes", _U32), ("reserved", _U32)]
+
+
 _SIZE = C.POINTER(C.c_size_t)
 _SIGNATURES = {
     "qd_workspace_create": [_I32, C.c_size_t, C.POINTER(_P)],
@@ -61,6 +66,15 @@ _SIGNATURES = {
     "qd_pages_fork_workspace": [_U32, _U32, _SIZE],
     "qd_beam_select": [_P, _P, _P],
     "qd_beam_select_workspace": [_U32, _U32, _U32, _U32, _SIZE],
+    "qd_paged_append_at": [_P, _P, _P, _P],
+    "qd_tree_attention": [_P, _P, _P, _P],
+    "qd_tree_attention_workspace": [_U32, _U32, _U32, _U32, _U32, _SIZE],
+    "qd_tree_accept": [_P, _P, _P],
+    "qd_tree_accept_workspace": [_U32, _U32, _U32, _SIZE],
+    "qd_tree_commit": [_P, _P],
+    "qd_page_bounds": [_P, _P, _U32, _P],
+    "qd_sparse_attention": [_P, _P, _P, _P],
+    "qd_sparse_attention_workspace": [_U32, _U32, _U32, _U32, _U32, _U32, _SIZE],
 }
 
 _lib = None
@@ -76,7 +90,8 @@ def lib():
             fn.restype = C.c_int
             fn.argtypes = args
         _qd_tensors.bind(*(C.cast(getattr(handle, name), _P).value for name in (
-            "qd_paged_append", "qd_paged_attention", "qd_pages_fork", "qd_beam_select")))
+            "qd_paged_append_at", "qd_paged_attention", "qd_pages_fork", "qd_beam_select", "qd_tree_attention",
+            "qd_tree_accept", "qd_tree_commit", "qd_page_bounds", "qd_sparse_attention")))
         _lib = handle
     return _lib
 
@@ -144,6 +159,18 @@ def select_workspace(groups, beams, k, vocab):
     return _bytes("qd_beam_select_workspace", groups, beams, k, vocab)
 
 
+def tree_attention_workspace(rows, nodes, heads, kv_heads, head_dim):
+    return _bytes("qd_tree_attention_workspace", rows, nodes, heads, kv_heads, head_dim)
+
+
+def tree_accept_workspace(rows, nodes, vocab):
+    return _bytes("qd_tree_accept_workspace", rows, nodes, vocab)
+
+
+def sparse_attention_workspace(rows, heads, kv_heads, head_dim, table_width, budget):
+    return _bytes("qd_sparse_attention_workspace", rows, heads, kv_heads, head_dim, table_width, budget)
+
+
 class Workspace:
     """Device memory for partial results, for one call at a time: work that may run at the
     same time (two streams, graphs on two streams) needs one each."""
@@ -196,13 +223,13 @@ class PagedCache:
 
 
 def paged_append(cache, q_out, q, k, v, positions, rows=None, cos=None, sin=None, interleaved=False, position_bias=0,
-                 stream=0):
+                 stream=0, slots=None):
     """Rotates new tokens' queries into q_out and writes their keys (rotated) and values into
-    pages. q, q_out [tokens, heads, head_dim] (both None: keys and values only), k, v
-    [tokens, kv_heads, head_dim], positions and rows [tokens] int32, cos and sin
+    pages, at position slots[t] of the row (None: where it is rotated for, positions[t]). q, q_out [tokens, heads, head_dim] (both None: keys and values only), k, v
+    [tokens, kv_heads, head_dim], positions, rows and slots [tokens] int32, cos and sin
     [positions, rotary_dim / 2] FP32 (None: no rotation)."""
     r = _qd_tensors.append(cache.at, q_out, q, k, v, positions, rows, cos, sin, interleaved, position_bias, stream,
-                           cache.tensors)
+                           cache.tensors, slots)
     if r is not None:
         _answer(r)
 
@@ -255,6 +282,85 @@ def beam_select(logits, scores, scores_out, parents, tokens, workspace, done=Non
     """The best k = scores_out.shape[1] continuations of each group: logits [groups, beams, vocab],
     scores and done [groups, beams], the results [groups, k]."""
     r = _qd_tensors.select(logits, scores, scores_out, parents, tokens, workspace.handle, done, done_out, eos, stream)
+    if r is not None:
+        _answer(r)
+
+
+def tree_attention(cache, out, q, parents, workspace, scale=None, stream=0):
+    """Attention of a tree of drafted tokens in each cache row, whose keys and values are the row's last
+    positions: q and out [rows, nodes, heads, head_dim], parents [rows, nodes] int32 (an earlier node,
+    -1: none, -2: no such node); scale None: 1 / sqrt(head_dim)."""
+    r = _qd_tensors.tree_attention(cache.at, out, q, parents, workspace.handle, scale, stream, cache.tensors)
+    if r is not None:
+        _answer(r)
+
+
+def tree_accept(logits, tokens, parents, path, counts, next_tokens, workspace, draws=None, temperature=1.0, errors=None,
+                stream=0):
+    """Which nodes of each row's tree stand: logits [rows, nodes, vocab], tokens and parents [rows, nodes]
+    int32; the walk's nodes into path [rows, nodes], their number into counts and the token after them into
+    next_tokens [rows]. draws [rows, nodes] FP32 from 0 up to 1: tokens are drawn; None: the likeliest."""
+    r = _qd_tensors.tree_accept(logits, tokens, parents, path, counts, next_tokens, workspace.handle, draws, temperature, errors,
+                                stream)
+    if r is not None:
+        _answer(r)
+
+
+class TokenMemory:
+    """Tensors that hold something of each position: [planes, pages, page_size, heads, values] or, without
+    planes, [pages, page_size, heads, values], with any strides but a contiguous last dimension."""
+
+    def __init__(self, tensors, planes=True):
+        self.tensors = tuple(tensors)
+        if not self.tensors:
+            _refuse("a memory without tensors")
+        p = 1 if planes else 0
+        self.pages, self.page_size = _dims("a memory", self.tensors[0], 4 + p)[p:p + 2]
+        self.device = self.tensors[0].get_device()
+        self.memories = (TokenStruct * len(self.tensors))()
+        for m, t in zip(self.memories, self.tensors):
+            shape = _dims("a memory", t, 4 + p)
+            if tuple(shape[p:p + 2]) != (self.pages, self.page_size) or t.get_device() != self.device:
+                _refuse(f"a tensor of shape {tuple(shape)} on {t.device} does not hold {self.pages} pages of {self.page_size} "
+                        f"positions of device {self.device}")
+            if t.numel() == 0:
+                _refuse(f"a tensor of shape {tuple(shape)} holds nothing")
+            if t.stride(-1) != 1 and shape[-1] > 1:
+                _refuse(f"a tensor of strides {t.stride()} is not contiguous in its last dimension")
+            size = t.element_size()
+            m.base, m.piece_bytes, m.pieces = t.data_ptr(), shape[-1] * size, shape[-2]
+            m.planes, m.plane_stride = (shape[0], t.stride(0) * size) if planes and shape[0] > 1 else (1, 0)
+            # (The stride of a dimension of one element is not used and may be anything.)
+            m.page_stride = t.stride(p) * size if self.pages > 1 else 0
+            m.token_stride = t.stride(p + 1) * size if self.page_size > 1 else m.piece_bytes
+            m.piece_stride = t.stride(p + 2) * size if m.pieces > 1 else 0
+        self.at = C.addressof(self.memories)
+        lib()
+
+
+def tree_commit(memory, table, lengths, path, counts, lengths_out, errors=None, stream=0):
+    """Moves what the memory holds of the nodes path[r][: counts[r]] of each row's tree, its last path.shape[1]
+    positions, to the first of those, and writes the lengths that this leaves."""
+    r = _qd_tensors.tree_commit(memory.page_size, memory.pages, memory.device, memory.at, len(memory.tensors), table, lengths, path,
+                                counts, lengths_out, errors, stream, memory.tensors)
+    if r is not None:
+        _answer(r)
+
+
+def page_bounds(cache, bounds, recent, stream=0):
+    """The least and the largest value of each element of the keys in each page that holds one of a row's last
+    `recent` positions: bounds [pages, kv_heads, 2, head_dim]."""
+    r = _qd_tensors.page_bounds(cache.at, bounds, recent, stream, cache.tensors)
+    if r is not None:
+        _answer(r)
+
+
+def sparse_attention(cache, bounds, out, q, workspace, budget, first=1, last=1, chosen=None, scale=None, stream=0):
+    """paged_attention over up to `budget` pages of each row and KV head: the first and the last ones, and of the
+    others those whose bounds allow the largest products with the queries. chosen [rows, kv_heads, budget] int32
+    gets the columns of the table that were read."""
+    r = _qd_tensors.sparse_attention(cache.at, bounds, out, q, workspace.handle, budget, first, last, chosen, scale, stream,
+                                     cache.tensors)
     if r is not None:
         _answer(r)
 

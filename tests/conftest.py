@@ -13,7 +13,8 @@ for sub in ("oracle", "light-rocm-runtime_amd"):
 
 # The operators' binding is built for torch, and the converter's tests compare with its
 # conversions: without it these are left out.
-NEED_TORCH = ["test_operators.py", "test_gpu_operators.py", "test_converter.py", "test_gpu_converter.py"]
+NEED_TORCH = ["test_operators.py", "test_gpu_operators.py", "test_converter.py", "test_gpu_converter.py",
+              "test_drafts.py", "test_gpu_drafts.py", "test_gpu_sparse.py"]
 collect_ignore = [] if importlib.util.find_spec("torch") else NEED_TORCH
 
 
