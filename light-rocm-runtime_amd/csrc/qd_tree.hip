@@ -747,32 +747,35 @@ TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_he
 }
 
 // ---- accept ------------------------------------------------------------------------
-// A workgroup takes a share of one node's logits: its largest, or (draws) the sum of
-// exp(x / T) in 64 bits relative to a power of two. Greedy, the last share of a row to
-// arrive walks the tree; with draws the last share of a node finds the share in which the
-// running sum passes the draw, reads it again and picks the token, and the last node of a
-// row walks. Bound by memory for large batches, by the chain of hand-overs for small ones.
-constexpr int kAcceptT = 256;
+// A workgroup takes a share of one node's logits, a quarter of it each wave: the largest, or
+// (draws) each wave's sum of exp(x / T) in 64 bits, relative to a power of two. Greedy, the last
+// share of a row to arrive finds each node's largest and walks the tree; with draws the last
+// share of a node finds the quarter in which the running sum passes the draw, reads that one
+// again and picks the token, and the last node of a row walks. Bound by memory for large
+// batches, by the chain of hand-overs for small ones.
+constexpr int kAcceptT = 256, kAcceptWaves = kAcceptT / kWave;
 constexpr uint32_t kAcceptShares = 64;    // of a node at most: a lane each
-constexpr uint32_t kAcceptAim = 1024;     // shares in all
-constexpr uint32_t kAcceptLeast = 4096;   // logits of a share at least
+constexpr uint32_t kAcceptAim = 2048;     // shares in all
+constexpr uint32_t kAcceptLeast = 16384;  // logits of a share at least
 constexpr float kHuge = 1e30f;            // logits past it are not exponentiated
 
 struct AcceptShare {
-  double sum;    // of 2^(x c - r), or the largest logit and its token
-  float r;
-  uint32_t pad;
+  double sum[kAcceptWaves];  // of 2^(x c - r), r the whole number above the largest logit's x c
+  float top;                 // the largest logit
+  uint32_t id;               // greedy: its token
+  uint32_t pad[2];
 };
 struct AcceptLaunch {
   qd_accept_args a;
   AcceptShare *share;   // [rows * nodes][shares]
   int32_t *picks;       // [rows * nodes]
   uint32_t *counters;   // [rows * nodes] nodes, then [rows] rows
+  uint32_t apart;       // words between two counters
   uint32_t shares;
   float c_hi, c_lo;     // log2(e) / temperature
 };
 
-// Logits `at` .. of a row that may start anywhere: as FP32.
+// A row's logit i as FP32.
 template <typename E>
 __device__ __forceinline__ float logit(const void *row, uint32_t i) {
   if constexpr (std::is_same_v<E, float>) {
@@ -789,18 +792,69 @@ __device__ __forceinline__ float power(float x, float c_hi, float c_lo, float r)
   return exp2_fast((hi - r) + lo);
 }
 __device__ __forceinline__ double scaled(double s, float by) { return ldexp(s, static_cast<int>(fmaxf(by, -4000.f))); }
+// Sum over the lanes up to this one.
+__device__ __forceinline__ double lanes_upto(double v) {
+#pragma unroll
+  for (int step = 1; step < kWave; step <<= 1) {
+    const double x = lane_of(v, max(lane_id() - step, 0));
+    if (lane_id() >= step) v += x;
+  }
+  return v;
+}
+
+// One row's logits in 16-byte pieces, shares of them and quarters of shares. The row may start
+// anywhere: the first quarter has what lies before the first piece too, the last one what lies
+// behind the last.
+template <typename E>
+struct Logits {
+  static constexpr int kPer = std::is_same_v<E, float> ? 4 : 8;
+  const char *x;
+  uint32_t vocab, head, pieces, each;
+  __device__ __forceinline__ Logits(const char *at, uint32_t n, uint32_t quarters) : x(at), vocab(n) {
+    const uint32_t skew = static_cast<uint32_t>(-(reinterpret_cast<uintptr_t>(x) / (16 / kPer))) % kPer;
+    head = min(skew, vocab);
+    pieces = (vocab - head) / kPer;
+    each = (pieces + quarters - 1) / quarters;
+  }
+  __device__ __forceinline__ uint32_t first(uint32_t quarter) const { return min(pieces, quarter * each); }
+  __device__ __forceinline__ uint32_t token(uint32_t piece) const { return head + piece * kPer; }
+  __device__ __forceinline__ u4v load(uint32_t piece) const { return reinterpret_cast<const u4v *>(x + head * (16 / kPer))[piece]; }
+  static __device__ __forceinline__ void values(const u4v &v, float (&y)[kPer]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t word = v[i];
+      if constexpr (std::is_same_v<E, float>) {
+        y[i] = __uint_as_float(word);
+      } else {
+        y[2 * i] = E::lo(word);
+        y[2 * i + 1] = E::hi(word);
+      }
+    }
+  }
+};
 
 template <typename E, bool kSampled>
 __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
-  constexpr int kW = kAcceptT / kWave, kPer = std::is_same_v<E, float> ? 4 : 8, kAhead = 4;
-  __shared__ double sums[kAcceptT];
-  __shared__ float tops[kW];
-  __shared__ uint32_t ids[kW], last;
-  __shared__ int32_t picked;
+  using Row = Logits<E>;
+  constexpr int kPer = Row::kPer, kAhead = 4;
+  __shared__ double sums[kAcceptWaves];
+  __shared__ float tops[kAcceptWaves];
+  __shared__ uint32_t ids[kAcceptWaves], last;
+  __shared__ int32_t picks[64];
   const uint32_t node = blockIdx.y % p.a.nodes, row = blockIdx.y / p.a.nodes, share = blockIdx.x;
-  const int lane = lane_id(), w = wave_id();
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
   const size_t at = static_cast<size_t>(row) * p.a.nodes;
   const int32_t parent = static_cast<uint32_t>(lane) < p.a.nodes ? p.a.parents[at + lane] : -2;
+  const Row x(static_cast<const char *>(p.a.logits) + (row * p.a.row_stride + node * p.a.node_stride) * static_cast<int64_t>(16 / kPer),
+              p.a.vocab, p.shares * kAcceptWaves);
+  const uint32_t quarter = share * kAcceptWaves + w, from = x.first(quarter), to = x.first(quarter + 1);
+  // (On their way before the tree is looked at.)
+  u4v v[kAhead];
+  const auto fetch = [&](uint32_t j) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) v[u] = x.load(min(j + u * kWave, to - 1));
+  };
+  if (from < to) fetch(from + lane);
   const uint64_t there = __ballot(parent >= -1);
   const bool bad = __any(parent >= lane || (parent >= 0 && !(there >> parent & 1)));
   if (bad || !(there & 1)) {
@@ -816,22 +870,13 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
   }
   if (!(there >> node & 1)) return;
   const uint32_t present = __popcll(there);
-  const char *x = static_cast<const char *>(p.a.logits) + (row * p.a.row_stride + node * p.a.node_stride) * static_cast<int64_t>(16 / kPer);
-  // The row's 16-byte pieces, and what lies before the first of them.
-  const uint32_t skew = static_cast<uint32_t>(-(reinterpret_cast<uintptr_t>(x) / (16 / kPer))) % kPer;
-  const uint32_t head = min(skew, p.a.vocab), pieces = (p.a.vocab - head) / kPer;
-  // Piece j of share s: [s * each, (s + 1) * each); the first has the head, the last the tail too.
-  const uint32_t each = (pieces + p.shares - 1) / p.shares;
-  const auto begin_of = [&](uint32_t s) { return s == 0 ? 0u : min(pieces, s * each) * kPer + head; };
-  const auto end_of = [&](uint32_t s) { return s + 1 == p.shares ? p.a.vocab : min(pieces, (s + 1) * each) * kPer + head; };
-  const uint32_t from = min(pieces, share * each), to = min(pieces, (share + 1) * each);
   float top = -INFINITY;
   uint32_t best = UINT32_MAX;
   double sum = 0.0;
   float r = -INFINITY;  // (a whole number)
-  const auto take = [&](float v, uint32_t i) {
-    if (v > top) {
-      top = v;
+  const auto take = [&](float y, uint32_t i) {
+    if (y > top) {
+      top = y;
       best = i;
     }
   };
@@ -846,107 +891,97 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       }
     }
   };
-  const auto values = [&](const u4v &v, float (&y)[kPer]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t word = v[i];
-      if constexpr (std::is_same_v<E, float>) {
-        y[i] = __uint_as_float(word);
-      } else {
-        y[2 * i] = E::lo(word);
-        y[2 * i + 1] = E::hi(word);
-      }
-    }
-  };
   const auto single = [&](uint32_t i) {
-    const float v = logit<E>(x, i);
+    const float y = logit<E>(x.x, i);
     if constexpr (kSampled) {
-      raise(fmaxf(v, -kHuge));
-      sum += power(v, p.c_hi, p.c_lo, r);
+      raise(fmaxf(y, -kHuge));
+      sum += power(y, p.c_hi, p.c_lo, r);
     } else {
-      take(v, i);
+      take(y, i);
     }
   };
-  if (share == 0 && threadIdx.x < head) single(threadIdx.x);
-  const u4v *body = reinterpret_cast<const u4v *>(x + head * (16 / kPer));
-  for (uint32_t j = from + threadIdx.x; j < to; j += kAhead * kAcceptT) {
-    u4v v[kAhead];
+  if (quarter == 0 && static_cast<uint32_t>(lane) < x.head) single(lane);
+  for (uint32_t j = from + lane; j < to; j += kAhead * kWave) {
+    u4v now[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) v[u] = body[min(j + u * kAcceptT, to - 1)];
+    for (int u = 0; u < kAhead; ++u) now[u] = v[u];
+    if (j + kAhead * kWave < to) fetch(j + kAhead * kWave);
+    if constexpr (kSampled) {
+      float most = -kHuge;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const uint32_t k = j + u * kAcceptT;
-      if (k >= to) break;
-      float y[kPer];
-      values(v[u], y);
-      if constexpr (kSampled) {
-        float most = -kHuge;
+      for (int u = 0; u < kAhead; ++u) {
+        float y[kPer];
+        Row::values(now[u], y);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) most = fmaxf(most, y[i]);
-        raise(most);
+        for (int i = 0; i < kPer; ++i) most = fmaxf(most, y[i]);  // (a piece past the end is the last one again)
+      }
+      raise(most);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += power(y[i], p.c_hi, p.c_lo, r);
-      } else {
+      for (int u = 0; u < kAhead; ++u) {
+        if (j + u * kWave >= to) break;
+        float y[kPer], s = 0.f;
+        Row::values(now[u], y);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) take(y[i], head + k * kPer + i);
+        for (int i = 0; i < kPer; ++i) s += power(y[i], p.c_hi, p.c_lo, r);
+        sum += s;
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const uint32_t k = j + u * kWave;
+        if (k >= to) break;
+        float y[kPer];
+        Row::values(now[u], y);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) take(y[i], x.token(k) + i);
       }
     }
   }
-  if (share + 1 == p.shares && head + pieces * kPer + threadIdx.x < p.a.vocab) single(head + pieces * kPer + threadIdx.x);
+  if (quarter + 1 == p.shares * kAcceptWaves && x.token(x.pieces) + lane < p.a.vocab) single(x.token(x.pieces) + lane);
   // The workgroup's share.
-  AcceptShare mine{0.0, 0.f, 0u};
+  constexpr uint32_t kWords = sizeof(AcceptShare) / 4;
+  const Coherent shares(p.share + at * p.shares, static_cast<uint32_t>(p.a.nodes * p.shares * sizeof(AcceptShare)));
+  const auto word = [&](uint32_t n, uint32_t s) { return (n * p.shares + s) * kWords; };
+  const uint32_t mine = word(node, share);
   if constexpr (kSampled) {
     const float wave_top = wave_max(top);
     if (lane == 0) tops[w] = wave_top;
     __syncthreads();
     float all = tops[0];
 #pragma unroll
-    for (int u = 1; u < kW; ++u) all = fmaxf(all, tops[u]);
-    mine.r = all;  // the largest logit; sums relative to the whole number above it
-    const float up = ceilf(fminf(all, kHuge) * p.c_hi);
-    double s = r == -INFINITY ? 0.0 : scaled(sum, r - up);
+    for (int u = 1; u < kAcceptWaves; ++u) all = fmaxf(all, tops[u]);
+    double s = r == -INFINITY ? 0.0 : scaled(sum, r - ceilf(fminf(all, kHuge) * p.c_hi));
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1) s += lane_of(s, lane ^ step);
-    if (lane == 0) sums[w] = s;
-    __syncthreads();
-    mine.sum = sums[0];
-#pragma unroll
-    for (int u = 1; u < kW; ++u) mine.sum += sums[u];
-  } else {
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) {
-      const float v = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane ^ step) << 2, __builtin_bit_cast(int, top)));
-      const uint32_t i = __builtin_amdgcn_ds_bpermute((lane ^ step) << 2, static_cast<int>(best));
-      if (better(v, i, top, best)) {
-        top = v;
-        best = i;
-      }
-    }
     if (lane == 0) {
-      tops[w] = top;
+      const uint64_t bits = __builtin_bit_cast(uint64_t, s);
+      shares.stu(mine + 2 * w, static_cast<uint32_t>(bits));
+      shares.stu(mine + 2 * w + 1, static_cast<uint32_t>(bits >> 32));
+      if (w == 0) shares.st(mine + 2 * kAcceptWaves, all);
+    }
+  } else {
+    const float wave_top = wave_max(top);
+    // The lowest token of those that reach it.
+    best = top == wave_top ? best : UINT32_MAX;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) best = min(best, static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute((lane ^ step) << 2, static_cast<int>(best))));
+    if (lane == 0) {
+      tops[w] = wave_top;
       ids[w] = best;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int u = 1; u < kW; ++u)
-        if (better(tops[u], ids[u], top, best)) {
-          top = tops[u];
+      float all = tops[0];
+      best = ids[0];
+#pragma unroll
+      for (int u = 1; u < kAcceptWaves; ++u)
+        if (better(tops[u], ids[u], all, best)) {
+          all = tops[u];
           best = ids[u];
         }
-      mine.r = top;
-      mine.pad = best;
+      shares.st(mine + 2 * kAcceptWaves, all);
+      shares.stu(mine + 2 * kAcceptWaves + 1, best);
     }
-  }
-  const size_t shares_of_node = (at + node) * p.shares;
-  const Coherent shares(p.share + at * p.shares, static_cast<uint32_t>(p.a.nodes * p.shares * sizeof(AcceptShare)));
-  const auto word = [&](uint32_t n, uint32_t s) { return (n * p.shares + s) * 4; };
-  (void)shares_of_node;
-  if (threadIdx.x == 0) {
-    const uint64_t bits = __builtin_bit_cast(uint64_t, mine.sum);
-    shares.stu(word(node, share), static_cast<uint32_t>(bits));
-    shares.stu(word(node, share) + 1, static_cast<uint32_t>(bits >> 32));
-    shares.st(word(node, share) + 2, mine.r);
-    shares.stu(word(node, share) + 3, mine.pad);
   }
   const auto arrive = [&](uint32_t *counter, uint32_t of) {
     wait_vm_stores();
@@ -958,100 +993,141 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(last) != 0;
   };
-  uint32_t *row_counter = p.counters + static_cast<size_t>(p.a.rows) * p.a.nodes + row;
-  int32_t pick = 0;  // lane n's: node n's
+  uint32_t *row_counter = p.counters + (static_cast<size_t>(p.a.rows) * p.a.nodes + row) * p.apart;
   if constexpr (!kSampled) {
     if (!arrive(row_counter, present * p.shares)) return;
-    if (w != 0) return;
-    float v = -INFINITY;
-    uint32_t id = UINT32_MAX;
-    if (there >> lane & 1)
-      for (uint32_t s = 0; s < p.shares; ++s) {
-        const float y = shares.ld(word(lane, s) + 2);
-        const uint32_t i = shares.ldu(word(lane, s) + 3);
-        if (better(y, i, v, id)) {
-          v = y;
-          id = i;
+    // A group of lanes takes a node, a lane a share.
+    const uint32_t lanes = p.shares <= 1 ? 1u : 1u << (32 - __builtin_clz(p.shares - 1));
+    for (uint32_t n = threadIdx.x / lanes; n < (p.a.nodes + kAcceptT / lanes - 1) / (kAcceptT / lanes) * (kAcceptT / lanes); n += kAcceptT / lanes) {
+      const uint32_t s = threadIdx.x % lanes;
+      float y = -INFINITY;
+      uint32_t i = UINT32_MAX;
+      if (n < p.a.nodes && there >> n & 1 && s < p.shares) {
+        y = shares.ld(word(n, s) + 2 * kAcceptWaves);
+        i = shares.ldu(word(n, s) + 2 * kAcceptWaves + 1);
+      }
+      for (uint32_t step = lanes / 2; step > 0; step >>= 1) {
+        const float z = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane ^ step) << 2, __builtin_bit_cast(int, y)));
+        const uint32_t k = __builtin_amdgcn_ds_bpermute((lane ^ step) << 2, static_cast<int>(i));
+        if (better(z, k, y, i)) {
+          y = z;
+          i = k;
         }
       }
-    pick = id == UINT32_MAX ? 0 : static_cast<int32_t>(id);  // (nothing above -inf)
+      if (s == 0 && n < p.a.nodes) picks[n] = i == UINT32_MAX ? 0 : static_cast<int32_t>(i);  // (nothing above -inf)
+    }
+    __syncthreads();
+    if (w != 0) return;
   } else {
-    if (!arrive(p.counters + at + node, p.shares)) return;
+    if (!arrive(p.counters + (at + node) * p.apart, p.shares)) return;
     // Every wave: all shares, a lane each.
     float most = -INFINITY;
-    double s = 0.0;
+    double part[kAcceptWaves] = {}, s = 0.0;
     if (static_cast<uint32_t>(lane) < p.shares) {
-      most = shares.ld(word(node, lane) + 2);
-      const uint64_t lo = shares.ldu(word(node, lane)), hi = shares.ldu(word(node, lane) + 1);
-      s = __builtin_bit_cast(double, hi << 32 | lo);
+      most = shares.ld(word(node, lane) + 2 * kAcceptWaves);
+#pragma unroll
+      for (int u = 0; u < kAcceptWaves; ++u) {
+        const uint64_t lo = shares.ldu(word(node, lane) + 2 * u), hi = shares.ldu(word(node, lane) + 2 * u + 1);
+        part[u] = __builtin_bit_cast(double, hi << 32 | lo);
+      }
     }
     const float all = wave_max(most);
-    if (threadIdx.x == 0) picked = -1;
-    __syncthreads();
     if (!(all > -kHuge && all < kHuge)) {
       // The largest logit, read again by the whole workgroup.
       top = -INFINITY;
       best = UINT32_MAX;
-      for (uint32_t i = threadIdx.x; i < p.a.vocab; i += kAcceptT) take(logit<E>(x, i), i);
+      for (uint32_t i = threadIdx.x; i < p.a.vocab; i += kAcceptT) take(logit<E>(x.x, i), i);
       const float wave_top = wave_max(top);
+      __syncthreads();
       if (lane == 0) tops[w] = wave_top;
       if (threadIdx.x == 0) ids[0] = UINT32_MAX;
       __syncthreads();
       const float m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       if (top == m && best != UINT32_MAX) atomicMin(&ids[0], best);
       __syncthreads();
-      if (threadIdx.x == 0) picked = ids[0] == UINT32_MAX ? 0 : static_cast<int32_t>(ids[0]);
+      if (threadIdx.x == 0) picks[0] = ids[0] == UINT32_MAX ? 0 : static_cast<int32_t>(ids[0]);
     } else {
-      const float up = ceilf(all * p.c_hi);
-      s = scaled(s, ceilf(fminf(most, kHuge) * p.c_hi) - up);
-      double upto = s;
+      const float up = ceilf(all * p.c_hi), by = ceilf(fminf(most, kHuge) * p.c_hi) - up;
 #pragma unroll
-      for (int step = 1; step < kWave; step <<= 1) {
-        const double v = lane_of(upto, max(lane - step, 0));
-        if (lane >= step) upto += v;
+      for (int u = 0; u < kAcceptWaves; ++u) {
+        part[u] = scaled(part[u], by);
+        s += part[u];
       }
-      const double total = lane_of(upto, kWave - 1), aim = static_cast<double>(p.a.draws[at + node]) * total;
+      const double upto = lanes_upto(s), aim = static_cast<double>(p.a.draws[at + node]) * lane_of(upto, kWave - 1);
       const uint64_t past = __ballot(upto > aim), some = __ballot(s > 0.0);
       // (A draw of 1 or more passes nothing: the last share with a token.)
-      const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<unsigned long long>(some));
-      const double before = lane_of(upto - s, in);
-      const uint32_t begin = begin_of(in), end = end_of(in), n = (end - begin + kAcceptT - 1) / kAcceptT;
-      const uint32_t a = min(end, begin + threadIdx.x * n), b = min(end, a + n);
+      const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(some));
+      // Its quarter: the first that passes, or the last with a token.
+      double before = lane_of(upto - s, in);
+      int which = -1;
+      double begins = before;
+#pragma unroll
+      for (int u = 0; u < kAcceptWaves; ++u) {
+        const double y = lane_of(part[u], in);
+        if (y > 0.0 && (which < 0 || !(begins + lane_of(part[max(which, 0)], in) > aim))) {
+          which = u;
+          begins = before;
+        }
+        before += y;
+      }
+      const uint32_t q = in * kAcceptWaves + which, a0 = x.first(q), b0 = x.first(q + 1);
+      // Its logits again, a run of pieces each thread; what lies before and behind the pieces with the first and last thread.
+      const uint32_t n = (b0 - a0 + kAcceptT - 1) / kAcceptT, a = min(b0, a0 + threadIdx.x * n), b = min(b0, a + n);
+      const uint32_t begin = q == 0 && threadIdx.x == 0 ? 0 : x.token(a);
+      const uint32_t end = q + 1 == p.shares * kAcceptWaves && threadIdx.x == kAcceptT - 1 ? p.a.vocab : x.token(b);
+      const auto each = [&](auto f) {  // f(token, probability), until it says so
+        for (uint32_t i = begin; i < x.token(a) && i < end; ++i)
+          if (f(i, power(logit<E>(x.x, i), p.c_hi, p.c_lo, up))) return;
+        for (uint32_t k = a; k < b; ++k) {
+          float y[kPer];
+          Row::values(x.load(k), y);
+#pragma unroll
+          for (int i = 0; i < kPer; ++i)
+            if (f(x.token(k) + i, power(y[i], p.c_hi, p.c_lo, up))) return;
+        }
+        for (uint32_t i = x.token(b); i < end; ++i)
+          if (f(i, power(logit<E>(x.x, i), p.c_hi, p.c_lo, up))) return;
+      };
       double run = 0.0;
-      for (uint32_t i = a; i < b; ++i) run += power(logit<E>(x, i), p.c_hi, p.c_lo, up);
-      sums[threadIdx.x] = run;
+      each([&](uint32_t, float y) {
+        run += y;
+        return false;
+      });
+      const double wave_upto = lanes_upto(run);
       __syncthreads();
+      if (lane == kWave - 1) sums[w] = wave_upto;
+      __syncthreads();
+      double mine_before = begins + (wave_upto - run);
+      for (int u = 0; u < w; ++u) mine_before += sums[u];
       // The first thread whose run passes the draw, or the last with a token.
-      double mine_before = before;
-      for (int u = 0; u < static_cast<int>(threadIdx.x); ++u) mine_before += sums[u];
       const uint64_t passes = __ballot(run > 0.0 && mine_before + run > aim), any = __ballot(run > 0.0);
       if (lane == 0) {
         ids[w] = passes ? w * kWave + __ffsll(static_cast<unsigned long long>(passes)) - 1 : UINT32_MAX;
-        tops[w] = any ? static_cast<float>(w * kWave + 63 - __clzll(static_cast<unsigned long long>(any))) : -1.f;
+        tops[w] = any ? static_cast<float>(w * kWave + 63 - __clzll(static_cast<long long>(any))) : -1.f;
       }
       __syncthreads();
       uint32_t who = min(min(ids[0], ids[1]), min(ids[2], ids[3]));
       if (who == UINT32_MAX) who = static_cast<uint32_t>(fmaxf(0.f, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))));
       if (threadIdx.x == who) {
-        uint32_t found = a;
-        for (uint32_t i = a; i < b; ++i) {
-          const float y = power(logit<E>(x, i), p.c_hi, p.c_lo, up);
+        uint32_t found = begin;
+        each([&](uint32_t i, float y) {
           if (y > 0.f) found = i;
           mine_before += y;
-          if (y > 0.f && mine_before > aim) break;
-        }
-        picked = static_cast<int32_t>(found);
+          return y > 0.f && mine_before > aim;
+        });
+        picks[0] = static_cast<int32_t>(found);
       }
     }
     __syncthreads();
-    const Coherent picks(p.picks + at, static_cast<uint32_t>(p.a.nodes * sizeof(int32_t)));
-    if (threadIdx.x == 0) picks.stu(node, static_cast<uint32_t>(picked));
+    const Coherent out(p.picks + at, static_cast<uint32_t>(p.a.nodes * sizeof(int32_t)));
+    if (threadIdx.x == 0) out.stu(node, static_cast<uint32_t>(picks[0]));
     if (!arrive(row_counter, present)) return;
     if (w != 0) return;
-    if (there >> lane & 1) pick = static_cast<int32_t>(picks.ldu(lane));
+    if (there >> lane & 1) picks[lane] = static_cast<int32_t>(out.ldu(lane));
   }
   // The walk: lane n is node n.
   const int32_t token = static_cast<uint32_t>(lane) < p.a.nodes ? p.a.tokens[at + lane] : -1;
+  const int32_t pick = there >> lane & 1 ? picks[lane] : -1;
   const int32_t wanted = __builtin_amdgcn_ds_bpermute(max(parent, 0) << 2, pick);
   const bool fits = parent >= 0 && token == wanted;
   int32_t here = 0, path = -1;
@@ -1222,6 +1298,7 @@ hipError_t launch_tree_accept(hipStream_t s, const qd_accept_args &a, const OpSc
   p.share = reinterpret_cast<AcceptShare *>(w.scratch);
   p.picks = reinterpret_cast<int32_t *>(w.scratch + round256(std::min(all * kAcceptShares, all + kAcceptAim) * sizeof(AcceptShare)));
   p.counters = w.counters;
+  for (p.apart = 32; (all + a.rows) * p.apart > kOpCounters;) p.apart /= 2;
   if (a.draws) {
     const double c = 1.4426950408889634074 / a.temperature;
     p.c_hi = static_cast<float>(c);
