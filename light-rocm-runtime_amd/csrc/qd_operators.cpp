@@ -431,11 +431,11 @@ qd_status qd_tree_attention(const qd_paged_cache *c, const qd_tree_attention_arg
     if (!a->parents) return invalid("null parents");
   }
   // A grid has fewer than 2^32 threads, 512 of a workgroup; a block has 16 columns or more.
-  const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((static_cast<uint64_t>(a->heads / c->kv_heads) * a->nodes + 127) / 128);
+  const uint64_t parts = static_cast<uint64_t>(c->kv_heads) * ((static_cast<uint64_t>(a->heads / c->kv_heads) * a->nodes + 63) / 64);
   if (c->rows * parts > 0x3f0000u)
     return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows of %u nodes and %u heads are too much for one call", c->rows, a->nodes, a->heads);
   qd::OpScratch scratch{};
-  QD_TRY(check_workspace(w, c->device, qd::tree_attention_scratch(c->rows, a->nodes, a->heads, c->kv_heads, c->head_dim), &scratch));
+  QD_TRY(check_workspace(w, c->device, qd::tree_attention_scratch(c->dtype, c->rows, a->nodes, a->heads, c->kv_heads, c->head_dim), &scratch));
   Device on;
   QD_TRY(on.enter(c->device));
   return launched(qd::launch_tree_attention(static_cast<hipStream_t>(stream), *c, *a, scratch), "tree attention launch");

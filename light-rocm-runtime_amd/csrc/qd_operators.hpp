@@ -47,7 +47,7 @@ size_t beam_select_scratch(uint32_t groups, uint32_t beams, uint32_t k, uint32_t
 size_t beam_select_scratch_most(uint32_t groups, uint32_t beams, uint32_t k, uint32_t vocab);
 hipError_t launch_beam_select(hipStream_t s, const qd_select_args &a, const OpScratch &w);
 
-size_t tree_attention_scratch(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
+size_t tree_attention_scratch(uint32_t dtype, uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 size_t tree_attention_scratch_most(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim);
 hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const qd_tree_attention_args &a, const OpScratch &w);
 

@@ -51,39 +51,44 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t *parents, uint32_t n
 // row's positions, in stages of 32 WP: K and V of a stage go to LDS without passing
 // registers, the next stages' on their way, and are read from there by WC x WP waves,
 // each for 16 NB columns and 32 positions of the stage:
-//   S^T = K Q^T   lane l: column l % 16, positions 4 (l / 16) + r of each half
+//   S^T = K Q^T    lane l: column l % 16, positions 4 (l / 16) + r of each 16
 //   O^T += V^T P^T with the lane's own probabilities as the operand; V is read in the
-//                 operand's layout, 16-bit types by transposing reads.
+//                  operand's layout, 16-bit types by transposing reads.
 // Positions before the tree are seen by every node; in the tree a bit of the node's
 // mask says so. What does not is hidden from the sum by its score, and by zeros in V's
 // place where V is not finite: the outputs that do see such a value become NaN.
 // Few rows are cut into runs that fill the card, which the last one joins in order.
 constexpr int kStep = 32;                // positions of a wave's step
 constexpr uint32_t kTreePieces = 64;     // of an item at most
-constexpr uint32_t kTreeLeast = 256;     // positions of a piece at least
+constexpr uint32_t kTreeLeast = 128;     // positions of a piece at least
 constexpr uint32_t kTreeCus = 256, kXcds = 8;
 constexpr uint32_t kLds = 160 * 1024;
-// As in the attention of one token (qd_paged.hip): a maximum is taken up once it passes
-// the one in use by so many powers of two, and FP16's scaled weights.
+// A maximum is taken up once it passes the one in use by so many powers of two, as in the
+// attention of one token (qd_paged.hip).
 template <typename E>
 constexpr float kLazy = 8.f;
 template <>
 constexpr float kLazy<Half> = 1.f;
-constexpr float kTreeWeight = 0x1p14f, kTreeRest = 0x1p12f;
+// FP16 takes 2^14 times a probability (at most 2 before it is rounded), and what rounding
+// that left: off by 2^-22 of it, or, at the end of FP16's range, 2^-39 of the largest. Sums
+// have the same factor, which the division takes out.
+template <typename E>
+constexpr float kUnit = 0.f;
+template <>
+constexpr float kUnit<Half> = 14.f;
 
 struct TreeLaunch {
   qd_paged_cache c;
   qd_tree_attention_args a;
-  float *records;      // [pieces][kv_heads * blocks][rec_floats]: acc [rec_columns][head_dim], maxima, sums
+  float *records;      // [pieces][kv_heads * blocks][columns of a block * (head_dim + 2)]
   uint32_t *counters;  // [rows][kv_heads * blocks]
   uint32_t apart;      // words between two counters
   uint32_t group;      // query heads of a KV head
   uint32_t columns;    // nodes * group
   uint32_t blocks;     // of columns
-  uint32_t rec_columns, rec_floats;
   uint32_t page_shift;
-  uint32_t target;     // pieces aimed at besides one of each row; 0: rows are not cut
-  uint32_t units;      // pieces x KV heads in the grid
+  uint32_t target;     // pieces of one KV head and block that the card holds at once; 0: rows are not cut
+  uint32_t units;      // pieces in the grid, of all rows and one KV head
 };
 
 // One 16-byte global -> LDS DMA per lane (lane l's bytes land at lds + 16 l), from
@@ -93,10 +98,20 @@ struct TreeLaunch {
 __device__ __forceinline__ void dma_to_lds(const void *src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
+__device__ __forceinline__ void dma_to_lds(const void *base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
 #pragma clang diagnostic pop
+// Waits until at most kEach x `left` of this wave's transfers are on their way.
 template <int kLeft>
 __device__ __forceinline__ void dma_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLeft) : "memory");
+}
+template <int kEach, int kMost>
+__device__ __forceinline__ void dma_wait(uint32_t left) {
+  if constexpr (kMost > 0)
+    if (left < kMost) return dma_wait<kEach, kMost - 1>(left);
+  dma_wait<kEach * kMost>();
 }
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
@@ -119,18 +134,25 @@ struct TreeShape {
   static constexpr bool kWide = std::is_same_v<E, float>;
   static constexpr int kElem = kWide ? 4 : 2;
   static constexpr int kWaves = WC * WP, kThreads = kWaves * kWave;
-  static constexpr int kRowBytes = D * kElem, kPositions = kStep * WP;
-  static constexpr int kHalf = kPositions * kRowBytes;  // K or V of a stage
-  static constexpr int kStages = 2;
+  static constexpr int kStage = kStep * WP;
+  static constexpr int kRowBytes = D * kElem;
+  static constexpr int kHalf = kStage * kRowBytes;  // K or V of a stage
+  // So many of them in LDS. Where memory is what bounds a stage they are waited for one by one
+  // and all but one are on their way, 128 KB to a CU with two workgroups (96: 64 rows of 0 to
+  // 8,192 with 8 nodes 260 us); where products do, by stages, three of them on their way.
+  static constexpr bool kByHalves = WP == 1;
+  static constexpr int kHalves = !kByHalves ? 8 : kRowBytes == 512 ? 4 : 9;
   static constexpr int kColumns = 16 * NB * WC;
   static constexpr int kRowsPerDma = 1024 / kRowBytes, kLanesPerRow = kRowBytes / 16;
-  static constexpr int kDmas = kPositions / kRowsPerDma / kWaves;  // of K, and of V, per wave and stage
+  static constexpr int kRows = kStage / kWaves;                // of a half, that a wave transfers
+  static constexpr int kDmas = kRows / kRowsPerDma;
+  static constexpr int kIds = (kRows + 15) / 16;               // groups of 16 of them
   static constexpr int kAcc = D / 16;
-  static constexpr int kMerge = (WP - 1) * WC * (NB * kAcc * 1024 + NB * 512);
-  static constexpr int kJoin = kColumns * (static_cast<int>(kTreePieces) + 1) * 4;
-  static constexpr int kBytes = std::max(kStages * 2 * kHalf, std::max(kMerge, kJoin));
-  static constexpr int kPerCu = 2 * (kBytes + 2048) <= static_cast<int>(kLds) ? 2 : 1;
-  static_assert(kDmas >= 1 && kDmas * kRowsPerDma * kWaves == kPositions, "whole transfers");
+  static constexpr int kMerge = WP > 1 ? WC * NB * (kAcc * 1024 + 512) : 0;
+  static constexpr int kBytes = std::max(kHalves * kHalf, kMerge);
+  static constexpr int kPerCu = std::min(8 / kWaves < 1 ? 1 : 8 / kWaves, static_cast<int>(kLds) / (kBytes + 2048));
+  static_assert(WP <= 2 && kDmas >= 1 && kDmas * kRowsPerDma * kWaves == kStage, "whole transfers");
+  static_assert((kHalves - 2) * kDmas < 64, "the wait's count");
   static_assert(kBytes + 2048 <= static_cast<int>(kLds), "LDS");
 };
 
@@ -155,20 +177,20 @@ struct TreeAttention {
   using S = TreeShape<E, D, NB, WC, WP>;
   using Shared = TreeShared<S>;
   static constexpr bool kWide = S::kWide;
-  static constexpr bool kScaled = std::is_same_v<E, Half>;
+  static constexpr int kStage = S::kStage, kRows = S::kRows;
   static constexpr int kQ = D * S::kElem / 64;  // 16-byte pieces of a query per lane
 
   const TreeLaunch &p;
   Shared &sh;
   const Piece &it;
   const int w, lane, col, quad, wc, wp;
-  const float scale;
+  const float scale;  // of the sizes of scores, in powers of two: the queries have its sign
   const uint32_t token_bytes;
   u4v q[NB][kQ];
   f4v o[NB][S::kAcc];
   float m[NB], ms[NB], l[NB];
-  int32_t ids[S::kDmas];  // the pages of the stage that is loaded next
   uint32_t errors = 0;
+  uint32_t lane_off[S::kDmas / S::kIds];  // of a lane's bytes in a group of 16 rows
 
   __device__ __forceinline__ TreeAttention(const TreeLaunch &launch, Shared &shared, const Piece &piece)
       : p(launch),
@@ -180,41 +202,68 @@ struct TreeAttention {
         quad(lane >> 4),
         wc(w % WC),
         wp(w / WC),
-        scale(p.a.scale * 1.44269504088896340736f),
-        token_bytes(static_cast<uint32_t>(p.c.token_stride) * S::kElem) {}
-
-  // This wave's n-th transfer of a stage begins at this row of it.
-  __device__ __forceinline__ uint32_t dma_row(int n) const { return (n * S::kWaves + w) * S::kRowsPerDma; }
-  __device__ __forceinline__ void pages_of(uint32_t stage) {
-    if (stage >= it.last) return;
+        scale(fabsf(p.a.scale) * 1.44269504088896340736f),
+        token_bytes(static_cast<uint32_t>(p.c.token_stride) * S::kElem) {
 #pragma unroll
-    for (int n = 0; n < S::kDmas; ++n) {
-      const uint32_t pos = min(stage * S::kPositions + dma_row(n), static_cast<uint32_t>(it.length - 1));
-      ids[n] = load_uniform(p.c.table + it.row * p.c.table_stride + (pos >> p.page_shift));
+    for (int n = 0; n < S::kDmas / S::kIds; ++n) {
+      const uint32_t row = n * S::kRowsPerDma + lane / S::kLanesPerRow;
+      lane_off[n] = row * token_bytes + 16 * ((lane % S::kLanesPerRow) ^ swizzle<S::kRowBytes, kWide>(w * kRows + row));
     }
   }
-  // Positions past the length read the last one: nothing behind it is touched.
-  __device__ __forceinline__ void load(uint32_t stage) {
-    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)sh.stage)) +
-                         (stage - it.first) % S::kStages * (2 * S::kHalf);
-    const int64_t head = static_cast<int64_t>(it.kv) * p.c.head_stride;
+
+  // A wave transfers rows of its own of each half.
+  struct Ids {
+    int32_t id[S::kIds];
+  };
+  // Their pages. (Past the length: the last position's.)
+  __device__ __forceinline__ Ids pages_of(uint32_t stage) const {
+    Ids x{};
+    if (stage >= it.last) return x;
 #pragma unroll
-    for (int n = 0; n < S::kDmas; ++n) {
-      const uint32_t row = dma_row(n), mine = row + lane / S::kLanesPerRow;
-      if (ids[n] < 0 || static_cast<uint32_t>(ids[n]) >= p.c.pages) {
+    for (int n = 0; n < S::kIds; ++n) {
+      const uint32_t pos = min(stage * kStage + w * kRows + 16 * n, static_cast<uint32_t>(it.length - 1));
+      x.id[n] = load_uniform(p.c.table + it.row * p.c.table_stride + (pos >> p.page_shift));
+    }
+    return x;
+  }
+  // K (0) or V (1) of a stage. Positions past the length read the last one: nothing behind it is
+  // touched. (A group of 16 rows lies in one page: its address is the wave's, and a lane's share of it
+  // is the same in every full group.)
+  template <int kOf>
+  __device__ __forceinline__ void load(uint32_t stage, const Ids &pages) {
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char *)sh.stage)) +
+                         (2 * (stage - it.first) + kOf) % S::kHalves * S::kHalf + w * kRows * S::kRowBytes;
+    const int64_t head = static_cast<int64_t>(it.kv) * p.c.head_stride;
+    constexpr int kPerGroup = S::kDmas / S::kIds;
+#pragma unroll
+    for (int g = 0; g < S::kIds; ++g) {
+      const int32_t id = pages.id[g];
+      const uint32_t first = stage * kStage + w * kRows + 16 * g;
+      if (id < 0 || static_cast<uint32_t>(id) >= p.c.pages) {
         errors |= QD_PAGED_BAD_PAGE;
         continue;
       }
-      const uint32_t pos = min(stage * S::kPositions + mine, static_cast<uint32_t>(it.length - 1)) & (p.c.page_size - 1);
-      const uint32_t chunk = (lane % S::kLanesPerRow) ^ swizzle<S::kRowBytes, kWide>(mine);
-      const int64_t base = (ids[n] * p.c.page_stride + head) * S::kElem;
-      const uint64_t off = static_cast<uint64_t>(pos) * token_bytes + 16 * chunk;
-      dma_to_lds(static_cast<const char *>(p.c.k) + base + off, lds + row * S::kRowBytes);
-      dma_to_lds(static_cast<const char *>(p.c.v) + base + off, lds + S::kHalf + row * S::kRowBytes);
+      const char *base = static_cast<const char *>(kOf ? p.c.v : p.c.k) + (id * p.c.page_stride + head) * S::kElem;
+      if (first + std::min(kRows, 16) <= static_cast<uint32_t>(it.length)) {
+        const char *group = base + static_cast<uint64_t>(first & (p.c.page_size - 1)) * token_bytes;
+#pragma unroll
+        for (int n = 0; n < kPerGroup; ++n) dma_to_lds(group, lane_off[n], lds + (g * kPerGroup + n) * 1024);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kPerGroup; ++n) {
+          const uint32_t row = n * S::kRowsPerDma + lane / S::kLanesPerRow;
+          const uint32_t pos = min(first + row, static_cast<uint32_t>(it.length - 1)) & (p.c.page_size - 1);
+          dma_to_lds(base + (static_cast<uint64_t>(pos) * token_bytes + lane_off[n] - row * token_bytes), lds + (g * kPerGroup + n) * 1024);
+        }
+      }
     }
+  }
+  __device__ __forceinline__ const char *half(uint32_t stage, int of) const {
+    return sh.stage + (2 * (stage - it.first) + of) % S::kHalves * S::kHalf;
   }
   __device__ __forceinline__ uint32_t column(int nb) const { return it.block * S::kColumns + (wc * NB + nb) * 16 + col; }
   __device__ __forceinline__ void load_queries() {
+    const uint32_t sign = p.a.scale < 0.f ? kWide ? 0x80000000u : 0x80008000u : 0u;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const uint32_t c = column(nb);
@@ -223,22 +272,19 @@ struct TreeAttention {
         const char *at = static_cast<const char *>(p.a.q) +
                          (it.row * p.a.q_stride + node * p.a.q_node_stride + head * p.a.q_head_stride) * S::kElem + 16 * quad;
 #pragma unroll
-        for (int s = 0; s < kQ; ++s) q[nb][s] = *reinterpret_cast<const u4v *>(at + 64 * s);
+        for (int s = 0; s < kQ; ++s) q[nb][s] = *reinterpret_cast<const u4v *>(at + 64 * s) ^ sign;
       } else {
 #pragma unroll
         for (int s = 0; s < kQ; ++s) q[nb][s] = u4v{0u, 0u, 0u, 0u};
       }
     }
   }
-  __device__ __forceinline__ const char *slot(uint32_t stage) const {
-    return sh.stage + (stage - it.first) % S::kStages * (2 * S::kHalf);
-  }
   // Positions of the tree in a stage, and those past it: V's values that are not finite
   // make way for zeros, and the nodes that see them are marked.
   __device__ __forceinline__ void clean(uint32_t stage) {
-    char *v = const_cast<char *>(slot(stage)) + S::kHalf;
-    const int base = stage * S::kPositions;
-    for (int i = threadIdx.x; i < S::kPositions * S::kLanesPerRow; i += S::kThreads) {
+    char *v = const_cast<char *>(half(stage, 1));
+    const int base = stage * kStage;
+    for (int i = threadIdx.x; i < kStage * S::kLanesPerRow; i += S::kThreads) {
       const int row = i / S::kLanesPerRow, node = base + row - it.start;
       if (node < 0) continue;
       u4v *at = reinterpret_cast<u4v *>(v + i * 16);
@@ -276,10 +322,11 @@ struct TreeAttention {
       *at = u4v{y[0], y[1], y[2], y[3]};
     }
   }
+  // The probabilities of this wave's half of a stage: pr[nb][s][r] of its position 16 s + 4 quad + r.
   template <bool kTree>
-  __device__ __forceinline__ void step(uint32_t stage) {
-    const char *k = slot(stage) + wp * kStep * S::kRowBytes, *v = k + S::kHalf;
-    const int base = stage * S::kPositions + wp * kStep;
+  __device__ __forceinline__ void weigh(uint32_t stage, float (&pr)[NB][2][4]) {
+    const char *k = half(stage, 0) + wp * kStep * S::kRowBytes;
+    const int base = stage * kStage + wp * kStep;
     f4v s[2][NB];
 #pragma unroll
     for (int sub = 0; sub < 2; ++sub)
@@ -302,28 +349,27 @@ struct TreeAttention {
           }
         }
       }
-    float pr[NB][2][4], top[NB];
+    float top[NB];
     bool rises = false;
+    bool hidden[kTree ? NB : 1][2][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      uint64_t mask = 0;
       if constexpr (kTree) {
         const uint32_t c = column(nb);
-        mask = c < p.columns ? sh.mask[c / p.group] : 0ull;
-      }
-      top[nb] = -INFINITY;
+        const uint64_t mask = c < p.columns ? sh.mask[c / p.group] : 0ull;
 #pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
+        for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = s[sub][nb][r] * scale;
-          if constexpr (kTree) {
+          for (int r = 0; r < 4; ++r) {
             const int node = base + 16 * sub + 4 * quad + r - it.start;
-            if (node >= 0 && (node >= static_cast<int>(p.a.nodes) || !(mask >> node & 1))) x = -INFINITY;
+            hidden[nb][sub][r] = node >= 0 && (node >= static_cast<int>(p.a.nodes) || !(mask >> node & 1));
+            if (hidden[nb][sub][r]) s[sub][nb][r] = -INFINITY;
           }
-          pr[nb][sub][r] = x;
-          top[nb] = fmaxf(top[nb], x);
-        }
+      }
+      float x = s[0][nb][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) x = fmaxf(x, s[i >> 2][nb][i & 3]);
+      top[nb] = kTree && x == -INFINITY ? x : x * scale;
       rises |= top[nb] > m[nb] + kLazy<E>;
     }
     if (__any(rises)) {
@@ -332,7 +378,7 @@ struct TreeAttention {
         const float n = fmaxf(m[nb], quarters_max(top[nb]));
         const float f = n == m[nb] ? 1.f : exp2_fast(m[nb] - n);
         m[nb] = n;
-        ms[nb] = n == -INFINITY ? 0.f : n;
+        ms[nb] = n == -INFINITY ? -kUnit<E> : n - kUnit<E>;
         l[nb] *= f;
 #pragma unroll
         for (int j = 0; j < S::kAcc; ++j) o[nb][j] *= f;
@@ -345,11 +391,17 @@ struct TreeAttention {
       for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          pr[nb][sub][r] = exp2_fast(pr[nb][sub][r] - ms[nb]);
-          sum += pr[nb][sub][r];
+          float x = exp2_fast(fmaf(s[sub][nb][r], scale, -ms[nb]));
+          if constexpr (kTree)
+            if (hidden[nb][sub][r]) x = 0.f;
+          pr[nb][sub][r] = x;
+          sum += x;
         }
       l[nb] += sum;
     }
+  }
+  __device__ __forceinline__ void accumulate(uint32_t stage, const float (&pr)[NB][2][4]) {
+    const char *v = half(stage, 1) + wp * kStep * S::kRowBytes;
     if constexpr (kWide) {
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub)
@@ -368,20 +420,16 @@ struct TreeAttention {
           }
         }
     } else {
-      // Probabilities as two numbers of the type, as in the attention of one token.
+      // Probabilities as two numbers of the type, rounded and what that left, as in the
+      // attention of one token.
       u4v b[NB], rest[NB];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float x = pr[nb][i >> 1][2 * (i & 1)], y = pr[nb][i >> 1][2 * (i & 1) + 1];
-          if constexpr (kScaled) {
-            b[nb][i] = E::pack(x * kTreeWeight, y * kTreeWeight);
-            rest[nb][i] = E::pack(fmaf(x, kTreeWeight, -E::lo(b[nb][i])) * kTreeRest, fmaf(y, kTreeWeight, -E::hi(b[nb][i])) * kTreeRest);
-          } else {
-            b[nb][i] = E::pack(x, y);
-            rest[nb][i] = E::pack(x - E::lo(b[nb][i]), y - E::hi(b[nb][i]));
-          }
+          b[nb][i] = E::pack(x, y);
+          rest[nb][i] = E::pack(x - E::lo(b[nb][i]), y - E::hi(b[nb][i]));
         }
 #pragma unroll
       for (int j = 0; j < S::kAcc; ++j) {
@@ -397,45 +445,85 @@ struct TreeAttention {
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          if constexpr (kScaled) {
-            const f4v r = E::mfma(a, rest[nb], f4v{0.f, 0.f, 0.f, 0.f});
-            o[nb][j] = E::mfma(a, b[nb], o[nb][j]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[nb][j][c] = fmaf(r[c], 1.f / kTreeRest, o[nb][j][c]);
-          } else {
-            o[nb][j] = E::mfma(a, rest[nb], o[nb][j]);
-            o[nb][j] = E::mfma(a, b[nb], o[nb][j]);
-          }
+          o[nb][j] = E::mfma(a, rest[nb], o[nb][j]);
+          o[nb][j] = E::mfma(a, b[nb], o[nb][j]);
         }
       }
     }
+  }
+  // All but one half (a stage) of what LDS holds is on its way when this returns.
+  static constexpr int kFirst = S::kHalves / 2 - !S::kByHalves;  // stages
+  Ids ahead;  // the pages of the stage that is loaded next
+  __device__ __forceinline__ void begin() {
+    if (it.length == 0) return;
+    Ids early[kFirst];
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) early[i] = pages_of(it.first + i);
+#pragma unroll
+    for (int i = 0; i < kFirst; ++i) {
+      if (it.first + i >= it.last) break;
+      load<0>(it.first + i, early[i]);
+      if (!S::kByHalves || S::kHalves % 2 || i + 1 < kFirst) load<1>(it.first + i, early[i]);
+    }
+    ahead = S::kByHalves && S::kHalves % 2 == 0 ? early[kFirst - 1] : pages_of(it.first + kFirst);
+  }
+  template <bool kTree>
+  __device__ __forceinline__ void stage_through(uint32_t stage) {
+    // (The last stage's second half may lie behind the row.)
+    const bool some = WP == 1 || static_cast<int>(stage * kStage + wp * kStep) < it.length;
+    const uint32_t more = it.last - 1 - stage;  // stages behind this one
+    float pr[NB][2][4];
+    if constexpr (S::kByHalves) {
+      // A half that is read makes room for the one kHalves - 1 behind it.
+      dma_wait<S::kDmas, S::kHalves - 2>(1 + 2 * more);
+      lds_barrier();
+      if constexpr (S::kHalves % 2) {
+        if (more >= kFirst) load<0>(stage + kFirst, ahead);
+      } else if (more >= kFirst - 1) {
+        load<1>(stage + kFirst - 1, ahead);
+        ahead = pages_of(stage + kFirst);
+      }
+      weigh<kTree>(stage, pr);
+      dma_wait<S::kDmas, S::kHalves - 2>(2 * more);
+      lds_barrier();
+      if (more >= kFirst) {
+        if constexpr (S::kHalves % 2) {
+          load<1>(stage + kFirst, ahead);
+          ahead = pages_of(stage + kFirst + 1);
+        } else {
+          load<0>(stage + kFirst, ahead);
+        }
+      }
+    } else {
+      dma_wait<2 * S::kDmas, kFirst - 1>(more);
+      lds_barrier();
+      if (more >= kFirst) {
+        load<0>(stage + kFirst, ahead);
+        load<1>(stage + kFirst, ahead);
+        ahead = pages_of(stage + kFirst + 1);
+      }
+      if (some) weigh<kTree>(stage, pr);
+    }
+    if constexpr (kTree) {
+      clean(stage);
+      lds_barrier();
+    }
+    if (some) accumulate(stage, pr);
   }
   __device__ __forceinline__ void run() {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       m[nb] = -INFINITY;
-      ms[nb] = l[nb] = 0.f;
+      ms[nb] = -kUnit<E>;
+      l[nb] = 0.f;
 #pragma unroll
       for (int j = 0; j < S::kAcc; ++j) o[nb][j] = f4v{0.f, 0.f, 0.f, 0.f};
     }
-    if (it.length == 0) {
-      __syncthreads();
-      return;
-    }
-    for (uint32_t stage = it.first; stage < it.last; ++stage) {
-      dma_wait<0>();
-      lds_barrier();
-      if (stage + 1 < it.last) {
-        load(stage + 1);
-        pages_of(stage + 2);
-      }
-      if (static_cast<int>((stage + 1) * S::kPositions) > it.start) {
-        clean(stage);
-        lds_barrier();
-        if (static_cast<int>(stage * S::kPositions + wp * kStep) < it.length) step<true>(stage);
-      } else {
-        step<false>(stage);
-      }
+    if (it.length) {
+      uint32_t stage = it.first;
+      const uint32_t plain = min(it.last, static_cast<uint32_t>(it.start) / kStage);  // stages before the tree
+      for (; stage < plain; ++stage) stage_through<false>(stage);
+      for (; stage < it.last; ++stage) stage_through<true>(stage);
     }
     lds_barrier();
   }
@@ -450,50 +538,39 @@ struct TreeAttention {
     else
       return make_float4(o[nb][i][0], o[nb][i][1], o[nb][i][2], o[nb][i][3]);
   }
-  // The waves' shares of the positions together, in the first WC waves.
+  // The sums of a stage's two waves together, in the first WC waves.
   __device__ __forceinline__ void merge() {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) l[nb] = quarters_sum(l[nb]);
-    if constexpr (WP > 1) {
-      constexpr int kShare = NB * S::kAcc * 1024 + NB * 512;
-      if (wp > 0) {
-        char *to = sh.stage + ((wp - 1) * WC + wc) * kShare;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-          for (int j = 0; j < S::kAcc; ++j) *reinterpret_cast<f4v *>(to + (nb * S::kAcc + j) * 1024 + lane * 16) = o[nb][j];
-          *reinterpret_cast<float2 *>(to + NB * S::kAcc * 1024 + nb * 512 + lane * 8) = make_float2(m[nb], l[nb]);
-        }
-      }
+    if constexpr (WP == 1) {
       __syncthreads();
-      if (wp == 0) {
+      return;
+    }
+    constexpr int kShare = NB * (S::kAcc * 1024 + 512);
+    char *at = sh.stage + wc * kShare;
+    if (wp > 0) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float2 x[WP - 1];
-          float top = m[nb];
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-          for (int u = 0; u < WP - 1; ++u) {
-            x[u] = *reinterpret_cast<const float2 *>(sh.stage + (u * WC + wc) * kShare + NB * S::kAcc * 1024 + nb * 512 + lane * 8);
-            top = fmaxf(top, x[u].x);
-          }
-          const float f = m[nb] == top ? 1.f : exp2_fast(m[nb] - top);
-          l[nb] *= f;
-#pragma unroll
-          for (int j = 0; j < S::kAcc; ++j) o[nb][j] *= f;
-#pragma unroll
-          for (int u = 0; u < WP - 1; ++u) {
-            const float g = x[u].x == top ? 1.f : exp2_fast(x[u].x - top);
-            l[nb] = fmaf(g, x[u].y, l[nb]);
-#pragma unroll
-            for (int j = 0; j < S::kAcc; ++j) {
-              const f4v y = *reinterpret_cast<const f4v *>(sh.stage + (u * WC + wc) * kShare + (nb * S::kAcc + j) * 1024 + lane * 16);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) o[nb][j][c] = fmaf(g, y[c], o[nb][j][c]);
-            }
-          }
-          m[nb] = top;
-        }
+        for (int j = 0; j < S::kAcc; ++j) *reinterpret_cast<f4v *>(at + (nb * S::kAcc + j) * 1024 + lane * 16) = o[nb][j];
+        *reinterpret_cast<float2 *>(at + NB * S::kAcc * 1024 + nb * 512 + lane * 8) = make_float2(m[nb], l[nb]);
       }
+    }
+    __syncthreads();
+    if (wp > 0) return;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const float2 x = *reinterpret_cast<const float2 *>(at + NB * S::kAcc * 1024 + nb * 512 + lane * 8);
+      const float top = fmaxf(m[nb], x.x);
+      const float f = m[nb] == top ? 1.f : exp2_fast(m[nb] - top), g = x.x == top ? 1.f : exp2_fast(x.x - top);
+      l[nb] = fmaf(g, x.y, l[nb] * f);
+#pragma unroll
+      for (int j = 0; j < S::kAcc; ++j) {
+        const f4v y = *reinterpret_cast<const f4v *>(at + (nb * S::kAcc + j) * 1024 + lane * 16);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[nb][j][c] = fmaf(g, y[c], o[nb][j][c] * f);
+      }
+      m[nb] = top;
     }
   }
   // Column c's four outputs from dimension d on.
@@ -508,41 +585,41 @@ struct TreeAttention {
     if (poison != 0.f) x = make_float4(poison, poison, poison, poison);  // NaN
     store4<E>(p.a.out, it.row * p.a.out_stride + node * p.a.out_node_stride + head * p.a.out_head_stride + d, x);
   }
+  // A record is as the lanes hold it, whole lines at a time: [block of 16 columns][four][lane] float4,
+  // then each column's maximum and sum.
+  static constexpr uint32_t kFours = S::kAcc * kWave, kRecord = S::kColumns * (D + 2);  // float4 of 16 columns; floats
+  __device__ __forceinline__ uint32_t record_four(int nb, int i) const { return (wc * NB + nb) * kFours + i * kWave + lane; }
+  __device__ __forceinline__ uint32_t record_sums(int nb) const { return S::kColumns * D + ((wc * NB + nb) * 16 + col) * 2; }
   // The piece's result, out or to its record.
   __device__ __forceinline__ void put(float *record) {
     const float nan = __uint_as_float(kNan);
     const bool spoilt = sh.errors != 0, whole = it.pieces == 1;
-    const bool tree = static_cast<int>(it.last * S::kPositions) > it.start && it.length > 0;
+    const bool tree = static_cast<int>(it.last * kStage) > it.start && it.length > 0;
     if (threadIdx.x == 0 && spoilt) raise_error(p.c.errors, sh.errors);
     if (wp > 0) return;
-    constexpr float unit = kScaled ? 1.f / kTreeWeight : 1.f;
-    const Coherent rec(record, p.rec_floats * static_cast<uint32_t>(sizeof(float)));
+    const Coherent rec(record, kRecord * static_cast<uint32_t>(sizeof(float)));
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t c = column(nb), mine = c - it.block * S::kColumns;
-      if (c >= p.columns) continue;
-      const uint32_t node = c / p.group;
+      const uint32_t c = column(nb);
+      const uint32_t node = min(c / p.group, p.a.nodes - 1);
 #pragma unroll
       for (int i = 0; i < S::kAcc; ++i) {
         const int d = dim_of(i);
         float4 x = four(nb, i);
-        x = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
         if (tree) {
           if (sh.poison[d] >> node & 1) x.x = nan;
           if (sh.poison[d + 1] >> node & 1) x.y = nan;
           if (sh.poison[d + 2] >> node & 1) x.z = nan;
           if (sh.poison[d + 3] >> node & 1) x.w = nan;
         }
-        if (whole) {
+        if (!whole)
+          rec.st4(record_four(nb, i), x);
+        else if (c < p.columns)
           emit(c, d, x, l[nb], spoilt ? nan : 0.f);
-        } else {
-          if (spoilt) x = make_float4(nan, nan, nan, nan);
-          rec.st4((mine * D + d) / 4, x);
-        }
       }
       if (!whole && quad == 0) {
-        rec.st(p.rec_columns * D + mine, spoilt ? nan : m[nb]);
-        rec.st(p.rec_columns * (D + 1) + mine, l[nb]);
+        rec.st(record_sums(nb), spoilt ? nan : m[nb]);
+        rec.st(record_sums(nb) + 1, l[nb]);
       }
     }
   }
@@ -558,62 +635,71 @@ struct TreeAttention {
     __syncthreads();
     return __builtin_amdgcn_readfirstlane(sh.last);
   }
-  // Joins the pieces in their order. Piece u's record is u * stride floats behind the first.
+  // Joins the pieces in their order, each wave its columns (of two waves at the same ones each half of the
+  // dimensions). Piece u's record is u * stride floats behind the first.
   __device__ __forceinline__ void join(const float *first, uint32_t stride) {
-    float *weight = reinterpret_cast<float *>(sh.stage);  // [columns][pieces]
-    float *sums = weight + S::kColumns * kTreePieces;
-    const uint32_t n = it.pieces, columns = min(static_cast<uint32_t>(S::kColumns), p.columns - it.block * S::kColumns);
-    const Coherent rec(first, ((n - 1) * stride + p.rec_floats) * static_cast<uint32_t>(sizeof(float)));
-    for (uint32_t c = threadIdx.x; c < columns; c += S::kThreads) {
+    constexpr int kMine = S::kAcc / WP, kAhead = 4;  // fours of a lane; pieces on their way
+    const uint32_t n = it.pieces;
+    const Coherent rec(first, ((n - 1) * stride + kRecord) * static_cast<uint32_t>(sizeof(float)));
+    const float nan = __uint_as_float(kNan);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float4 acc[kMine];
       float top = -INFINITY, sum = 0.f;
       bool spoilt = false;
-      for (uint32_t u = 0; u < n; ++u) {
-        const float x = rec.ld(u * stride + p.rec_columns * D + c);
-        spoilt |= x != x;
-        top = fmaxf(top, x);
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (uint32_t u0 = 0; u0 < n; u0 += kAhead) {
+        float mu[kAhead], lu[kAhead];
+        float4 x[kAhead][kMine];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const uint32_t at = min(u0 + a, n - 1) * stride;
+          mu[a] = rec.ld(at + record_sums(nb));
+          lu[a] = rec.ld(at + record_sums(nb) + 1);
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) x[a][i] = rec.ld4(at / 4 + record_four(nb, wp * kMine + i));
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          if (u0 + a >= n) break;
+          spoilt |= mu[a] != mu[a];
+          const float t = fmaxf(top, mu[a]);
+          const float g = top == t ? 1.f : exp2_fast(top - t), f = mu[a] == t ? 1.f : exp2_fast(mu[a] - t);
+          top = t;
+          sum = fmaf(f, lu[a], sum * g);
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            acc[i].x = fmaf(f, x[a][i].x, acc[i].x * g);
+            acc[i].y = fmaf(f, x[a][i].y, acc[i].y * g);
+            acc[i].z = fmaf(f, x[a][i].z, acc[i].z * g);
+            acc[i].w = fmaf(f, x[a][i].w, acc[i].w * g);
+          }
+        }
       }
-      for (uint32_t u = 0; u < n; ++u) {
-        const float x = rec.ld(u * stride + p.rec_columns * D + c);
-        const float f = spoilt ? __uint_as_float(kNan) : x == top ? 1.f : exp2_fast(x - top);
-        weight[c * kTreePieces + u] = f;
-        sum = fmaf(f, rec.ld(u * stride + p.rec_columns * (D + 1) + c), sum);
-      }
-      sums[c] = sum;
-    }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < columns * (D / 4); i += S::kThreads) {
-      const uint32_t c = i / (D / 4), d = 4 * (i % (D / 4));
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (uint32_t u = 0; u < n; ++u) {
-        const float f = weight[c * kTreePieces + u];
-        const float4 x = rec.ld4((u * stride + c * D + d) / 4);
-        acc.x = fmaf(f, x.x, acc.x);
-        acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z);
-        acc.w = fmaf(f, x.w, acc.w);
-      }
-      const float sum = sums[c];
-      emit(it.block * S::kColumns + c, d, acc, sum, weight[c * kTreePieces] != weight[c * kTreePieces] ? __uint_as_float(kNan) : 0.f);
+      const uint32_t c = column(nb);
+      if (c >= p.columns) continue;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) emit(c, dim_of(wp * kMine + i), acc[i], sum, spoilt ? nan : 0.f);
     }
   }
 };
 
-// The piece that a workgroup takes: rows are cut into pieces of `size` stages, so
-// that there are about `target` of them besides one of each row.
-template <int kPositions>
+// The piece that a workgroup takes: rows are cut into pieces of `size` stages, as few as let
+// all of them be on the card at once (p.target of one KV head and block); where rows alone are a
+// quarter of that, four times as many, since each place takes several of them then.
+template <int kStage>
 __device__ __forceinline__ bool find_piece(const TreeLaunch &p, Piece &it) {
-  // Consecutive workgroups go to consecutive XCDs: the blocks of a piece, which read
-  // the same positions, come to one.
+  // Consecutive workgroups go to consecutive XCDs: the heads and blocks of a piece come to one.
   const uint32_t xcd = blockIdx.x % kXcds, idx = blockIdx.x / kXcds;
-  const uint32_t unit = idx / p.blocks * kXcds + xcd;
-  if (unit >= p.units) return false;
+  const uint32_t x = idx / (p.blocks * p.c.kv_heads) * kXcds + xcd;
+  if (x >= p.units) return false;
   it.block = idx % p.blocks;
-  it.kv = unit % p.c.kv_heads;
-  const uint32_t x = unit / p.c.kv_heads;
+  it.kv = idx / p.blocks % p.c.kv_heads;
   const int lane = lane_id();
   const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
   const auto wrong = [&](int32_t n) { return n != 0 && (n < static_cast<int32_t>(p.a.nodes) || n > most); };
-  const auto stages_of = [&](int32_t n) { return wrong(n) || n == 0 ? 1u : (static_cast<uint32_t>(n) + kPositions - 1) / kPositions; };
+  const auto stages_of = [&](int32_t n) { return wrong(n) || n == 0 ? 1u : (static_cast<uint32_t>(n) + kStage - 1) / kStage; };
   uint32_t size = 0x7fffffffu, row = x;
   int32_t n = 0;
   it.number = x;
@@ -626,15 +712,19 @@ __device__ __forceinline__ bool find_piece(const TreeLaunch &p, Piece &it) {
       longest = max(longest, stages_of(n));
     }
     total = __builtin_amdgcn_readlane(lanes_upto(total), kWave - 1);
-    size = max(max((kTreeLeast + kPositions - 1) / kPositions, (total + p.target - 1) / p.target), (lanes_max(longest) + kTreePieces - 1) / kTreePieces);
-    const bool once = p.c.rows <= kWave;
+    const bool once = p.c.rows <= kWave, few = 4 * p.c.rows <= p.target;
+    const uint32_t aim = few ? p.target : 4 * p.target;
+    size = max(max(kTreeLeast / kStage, (total + aim - 1) / aim), (lanes_max(longest) + kTreePieces - 1) / kTreePieces);
+    const auto pieces_of = [&](uint32_t r, int32_t length) { return r < p.c.rows ? (stages_of(length) + size - 1) / size : 0u; };
+    if (few && once)  // (a size of total / (target - rows) will do)
+      while (__builtin_amdgcn_readlane(lanes_upto(pieces_of(lane, n)), kWave - 1) > p.target) size += max(1u, size / 16);
     uint32_t base = 0, upto, mine;
     it.number = 0;
     uint64_t past;
     for (;; base += kWave) {
       if (base >= p.c.rows) return false;
       if (!once) n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
-      mine = base + lane < p.c.rows ? (stages_of(n) + size - 1) / size : 0u;
+      mine = pieces_of(base + lane, n);
       upto = lanes_upto(mine);
       past = __ballot(it.number + upto > x);
       if (past) break;
@@ -664,13 +754,10 @@ __global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunc
   using S = TreeShape<E, D, NB, WC, WP>;
   __shared__ TreeShared<S> sh;
   Piece it;
-  if (!find_piece<S::kPositions>(p, it)) return;
+  if (!find_piece<S::kStage>(p, it)) return;
   TreeAttention<E, D, NB, WC, WP> a(p, sh, it);
-  if (it.length) {
-    a.pages_of(it.first);
-    a.load(it.first);
-    a.pages_of(it.first + 1);
-  }
+  a.load_queries();
+  a.begin();
   if (threadIdx.x == 0) sh.errors = 0;
   for (int i = threadIdx.x; i < 128; i += S::kThreads) sh.poison[i] = 0;
   if (a.w == 0) {
@@ -680,67 +767,59 @@ __global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunc
     if (bad) a.errors |= QD_TREE_BAD_PARENT;
   }
   if (it.bad) a.errors |= QD_PAGED_BAD_LENGTH;
-  a.load_queries();
   a.run();
   if (a.errors && a.lane == 0) atomicOr(&sh.errors, a.errors);
   a.merge();
-  if constexpr (WP == 1) __syncthreads();
-  // (Without columns of its own a block has none to put together.)
-  const uint32_t stride = p.c.kv_heads * p.blocks * p.rec_floats;
-  float *first = p.records + (static_cast<size_t>(it.number) * p.c.kv_heads * p.blocks + it.kv * p.blocks + it.block) * p.rec_floats;
+  const uint32_t stride = p.c.kv_heads * p.blocks * a.kRecord;
+  float *first = p.records + (static_cast<size_t>(it.number) * p.c.kv_heads * p.blocks + it.kv * p.blocks + it.block) * a.kRecord;
   a.put(first + static_cast<size_t>(it.index) * stride);
   if (it.pieces == 1) return;
   if (a.arrive()) a.join(first, stride);
 }
 
 struct TreePlan {
-  uint32_t group, columns, block_columns, blocks, rec_columns, rec_floats, apart, target, positions, records;
+  uint32_t group, columns, blocks, rec_floats, apart, target, records;
 };
-// The columns of a workgroup: as many as there are, by steps that the kernels come in.
-constexpr uint32_t block_columns_of(uint32_t columns) { return columns <= 16 ? 16 : columns <= 32 ? 32 : columns <= 64 ? 64 : 128; }
 
-// Calls f with the kernel's shape for so many columns.
+// Calls f with the shape and kernel for so many columns: as many of them to a workgroup as there
+// are, by steps that the kernels come in.
 template <typename E, int D, typename F>
-auto with_shape(uint32_t block_columns, F &&f) {
-  // FP32 heads of 128: half as many positions a stage.
-  constexpr int kFew = std::is_same_v<E, float> && D == 128 ? 2 : 4;
-  switch (block_columns) {
-    case 16: return f(TreeShape<E, D, 1, 1, kFew>{}, tree_attention_kernel<E, D, 1, 1, kFew>);
-    case 32:
-      if constexpr (std::is_same_v<E, float>)
-        return f(TreeShape<E, D, 1, 2, kFew>{}, tree_attention_kernel<E, D, 1, 2, kFew>);
-      else
-        return f(TreeShape<E, D, 2, 1, kFew>{}, tree_attention_kernel<E, D, 2, 1, kFew>);
-    case 64:
-      if constexpr (std::is_same_v<E, float>)
-        return f(TreeShape<E, D, 1, 4, 2>{}, tree_attention_kernel<E, D, 1, 4, 2>);
-      else
-        return f(TreeShape<E, D, 2, 2, 4>{}, tree_attention_kernel<E, D, 2, 2, 4>);
-    default: return f(TreeShape<E, D, 2, 4, 2>{}, tree_attention_kernel<E, D, 2, 4, 2>);
+auto with_shape(uint32_t columns, F &&f) {
+  const auto shape = [&](auto nb, auto wc, auto wp) {
+    constexpr int NB = decltype(nb)::value, WC = decltype(wc)::value, WP = decltype(wp)::value;
+    return f(TreeShape<E, D, NB, WC, WP>{}, tree_attention_kernel<E, D, NB, WC, WP>);
+  };
+  std::integral_constant<int, 1> one;
+  std::integral_constant<int, 2> two;
+  std::integral_constant<int, 4> four;
+  if (columns <= 16) return shape(one, one, one);
+  if (columns <= 32) return shape(one, two, one);
+  if constexpr (std::is_same_v<E, float>) {
+    return shape(one, four, one);
+  } else {
+    return columns <= 64 ? shape(two, two, one) : shape(two, four, two);
   }
 }
 template <typename F>
-auto with_type(uint32_t dtype, uint32_t head_dim, uint32_t block_columns, F &&f) {
+auto with_type(uint32_t dtype, uint32_t head_dim, uint32_t columns, F &&f) {
   const bool wide = head_dim == 128;
   switch (dtype) {
-    case QD_DTYPE_F32: return wide ? with_shape<float, 128>(block_columns, f) : with_shape<float, 64>(block_columns, f);
-    case QD_DTYPE_BF16: return wide ? with_shape<Brain, 128>(block_columns, f) : with_shape<Brain, 64>(block_columns, f);
-    default: return wide ? with_shape<Half, 128>(block_columns, f) : with_shape<Half, 64>(block_columns, f);
+    case QD_DTYPE_F32: return wide ? with_shape<float, 128>(columns, f) : with_shape<float, 64>(columns, f);
+    case QD_DTYPE_BF16: return wide ? with_shape<Brain, 128>(columns, f) : with_shape<Brain, 64>(columns, f);
+    default: return wide ? with_shape<Half, 128>(columns, f) : with_shape<Half, 64>(columns, f);
   }
 }
 
-TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t block_columns) {
   TreePlan s{};
   s.group = heads / kv_heads;
   s.columns = nodes * s.group;
-  s.block_columns = block_columns_of(s.columns);
-  s.blocks = (s.columns + s.block_columns - 1) / s.block_columns;
-  s.rec_columns = std::min(s.columns, s.block_columns);
-  s.rec_floats = (s.rec_columns * (head_dim + 2) + 3) / 4 * 4;
+  s.blocks = (s.columns + block_columns - 1) / block_columns;
+  s.rec_floats = block_columns * (head_dim + 2);
   const uint64_t items = static_cast<uint64_t>(rows) * kv_heads * s.blocks;
   if (items <= kOpCounters) {
-    s.target = std::max(1u, 2 * kTreeCus / (kv_heads * s.blocks));
-    s.records = (rows + s.target) * kv_heads * s.blocks;
+    s.target = std::max(1u, 4 * kTreeCus / (kv_heads * s.blocks));
+    s.records = (rows + 4 * s.target) * kv_heads * s.blocks;  // (where there are more pieces than rows)
     for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
   }
   return s;
@@ -1239,45 +1318,47 @@ uint32_t accept_shares(uint32_t rows, uint32_t nodes, uint32_t vocab) {
 
 }  // namespace
 
-size_t tree_attention_scratch(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
-  const TreePlan s = tree_plan(rows, nodes, heads, kv_heads, head_dim);
-  return static_cast<size_t>(s.records) * s.rec_floats * sizeof(float);
+size_t tree_attention_scratch(uint32_t dtype, uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
+  return with_type(dtype, head_dim, nodes * (heads / kv_heads), [&](auto shape, auto) {
+    const TreePlan s = tree_plan(rows, nodes, heads, kv_heads, head_dim, decltype(shape)::kColumns);
+    return static_cast<size_t>(s.records) * s.rec_floats * sizeof(float);
+  });
 }
 
 size_t tree_attention_scratch_most(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
   size_t most = 0;
   // (More rows than there are counters for are not cut and keep nothing; fewer are. A
   // few nodes less may take narrower blocks.)
-  for (uint32_t n = 1; n <= nodes; ++n) {
-    const uint32_t parts = kv_heads * tree_plan(0, n, heads, kv_heads, head_dim).blocks;
-    most = std::max(most, tree_attention_scratch(std::min(rows, static_cast<uint32_t>(kOpCounters / parts)), n, heads, kv_heads, head_dim));
-  }
+  for (const uint32_t dtype : {QD_DTYPE_F32, QD_DTYPE_BF16})
+    for (uint32_t n = 1; n <= nodes; ++n)
+      with_type(dtype, head_dim, n * (heads / kv_heads), [&](auto shape, auto) {
+        const uint32_t parts = kv_heads * tree_plan(0, n, heads, kv_heads, head_dim, decltype(shape)::kColumns).blocks;
+        most = std::max(most, tree_attention_scratch(dtype, std::min(rows, static_cast<uint32_t>(kOpCounters / parts)), n, heads, kv_heads, head_dim));
+      });
   return most;
 }
 
 hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const qd_tree_attention_args &a, const OpScratch &w) {
   if (c.rows == 0 || a.nodes == 0) return hipSuccess;
-  const TreePlan plan = tree_plan(c.rows, a.nodes, a.heads, c.kv_heads, c.head_dim);
   TreeLaunch p{};
   p.c = c;
   p.a = a;
   p.records = reinterpret_cast<float *>(w.scratch);
   p.counters = w.counters;
-  p.apart = plan.apart;
-  p.group = plan.group;
-  p.columns = plan.columns;
-  p.blocks = plan.blocks;
-  p.rec_columns = plan.rec_columns;
-  p.rec_floats = plan.rec_floats;
   p.page_shift = log2_of(c.page_size);
-  return with_type(c.dtype, c.head_dim, plan.block_columns, [&](auto shape, auto kernel) {
+  return with_type(c.dtype, c.head_dim, a.nodes * (a.heads / c.kv_heads), [&](auto shape, auto kernel) {
     using S = decltype(shape);
+    const TreePlan plan = tree_plan(c.rows, a.nodes, a.heads, c.kv_heads, c.head_dim, S::kColumns);
+    p.apart = plan.apart;
+    p.group = plan.group;
+    p.columns = plan.columns;
+    p.blocks = plan.blocks;
     const uint64_t most = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + kTreeLeast - 1) / kTreeLeast;
-    p.target = plan.target == 0 || most <= 1 ? 0 : std::max(1u, plan.target * S::kPerCu / 2);
+    p.target = plan.target == 0 || most <= 1 ? 0 : std::max(1u, plan.target * S::kPerCu / 4);
     uint64_t x = c.rows;
-    if (p.target) x = std::min<uint64_t>(x + p.target, x * most);
-    p.units = static_cast<uint32_t>(x * c.kv_heads);
-    const uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.blocks;
+    if (p.target) x = std::min<uint64_t>(4 * x <= p.target ? x + p.target : x + 4 * p.target, x * most);
+    p.units = static_cast<uint32_t>(x);
+    const uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.blocks * c.kv_heads;
     return launch(kernel, dim3(grid), dim3(S::kThreads), s, p);
   });
 }
