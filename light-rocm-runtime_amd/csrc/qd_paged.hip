@@ -181,11 +181,7 @@ __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
 // page, K, the other waves, the other pieces, each near 1 us (one row of 129 6.75 us,
 // 16 beams at 576 8.5).
 constexpr int kTile = 32, kSub = 16;
-constexpr uint32_t kMostPieces = 256;  // of an item
 constexpr int kWaves = 4;              // of a workgroup
-// Tiles that an item's results cost the long kernel as much time as: 128 rows of 0 to
-// 4,000 took 171 us, counted as none 177, as one 176, as four 173.
-constexpr uint32_t kEdge = 2;
 // The short kernel: tiles of a piece at least, of an item that stays whole (one row of
 // 129 positions 7.4 us, with items of 5 tiles cut 8.6; 8 rows of 448 8.8, with items
 // of 14 whole 11.6), and pieces of an item at most (one row of 30,000 18.9 us, in up
@@ -234,115 +230,6 @@ struct PageRows {
   }
 };
 
-// An item and the run of its tiles that a workgroup takes: wave-uniform.
-struct Item {
-  int row, length;
-  uint32_t part;
-  uint32_t at, tiles;        // its first tile among all in the deal, and how many it has (one at least)
-  uint32_t first, last;      // the run
-  uint32_t home, pieces;     // the workgroup of its first piece, and how many there are
-  bool bad;                  // the row's length
-};
-
-// The runs of all workgroups: run i is [i share, (i + 1) share) of all tiles, but
-// for the cuts that move. Before its tiles each item has kEdge more that stand for
-// the time that its results take.
-struct Deal {
-  uint32_t share, total;
-};
-
-__device__ __forceinline__ uint32_t tiles_of(const AttnLaunch &p, int32_t n, int64_t most) {
-  return n <= 0 || n > most ? 1u : (static_cast<uint32_t>(n) + kTile - 1) / kTile;
-}
-
-// How a cut `off` tiles into an item of n moves: 0 to its start, 1 not, 2 to its end.
-__device__ __forceinline__ int cut_of(const AttnLaunch &p, uint32_t off, uint32_t n) {
-  if (p.least && n >= 2 * p.least) return off < p.least ? 0 : n - off < p.least ? 2 : 1;
-  return 2 * off < n ? 0 : 2;
-}
-
-__device__ __forceinline__ void set_item(const AttnLaunch &p, const Deal &d, Item &it, uint32_t row, uint32_t part,
-                                         uint32_t at, int32_t n, int64_t most) {
-  it.row = static_cast<int>(row);
-  it.part = part;
-  it.at = at + kEdge;
-  it.bad = n < 0 || n > most;
-  it.length = it.bad ? 0 : n;
-  it.tiles = tiles_of(p, n, most);
-  it.first = 0;
-  it.last = it.tiles;
-  it.home = 0;
-  it.pieces = 1;
-  if (p.least && it.tiles >= 2 * p.least) {
-    const uint32_t lo = (it.at + p.least + d.share - 1) / d.share, hi = (it.at + it.tiles - p.least) / d.share;
-    if (hi >= lo) {
-      it.pieces = hi - lo + 2;
-      it.home = lo - 1;
-    }
-  }
-}
-
-// Ends the run of `it` where workgroup i's does; false: the item is the next one's.
-__device__ __forceinline__ bool end_run(const AttnLaunch &p, const Deal &d, uint32_t i, Item &it) {
-  const uint32_t end = (i + 1) * d.share;
-  if (it.at + it.tiles <= end || end >= d.total) return true;
-  if (end <= it.at) return false;
-  const int cut = cut_of(p, end - it.at, it.tiles);
-  if (cut == 1) it.last = end - it.at;
-  return cut != 0;
-}
-
-// Workgroup i's first item; false if it has none. Lane l looks at rows l, l + 64, ...
-__device__ __forceinline__ bool first_item(const AttnLaunch &p, uint32_t i, uint32_t groups, Deal &d, Item &it) {
-  const int lane = lane_id();
-  const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
-  uint32_t total = 0, longest = 0;
-  int32_t n = 0;  // of the row looked at last
-  for (uint32_t r = lane; r < p.c.rows; r += kWave) {
-    n = p.c.lengths[r];
-    const uint32_t tiles = tiles_of(p, n, most) + kEdge;
-    total += tiles;
-    longest = max(longest, tiles);
-  }
-  uint32_t upto = lanes_upto(total);
-  total = __builtin_amdgcn_readlane(upto, kWave - 1) * p.parts;
-  longest = lanes_max(longest);
-  d.total = total;
-  d.share = max((total + groups - 1) / groups, (longest + kMostPieces - 3) / (kMostPieces - 2));
-  const uint32_t begin = i * d.share;
-  if (static_cast<uint64_t>(i) * d.share >= total) return false;
-  // The row in which the run begins.
-  uint32_t before = 0, base = 0;
-  const bool once = p.c.rows <= kWave;
-  uint64_t past;
-  for (;;) {
-    if (!once) {
-      n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
-      upto = lanes_upto(base + lane < p.c.rows ? tiles_of(p, n, most) + kEdge : 0u);
-    }
-    past = __ballot(before + upto * p.parts > begin);
-    if (past) break;
-    before += __builtin_amdgcn_readlane(upto, kWave - 1) * p.parts;
-    base += kWave;
-  }
-  const int at = __ffsll(static_cast<unsigned long long>(past)) - 1;
-  const int32_t length = __builtin_amdgcn_readlane(n, at);
-  const uint32_t tiles = tiles_of(p, length, most), each = tiles + kEdge, row = base + at;
-  before += (__builtin_amdgcn_readlane(upto, at) - each) * p.parts;
-  const uint32_t part = (begin - before) / each, in = begin - before - part * each;
-  const int cut = in > kEdge ? cut_of(p, in - kEdge, tiles) : 0;
-  if (cut < 2) {
-    set_item(p, d, it, row, part, before + part * each, length, most);
-    if (cut == 1) it.first = in - kEdge;
-  } else if (part + 1 < p.parts) {  // from the next item on
-    set_item(p, d, it, row, part + 1, before + (part + 1) * each, length, most);
-  } else {
-    if (row + 1 >= p.c.rows) return false;
-    set_item(p, d, it, row + 1, 0, before + (part + 1) * each, load_uniform(p.c.lengths + row + 1), most);
-  }
-  return end_run(p, d, i, it);
-}
-
 // The short kernel's pieces: a row of n tiles has max(1, ceil(n / size)) of each
 // item, where size makes about `target` of them. Piece x of all rows' (counted for
 // one part); it.home is its number within the row, `begin` the number of its
@@ -357,7 +244,7 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint
     uint32_t total = 0, longest = 0;
     for (uint32_t r = lane; r < p.c.rows; r += kWave) {
       n = p.c.lengths[r];
-      const uint32_t tiles = tiles_of(p, n, most);
+      const uint32_t tiles = tiles_of<kTile>(p, n, most);
       total += tiles;
       longest = max(longest, tiles);
     }
@@ -371,7 +258,7 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint
     for (;; base += kWave) {
       if (base >= p.c.rows) return false;
       if (!once) n = base + lane < p.c.rows ? p.c.lengths[base + lane] : 0;
-      mine = base + lane < p.c.rows ? pieces_of(tiles_of(p, n, most)) : 0u;
+      mine = base + lane < p.c.rows ? pieces_of(tiles_of<kTile>(p, n, most)) : 0u;
       upto = lanes_upto(mine);
       past = __ballot(begin + upto > x);
       if (past) break;
@@ -391,24 +278,11 @@ __device__ __forceinline__ bool find_piece(const AttnLaunch &p, uint32_t x, uint
   it.bad = n < 0 || n > most;
   it.length = it.bad ? 0 : n;
   it.at = 0;
-  it.tiles = tiles_of(p, n, most);
+  it.tiles = tiles_of<kTile>(p, n, most);
   it.home = x - begin;
   it.first = it.pieces == 1 ? 0 : it.home * size;
   it.last = it.pieces == 1 ? it.tiles : min(it.tiles, it.first + size);
   return true;
-}
-
-// The item behind `it` in workgroup i's run; false at its end.
-__device__ __forceinline__ bool next_item(const AttnLaunch &p, const Deal &d, uint32_t i, const Item &it, Item &next) {
-  const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
-  const uint32_t at = it.at + it.tiles;
-  if (it.last < it.tiles || at >= d.total || at >= (i + 1) * d.share) return false;
-  if (it.part + 1 < p.parts) {
-    set_item(p, d, next, it.row, it.part + 1, at, it.bad ? -1 : it.length, most);
-  } else {
-    set_item(p, d, next, it.row + 1, 0, at, load_uniform(p.c.lengths + it.row + 1), most);
-  }
-  return end_run(p, d, i, next);
 }
 
 // kStages tiles are loaded ahead. kEarly (one stage): the next tile's V comes with its
@@ -924,7 +798,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
   const uint32_t group_id = blockIdx.x;
   Deal deal;
   Item it;
-  if (!first_item(p, group_id, gridDim.x, deal, it)) return;
+  if (!first_item<kTile>(p, group_id, gridDim.x, deal, it)) return;
   if (threadIdx.x == 0) sh.spoilt = 0u;
   Attention<E, D, kStages, kPolicyNt, false> a(p, sh);
   // The record of an item's piece: its workgroup's first if it begins inside the item, else the second.
@@ -941,7 +815,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
     a.put_partials();
     // The next item's loads are under way while this one's results are put together.
     Item next;
-    const bool more = next_item(p, deal, group_id, it, next);
+    const bool more = next_item<kTile>(p, deal, group_id, it, next);
     bool next_bad = false;
     if (more) a.begin(next, next_bad);
     __syncthreads();

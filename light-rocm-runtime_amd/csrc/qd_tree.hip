@@ -60,8 +60,8 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t *parents, uint32_t n
 // Few rows are cut into runs that fill the card, which the last one joins in order.
 constexpr int kStep = 32;                // positions of a wave's step
 constexpr uint32_t kTreePieces = 64;     // of an item at most
-constexpr uint32_t kTreeLeast = 128;     // positions of a piece at least
-constexpr uint32_t kTreeCus = 256, kXcds = 8;
+constexpr uint32_t kTreeLeast = 64;      // positions of a piece at least
+constexpr uint32_t kTreeCus = 256, kTreePerCu = 4, kXcds = 8;
 constexpr uint32_t kLds = 160 * 1024;
 // A maximum is taken up once it passes the one in use by so many powers of two, as in the
 // attention of one token (qd_paged.hip).
@@ -87,18 +87,26 @@ struct TreeLaunch {
   uint32_t columns;    // nodes * group
   uint32_t blocks;     // of columns
   uint32_t page_shift;
-  uint32_t target;     // pieces of one KV head and block that the card holds at once; 0: rows are not cut
-  uint32_t units;      // pieces in the grid, of all rows and one KV head
+  uint32_t parts;      // items of a row: KV heads x blocks
+  uint32_t target;     // pieces of one item that the card holds at once; 0: rows are not cut
+  uint32_t units;      // pieces in the grid, of all rows and one item each; 0: equal runs of all stages
+  uint32_t least;      // (equal runs) stages on either side of a cut
 };
 
 // One 16-byte global -> LDS DMA per lane (lane l's bytes land at lds + 16 l), from
 // inline assembly: the compiler would guard every later LDS read with a wait for it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: set before each use, never saved
+// (lds and base are the wave's: the compiler is told where it cannot see it.)
 __device__ __forceinline__ void dma_to_lds(const void *src, uint32_t lds) {
+  lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
 __device__ __forceinline__ void dma_to_lds(const void *base, uint32_t off, uint32_t lds) {
+  const uint64_t at = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+  base = reinterpret_cast<const void *>(static_cast<uint64_t>(hi) << 32 | lo);
+  lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -141,7 +149,7 @@ struct TreeShape {
   // and all but one are on their way, 128 KB to a CU with two workgroups (96: 64 rows of 0 to
   // 8,192 with 8 nodes 260 us); where products do, by stages, three of them on their way.
   static constexpr bool kByHalves = WP == 1;
-  static constexpr int kHalves = !kByHalves ? 8 : kRowBytes == 512 ? 4 : 9;
+  static constexpr int kHalves = !kByHalves ? 8 : kRowBytes == 512 ? 4 : kRowBytes == 256 ? 5 : 9;
   static constexpr int kColumns = 16 * NB * WC;
   static constexpr int kRowsPerDma = 1024 / kRowBytes, kLanesPerRow = kRowBytes / 16;
   static constexpr int kRows = kStage / kWaves;                // of a half, that a wave transfers
@@ -150,10 +158,11 @@ struct TreeShape {
   static constexpr int kAcc = D / 16;
   static constexpr int kMerge = WP > 1 ? WC * NB * (kAcc * 1024 + 512) : 0;
   static constexpr int kBytes = std::max(kHalves * kHalf, kMerge);
-  static constexpr int kPerCu = std::min(8 / kWaves < 1 ? 1 : 8 / kWaves, static_cast<int>(kLds) / (kBytes + 2048));
+  static constexpr uint32_t kRecord = kColumns * (D + 2);  // floats
+  static constexpr int kPerCu = kWaves == 8 ? 1 : std::min(NB == 2 ? 2 : 4, static_cast<int>(kLds) / (kBytes + 2048));
   static_assert(WP <= 2 && kDmas >= 1 && kDmas * kRowsPerDma * kWaves == kStage, "whole transfers");
   static_assert((kHalves - 2) * kDmas < 64, "the wait's count");
-  static_assert(kBytes + 2048 <= static_cast<int>(kLds), "LDS");
+  static_assert(kBytes + 2048 <= static_cast<int>(kLds) && kPerCu <= static_cast<int>(kTreePerCu), "LDS");
 };
 
 template <typename S>
@@ -182,7 +191,7 @@ struct TreeAttention {
 
   const TreeLaunch &p;
   Shared &sh;
-  const Piece &it;
+  Piece it;
   const int w, lane, col, quad, wc, wp;
   const float scale;  // of the sizes of scores, in powers of two: the queries have its sign
   const uint32_t token_bytes;
@@ -192,10 +201,9 @@ struct TreeAttention {
   uint32_t errors = 0;
   uint32_t lane_off[S::kDmas / S::kIds];  // of a lane's bytes in a group of 16 rows
 
-  __device__ __forceinline__ TreeAttention(const TreeLaunch &launch, Shared &shared, const Piece &piece)
+  __device__ __forceinline__ TreeAttention(const TreeLaunch &launch, Shared &shared)
       : p(launch),
         sh(shared),
-        it(piece),
         w(__builtin_amdgcn_readfirstlane(wave_id())),
         lane(lane_id()),
         col(lane & 15),
@@ -587,7 +595,7 @@ struct TreeAttention {
   }
   // A record is as the lanes hold it, whole lines at a time: [block of 16 columns][four][lane] float4,
   // then each column's maximum and sum.
-  static constexpr uint32_t kFours = S::kAcc * kWave, kRecord = S::kColumns * (D + 2);  // float4 of 16 columns; floats
+  static constexpr uint32_t kFours = S::kAcc * kWave, kRecord = S::kRecord;  // float4 of 16 columns
   __device__ __forceinline__ uint32_t record_four(int nb, int i) const { return (wc * NB + nb) * kFours + i * kWave + lane; }
   __device__ __forceinline__ uint32_t record_sums(int nb) const { return S::kColumns * D + ((wc * NB + nb) * 16 + col) * 2; }
   // The piece's result, out or to its record.
@@ -627,7 +635,7 @@ struct TreeAttention {
   __device__ __forceinline__ bool arrive() {
     wait_vm_stores();
     __syncthreads();
-    uint32_t *cnt = p.counters + (static_cast<size_t>(it.row) * p.c.kv_heads * p.blocks + it.kv * p.blocks + it.block) * p.apart;
+    uint32_t *cnt = p.counters + (static_cast<size_t>(it.row) * p.parts + it.kv * p.blocks + it.block) * p.apart;
     if (threadIdx.x == 0) {
       sh.last = atomicAdd(cnt, 1u) == it.pieces - 1;
       if (sh.last) *cnt = 0u;
@@ -636,11 +644,11 @@ struct TreeAttention {
     return __builtin_amdgcn_readfirstlane(sh.last);
   }
   // Joins the pieces in their order, each wave its columns (of two waves at the same ones each half of the
-  // dimensions). Piece u's record is u * stride floats behind the first.
-  __device__ __forceinline__ void join(const float *first, uint32_t stride) {
+  // dimensions).
+  __device__ __forceinline__ void join(const float *first, uint32_t second, uint32_t stride) {
     constexpr int kMine = S::kAcc / WP, kAhead = 4;  // fours of a lane; pieces on their way
     const uint32_t n = it.pieces;
-    const Coherent rec(first, ((n - 1) * stride + kRecord) * static_cast<uint32_t>(sizeof(float)));
+    const Coherent rec(first, (second + (n - 2) * stride + kRecord) * static_cast<uint32_t>(sizeof(float)));
     const float nan = __uint_as_float(kNan);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
@@ -654,7 +662,7 @@ struct TreeAttention {
         float4 x[kAhead][kMine];
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-          const uint32_t at = min(u0 + a, n - 1) * stride;
+          const uint32_t u = min(u0 + a, n - 1), at = u == 0 ? 0u : second + (u - 1) * stride;
           mu[a] = rec.ld(at + record_sums(nb));
           lu[a] = rec.ld(at + record_sums(nb) + 1);
 #pragma unroll
@@ -685,21 +693,28 @@ struct TreeAttention {
   }
 };
 
-// The piece that a workgroup takes: rows are cut into pieces of `size` stages, as few as let
-// all of them be on the card at once (p.target of one KV head and block); where rows alone are a
-// quarter of that, four times as many, since each place takes several of them then.
+// The row of a piece, of length n.
+__device__ __forceinline__ void set_row(const TreeLaunch &p, Piece &it, uint32_t row, int32_t n) {
+  it.row = row;
+  it.bad = n != 0 && (n < static_cast<int32_t>(p.a.nodes) || n > static_cast<int64_t>(p.c.table_width) << p.page_shift);
+  it.length = it.bad ? 0 : n;
+  it.start = it.length - static_cast<int>(p.a.nodes);
+}
+
+// The one piece that a workgroup takes: rows are cut into pieces of `size` stages, as few as let
+// all of them be on the card at once (p.target of one item); where rows alone are a quarter of
+// that, four times as many, since each place takes several of them then.
 template <int kStage>
 __device__ __forceinline__ bool find_piece(const TreeLaunch &p, Piece &it) {
   // Consecutive workgroups go to consecutive XCDs: the heads and blocks of a piece come to one.
   const uint32_t xcd = blockIdx.x % kXcds, idx = blockIdx.x / kXcds;
-  const uint32_t x = idx / (p.blocks * p.c.kv_heads) * kXcds + xcd;
+  const uint32_t x = idx / p.parts * kXcds + xcd;
   if (x >= p.units) return false;
   it.block = idx % p.blocks;
   it.kv = idx / p.blocks % p.c.kv_heads;
   const int lane = lane_id();
   const int64_t most = static_cast<int64_t>(p.c.table_width) << p.page_shift;
-  const auto wrong = [&](int32_t n) { return n != 0 && (n < static_cast<int32_t>(p.a.nodes) || n > most); };
-  const auto stages_of = [&](int32_t n) { return wrong(n) || n == 0 ? 1u : (static_cast<uint32_t>(n) + kStage - 1) / kStage; };
+  const auto stages_of = [&](int32_t n) { return tiles_of<kStage>(p, n, most); };
   uint32_t size = 0x7fffffffu, row = x;
   int32_t n = 0;
   it.number = x;
@@ -738,10 +753,7 @@ __device__ __forceinline__ bool find_piece(const TreeLaunch &p, Piece &it) {
   } else {
     n = load_uniform(p.c.lengths + row);
   }
-  it.row = row;
-  it.bad = wrong(n);
-  it.length = it.bad ? 0 : n;
-  it.start = it.length - static_cast<int>(p.a.nodes);
+  set_row(p, it, row, n);
   it.index = x - it.number;
   const uint32_t stages = stages_of(n);
   it.first = it.pieces == 1 ? 0 : it.index * size;
@@ -753,28 +765,80 @@ template <typename E, int D, int NB, int WC, int WP>
 __global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunch p) {
   using S = TreeShape<E, D, NB, WC, WP>;
   __shared__ TreeShared<S> sh;
-  Piece it;
-  if (!find_piece<S::kStage>(p, it)) return;
-  TreeAttention<E, D, NB, WC, WP> a(p, sh, it);
-  a.load_queries();
-  a.begin();
-  if (threadIdx.x == 0) sh.errors = 0;
-  for (int i = threadIdx.x; i < 128; i += S::kThreads) sh.poison[i] = 0;
-  if (a.w == 0) {
-    bool bad;
-    const uint64_t mask = ancestors(p.a.parents + static_cast<size_t>(it.row) * p.a.nodes, p.a.nodes, bad);
-    sh.mask[a.lane] = mask;
-    if (bad) a.errors |= QD_TREE_BAD_PARENT;
+  constexpr uint32_t kRecord = S::kRecord;
+  TreeAttention<E, D, NB, WC, WP> a(p, sh);
+  // (Told to the compiler: all lanes have the same.)
+  const auto same = [](auto v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
+  const auto piece_of = [&](const Item &item) __attribute__((always_inline)) {
+    Piece x;
+    set_row(p, x, same(item.row), same(item.bad ? -1 : item.length));
+    x.kv = same(item.part) / p.blocks;
+    x.block = same(item.part) % p.blocks;
+    x.first = same(item.first);
+    x.last = same(item.last);
+    x.pieces = same(item.pieces);
+    x.number = same(item.home);
+    x.index = x.pieces > 1 ? blockIdx.x - x.number : 0;
+    return x;
+  };
+  // (A stage of two waves has no runs: its columns are so many that products bound it.)
+  const bool single = WP > 1 || p.units;
+  Deal deal{};
+  Item item{};
+  if (single) {
+    if (!find_piece<S::kStage>(p, a.it)) return;
+  } else {
+    if (!same(first_item<S::kStage>(p, blockIdx.x, gridDim.x, deal, item) ? 1 : 0)) return;
+    a.it = piece_of(item);
   }
-  if (it.bad) a.errors |= QD_PAGED_BAD_LENGTH;
-  a.run();
-  if (a.errors && a.lane == 0) atomicOr(&sh.errors, a.errors);
-  a.merge();
-  const uint32_t stride = p.c.kv_heads * p.blocks * a.kRecord;
-  float *first = p.records + (static_cast<size_t>(it.number) * p.c.kv_heads * p.blocks + it.kv * p.blocks + it.block) * a.kRecord;
-  a.put(first + static_cast<size_t>(it.index) * stride);
-  if (it.pieces == 1) return;
-  if (a.arrive()) a.join(first, stride);
+  a.begin();
+  for (;;) {
+    a.load_queries();
+    if (threadIdx.x == 0) sh.errors = 0;
+    for (int i = threadIdx.x; i < 128; i += S::kThreads) sh.poison[i] = 0;
+    if (a.w == 0) {
+      bool bad;
+      const uint64_t mask = ancestors(p.a.parents + static_cast<size_t>(a.it.row) * p.a.nodes, p.a.nodes, bad);
+      sh.mask[a.lane] = mask;
+      if (bad) a.errors |= QD_TREE_BAD_PARENT;
+    }
+    if (a.it.bad) a.errors |= QD_PAGED_BAD_LENGTH;
+    a.run();
+    if (a.errors && a.lane == 0) atomicOr(&sh.errors, a.errors);
+    a.merge();
+    // The next piece's loads are under way while this one's results are put together.
+    const Piece now = a.it;
+    Item next{};
+    const bool more = !single && same(next_item<S::kStage>(p, deal, blockIdx.x, item, next) ? 1 : 0);
+    uint32_t errors = 0;
+    if (more) {
+      a.it = piece_of(next);
+      a.errors = 0;
+      a.begin();
+      errors = a.errors;
+    }
+    const Piece then = a.it;
+    a.it = now;
+    // Records: of pieces of an item one after the other; or (equal runs) a workgroup's first where a
+    // piece begins inside its item, else the second.
+    float *first;
+    uint32_t second, stride;
+    if (single) {
+      first = p.records + (static_cast<size_t>(now.number) * p.parts + now.kv * p.blocks + now.block) * kRecord;
+      second = stride = p.parts * kRecord;
+    } else {
+      first = p.records + (2 * static_cast<size_t>(now.number) + 1) * kRecord;
+      second = kRecord;
+      stride = 2 * kRecord;
+    }
+    a.put(first + (now.index ? second + static_cast<size_t>(now.index - 1) * stride : 0));
+    if (now.pieces > 1 && a.arrive()) a.join(first, second, stride);
+    if (!more) break;
+    a.it = then;
+    a.errors = errors;
+    item = next;
+    __syncthreads();  // the masks and marks are written again
+  }
 }
 
 struct TreePlan {
@@ -818,8 +882,8 @@ TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_he
   s.rec_floats = block_columns * (head_dim + 2);
   const uint64_t items = static_cast<uint64_t>(rows) * kv_heads * s.blocks;
   if (items <= kOpCounters) {
-    s.target = std::max(1u, 4 * kTreeCus / (kv_heads * s.blocks));
-    s.records = (rows + 4 * s.target) * kv_heads * s.blocks;  // (where there are more pieces than rows)
+    s.target = std::max(1u, kTreePerCu * kTreeCus / (kv_heads * s.blocks));
+    s.records = std::max((rows + 4 * s.target) * kv_heads * s.blocks, 2 * kTreeCus * kTreePerCu);
     for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
   }
   return s;
@@ -1353,12 +1417,23 @@ hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const q
     p.group = plan.group;
     p.columns = plan.columns;
     p.blocks = plan.blocks;
+    p.parts = c.kv_heads * plan.blocks;
     const uint64_t most = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + kTreeLeast - 1) / kTreeLeast;
-    p.target = plan.target == 0 || most <= 1 ? 0 : std::max(1u, plan.target * S::kPerCu / 4);
+    // FP32's products bound it: no more pieces than CUs (16 rows of 576 with 16 nodes 19.1 us, as
+    // many as the card holds 22.9).
+    constexpr uint32_t kAim = S::kWide ? 1 : S::kPerCu;
+    p.target = plan.target == 0 || most <= 1 ? 0 : std::max(1u, plan.target * kAim / kTreePerCu);
     uint64_t x = c.rows;
     if (p.target) x = std::min<uint64_t>(4 * x <= p.target ? x + p.target : x + 4 * p.target, x * most);
     p.units = static_cast<uint32_t>(x);
-    const uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.blocks * c.kv_heads;
+    uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.parts;
+    // Many rows whose items read nothing twice: equal runs. (Stages are counted in 31 bits.)
+    const uint64_t stages = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + S::kStage - 1) / S::kStage;
+    if (S::kByHalves && p.target && p.blocks == 1 && 4ull * c.rows > p.target && c.rows * p.parts * (stages + kEdge) <= 0x7f000000u) {
+      p.units = 0;
+      p.least = kTreeLeast / S::kStage;
+      grid = kTreeCus * S::kPerCu;
+    }
     return launch(kernel, dim3(grid), dim3(S::kThreads), s, p);
   });
 }
