@@ -284,9 +284,9 @@ QD_API qd_status qd_paged_append_at(const qd_paged_cache *cache, const qd_append
  * them: node i attends to the positions before the tree, to the nodes above it and to
  * itself,
  *   out[r][i][h] = sum_j softmax_j(scale q[r][i][h] . K_j) V_j,
- * each position read once for all nodes where up to 128 pairs of a node and a query head
- * of one KV head allow it. Precision is qd_paged_attention's. Nodes that are not there
- * and rows of length 0 get zeros; K and V of nodes that are not seen may hold anything,
+ * each position read once for up to 128 (FP32: 64) pairs of a node and a query head of one
+ * KV head. Precision is qd_paged_attention's, but that a weight in FP16 is off by 2^-22 of
+ * it or 2^-39 of the row's largest. Nodes that are not there and rows of length 0 get zeros; K and V of nodes that are not seen may hold anything,
  * also values that are not finite: outputs that see such a V become NaN or infinite. A row with
  * a bad page, a bad parent, or a length that is not 0 and below `nodes` or past its
  * table gets NaN. q and out are [rows][nodes][heads][head_dim] with strides that are
@@ -320,9 +320,10 @@ QD_API qd_status qd_tree_attention_workspace(uint32_t rows, uint32_t nodes, uint
  * Picked is the token of the largest logit, the lowest of equal ones; NaN counts as -inf.
  * With draws (numbers u from 0 up to 1), the least token t with
  *   sum_{i <= t} p_i > u sum_i p_i,  p_i = exp(logits[i] / temperature)
- * (p_i in FP32, off by about 2^-23 of it; sums in 64 bits), so that the tokens that come
- * out are distributed as the model's own; where the largest logit is past 1e30 either
- * way, the token of the largest logit. A row whose node 0 is not there gets count 0 and
+ * (p_i and sums of up to 8 of them in FP32, off by about 2^-22; sums beyond in 64 bits), so
+ * that the tokens that come out are distributed as the model's own. A draw below 0 or NaN
+ * counts as 0, one of 1 or more picks the last token that has a probability; where the
+ * largest logit is past 1e30 either way, the token of the largest logit. A row whose node 0 is not there gets count 0 and
  * -1, and so does one with a bad parent. */
 typedef struct qd_accept_args {
   const void *logits;      /* [rows][nodes][vocab] */
@@ -368,7 +369,8 @@ typedef struct qd_token_memory {
  * a row of length 0, whose path is not read. Positions behind are left as they are. A row
  * with a bad length (not 0 and below `nodes`, or past the table), count, path (its nodes
  * ascend) or page moves nothing and hands its length on. Rows whose trees lie in the same
- * pages must not be committed in one call; lengths_out must not be lengths. */
+ * pages must not be committed in one call, nor memories that overlap; lengths_out must
+ * not be lengths. */
 typedef struct qd_commit_args {
   const int32_t *table;
   const int32_t *lengths;

@@ -494,6 +494,7 @@ qd_status qd_tree_commit(const qd_commit_args *a, void *stream) {
         p.piece_stride % 16 != 0 || p.plane_stride < 0 || p.plane_stride > most || p.page_stride < 0 || p.page_stride > most ||
         p.token_stride < static_cast<int64_t>(p.piece_bytes) || p.token_stride > most || p.piece_stride < 0 || p.piece_stride > most ||
         (p.pieces > 1 && p.piece_stride < static_cast<int64_t>(p.piece_bytes)) ||
+        (a->pages > 1 && p.page_stride < static_cast<int64_t>(p.piece_bytes)) ||
         (p.planes > 1 && p.plane_stride < static_cast<int64_t>(p.piece_bytes)))
       return invalid("a memory's bytes and strides: multiples of 16, strides of at least the bytes");
     const uint64_t row = static_cast<uint64_t>(p.piece_bytes / 16) * p.pieces;

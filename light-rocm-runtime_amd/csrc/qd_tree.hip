@@ -1196,7 +1196,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
         part[u] = scaled(part[u], by);
         s += part[u];
       }
-      const double upto = lanes_upto(s), aim = static_cast<double>(p.a.draws[at + node]) * lane_of(upto, kWave - 1);
+      const double upto = lanes_upto(s), aim = static_cast<double>(fmaxf(p.a.draws[at + node], 0.f)) * lane_of(upto, kWave - 1);
       const uint64_t past = __ballot(upto > aim), some = __ballot(s > 0.0);
       // (A draw of 1 or more passes nothing: the last share with a token.)
       const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(some));

@@ -119,7 +119,7 @@ def test_accept_refusals(status, changes):
     (qd.INVALID_ARGUMENT, dict(base=None), {}), (qd.INVALID_ARGUMENT, dict(base=AT + 4), {}), (qd.INVALID_ARGUMENT, dict(piece_bytes=8), {}),
     (qd.INVALID_ARGUMENT, dict(piece_bytes=0), {}), (qd.INVALID_ARGUMENT, dict(pieces=0), {}), (qd.INVALID_ARGUMENT, dict(planes=0), {}),
     (qd.INVALID_ARGUMENT, dict(token_stride=128), {}), (qd.INVALID_ARGUMENT, dict(piece_stride=128), {}),
-    (qd.INVALID_ARGUMENT, dict(plane_stride=-16), {}), (qd.INVALID_ARGUMENT, dict(page_stride=8), {}),
+    (qd.INVALID_ARGUMENT, dict(plane_stride=-16), {}), (qd.INVALID_ARGUMENT, dict(page_stride=8), {}), (qd.INVALID_ARGUMENT, dict(page_stride=0), {}),
     (qd.INVALID_ARGUMENT, dict(plane_stride=0), {}), (qd.NOT_SUPPORTED, dict(pieces=1 << 28, planes=1), {}),
     (qd.NOT_SUPPORTED, dict(pieces=1 << 26, planes=1), dict(rows=65535))])
 def test_commit_refusals(status, memory, changes):

@@ -105,6 +105,44 @@ def test_tree_attention_of_cut_rows(dtype, heads, kv_heads, dim, nodes, lengths)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,nodes,page", [(2, 2, 64, 3, 16), (8, 2, 128, 4, 32), (8, 4, 64, 5, 64), (7, 1, 128, 9, 16)])
+def test_tree_attention_of_many_rows(dtype, heads, kv_heads, dim, nodes, page):
+    """Dealt in equal runs, cut where they end; rows that are bad spoil no others."""
+    say("tree attention, many rows", dtype, heads, kv_heads, dim, nodes, page)
+    g, rows = seeded(heads), 300 // kv_heads
+    lengths = [int(n) for n in torch.randint(0, 500, (rows,), generator=g)]
+    lengths[7], lengths[rows - 1], lengths[11] = 2900, 1700, 0
+    lengths = [n if n >= nodes else 0 for n in lengths]
+    table, pages = tables_for(g, lengths, page, -(-2900 // page))
+    k, v = pool(g, pages, page, kv_heads, dim, dtype)
+    q = normal(g, (rows, nodes, heads, dim), dtype, 1.5)
+    parents = some_trees(g, rows, nodes)
+    parents[7] = int32(tree(g, nodes))
+    some = [0, 1, 2, 3, 4, 5, 6, 7, 8, 11, 12, 50, rows - 2, rows - 1]
+    want, bound = oracle.tree_attention(q[some], k, v, table[some], [lengths[r] for r in some], parents[some], 0.1)
+    close(run_tree(q, k, v, table, lengths, parents, 0.1)[some], want, bound, "out")
+    table[9, 0], lengths[10], parents[13, -1] = pages, -4, nodes
+    lengths[9] = max(lengths[9], nodes)
+    lengths[13] = max(lengths[13], nodes)
+    table[13, : -(-lengths[13] // page)] = table[7, : -(-lengths[13] // page)]
+    got = run_tree(q, k, v, table, lengths, parents, 0.1, errors=ops.BAD_PAGE | ops.BAD_LENGTH | ops.BAD_PARENT)
+    close(got[some], want, bound, "out beside bad rows")
+    assert torch.isnan(got[[9, 10, 13]]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+def test_scales_of_any_sign(dtype, scale):
+    g, nodes, page, lengths = seeded(3), 9, 16, [150, 9]
+    table, pages = tables_for(g, lengths, page, 10)
+    k, v = pool(g, pages, page, 2, 64, dtype)
+    q = normal(g, (2, nodes, 6, 64), dtype, 1.5)
+    parents = some_trees(g, 2, nodes)
+    want, bound = oracle.tree_attention(q, k, v, table, lengths, parents, scale)
+    close(run_tree(q, k, v, table, lengths, parents, scale), want, bound, "out")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("length", [70, 1500])
 @pytest.mark.parametrize("bad", [NAN, math.inf, -math.inf])
 def test_what_is_not_seen_may_be_anything(dtype, length, bad):
@@ -366,12 +404,12 @@ def test_accept_drawn_tokens(dtype, rows, nodes, vocab, temperature):
 
 
 def test_draws_at_the_ends():
-    """0 is the first token that has a probability, just below 1 the last one, 1 and more too."""
-    logits = torch.full((4, 1, 5001), -math.inf)
+    """0 is the first token that has a probability, and so is less; just below 1 the last one, 1 and more too."""
+    logits = torch.full((6, 1, 5001), -math.inf)
     logits[:, 0, [17, 4000, 4999]] = torch.tensor([0.0, 1.0, -1.0])
-    draws = torch.tensor([[0.0], [1 - 2.0 ** -24], [1.0], [2.0]])
-    parents, tokens = int32([[-1]] * 4), int32([[0]] * 4)
-    assert run_accept(logits, tokens, parents, draws)[2].tolist() == [17, 4999, 4999, 4999]
+    draws = torch.tensor([[0.0], [1 - 2.0 ** -24], [1.0], [2.0], [-1.0], [NAN]])
+    parents, tokens = int32([[-1]] * 6), int32([[0]] * 6)
+    assert run_accept(logits, tokens, parents, draws)[2].tolist() == [17, 4999, 4999, 4999, 17, 17]
 
 
 @pytest.mark.parametrize("sampled", [False, True])
@@ -483,6 +521,17 @@ def test_commit(dtype, nodes, page):
     assert out == [n - nodes + int(k) if n else 0 for n, k in zip(lengths, counts)]
     for x, y in zip((a, b, c), tensors):
         assert torch.equal(y.cpu(), committed(x, table, lengths, path, counts, page))
+
+
+def test_commit_of_a_path_over_page_ends():
+    """Every source a page behind its target, each target the source of the move before."""
+    g, page, nodes = seeded(3), 16, 64
+    table, pages = tables_for(g, [90], page, 6)
+    x = normal(g, (24, pages, page, 1, 64), F32)
+    y = x.cuda()
+    path, counts = int32([[*range(16, 64)] + [-1] * 16]), int32([48])
+    assert run_commit(ops.TokenMemory([y]), table, [90], path, counts) == [74]
+    assert torch.equal(y.cpu(), committed(x, table, [90], path, counts, page))
 
 
 def test_commit_without_planes():
