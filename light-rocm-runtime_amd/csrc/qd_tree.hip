@@ -58,8 +58,15 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t *parents, uint32_t n
 // mask says so. What does not is hidden from the sum by its score, and by zeros in V's
 // place where V is not finite: the outputs that do see such a value become NaN.
 // Few rows are cut into runs that fill the card, which the last one joins in order.
+// 64 BF16 rows of 0 to 8,192 with 8 nodes of 4 heads on 8 KV heads of 128 take 212 us, 1,087 MB at
+// 5.1 TB/s, bound by memory and by what ends a piece (187 us without results and joins); two FP16 rows of
+// 30,001 to 40,001 with 63 nodes of 7 on 4 KV heads 140 us, 63 GFLOP at 0.45 PFLOP/s, bound by the
+// sum of products and the exponentials' vector work, which overlap little (without K's half of a stage
+// 96 us, without V's 100, without either 77; without the second number of a weight 117). 16 FP32 rows
+// of 576 with 16 nodes of 7 on 2 heads of 64 19 us, one of 129 with 8 12.4: a chain of latencies.
 constexpr int kStep = 32;                // positions of a wave's step
 constexpr uint32_t kTreePieces = 64;     // of an item at most
+// (128: one row of 129 with 8 nodes 15.0 us instead of 12.5, 16 of 576 with 16 19.3 and 19.1)
 constexpr uint32_t kTreeLeast = 64;      // positions of a piece at least
 constexpr uint32_t kTreeCus = 256, kTreePerCu = 4, kXcds = 8;
 constexpr uint32_t kLds = 160 * 1024;
@@ -145,11 +152,13 @@ struct TreeShape {
   static constexpr int kStage = kStep * WP;
   static constexpr int kRowBytes = D * kElem;
   static constexpr int kHalf = kStage * kRowBytes;  // K or V of a stage
-  // So many of them in LDS. Where memory is what bounds a stage they are waited for one by one
-  // and all but one are on their way, 128 KB to a CU with two workgroups (96: 64 rows of 0 to
-  // 8,192 with 8 nodes 260 us); where products do, by stages, three of them on their way.
-  static constexpr bool kByHalves = WP == 1;
-  static constexpr int kHalves = !kByHalves ? 8 : kRowBytes == 512 ? 4 : kRowBytes == 256 ? 5 : 9;
+  // So many of them in LDS. Up to 64 columns they are waited for one by one and all but one are
+  // on their way, to three workgroups of a CU (five halves of 8 KB; nine and two workgroups: 64
+  // rows of 0 to 8,192 with 8 nodes 227 us instead of 212); where products bound a stage, by
+  // stages, three of them on their way.
+  static constexpr bool kWhole = WP > 1;
+  static constexpr bool kByHalves = !kWhole;
+  static constexpr int kHalves = kWhole ? 8 : kRowBytes == 512 ? 4 : kRowBytes == 256 ? 5 : 9;
   static constexpr int kColumns = 16 * NB * WC;
   static constexpr int kRowsPerDma = 1024 / kRowBytes, kLanesPerRow = kRowBytes / 16;
   static constexpr int kRows = kStage / kWaves;                // of a half, that a wave transfers
@@ -159,7 +168,9 @@ struct TreeShape {
   static constexpr int kMerge = WP > 1 ? WC * NB * (kAcc * 1024 + 512) : 0;
   static constexpr int kBytes = std::max(kHalves * kHalf, kMerge);
   static constexpr uint32_t kRecord = kColumns * (D + 2);  // floats
-  static constexpr int kPerCu = kWaves == 8 ? 1 : std::min(NB == 2 ? 2 : 4, static_cast<int>(kLds) / (kBytes + 2048));
+  // Workgroups of a CU that pieces are made for (four: 16 FP16 rows of 513 to 4,000 with 9 nodes of 7
+  // heads of 64 34.2 us, three 28.3).
+  static constexpr int kPerCu = std::min(kWhole ? 1 : 3, static_cast<int>(kLds) / (kBytes + 2048));
   static_assert(WP <= 2 && kDmas >= 1 && kDmas * kRowsPerDma * kWaves == kStage, "whole transfers");
   static_assert((kHalves - 2) * kDmas < 64, "the wait's count");
   static_assert(kBytes + 2048 <= static_cast<int>(kLds) && kPerCu <= static_cast<int>(kTreePerCu), "LDS");
@@ -782,7 +793,7 @@ __global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunc
     return x;
   };
   // (A stage of two waves has no runs: its columns are so many that products bound it.)
-  const bool single = WP > 1 || p.units;
+  const bool single = S::kWhole || p.units;
   Deal deal{};
   Item item{};
   if (single) {
@@ -845,8 +856,13 @@ struct TreePlan {
   uint32_t group, columns, blocks, rec_floats, apart, target, records;
 };
 
-// Calls f with the shape and kernel for so many columns: as many of them to a workgroup as there
-// are, by steps that the kernels come in.
+// Calls f with the shape and kernel for so many columns. A wave of 32 columns has 340 registers and
+// its SIMD to itself, which only more than 64 columns make up for (64 BF16 rows of 0 to 8,192, 8 KV heads
+// of 128: 64 columns by four waves of 16 253 us, by two of 32 319, by the eight of 128 columns 294; 128
+// columns by those 312, as two blocks of four waves 410; two rows of 1,000: 64 columns 18.5, 31 and 26,
+// 128 28 and 21.5). Up to 32 columns two waves (16 columns by one wave 203 us and 18.0, by these
+// 212 and 17.3; FP32, 16 rows of 513 to 4,000 with 14 columns 31.7 and 28.9; 28 columns by four 30.1,
+// by two 29.0).
 template <typename E, int D, typename F>
 auto with_shape(uint32_t columns, F &&f) {
   const auto shape = [&](auto nb, auto wc, auto wp) {
@@ -856,12 +872,11 @@ auto with_shape(uint32_t columns, F &&f) {
   std::integral_constant<int, 1> one;
   std::integral_constant<int, 2> two;
   std::integral_constant<int, 4> four;
-  if (columns <= 16) return shape(one, one, one);
   if (columns <= 32) return shape(one, two, one);
   if constexpr (std::is_same_v<E, float>) {
     return shape(one, four, one);
   } else {
-    return columns <= 64 ? shape(two, two, one) : shape(two, four, two);
+    return columns <= 64 ? shape(one, four, one) : shape(two, four, two);
   }
 }
 template <typename F>
@@ -895,10 +910,13 @@ TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_he
 // share of a row to arrive finds each node's largest and walks the tree; with draws the last
 // share of a node finds the quarter in which the running sum passes the draw, reads that one
 // again and picks the token, and the last node of a row walks. Bound by memory for large
-// batches, by the chain of hand-overs for small ones.
+// batches (16 drawn trees of 16 over 151,936 tokens in FP32, 130 MB, 38 us; arithmetic left out
+// changed nothing), by the chain of hand-overs for small ones (a tree of 8 6.5 us).
 constexpr int kAcceptT = 256, kAcceptWaves = kAcceptT / kWave;
 constexpr uint32_t kAcceptShares = 64;    // of a node at most: a lane each
+// (1,024: 16 drawn trees of 16 41 us instead of 38, 4,096 44)
 constexpr uint32_t kAcceptAim = 2048;     // shares in all
+// (4,096: one tree of 8 9.1 us instead of 6.5, 8,192 6.9, 32,768 7.3: arrivals at one counter)
 constexpr uint32_t kAcceptLeast = 16384;  // logits of a share at least
 constexpr float kHuge = 1e30f;            // logits past it are not exponentiated
 
@@ -1293,8 +1311,9 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
 // ---- commit --------------------------------------------------------------------------
 // Lane n of every wave looks up node n's move; a workgroup takes 64 columns of 16 bytes of
 // one row, its waves every fourth move, and stores when all of them are loaded: a move's
-// target is an earlier move's source. Bound by memory for large trees, else by the chain
-// length, path, page, load, store.
+// target is an earlier move's source. Bound by memory for large trees (64 of 63 nodes, 8 layers of 8 heads
+// of 128 in BF16, 70 MB read and written, 16.7 us: 4.2 TB/s), else by the chain length, path, page,
+// load, store (16 of 16, 24 layers of 2 of 64 in FP32, 4.9 us).
 constexpr int kCommitT = 256;
 constexpr int kMovesPerWave = 64 / (kCommitT / kWave);
 struct CommitLaunch {
@@ -1427,7 +1446,10 @@ hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const q
     if (p.target) x = std::min<uint64_t>(4 * x <= p.target ? x + p.target : x + 4 * p.target, x * most);
     p.units = static_cast<uint32_t>(x);
     uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.parts;
-    // Many rows whose items read nothing twice: equal runs. (Stages are counted in 31 bits.)
+    // Many rows whose items read nothing twice: equal runs (64 BF16 rows of 0 to 8,192 with 16 columns
+    // 203 us, in pieces 229, with 32 212 and 234; for few rows their two halves of a record cost more
+    // than they even out: two of 1,000 24.5 us, in pieces 17.4, 16 FP32 of 513 to 4,000 33 and 29).
+    // (Stages are counted in 31 bits.)
     const uint64_t stages = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + S::kStage - 1) / S::kStage;
     if (S::kByHalves && p.target && p.blocks == 1 && 4ull * c.rows > p.target && c.rows * p.parts * (stages + kEdge) <= 0x7f000000u) {
       p.units = 0;
