@@ -82,15 +82,20 @@ __device__ __forceinline__ float4 turn4(float4 x, float4 y, float4 c, float4 s, 
   return a;
 }
 
-template <typename E>
+// (kSlots: tokens go where p.slots says. The others look no further: 16 tokens 3.1 us, with a test of
+// the pointer 3.6.)
+template <typename E, bool kSlots>
 __global__ __launch_bounds__(kBlock) void append_kernel(AppendLaunch p) {
   const uint32_t id = blockIdx.x * kWavesPerBlock + __builtin_amdgcn_readfirstlane(wave_id());
   const uint32_t token = id / p.waves;
   if (token >= p.a.tokens) return;
   const int64_t position = static_cast<int64_t>(load_uniform(p.a.positions + token)) + p.a.position_bias;
   if (position < 0) return;
-  const int64_t place = p.slots ? static_cast<int64_t>(load_uniform(p.slots + token)) + p.a.position_bias : position;
-  if (place < 0) return;
+  int64_t place = position;
+  if constexpr (kSlots) {
+    place = static_cast<int64_t>(load_uniform(p.slots + token)) + p.a.position_bias;
+    if (place < 0) return;
+  }
   const uint32_t dim = p.c.head_dim, lane = lane_id();
   const uint32_t heads = p.a.q ? p.a.heads : 0, all = heads + 2 * p.c.kv_heads;  // queries, then keys, then values
   const uint32_t j = (id - token * p.waves) * (kWave >> p.lanes_shift) + (lane >> p.lanes_shift);  // this lane's row
@@ -417,7 +422,9 @@ struct AttnShared {
   uint32_t spoilt, last;
 };
 
-template <typename E, int D, int kStages, int kPolicy, bool kEarly>
+// kOwn: each KV head has a table of its own (p.head_table apart). (One row of 129 positions 6.55 us,
+// with that distance looked at in every call 7.1.)
+template <typename E, int D, int kStages, int kPolicy, bool kEarly, bool kOwn>
 struct Attention {
   static_assert(!kEarly || kStages == 1, "one stage");
   using Tiles = WaveTiles<E, D, kStages, kEarly>;
@@ -482,9 +489,9 @@ struct Attention {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const uint32_t pos = at * kTile + s * kSub;
-      id[s] = at < x.last && pos < static_cast<uint32_t>(x.length)
-                  ? load_uniform(p.c.table + x.row * p.c.table_stride + x.part / p.blocks * p.head_table + (pos >> p.page_shift))
-                  : -1;
+      const int32_t *table = p.c.table + x.row * p.c.table_stride;
+      if constexpr (kOwn) table += x.part / p.blocks * p.head_table;
+      id[s] = at < x.last && pos < static_cast<uint32_t>(x.length) ? load_uniform(table + (pos >> p.page_shift)) : -1;
     }
   }
   // The queries and the first tiles of a run are on their way when this returns.
@@ -767,7 +774,7 @@ constexpr uint32_t short_per_cu(uint32_t head_dim) { return head_dim == 128 ? 2 
 // Few positions in all: a workgroup per piece, no more than `target` pieces
 // besides one for each item. Short code and one dependent load less, because each
 // step of such a call waits for the one before it.
-template <typename E, int D>
+template <typename E, int D, bool kOwn>
 __global__ __launch_bounds__(kWaves *kWave, short_per_cu(D)) void attention_short_kernel(AttnLaunch p) {
   __shared__ AttnShared<E, D, 1> sh;
   Item it;
@@ -775,7 +782,7 @@ __global__ __launch_bounds__(kWaves *kWave, short_per_cu(D)) void attention_shor
   uint32_t begin;
   if (!find_piece(p, blockIdx.x / p.parts, part, it, begin)) return;
   if (threadIdx.x == 0) sh.spoilt = 0u;
-  Attention<E, D, 1, 0, D == 64> a(p, sh);
+  Attention<E, D, 1, 0, D == 64, kOwn> a(p, sh);
   bool bad = false;
   a.begin(it, bad);
   a.run(it, bad);
@@ -792,7 +799,7 @@ __global__ __launch_bounds__(kWaves *kWave, short_per_cu(D)) void attention_shor
 // as a stream, as so much is not read again before others have taken its place: 16 rows
 // of 2,000 to 4,000 of one layer after the other 45.6 us, by the caches 48.6 (of one
 // layer again and again, 208 MB, 40.0 and 38.6), 64 of 0 to 8,192 182 and 202.
-template <typename E, int D, int kStages>
+template <typename E, int D, int kStages, bool kOwn>
 __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunch p) {
   __shared__ AttnShared<E, D, kStages> sh;
   const uint32_t group_id = blockIdx.x;
@@ -800,7 +807,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attention_long_kernel(AttnLaunc
   Item it;
   if (!first_item<kTile>(p, group_id, gridDim.x, deal, it)) return;
   if (threadIdx.x == 0) sh.spoilt = 0u;
-  Attention<E, D, kStages, kPolicyNt, false> a(p, sh);
+  Attention<E, D, kStages, kPolicyNt, false, kOwn> a(p, sh);
   // The record of an item's piece: its workgroup's first if it begins inside the item, else the second.
   auto record_of = [&](const Item &x, uint32_t piece) {
     return p.records + (2 * static_cast<size_t>(x.home + piece) + (piece == 0)) * p.rec_floats;
@@ -1195,10 +1202,11 @@ hipError_t launch_paged_append(hipStream_t s, const qd_paged_cache &c, const qd_
   p.waves = (rows + at_once - 1) / at_once;
   const dim3 grid((static_cast<uint64_t>(a.tokens) * p.waves + kWavesPerBlock - 1) / kWavesPerBlock);
   const dim3 block(kBlock);
+  const auto run = [&](auto plain, auto slotted) { return launch(slots ? slotted : plain, grid, block, s, p); };
   switch (c.dtype) {
-    case QD_DTYPE_F32: return launch(append_kernel<float>, grid, block, s, p);
-    case QD_DTYPE_BF16: return launch(append_kernel<Brain>, grid, block, s, p);
-    default: return launch(append_kernel<Half>, grid, block, s, p);
+    case QD_DTYPE_F32: return run(append_kernel<float, false>, append_kernel<float, true>);
+    case QD_DTYPE_BF16: return run(append_kernel<Brain, false>, append_kernel<Brain, true>);
+    default: return run(append_kernel<Half, false>, append_kernel<Half, true>);
   }
 }
 
@@ -1230,9 +1238,9 @@ static hipError_t launch_attention(hipStream_t s, AttnLaunch &p) {
     if (most <= kShortWhole) p.target = 0;
     uint64_t x = p.c.rows;
     if (p.target) x = std::min<uint64_t>(x + p.target, x * ((most + kShortLeast - 1) / kShortLeast));
-    return launch(attention_short_kernel<E, D>, dim3(static_cast<uint32_t>(x * p.parts)), block, s, p);
+    return launch(p.head_table ? attention_short_kernel<E, D, true> : attention_short_kernel<E, D, false>, dim3(static_cast<uint32_t>(x * p.parts)), block, s, p);
   }
-  return launch(attention_long_kernel<E, D, kStages>, dim3(kCus * per_cu), block, s, p);
+  return launch(p.head_table ? attention_long_kernel<E, D, kStages, true> : attention_long_kernel<E, D, kStages, false>, dim3(kCus * per_cu), block, s, p);
 }
 
 hipError_t launch_paged_attention(hipStream_t s, const qd_paged_cache &c, const qd_attention_args &a, const OpScratch &w,
