@@ -104,7 +104,8 @@ struct TreeLaunch {
 // inline assembly: the compiler would guard every later LDS read with a wait for it.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: set before each use, never saved
-// (lds and base are the wave's: the compiler is told where it cannot see it.)
+// (lds and base are the wave's: the compiler is told where it cannot see it, by a vector instruction
+// that writes scalar registers. A transfer may read those five wait states later.)
 __device__ __forceinline__ void dma_to_lds(const void *src, uint32_t lds) {
   lds = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
@@ -114,7 +115,7 @@ __device__ __forceinline__ void dma_to_lds(const void *base, uint32_t off, uint3
   const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
   base = reinterpret_cast<const void *>(static_cast<uint64_t>(hi) << 32 | lo);
   lds = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 // Waits until at most kEach x `left` of this wave's transfers are on their way.
