@@ -3,6 +3,7 @@ device work, the layout of their structures, the sizes of their workspaces, and 
 oracle's tree and choice are what they say."""
 import ctypes as C
 import math
+import os
 import random
 import re
 
@@ -206,6 +207,14 @@ def test_arguments_that_are_something_else_are_refused():
             (lambda: ops.paged_append(c, None, None, k[0, :1], k[0, :1], lengths, slots=lengths.long()), "slots has type")):
         with pytest.raises(qd.QdError, match=text):
             call()
+
+
+def test_transfers_wait_for_scalar_registers_of_vector_instructions():
+    """A transfer whose address is in scalar registers, which a vector instruction may have written right before:
+    five wait states between them."""
+    text = open(os.path.join(os.path.dirname(HEADER), "..", "..", "light-rocm-runtime_amd", "csrc", "qd_tree.hip")).read()
+    found = re.findall(r's_nop (\d+)\\n\\tglobal_load_lds_dwordx4 %1, %2', text)
+    assert found and all(int(n) >= 4 for n in found)
 
 
 def test_oracle_chains_and_choices():
