@@ -7,7 +7,9 @@
  * pages (qd_paged_append), one new token per row attends over its pages
  * (qd_paged_attention), and the best continuations are chosen from logits and
  * scores (qd_beam_select). qd_generate_beams (qwen_decode.h) runs a whole
- * search of an engine's model through them.
+ * search of an engine's model through them. Beside them: several drafted tokens
+ * per row at once (qd_tree_attention, qd_tree_accept, qd_tree_commit), and
+ * attention over a part of a long cache (qd_page_bounds, qd_sparse_attention).
  *
  * Conventions:
  *   - pointers are device memory unless they say host; sizes and strides are
@@ -52,7 +54,7 @@ enum {
 };
 
 /* ---- workspace --------------------------------------------------------------
- * Device memory that attention, fork and select keep partial results in. Its
+ * Device memory that attention, fork, select and accept keep partial results in. Its
  * owner allocates one of the largest size its calls ask for and may pass it to
  * any of them, but to one call at a time: calls on the same stream, or graphs
  * replayed on the same stream, follow each other; work that may run at the same
