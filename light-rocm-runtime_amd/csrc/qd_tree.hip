@@ -68,7 +68,7 @@ constexpr int kStep = 32;                // positions of a wave's step
 constexpr uint32_t kTreePieces = 64;     // of an item at most
 // (128: one row of 129 with 8 nodes 15.0 us instead of 12.5, 16 of 576 with 16 19.3 and 19.1)
 constexpr uint32_t kTreeLeast = 64;      // positions of a piece at least
-constexpr uint32_t kTreeCus = 256, kTreePerCu = 4, kXcds = 8;
+constexpr uint32_t kTreeCus = 256, kTreePerCu = 3, kXcds = 8;
 constexpr uint32_t kLds = 160 * 1024;
 // A maximum is taken up once it passes the one in use by so many powers of two, as in the
 // attention of one token (qd_paged.hip).
