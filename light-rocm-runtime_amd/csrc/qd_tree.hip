@@ -920,6 +920,8 @@ constexpr uint32_t kAcceptAim = 2048;     // shares in all
 // (4,096: one tree of 8 9.1 us instead of 6.5, 8,192 6.9, 32,768 7.3: arrivals at one counter)
 constexpr uint32_t kAcceptLeast = 16384;  // logits of a share at least
 constexpr float kHuge = 1e30f;            // logits past it are not exponentiated
+// Where the largest logit's x c is past this either way, sums are relative to that logit, not to a whole number.
+constexpr float kFar = 0x1p22f;
 
 struct AcceptShare {
   double sum[kAcceptWaves];  // of 2^(x c - r), r the whole number above the largest logit's x c
@@ -935,6 +937,7 @@ struct AcceptLaunch {
   uint32_t apart;       // words between two counters
   uint32_t shares;
   float c_hi, c_lo;     // log2(e) / temperature
+  float most;           // 2 kFar / c
 };
 
 // A row's logit i as FP32.
@@ -947,12 +950,19 @@ __device__ __forceinline__ float logit(const void *row, uint32_t i) {
     return E::lo(v);
   }
 }
-// 2^(x c - r), where x c is computed to about 2^-46 of it. NaN and what is below -1e30 give 0.
-__device__ __forceinline__ float power(float x, float c_hi, float c_lo, float r) {
-  x = fmaxf(x, -kHuge);
-  const float hi = x * c_hi, lo = fmaf(x, c_lo, fmaf(x, c_hi, -hi));
+// The whole number above x c, of a sum whose largest logit is x. Logits count as +-2 kFar / c where they are past it, -inf
+// and NaN too: x c is at least kFar below the largest then, and the number has FP32's 24 bits.
+__device__ __forceinline__ float whole_above(const AcceptLaunch &p, float x) {
+  return ceilf(fminf(fmaxf(x, -p.most), p.most) * p.c_hi);
+}
+// 2^(x c - r), x no larger than the logit that r stands above.
+__device__ __forceinline__ float power(const AcceptLaunch &p, float x, float r) {
+  x = fmaxf(x, -p.most);
+  const float hi = x * p.c_hi, lo = fmaf(x, p.c_lo, fmaf(x, p.c_hi, -hi));
   return exp2_fast((hi - r) + lo);
 }
+// The same relative to the largest logit itself: where x c is past kFar, differences of logits are what is exact.
+__device__ __forceinline__ float power_far(const AcceptLaunch &p, float x, float top) { return exp2_fast((fmaxf(x, -INFINITY) - top) * p.c_hi); }
 __device__ __forceinline__ double scaled(double s, float by) { return ldexp(s, static_cast<int>(fmaxf(by, -4000.f))); }
 // Sum over the lanes up to this one.
 __device__ __forceinline__ double lanes_upto(double v) {
@@ -1035,7 +1045,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
   float top = -INFINITY;
   uint32_t best = UINT32_MAX;
   double sum = 0.0;
-  float r = -INFINITY;  // (a whole number)
+  float r = kSampled ? whole_above(p, -INFINITY) : 0.f;
   const auto take = [&](float y, uint32_t i) {
     if (y > top) {
       top = y;
@@ -1046,9 +1056,9 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
   const auto raise = [&](float most) {
     if (most > top) {
       top = most;
-      const float up = ceilf(fminf(most, kHuge) * p.c_hi);
+      const float up = whole_above(p, most);
       if (up > r) {
-        sum = r == -INFINITY ? 0.0 : scaled(sum, r - up);
+        sum = scaled(sum, r - up);
         r = up;
       }
     }
@@ -1056,8 +1066,8 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
   const auto single = [&](uint32_t i) {
     const float y = logit<E>(x.x, i);
     if constexpr (kSampled) {
-      raise(fmaxf(y, -kHuge));
-      sum += power(y, p.c_hi, p.c_lo, r);
+      raise(y);
+      sum += power(p, y, r);
     } else {
       take(y, i);
     }
@@ -1069,7 +1079,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
     for (int u = 0; u < kAhead; ++u) now[u] = v[u];
     if (j + kAhead * kWave < to) fetch(j + kAhead * kWave);
     if constexpr (kSampled) {
-      float most = -kHuge;
+      float most = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         float y[kPer];
@@ -1084,7 +1094,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
         float y[kPer], s = 0.f;
         Row::values(now[u], y);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) s += power(y[i], p.c_hi, p.c_lo, r);
+        for (int i = 0; i < kPer; ++i) s += power(p, y[i], r);
         sum += s;
       }
     } else {
@@ -1112,7 +1122,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
     float all = tops[0];
 #pragma unroll
     for (int u = 1; u < kAcceptWaves; ++u) all = fmaxf(all, tops[u]);
-    double s = r == -INFINITY ? 0.0 : scaled(sum, r - ceilf(fminf(all, kHuge) * p.c_hi));
+    double s = scaled(sum, r - whole_above(p, all));
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1) s += lane_of(s, lane ^ step);
     if (lane == 0) {
@@ -1194,7 +1204,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       }
     }
     const float all = wave_max(most);
-    if (!(all > -kHuge && all < kHuge)) {
+    if (!(fabsf(all) < kHuge)) {
       // The largest logit, read again by the whole workgroup.
       top = -INFINITY;
       best = UINT32_MAX;
@@ -1209,13 +1219,15 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       __syncthreads();
       if (threadIdx.x == 0) picks[0] = ids[0] == UINT32_MAX ? 0 : static_cast<int32_t>(ids[0]);
     } else {
-      const float up = ceilf(all * p.c_hi), by = ceilf(fminf(most, kHuge) * p.c_hi) - up;
+      const bool far = fabsf(all) * p.c_hi >= kFar;  // (then all of the node's logits are read again)
+      const float up = whole_above(p, all), by = whole_above(p, most) - up;
 #pragma unroll
       for (int u = 0; u < kAcceptWaves; ++u) {
         part[u] = scaled(part[u], by);
         s += part[u];
       }
-      const double upto = lanes_upto(s), aim = static_cast<double>(fmaxf(p.a.draws[at + node], 0.f)) * lane_of(upto, kWave - 1);
+      const double upto = lanes_upto(s), draw = fmaxf(p.a.draws[at + node], 0.f);
+      double aim = draw * lane_of(upto, kWave - 1);
       const uint64_t past = __ballot(upto > aim), some = __ballot(s > 0.0);
       // (A draw of 1 or more passes nothing: the last share with a token.)
       const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(some));
@@ -1232,23 +1244,24 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
         }
         before += y;
       }
-      const uint32_t q = in * kAcceptWaves + which, a0 = x.first(q), b0 = x.first(q + 1);
+      const uint32_t q = in * kAcceptWaves + which, a0 = far ? 0 : x.first(q), b0 = far ? x.pieces : x.first(q + 1);
       // Its logits again, a run of pieces each thread; what lies before and behind the pieces with the first and last thread.
       const uint32_t n = (b0 - a0 + kAcceptT - 1) / kAcceptT, a = min(b0, a0 + threadIdx.x * n), b = min(b0, a + n);
-      const uint32_t begin = q == 0 && threadIdx.x == 0 ? 0 : x.token(a);
-      const uint32_t end = q + 1 == p.shares * kAcceptWaves && threadIdx.x == kAcceptT - 1 ? p.a.vocab : x.token(b);
+      const uint32_t begin = (far || q == 0) && threadIdx.x == 0 ? 0 : x.token(a);
+      const uint32_t end = (far || q + 1 == p.shares * kAcceptWaves) && threadIdx.x == kAcceptT - 1 ? p.a.vocab : x.token(b);
+      const auto weight = [&](float y) { return far ? power_far(p, y, all) : power(p, y, up); };
       const auto each = [&](auto f) {  // f(token, probability), until it says so
         for (uint32_t i = begin; i < x.token(a) && i < end; ++i)
-          if (f(i, power(logit<E>(x.x, i), p.c_hi, p.c_lo, up))) return;
+          if (f(i, weight(logit<E>(x.x, i)))) return;
         for (uint32_t k = a; k < b; ++k) {
           float y[kPer];
           Row::values(x.load(k), y);
 #pragma unroll
           for (int i = 0; i < kPer; ++i)
-            if (f(x.token(k) + i, power(y[i], p.c_hi, p.c_lo, up))) return;
+            if (f(x.token(k) + i, weight(y[i]))) return;
         }
         for (uint32_t i = x.token(b); i < end; ++i)
-          if (f(i, power(logit<E>(x.x, i), p.c_hi, p.c_lo, up))) return;
+          if (f(i, weight(logit<E>(x.x, i)))) return;
       };
       double run = 0.0;
       each([&](uint32_t, float y) {
@@ -1259,6 +1272,10 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       __syncthreads();
       if (lane == kWave - 1) sums[w] = wave_upto;
       __syncthreads();
+      if (far) {
+        begins = 0.0;
+        aim = draw * ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+      }
       double mine_before = begins + (wave_upto - run);
       for (int u = 0; u < w; ++u) mine_before += sums[u];
       // The first thread whose run passes the draw, or the last with a token.
@@ -1482,6 +1499,7 @@ hipError_t launch_tree_accept(hipStream_t s, const qd_accept_args &a, const OpSc
     const double c = 1.4426950408889634074 / a.temperature;
     p.c_hi = static_cast<float>(c);
     p.c_lo = static_cast<float>(c - p.c_hi);
+    p.most = static_cast<float>(2.0 * kFar / c);
   }
   const dim3 grid(p.shares, static_cast<uint32_t>(all)), block(kAcceptT);
   const auto run = [&](auto greedy, auto sampled) { return launch(a.draws ? sampled : greedy, grid, block, s, p); };

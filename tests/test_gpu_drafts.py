@@ -412,6 +412,93 @@ def test_draws_at_the_ends():
     assert run_accept(logits, tokens, parents, draws)[2].tolist() == [17, 4999, 4999, 4999, 17, 17]
 
 
+TEMPERATURES = [float(torch.tensor(t)) for t in (0.05, 0.1, 0.2, 0.4, 0.5, 0.7, 0.75, 0.8, 0.85, 0.9, 1.0, 1.3, 1.5, 2.0)]
+
+
+def running_sums(x, temperature):
+    """Of rows [n, vocab]: each token's probability, the largest 1, their running sums, and how far two of those may be
+    off: p = 2^-d by (1.8 d + 4) 2^-24 of it, eight of them in FP32 by 3 x 2^-24 more."""
+    x = x.cuda().double()
+    x = torch.where(torch.isnan(x), -math.inf, x)
+    d = (x.amax(-1, keepdim=True) - x) / temperature / math.log(2)
+    p = torch.exp2(-d)
+    off = torch.where(p > 0, p * (1.8 * d + 7), 0.0).sum(-1) * 2.0 ** -24
+    return p, torch.cumsum(p, -1), 2 * off
+
+
+def draw_one_each(logits, draws, temperature):
+    """The tokens that follow trees of one node: logits [n, vocab], draws [n]."""
+    n = logits.shape[0]
+    return run_accept(logits[:, None], int32([[0]] * n), int32([[-1]] * n), draws[:, None].float(), temperature)[2].cuda().long()
+
+
+def check_draws(logits, draws, temperature, got):
+    p, upto, off = running_sums(logits, temperature)
+    n, vocab = p.shape
+    assert ((got >= 0) & (got < vocab)).all(), got
+    row, total = torch.arange(n, device="cuda"), upto[:, -1]
+    aim = draws.cuda().double().nan_to_num(nan=0.0).clamp(0, 1) * total
+    last = vocab - 1 - (p > 0).flip(-1).to(torch.uint8).argmax(-1)
+    assert (p[row, got] > 0).all(), "a token without a probability"
+    assert torch.equal(got[draws.cuda() >= 1], last[draws.cuda() >= 1])
+    assert ((upto[row, got] > aim - off) | (got == last)).all()
+    assert (upto[row, got] - p[row, got] <= aim + off).all()
+
+
+def middles(g, logits, temperature):
+    """A draw in the middle of a token of each row that has 2^-14 of the probability or more, and the tokens."""
+    p, upto, _ = running_sums(logits, temperature)
+    p, upto = (p / upto[:, -1:]).cpu(), (upto / upto[:, -1:]).cpu()
+    able = [(row > 2.0 ** -14).nonzero()[:, 0] for row in p]
+    token = torch.tensor([int(a[int(torch.randint(0, len(a), (1,), generator=g))]) for a in able])
+    row = torch.arange(len(able))
+    return (upto[row, token] - p[row, token] / 2).float(), token.cuda()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("mask", [-math.inf, "lowest", -1e30, -1e10])
+def test_draws_of_masked_logits(dtype, mask):
+    """Lanes, quarters and shares that hold nothing but masks, at temperatures of either sign of what rounding leaves of
+    their products."""
+    say("draws of masked logits", dtype, mask)
+    g, vocab = seeded(21), 151936
+    mask = torch.finfo(dtype).min if mask == "lowest" else mask
+    keep = torch.zeros(9, vocab, dtype=torch.bool)
+    keep[0, 100000] = True
+    keep[1, torch.randperm(vocab, generator=g)[:40]] = True
+    keep[2, vocab // 2:] = True
+    keep[3, : vocab // 2] = True
+    keep[4] = torch.arange(vocab) // 8 % 64 == 5
+    keep[5, 40000:43000] = True
+    keep[6, -1] = True
+    keep[7, 0] = True
+    keep[8, ::3000] = True
+    x = torch.randn(keep.shape, generator=g) * 0.5
+    x[:, ::1000] += 8.0
+    logits = torch.where(keep, x, mask).to(dtype)
+    for temperature in TEMPERATURES:
+        draws, want = middles(g, logits, temperature)
+        assert torch.equal(draw_one_each(logits, draws, temperature), want), temperature
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_draws_of_logits_of_any_size(dtype):
+    """Logits of many temperatures: ties and neighbours are told apart."""
+    say("draws of any size", dtype)
+    g, vocab = seeded(24), 20001
+    for temperature, scale, base in ((1e-6, 3.0, 0.0), (1e-3, 3.0, 50.0), (1.0, 1.0, 3e6), (1.0, 0.0, -1e10), (1.0, 0.0, 1e20), (0.7, 1e25, 0.0),
+                                     (1e6, 1e5, 0.0), (1e6, 1.0, 1e20), (1.0, 1.0, -1e9)):
+        temperature = float(torch.tensor(temperature))
+        logits = (torch.randn((12, vocab), generator=g) * scale + base).to(dtype)
+        logits[:6, ::2] = -math.inf
+        logits[2, 1:] = -math.inf
+        logits[3, :-1] = -math.inf
+        logits[3, -1] = logits[2, 0] = base
+        draws = torch.rand(12, generator=g)
+        draws[0], draws[1] = 0.0, 1.0
+        check_draws(logits, draws, temperature, draw_one_each(logits, draws, temperature))
+
+
 @pytest.mark.parametrize("sampled", [False, True])
 def test_accept_of_masked_and_infinite_logits(sampled):
     vocab = 9001
