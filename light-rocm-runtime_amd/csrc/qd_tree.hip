@@ -955,13 +955,15 @@ __device__ __forceinline__ float logit(const void *row, uint32_t i) {
 __device__ __forceinline__ float whole_above(const AcceptLaunch &p, float x) {
   return ceilf(fminf(fmaxf(x, -p.most), p.most) * p.c_hi);
 }
-// 2^(x c - r), x no larger than the logit that r stands above.
+// 2^(x c - r), x no larger than the logit that r stands above. Two roundings of an exponent -d, 2^-24 of it each, and the
+// exponential's 2^-23: off by (1.4 d + 4) 2^-24 of itself. (r is subtracted inside: a product that is rounded first can be
+// contracted with what follows, and is then corrected twice.)
 __device__ __forceinline__ float power(const AcceptLaunch &p, float x, float r) {
   x = fmaxf(x, -p.most);
-  const float hi = x * p.c_hi, lo = fmaf(x, p.c_lo, fmaf(x, p.c_hi, -hi));
-  return exp2_fast((hi - r) + lo);
+  return exp2_fast(fmaf(x, p.c_lo, fmaf(x, p.c_hi, -r)));
 }
-// The same relative to the largest logit itself: where x c is past kFar, differences of logits are what is exact.
+// The same relative to the largest logit itself: where x c is past kFar, differences of logits are what is exact. Off by
+// (1.8 d + 2) 2^-24 of itself: the difference, c and their product.
 __device__ __forceinline__ float power_far(const AcceptLaunch &p, float x, float top) { return exp2_fast((fmaxf(x, -INFINITY) - top) * p.c_hi); }
 __device__ __forceinline__ double scaled(double s, float by) { return ldexp(s, static_cast<int>(fmaxf(by, -4000.f))); }
 // Sum over the lanes up to this one.
@@ -1091,11 +1093,16 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (j + u * kWave >= to) break;
-        float y[kPer], s = 0.f;
+        float y[kPer];
         Row::values(now[u], y);
+        // In pairs: three roundings at most.
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) s += power(p, y[i], r);
-        sum += s;
+        for (int i = 0; i < kPer; ++i) y[i] = power(p, y[i], r);
+#pragma unroll
+        for (int step = 1; step < kPer; step *= 2)
+#pragma unroll
+          for (int i = 0; i < kPer; i += 2 * step) y[i] += y[i + step];
+        sum += y[0];
       }
     } else {
 #pragma unroll

@@ -481,6 +481,23 @@ def test_draws_of_masked_logits(dtype, mask):
         assert torch.equal(draw_one_each(logits, draws, temperature), want), temperature
 
 
+@pytest.mark.parametrize("temperature,base", [(0.05, 0.0), (0.05, 30.0), (0.05, -30.0), (0.1, 30.0), (0.7, 20.0), (1.0, 40.0), (1.3, 100.0), (0.7, -300.0)])
+def test_draws_at_the_ends_of_tokens(temperature, base):
+    """Within what sums may be off, to either side of each token's end."""
+    say("draws at the ends of tokens", temperature, base)
+    g, vocab, temperature = seeded(22), 4003, float(torch.tensor(temperature))
+    for _ in range(8):
+        x = torch.full((vocab,), base - 200 * temperature)
+        at = torch.randperm(vocab, generator=g)[:9].sort().values
+        x[at] = base + 2 * temperature * torch.rand(9, generator=g)
+        _, upto, off = running_sums(x[None], temperature)
+        end = (upto[0, at] / upto[0, -1]).cpu()[:-1]
+        by = float(off[0] / upto[0, -1])
+        draws = torch.cat([end * (1 - 4 * by), end * (1 - by), end, end * (1 + by), end * (1 + 4 * by)]).float()
+        logits = x.repeat(len(draws), 1)
+        check_draws(logits, draws, temperature, draw_one_each(logits, draws, temperature))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_draws_of_logits_of_any_size(dtype):
     """Logits of many temperatures: ties and neighbours are told apart."""
