@@ -1234,9 +1234,11 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
         s += part[u];
       }
       const double upto = lanes_upto(s), draw = fmaxf(p.a.draws[at + node], 0.f);
-      double aim = draw * lane_of(upto, kWave - 1);
-      const uint64_t past = __ballot(upto > aim), some = __ballot(s > 0.0);
-      // (A draw of 1 or more passes nothing: the last share with a token.)
+      // A draw of 1 or more passes nothing: the last share with a token, and there the last quarter and token.
+      const auto aim_at = [&](double total) { return draw < 1.0 ? draw * total : static_cast<double>(INFINITY); };
+      double aim = aim_at(lane_of(upto, kWave - 1));
+      // (Lanes add in orders of their own: behind the last share sums may be larger by a rounding.)
+      const uint64_t some = __ballot(s > 0.0), past = __ballot(upto > aim) & some;
       const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(some));
       // Its quarter: the first that passes, or the last with a token.
       double before = lane_of(upto - s, in);
@@ -1281,7 +1283,7 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       __syncthreads();
       if (far) {
         begins = 0.0;
-        aim = draw * ((sums[0] + sums[1]) + (sums[2] + sums[3]));
+        aim = aim_at((sums[0] + sums[1]) + (sums[2] + sums[3]));
       }
       double mine_before = begins + (wave_upto - run);
       for (int u = 0; u < w; ++u) mine_before += sums[u];

@@ -498,6 +498,17 @@ def test_draws_at_the_ends_of_tokens(temperature, base):
         check_draws(logits, draws, temperature, draw_one_each(logits, draws, temperature))
 
 
+def test_draws_of_one_and_almost_one():
+    """Many shares: the last token that has a probability, and never one behind the vocabulary."""
+    say("draws of one")
+    g, vocab, rows, temperature = seeded(23), 151936, 96, float(torch.tensor(0.7))
+    logits = normal(g, (rows, vocab), F32, 3.0)
+    logits[::3, -1000:] = -math.inf
+    logits[1::3, -40000:] = -math.inf
+    draws = torch.tensor([1.0, 1 - 2.0 ** -24, 2.0, math.inf]).repeat(rows // 4)
+    check_draws(logits, draws, temperature, draw_one_each(logits, draws, temperature))
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_draws_of_logits_of_any_size(dtype):
     """Logits of many temperatures: ties and neighbours are told apart."""
