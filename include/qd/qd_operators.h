@@ -325,10 +325,10 @@ QD_API qd_status qd_tree_attention_workspace(uint32_t rows, uint32_t nodes, uint
  * (in FP32, a p_i of 2^-d of the largest off by at most (1.8 d + 4) 2^-24 of itself and sums of
  * up to 8 of them by 3 x 2^-24; sums beyond in 64 bits), so that the tokens that come out are
  * distributed as the model's own. A draw below 0 or NaN
- * counts as 0, one of 1 or more picks the last token that has a probability, which -inf, NaN
- * and what is far below the largest logit have not; where the largest logit is past 1e30
- * either way, the token of the largest logit. A row whose node 0 is not there gets count 0 and
- * -1, and so does one with a bad parent. */
+ * counts as 0, one of 1 or more picks the last token that has a probability, which -inf and
+ * NaN have not; a p_i below 2^-126 of the largest may count as none. Where the largest logit
+ * is past 1e30 either way, the token of the largest logit is picked. A row whose node 0 is
+ * not there gets count 0 and -1, and so does one with a bad parent. */
 typedef struct qd_accept_args {
   const void *logits;      /* [rows][nodes][vocab] */
   int64_t row_stride;

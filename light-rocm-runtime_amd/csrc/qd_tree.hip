@@ -924,10 +924,8 @@ constexpr float kHuge = 1e30f;            // logits past it are not exponentiate
 constexpr float kFar = 0x1p22f;
 
 struct AcceptShare {
-  double sum[kAcceptWaves];  // of 2^(x c - r), r the whole number above the largest logit's x c
-  float top;                 // the largest logit
-  uint32_t id;               // greedy: its token
-  uint32_t pad[2];
+  double sum[kAcceptWaves];  // each wave's, of 2^(x c - r), r the whole number above the x c of
+  float top[kAcceptWaves];   // its largest logit. Greedy: the share's largest, and its token's bits
 };
 struct AcceptLaunch {
   qd_accept_args a;
@@ -1124,19 +1122,14 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
   const uint32_t mine = word(node, share);
   if constexpr (kSampled) {
     const float wave_top = wave_max(top);
-    if (lane == 0) tops[w] = wave_top;
-    __syncthreads();
-    float all = tops[0];
-#pragma unroll
-    for (int u = 1; u < kAcceptWaves; ++u) all = fmaxf(all, tops[u]);
-    double s = scaled(sum, r - whole_above(p, all));
+    double s = scaled(sum, r - whole_above(p, wave_top));
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1) s += lane_of(s, lane ^ step);
     if (lane == 0) {
       const uint64_t bits = __builtin_bit_cast(uint64_t, s);
       shares.stu(mine + 2 * w, static_cast<uint32_t>(bits));
       shares.stu(mine + 2 * w + 1, static_cast<uint32_t>(bits >> 32));
-      if (w == 0) shares.st(mine + 2 * kAcceptWaves, all);
+      shares.st(mine + 2 * kAcceptWaves + w, wave_top);
     }
   } else {
     const float wave_top = wave_max(top);
@@ -1200,16 +1193,20 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
   } else {
     if (!arrive(p.counters + (at + node) * p.apart, p.shares)) return;
     // Every wave: all shares, a lane each.
-    float most = -INFINITY;
+    float largest[kAcceptWaves], most = -INFINITY;
     double part[kAcceptWaves] = {}, s = 0.0;
+#pragma unroll
+    for (int u = 0; u < kAcceptWaves; ++u) largest[u] = -INFINITY;
     if (static_cast<uint32_t>(lane) < p.shares) {
-      most = shares.ld(word(node, lane) + 2 * kAcceptWaves);
 #pragma unroll
       for (int u = 0; u < kAcceptWaves; ++u) {
+        largest[u] = shares.ld(word(node, lane) + 2 * kAcceptWaves + u);
         const uint64_t lo = shares.ldu(word(node, lane) + 2 * u), hi = shares.ldu(word(node, lane) + 2 * u + 1);
         part[u] = __builtin_bit_cast(double, hi << 32 | lo);
       }
     }
+#pragma unroll
+    for (int u = 0; u < kAcceptWaves; ++u) most = fmaxf(most, largest[u]);
     const float all = wave_max(most);
     if (!(fabsf(all) < kHuge)) {
       // The largest logit, read again by the whole workgroup.
@@ -1227,10 +1224,10 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       if (threadIdx.x == 0) picks[0] = ids[0] == UINT32_MAX ? 0 : static_cast<int32_t>(ids[0]);
     } else {
       const bool far = fabsf(all) * p.c_hi >= kFar;  // (then all of the node's logits are read again)
-      const float up = whole_above(p, all), by = whole_above(p, most) - up;
+      const float up = whole_above(p, all);
 #pragma unroll
       for (int u = 0; u < kAcceptWaves; ++u) {
-        part[u] = scaled(part[u], by);
+        part[u] = scaled(part[u], whole_above(p, largest[u]) - up);
         s += part[u];
       }
       const double upto = lanes_upto(s), draw = fmaxf(p.a.draws[at + node], 0.f);
@@ -1241,24 +1238,29 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       const uint64_t some = __ballot(s > 0.0), past = __ballot(upto > aim) & some;
       const int in = past ? __ffsll(static_cast<unsigned long long>(past)) - 1 : 63 - __clzll(static_cast<long long>(some));
       // Its quarter: the first that passes, or the last with a token.
-      double before = lane_of(upto - s, in);
+      double before = lane_of(upto - s, in), begins = before, ends = before;
       int which = -1;
-      double begins = before;
+      float own = all;  // its largest logit
 #pragma unroll
       for (int u = 0; u < kAcceptWaves; ++u) {
         const double y = lane_of(part[u], in);
-        if (y > 0.0 && (which < 0 || !(begins + lane_of(part[max(which, 0)], in) > aim))) {
+        if (y > 0.0 && (which < 0 || !(ends > aim))) {
           which = u;
           begins = before;
+          ends = before + y;
+          own = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, largest[u]), in));
         }
         before += y;
       }
+      // The rest is relative to the quarter's own whole number: to the node's, FP32 may have nothing of it.
+      const float r_own = whole_above(p, own);
+      aim = ldexp(aim - begins, static_cast<int>(up - r_own));
       const uint32_t q = in * kAcceptWaves + which, a0 = far ? 0 : x.first(q), b0 = far ? x.pieces : x.first(q + 1);
       // Its logits again, a run of pieces each thread; what lies before and behind the pieces with the first and last thread.
       const uint32_t n = (b0 - a0 + kAcceptT - 1) / kAcceptT, a = min(b0, a0 + threadIdx.x * n), b = min(b0, a + n);
       const uint32_t begin = (far || q == 0) && threadIdx.x == 0 ? 0 : x.token(a);
       const uint32_t end = (far || q + 1 == p.shares * kAcceptWaves) && threadIdx.x == kAcceptT - 1 ? p.a.vocab : x.token(b);
-      const auto weight = [&](float y) { return far ? power_far(p, y, all) : power(p, y, up); };
+      const auto weight = [&](float y) { return far ? power_far(p, y, all) : power(p, y, r_own); };
       const auto each = [&](auto f) {  // f(token, probability), until it says so
         for (uint32_t i = begin; i < x.token(a) && i < end; ++i)
           if (f(i, weight(logit<E>(x.x, i)))) return;
@@ -1281,11 +1283,8 @@ __global__ __launch_bounds__(kAcceptT) void accept_kernel(AcceptLaunch p) {
       __syncthreads();
       if (lane == kWave - 1) sums[w] = wave_upto;
       __syncthreads();
-      if (far) {
-        begins = 0.0;
-        aim = aim_at((sums[0] + sums[1]) + (sums[2] + sums[3]));
-      }
-      double mine_before = begins + (wave_upto - run);
+      if (far) aim = aim_at((sums[0] + sums[1]) + (sums[2] + sums[3]));
+      double mine_before = wave_upto - run;
       for (int u = 0; u < w; ++u) mine_before += sums[u];
       // The first thread whose run passes the draw, or the last with a token.
       const uint64_t passes = __ballot(run > 0.0 && mine_before + run > aim), any = __ballot(run > 0.0);

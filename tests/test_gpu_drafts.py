@@ -509,6 +509,18 @@ def test_draws_of_one_and_almost_one():
     check_draws(logits, draws, temperature, draw_one_each(logits, draws, temperature))
 
 
+def test_draws_among_tokens_far_below_the_largest():
+    """What FP32 holds of the largest's size: nothing. It is a probability all the same, and masks beside it are none."""
+    say("draws far below")
+    vocab = 151936
+    logits = torch.full((4, vocab), -math.inf)
+    logits[:, 100:9000] = -120.0
+    logits[:, 90000] = 0.0
+    logits[:, 100000:130000] = -150.0
+    draws = torch.tensor([0.0, -1.0, 1.0, 0.5])
+    assert draw_one_each(logits, draws, 1.0).tolist() == [100, 100, 129999, 90000]
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_draws_of_logits_of_any_size(dtype):
     """Logits of many temperatures: ties and neighbours are told apart."""
