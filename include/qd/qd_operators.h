@@ -288,10 +288,11 @@ QD_API qd_status qd_paged_append_at(const qd_paged_cache *cache, const qd_append
  *   out[r][i][h] = sum_j softmax_j(scale q[r][i][h] . K_j) V_j,
  * each position read once for up to 128 (FP32: 64) pairs of a node and a query head of one
  * KV head. Precision is qd_paged_attention's, but that a weight in FP16 is off by 2^-22 of
- * it or 2^-39 of the row's largest. Nodes that are not there and rows of length 0 get zeros; K and V of nodes that are not seen may hold anything,
- * also values that are not finite: outputs that see such a V become NaN or infinite. A row with
- * a bad page, a bad parent, or a length that is not 0 and below `nodes` or past its
- * table gets NaN. q and out are [rows][nodes][heads][head_dim] with strides that are
+ * it or 2^-39 of the row's largest. Nodes that are not there get zeros, and so do rows of length 0, whose
+ * parents are not looked at. K and V of nodes that are not seen may hold anything,
+ * also values that are not finite: outputs that see such a V become NaN or infinite. A row of another length
+ * gets NaN if it has a bad page, a bad parent, or a length below `nodes` or past its
+ * table. q and out are [rows][nodes][heads][head_dim] with strides that are
  * multiples of 16 bytes; out may be q itself, with its strides. */
 typedef struct qd_tree_attention_args {
   const void *q;

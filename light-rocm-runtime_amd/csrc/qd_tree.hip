@@ -812,7 +812,7 @@ __global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunc
       bool bad;
       const uint64_t mask = ancestors(p.a.parents + static_cast<size_t>(a.it.row) * p.a.nodes, p.a.nodes, bad);
       sh.mask[a.lane] = mask;
-      if (bad) a.errors |= QD_TREE_BAD_PARENT;
+      if (bad && (a.it.length || a.it.bad)) a.errors |= QD_TREE_BAD_PARENT;  // (a row of nothing may have any)
     }
     if (a.it.bad) a.errors |= QD_PAGED_BAD_LENGTH;
     a.run();

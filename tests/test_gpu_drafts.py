@@ -230,6 +230,21 @@ def test_bad_rows_are_marked_and_no_others(length):
         assert torch.isnan(got).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_of_nothing_may_have_any_parents(dtype):
+    """A row that only fills the batch: what its parents hold is not looked at."""
+    g, nodes = seeded(25), 5
+    lengths = [0, 40, 0, 0]
+    table, pages = tables_for(g, lengths, 16, 4)
+    k, v = pool(g, pages, 16, 2, 64, dtype)
+    q = normal(g, (4, nodes, 4, 64), dtype)
+    parents = int32([[7, -9, 4, 3, 100], tree(g, nodes), [1 << 30] * nodes, [-1, 0, 1, 2, 3]])
+    want, bound = oracle.tree_attention(q[1:2], k, v, table[1:2], lengths[1:2], parents[1:2], 0.125)
+    out = run_tree(q, k, v, table, lengths, parents, 0.125)
+    close(out[1:2], want, bound, "out")
+    assert (out[[0, 2, 3]] == 0).all()
+
+
 def test_in_place_and_strides():
     g, nodes, page = seeded(8), 10, 32
     lengths = [300, 40, 0]
