@@ -411,8 +411,9 @@ QD_API qd_status qd_page_bounds(const qd_paged_cache *cache, void *bounds, uint3
  * between the ones that score highest, the lower of equal ones:
  *   score(page) = sum over the KV head's query heads and d of
  *                 max(q_d low_d, q_d high_d),
- * as much as the products of the page's keys can sum to, in 64 bits; a score that is
- * NaN counts as +inf.
+ * as much as the products of the page's keys can sum to, in 64 bits. Bounds are as
+ * qd_page_bounds makes them. A term with a product that is NaN (of 0 and an infinite bound,
+ * of a query that is NaN) is NaN, and a score that is NaN counts as +inf.
  *   chosen[r][kv_head][..]  the columns of the table that were read, ascending, -1 behind
  *                           them (NULL: not told)
  * A row of n <= budget pages reads all of them. A row with a bad length gets NaN, one

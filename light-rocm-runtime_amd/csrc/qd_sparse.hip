@@ -138,7 +138,9 @@ __global__ __launch_bounds__(kBoundsT) void bounds_kernel(BoundsLaunch p) {
 
 // ---- the choice ---------------------------------------------------------------------
 // The score is linear in a page's bounds: sum_d (sum_h min(q_h, 0)) low_d + (sum_h max(q_h, 0))
-// high_d, one product of 2 D in 64 bits whatever the number of query heads. Four lanes take a
+// high_d, one product of 2 D in 64 bits whatever the number of query heads, if all are finite: an
+// infinite bound, one without a number or a query without makes the product infinite or NaN, and the
+// score is then summed as it is defined. Four lanes take a
 // page, a quarter of its bounds each; a workgroup takes a share of the pages of one row and KV
 // head. Scores go out as whole numbers in their order; the last share of a row's head to
 // arrive finds the least chosen one by counting keys into bins between the least and the
@@ -165,6 +167,30 @@ struct ChooseLaunch {
   uint32_t page_shift;
   uint32_t share;      // pages
 };
+
+// One element, or a bound, as it is held.
+template <typename E>
+__device__ __forceinline__ double element(const void *base, int64_t i) {
+  if constexpr (std::is_same_v<E, float>)
+    return static_cast<const float *>(base)[i];
+  else
+    return E::lo(static_cast<const uint16_t *>(base)[i]);
+}
+// The terms of dimensions [from, from + n) as they are defined: bounds from element `at`, queries from `q` on.
+template <typename E, int D>
+__device__ __forceinline__ double defined_score(const ChooseLaunch &p, int64_t at, int64_t q, int from, int n) {
+  double s = 0.0;
+#pragma unroll 1
+  for (int d = from; d < from + n; ++d) {
+    const double low = element<E>(p.a.bounds, at + d), high = element<E>(p.a.bounds, at + D + d);
+#pragma unroll 1
+    for (uint32_t h = 0; h < p.group; ++h) {
+      const double x = element<E>(p.a.q, q + h * p.a.q_head_stride + d), a = x * low, b = x * high;
+      s += a != a || b != b ? __builtin_nan("") : a > b ? a : b;
+    }
+  }
+  return s;
+}
 
 // Whole numbers in the order of the scores; NaN as +inf.
 __device__ __forceinline__ uint64_t key_of(double s) {
@@ -224,17 +250,13 @@ __global__ __launch_bounds__(kChooseT) void choose_kernel(ChooseLaunch p) {
   // The pages between the first and the last ones: all that is scored.
   const uint32_t middle = pages - fixed, from = blockIdx.x * p.share, to = min(middle, from + p.share);
   if (from >= middle) return;
+  const int64_t queries = row * p.a.q_stride + static_cast<int64_t>(head) * p.group * p.a.q_head_stride;
   for (int d = threadIdx.x; d < D; d += kChooseT) {
     double low = 0.0, high = 0.0;
     for (uint32_t h = 0; h < p.group; ++h) {
-      const int64_t at = row * p.a.q_stride + (head * p.group + h) * p.a.q_head_stride + d;
-      float q;
-      if constexpr (std::is_same_v<E, float>)
-        q = static_cast<const float *>(p.a.q)[at];
-      else
-        q = E::lo(static_cast<const uint16_t *>(p.a.q)[at]);
-      low += q < 0.f ? q : q > 0.f ? 0.f : q;  // (NaN stays)
-      high += q > 0.f ? q : q < 0.f ? 0.f : q;
+      const double q = element<E>(p.a.q, queries + h * p.a.q_head_stride + d);
+      low += q < 0.0 ? q : q > 0.0 ? 0.0 : q;  // (NaN stays)
+      high += q > 0.0 ? q : q < 0.0 ? 0.0 : q;
     }
     weight[d + d / kQuarter * 2] = low;
     weight[D + d + (D + d) / kQuarter * 2] = high;
@@ -245,10 +267,10 @@ __global__ __launch_bounds__(kChooseT) void choose_kernel(ChooseLaunch p) {
   for (uint32_t i = from + threadIdx.x / 4; i < to; i += kChooseT / 4) {
     const int32_t page = table[p.a.first + i];
     const bool there = page >= 0 && static_cast<uint32_t>(page) < p.c.pages;
+    const int64_t first = (static_cast<int64_t>(page) * p.c.kv_heads + head) * 2 * D;
     double s = 0.0;
     if (there) {
-      const char *at = static_cast<const char *>(p.a.bounds) +
-                       ((static_cast<int64_t>(page) * p.c.kv_heads + head) * 2 * D + quarter * kQuarter) * (16 / kP);
+      const char *at = static_cast<const char *>(p.a.bounds) + (first + quarter * kQuarter) * (16 / kP);
       u4v v[kQuarter / kP];
 #pragma unroll
       for (int u = 0; u < kQuarter / kP; ++u) v[u] = *reinterpret_cast<const u4v *>(at + 16 * u);
@@ -263,6 +285,11 @@ __global__ __launch_bounds__(kChooseT) void choose_kernel(ChooseLaunch p) {
     }
     s += lane_of(s, lane ^ 1);
     s += lane_of(s, lane ^ 2);
+    if (!(fabs(s) < INFINITY)) {  // (all four lanes)
+      s = defined_score<E, D>(p, first, queries, quarter * (D / 4), D / 4);
+      s += lane_of(s, lane ^ 1);
+      s += lane_of(s, lane ^ 2);
+    }
     // A page that does not exist comes first: attention then says so.
     if (quarter == 0) __hip_atomic_store(keys + i, there ? key_of(s) : UINT64_MAX, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }

@@ -150,6 +150,49 @@ def test_scores_that_are_not_finite():
     assert chosen.flatten().tolist() == [0, 1, 2, 19] and torch.isnan(out[0, 0]).all() and torch.isfinite(out[0, 1]).all()
 
 
+def best_pages(q, low_high, table, pages, budget, first, last):
+    """What a KV head with queries q [group, dim] and bounds [pages, 2, dim] reads, from the score's definition."""
+    low, high = low_high[table.long(), 0].double(), low_high[table.long(), 1].double()
+    score = sum(torch.maximum(x * low, x * high).sum(-1) for x in q.double())
+    score = torch.where(torch.isnan(score), math.inf, score).tolist()
+    middle = sorted(range(first, pages - last), key=lambda i: (-score[i], i))[: budget - first - last]
+    return [*range(first), *sorted(middle), *range(pages - last, pages)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("dim,group", [(64, 1), (64, 3), (128, 2)])
+@pytest.mark.parametrize("signs", ["above", "below", "both"])
+def test_pages_whose_bounds_are_infinite(dtype, dim, group, signs):
+    """Keys that are infinite or no number in single elements: the bounds of their pages, and what queries of one sign or
+    of both make of them."""
+    say("infinite bounds", dtype, dim, group, signs)
+    g, page, pages, kv_heads = seeded(dim + group), 16, 30, 2
+    k, v = pool(g, pages, page, kv_heads, dim, dtype)
+    k[3, :, :, 5] = NAN            # no number: +inf and -inf
+    k[5, 2, :, 6] = math.inf
+    k[7, 2, :, 6] = -math.inf
+    k[9, :, :, 7] = math.inf       # all keys
+    k[11, :, :, 7] = -math.inf
+    k[13, 1, :, 40], k[13, 2, :, 41] = math.inf, -math.inf
+    k[15, 1, :, 40], k[15, 2, :, 40] = math.inf, -math.inf
+    k[17, 1, 0, 50] = math.inf     # one head's alone
+    k[19, :, 1] = NAN              # a head's whole page
+    k[21, 4, :, 8] = NAN           # one key's
+    q = normal(g, (1, kv_heads * group, dim), dtype).abs()
+    if signs == "below":
+        q = -q
+    elif signs == "both":
+        q[:, ::2, ::2] = -q[:, ::2, ::2]
+    q[:, :, 41] = 0.0
+    table = torch.randperm(pages, generator=g).to(torch.int32)[None]
+    low_high = run_bounds(k, table, [pages * page], 1 << 20, torch.zeros((pages, kv_heads, 2, dim), dtype=dtype))
+    for budget in (3, 5, 8, 11, 14, 20, 29):
+        _, chosen = run_sparse(q, k, v, low_high, table, [pages * page], budget, 1, 1, 0.125)
+        for h in range(kv_heads):
+            want = best_pages(q[0, h * group: (h + 1) * group], low_high[:, h], table[0], pages, budget, 1, 1)
+            assert chosen[0, h].tolist() == want, (budget, h)
+
+
 def test_bad_rows():
     g, page = seeded(7), 16
     lengths = [320] * 5
