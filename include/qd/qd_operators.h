@@ -375,7 +375,7 @@ typedef struct qd_token_memory {
  * with a bad length (not 0 and below `nodes`, or past the table), count, path (its nodes
  * ascend) or page moves nothing and hands its length on. Rows whose trees lie in the same
  * pages must not be committed in one call, nor memories that overlap; lengths_out must
- * not be lengths. */
+ * not overlap lengths, counts, path or table. */
 typedef struct qd_commit_args {
   const int32_t *table;
   const int32_t *lengths;

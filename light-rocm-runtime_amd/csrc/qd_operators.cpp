@@ -62,6 +62,15 @@ qd_status check_stride(int64_t stride, int64_t least, uint32_t bytes, const char
   return QD_SUCCESS;
 }
 
+// Whether two arrays of so many 32-bit words share some; `b` may be rows, `stride` words apart.
+bool overlap(const void *a, uint64_t a_words, const void *b, uint64_t b_words, uint64_t rows = 1, uint64_t stride = 0) {
+  if (!a || !b || a_words == 0 || b_words == 0 || rows == 0) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  if (x < y) return (y - x) / 4 < a_words;
+  const uint64_t in = (x - y) / 4, row = stride ? std::min(in / stride, rows - 1) : 0, at = in - row * stride;
+  return at < b_words || (row + 1 < rows && at + a_words > stride);
+}
+
 qd_status check_page_size(uint32_t n) {
   if (n < qd::kPageSizeLeast || n > qd::kPageSizeMost || (n & (n - 1)) != 0)
     return refuse(QD_ERROR_NOT_SUPPORTED, "page_size %u: a power of two from %u to %u is needed", n, qd::kPageSizeLeast,
@@ -478,7 +487,6 @@ qd_status qd_tree_commit(const qd_commit_args *a, void *stream) {
     return refuse(QD_ERROR_NOT_SUPPORTED, "rows of more than 2^30 positions");
   if (a->rows) {
     if (!a->table || !a->lengths || !a->path || !a->counts || !a->lengths_out) return invalid("null tensor");
-    if (a->lengths == a->lengths_out) return invalid("lengths_out must not be lengths");
     if (a->table_stride < static_cast<int64_t>(a->table_width) || a->table_stride > (int64_t(1) << 40))
       return invalid("table_stride is less than table_width");
   }
@@ -503,6 +511,11 @@ qd_status qd_tree_commit(const qd_commit_args *a, void *stream) {
   }
   // A grid has fewer than 2^32 threads, 256 for 64 columns.
   if ((columns / 64 + 1) * a->rows > 0xff0000u) return refuse(QD_ERROR_NOT_SUPPORTED, "%u rows are too much for one call", a->rows);
+  // (A row's first workgroup writes its length while the others still read the rest.)
+  if (overlap(a->lengths_out, a->rows, a->lengths, a->rows) || overlap(a->lengths_out, a->rows, a->counts, a->rows) ||
+      overlap(a->lengths_out, a->rows, a->path, static_cast<uint64_t>(a->rows) * a->nodes) ||
+      overlap(a->lengths_out, a->rows, a->table, a->table_width, a->rows, a->table_stride))
+    return invalid("lengths_out must not be lengths, counts, path or table, nor overlap them");
   Device on;
   QD_TRY(on.enter(a->device));
   return launched(qd::launch_tree_commit(static_cast<hipStream_t>(stream), *a), "commit launch");

@@ -127,6 +127,27 @@ def test_commit_refusals(status, memory, changes):
     refused(status, "qd_tree_commit", commit(memory, **changes), None)
 
 
+@pytest.mark.parametrize("other,at", [("lengths", 0), ("lengths", 2), ("counts", 0), ("counts", -2), ("path", 0), ("path", 14), ("path", -2),
+                                      ("table", 0), ("table", 7), ("table", 8), ("table", 23), ("table", 12), ("table", 17)])
+def test_commit_refuses_lengths_over_what_it_reads(other, at):
+    """Some of a row's workgroups would read what another has written."""
+    changes = {name: AT + 4096 * i for i, name in enumerate(("lengths", "counts", "path", "table"))}
+    changes.update(lengths_out=changes[other] + 4 * at, table_stride=10)
+    refused(qd.INVALID_ARGUMENT, "qd_tree_commit", commit(**changes), None)
+    assert b"lengths_out" in ops.lib().qd_last_error()
+
+
+@pytest.mark.parametrize("other,at", [("lengths", 3), ("lengths", -3), ("counts", 3), ("path", 15), ("path", -3), ("table", 30), ("table", -3),
+                                      ("table", 19), ("table", 8)])
+def test_commit_takes_lengths_beside_what_it_reads(other, at):
+    """(In the gap behind a row of the table too, if they fit.) The device is the next thing that is looked at."""
+    changes = {name: AT + 4096 * i for i, name in enumerate(("lengths", "counts", "path", "table"))}
+    rows = 2 if other == "table" and at == 8 else 3
+    changes.update(lengths_out=changes[other] + 4 * at, rows=rows, table_stride=10 if rows == 2 else 11, device=-1)
+    refused(qd.INVALID_ARGUMENT if torch.cuda.is_available() else qd.NOT_SUPPORTED, "qd_tree_commit", commit(**changes), None)
+    assert b"lengths_out" not in ops.lib().qd_last_error()
+
+
 @pytest.mark.parametrize("status,changes,bounds,recent", [
     (qd.INVALID_ARGUMENT, dict(dtype=7), AT, 1), (qd.INVALID_ARGUMENT, {}, None, 1), (qd.INVALID_ARGUMENT, {}, AT + 8, 1),
     (qd.NOT_SUPPORTED, dict(rows=1 << 20, table_width=1 << 10, table_stride=1 << 10), AT, 1 << 20)])
