@@ -329,7 +329,9 @@ QD_API qd_status qd_tree_attention_workspace(uint32_t rows, uint32_t nodes, uint
  * counts as 0, one of 1 or more picks the last token that has a probability, which -inf and
  * NaN have not; a p_i below 2^-126 of the largest may count as none. Where the largest logit
  * is past 1e30 either way, the token of the largest logit is picked. A row whose node 0 is
- * not there gets count 0 and -1, and so does one with a bad parent. */
+ * not there gets count 0 and -1, and so does one with a bad parent. The results must not
+ * overlap each other or what is read, but that next_tokens may be the tokens of trees of
+ * one node. */
 typedef struct qd_accept_args {
   const void *logits;      /* [rows][nodes][vocab] */
   int64_t row_stride;

@@ -10,6 +10,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <new>
 
 #include "qd_operators.hpp"
@@ -463,7 +464,17 @@ qd_status qd_tree_accept(const qd_accept_args *a, qd_workspace *w, void *stream)
   QD_TRY(check_accept(a->rows, a->nodes, a->vocab));
   if (a->rows) {
     if (!a->logits || !a->tokens || !a->parents || !a->path || !a->counts || !a->next_tokens) return invalid("null tensor");
-    if (a->path == a->tokens || a->path == a->parents) return invalid("path must not be tokens or parents");
+    // (Rows that are done write theirs while others still read.)
+    const uint64_t rows = a->rows, all = rows * a->nodes;
+    for (const void *read : {static_cast<const void *>(a->tokens), static_cast<const void *>(a->parents), static_cast<const void *>(a->draws)}) {
+      if (overlap(a->path, all, read, all)) return invalid("path must not be tokens or parents or draws, nor overlap them");
+      // (Of trees of one node a row's token is read where the next one is written.)
+      const bool own = a->nodes == 1 && read == a->tokens && a->next_tokens == a->tokens;
+      if (overlap(a->counts, rows, read, all) || (!own && overlap(a->next_tokens, rows, read, all)))
+        return invalid("counts and next_tokens must not overlap tokens, parents or draws");
+    }
+    if (overlap(a->path, all, a->counts, rows) || overlap(a->path, all, a->next_tokens, rows) || overlap(a->counts, rows, a->next_tokens, rows))
+      return invalid("path, counts and next_tokens must not overlap");
     if (reinterpret_cast<uintptr_t>(a->logits) % element_bytes(a->dtype) != 0) return invalid("misaligned logits");
     const int64_t most = int64_t(1) << 40;
     if (a->row_stride < 0 || a->node_stride < 0 || a->row_stride > most || a->node_stride > most)

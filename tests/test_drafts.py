@@ -110,6 +110,29 @@ def test_accept_refusals(status, changes):
     refused(status, "qd_tree_accept", accept(**changes), None, None)
 
 
+@pytest.mark.parametrize("result", ["path", "counts", "next_tokens"])
+@pytest.mark.parametrize("other,at", [("tokens", 0), ("tokens", 14), ("parents", 0), ("parents", -2), ("draws", 0), ("draws", 3), ("path", 14),
+                                      ("counts", 0), ("counts", -2), ("next_tokens", 2)])
+def test_accept_refuses_results_over_each_other_and_what_it_reads(result, other, at):
+    names = ("tokens", "parents", "draws", "path", "counts", "next_tokens")
+    changes = {name: AT + 4096 * i for i, name in enumerate(names)}
+    if result == other:
+        refused(qd.INVALID_ARGUMENT, "qd_tree_accept", accept(**changes), None, None)
+        assert b"null workspace" in ops.lib().qd_last_error()
+        return
+    changes[result] = changes[other] + 4 * at
+    refused(qd.INVALID_ARGUMENT, "qd_tree_accept", accept(**changes), None, None)
+    assert b"overlap" in ops.lib().qd_last_error()
+
+
+def test_accept_of_one_node_takes_its_tokens_in_place():
+    names = ("tokens", "parents", "draws", "path", "counts")
+    changes = {name: AT + 4096 * i for i, name in enumerate(names)}
+    for nodes, text in ((1, b"null workspace"), (5, b"overlap")):
+        refused(qd.INVALID_ARGUMENT, "qd_tree_accept", accept(nodes=nodes, next_tokens=AT, **changes), None, None)
+        assert text in ops.lib().qd_last_error()
+
+
 @pytest.mark.parametrize("status,memory,changes", [
     (qd.NOT_SUPPORTED, {}, dict(page_size=24)), (qd.NOT_SUPPORTED, {}, dict(nodes=0)), (qd.NOT_SUPPORTED, {}, dict(nodes=65)),
     (qd.NOT_SUPPORTED, {}, dict(rows=65536)), (qd.INVALID_ARGUMENT, {}, dict(pages=1 << 31)),
