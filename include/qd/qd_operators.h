@@ -417,7 +417,7 @@ QD_API qd_status qd_page_bounds(const qd_paged_cache *cache, void *bounds, uint3
  * qd_page_bounds makes them. A term with a product that is NaN (of 0 and an infinite bound,
  * of a query that is NaN) is NaN, and a score that is NaN counts as +inf.
  *   chosen[r][kv_head][..]  the columns of the table that were read, ascending, -1 behind
- *                           them (NULL: not told)
+ *                           them (NULL: not told; not over the table or the lengths)
  * A row of n <= budget pages reads all of them. A row with a bad length gets NaN, one
  * with a bad page at least where its page is chosen, as it then is. */
 typedef struct qd_sparse_args {

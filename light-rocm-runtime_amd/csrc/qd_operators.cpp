@@ -563,6 +563,10 @@ qd_status qd_sparse_attention(const qd_paged_cache *c, const qd_sparse_args *a, 
   if (c->rows) {
     QD_TRY(check_rows_of_heads(c, a->q, a->out, a->q_stride, a->q_head_stride, a->out_stride, a->out_head_stride, a->heads));
     if (c->pages && (!a->bounds || !aligned16(a->bounds))) return invalid("bounds need a 16-byte aligned address");
+    // (One row's list is written while another's table is read.)
+    const uint64_t listed = static_cast<uint64_t>(c->rows) * c->kv_heads * a->budget;
+    if (overlap(a->chosen, listed, c->table, c->table_width, c->rows, c->table_stride) || overlap(a->chosen, listed, c->lengths, c->rows))
+      return invalid("chosen must not overlap the table or the lengths");
   }
   const uint64_t positions = static_cast<uint64_t>(a->budget) * c->page_size;
   if (positions > (1u << 30)) return refuse(QD_ERROR_NOT_SUPPORTED, "a budget of more than 2^30 positions");

@@ -188,6 +188,14 @@ def test_sparse_refusals(status, changes):
     refused(status, "qd_sparse_attention", cache(), sparse(**changes), None, None)
 
 
+@pytest.mark.parametrize("place,text", [(AT, b"chosen"), (AT + 4 * 23, b"chosen"), (AT - 4 * 23, b"chosen"), (2 * AT + 8, b"chosen"),
+                                        (AT + 4 * 24, b"null workspace"), (AT - 4 * 24, b"null workspace")])
+def test_sparse_refuses_a_list_over_what_it_reads(place, text):
+    """Three rows of eight columns, lists of four for two heads."""
+    refused(qd.INVALID_ARGUMENT, "qd_sparse_attention", cache(lengths=2 * AT), sparse(chosen=place), None, None)
+    assert text in ops.lib().qd_last_error()
+
+
 def test_sparse_of_too_many_rows_is_refused():
     refused(qd.NOT_SUPPORTED, "qd_sparse_attention", cache(rows=40000), sparse(), None, None)
 
