@@ -899,6 +899,12 @@ TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_he
   const uint64_t items = static_cast<uint64_t>(rows) * kv_heads * s.blocks;
   if (items <= kOpCounters) {
     s.target = std::max(1u, kTreePerCu * kTreeCus / (kv_heads * s.blocks));
+    // A join's offsets and its buffer have 32 bits: rows of so many items that they would not do stay whole.
+    const uint64_t apart = static_cast<uint64_t>(kv_heads) * s.blocks * s.rec_floats * sizeof(float);
+    if (std::min(kTreePieces, 1 + 4 * s.target) * apart > UINT32_MAX) {
+      s.target = 0;
+      return s;
+    }
     s.records = std::max((rows + 4 * s.target) * kv_heads * s.blocks, 2 * kTreeCus * kTreePerCu);
     for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
   }

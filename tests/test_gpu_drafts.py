@@ -288,6 +288,26 @@ def test_tree_attention_of_more_rows_than_counters():
     close(got[some.cuda()], want, bound, "out")
 
 
+def test_tree_attention_of_very_many_heads():
+    """Rows of 24,576 items: the records of a few pieces of them would pass 32 bits."""
+    say("tree attention of very many heads")
+    g, kv_heads, group, nodes, dim, page, n = seeded(28), 4096, 11, 64, 128, 256, 256
+    gd = torch.Generator(device="cuda").manual_seed(28)
+    k, v = (torch.randn((1, page, kv_heads, dim), generator=gd, device="cuda", dtype=F16) for _ in range(2))
+    q = torch.randn((1, nodes, kv_heads * group, dim), generator=gd, device="cuda", dtype=F16)
+    parents, table = int32([tree(g, nodes)]), int32([[0]])
+    w = ops.Workspace(ops.tree_attention_workspace(1, nodes, kv_heads * group, kv_heads, dim))
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, NAN)
+    ops.tree_attention(ops.PagedCache(k, v, table.cuda(), int32([n]).cuda(), error), out, q, parents.cuda(), w, scale=0.1)
+    assert int(error) == 0
+    assert torch.isfinite(out).all()
+    for h in (0, 1, 2047, 4095):
+        heads = slice(h * group, (h + 1) * group)
+        want, bound = oracle.tree_attention(q[:, :, heads].cpu(), k[:, :, h:h + 1].cpu(), v[:, :, h:h + 1].cpu(), table, [n], parents, 0.1)
+        close(out[:, :, heads], want, bound, h)
+
+
 def test_offsets_past_32_bits():
     say("offsets past 32 bits")
     g, page, nodes, dim = seeded(11), 16, 3, 64
