@@ -854,7 +854,8 @@ __global__ __launch_bounds__(WC *WP *kWave) void tree_attention_kernel(TreeLaunc
 }
 
 struct TreePlan {
-  uint32_t group, columns, blocks, rec_floats, apart, target, records;
+  uint32_t group, columns, blocks, apart, target, records;
+  bool few;  // rows, for pieces of one item that the card holds at once
 };
 
 // Calls f with the shape and kernel for so many columns. A wave of 32 columns has 340 registers and
@@ -890,24 +891,28 @@ auto with_type(uint32_t dtype, uint32_t head_dim, uint32_t columns, F &&f) {
   }
 }
 
-TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t block_columns) {
+// What a launch of shape S does, and the records that it can write: no more pieces than one of each row and `target`
+// more, four times as many where rows are not few, or two of each workgroup that equal runs go to.
+template <typename S>
+TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads) {
   TreePlan s{};
   s.group = heads / kv_heads;
   s.columns = nodes * s.group;
-  s.blocks = (s.columns + block_columns - 1) / block_columns;
-  s.rec_floats = block_columns * (head_dim + 2);
-  const uint64_t items = static_cast<uint64_t>(rows) * kv_heads * s.blocks;
-  if (items <= kOpCounters) {
-    s.target = std::max(1u, kTreePerCu * kTreeCus / (kv_heads * s.blocks));
-    // A join's offsets and its buffer have 32 bits: rows of so many items that they would not do stay whole.
-    const uint64_t apart = static_cast<uint64_t>(kv_heads) * s.blocks * s.rec_floats * sizeof(float);
-    if (std::min(kTreePieces, 1 + 4 * s.target) * apart > UINT32_MAX) {
-      s.target = 0;
-      return s;
-    }
-    s.records = std::max((rows + 4 * s.target) * kv_heads * s.blocks, 2 * kTreeCus * kTreePerCu);
-    for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
-  }
+  s.blocks = (s.columns + S::kColumns - 1) / S::kColumns;
+  const uint32_t parts = kv_heads * s.blocks;
+  const uint64_t items = static_cast<uint64_t>(rows) * parts;
+  if (items > kOpCounters) return s;
+  for (s.apart = 32; items * s.apart > kOpCounters;) s.apart /= 2;
+  // FP32's products bound it: no more pieces than CUs (16 rows of 576 with 16 nodes 19.1 us, as
+  // many as the card holds 22.9).
+  constexpr uint32_t kAim = S::kWide ? 1 : S::kPerCu;
+  const uint32_t target = std::max(1u, std::max(1u, kTreePerCu * kTreeCus / parts) * kAim / kTreePerCu);
+  // A join's offsets and its buffer have 32 bits: rows of so many items that they would not do stay whole.
+  if (std::min(kTreePieces, 1 + 4 * target) * (parts * S::kRecord * sizeof(float)) > UINT32_MAX) return s;
+  s.target = target;
+  s.few = 4ull * rows <= target;
+  s.records = (s.few ? rows + target : rows + 4 * target) * parts;
+  if (S::kByHalves && s.blocks == 1 && !s.few) s.records = std::max(s.records, 2 * kTreeCus * S::kPerCu);
   return s;
 }
 
@@ -1435,8 +1440,8 @@ uint32_t accept_shares(uint32_t rows, uint32_t nodes, uint32_t vocab) {
 
 size_t tree_attention_scratch(uint32_t dtype, uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_heads, uint32_t head_dim) {
   return with_type(dtype, head_dim, nodes * (heads / kv_heads), [&](auto shape, auto) {
-    const TreePlan s = tree_plan(rows, nodes, heads, kv_heads, head_dim, decltype(shape)::kColumns);
-    return static_cast<size_t>(s.records) * s.rec_floats * sizeof(float);
+    using S = decltype(shape);
+    return static_cast<size_t>(tree_plan<S>(rows, nodes, heads, kv_heads).records) * S::kRecord * sizeof(float);
   });
 }
 
@@ -1447,7 +1452,7 @@ size_t tree_attention_scratch_most(uint32_t rows, uint32_t nodes, uint32_t heads
   for (const uint32_t dtype : {QD_DTYPE_F32, QD_DTYPE_BF16})
     for (uint32_t n = 1; n <= nodes; ++n)
       with_type(dtype, head_dim, n * (heads / kv_heads), [&](auto shape, auto) {
-        const uint32_t parts = kv_heads * tree_plan(0, n, heads, kv_heads, head_dim, decltype(shape)::kColumns).blocks;
+        const uint32_t parts = kv_heads * tree_plan<decltype(shape)>(0, n, heads, kv_heads).blocks;
         most = std::max(most, tree_attention_scratch(dtype, std::min(rows, static_cast<uint32_t>(kOpCounters / parts)), n, heads, kv_heads, head_dim));
       });
   return most;
@@ -1463,19 +1468,16 @@ hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const q
   p.page_shift = log2_of(c.page_size);
   return with_type(c.dtype, c.head_dim, a.nodes * (a.heads / c.kv_heads), [&](auto shape, auto kernel) {
     using S = decltype(shape);
-    const TreePlan plan = tree_plan(c.rows, a.nodes, a.heads, c.kv_heads, c.head_dim, S::kColumns);
+    const TreePlan plan = tree_plan<S>(c.rows, a.nodes, a.heads, c.kv_heads);
     p.apart = plan.apart;
     p.group = plan.group;
     p.columns = plan.columns;
     p.blocks = plan.blocks;
     p.parts = c.kv_heads * plan.blocks;
     const uint64_t most = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + kTreeLeast - 1) / kTreeLeast;
-    // FP32's products bound it: no more pieces than CUs (16 rows of 576 with 16 nodes 19.1 us, as
-    // many as the card holds 22.9).
-    constexpr uint32_t kAim = S::kWide ? 1 : S::kPerCu;
-    p.target = plan.target == 0 || most <= 1 ? 0 : std::max(1u, plan.target * kAim / kTreePerCu);
+    p.target = most <= 1 ? 0 : plan.target;
     uint64_t x = c.rows;
-    if (p.target) x = std::min<uint64_t>(4 * x <= p.target ? x + p.target : x + 4 * p.target, x * most);
+    if (p.target) x = std::min<uint64_t>(plan.few ? x + p.target : x + 4 * p.target, x * most);
     p.units = static_cast<uint32_t>(x);
     uint32_t grid = (p.units + kXcds - 1) / kXcds * kXcds * p.parts;
     // Many rows whose items read nothing twice: equal runs (64 BF16 rows of 0 to 8,192 with 16 columns
@@ -1483,7 +1485,7 @@ hipError_t launch_tree_attention(hipStream_t s, const qd_paged_cache &c, const q
     // than they even out: two of 1,000 24.5 us, in pieces 17.4, 16 FP32 of 513 to 4,000 33 and 29).
     // (Stages are counted in 31 bits.)
     const uint64_t stages = ((static_cast<uint64_t>(c.table_width) << p.page_shift) + S::kStage - 1) / S::kStage;
-    if (S::kByHalves && p.target && p.blocks == 1 && 4ull * c.rows > p.target && c.rows * p.parts * (stages + kEdge) <= 0x7f000000u) {
+    if (S::kByHalves && p.target && p.blocks == 1 && !plan.few && c.rows * p.parts * (stages + kEdge) <= 0x7f000000u) {
       p.units = 0;
       p.least = kTreeLeast / S::kStage;
       grid = kTreeCus * S::kPerCu;

@@ -224,6 +224,14 @@ def test_a_workspace_serves_every_smaller_call():
         assert ops.sparse_attention_workspace(rng.randint(1, rows), heads, kv_heads, dim, rng.randint(1, width), rng.randint(1, budget)) <= most
 
 
+@pytest.mark.parametrize("rows,nodes,heads,kv_heads,dim,most", [(2, 63, 28, 4, 128, 26 << 20), (1, 8, 14, 2, 64, 13 << 20), (64, 64, 32, 8, 128, 137 << 20),
+                                                                 (1, 64, 65536, 4096, 128, 4 << 30)])
+def test_tree_attention_asks_for_no_more_than_its_pieces_write(rows, nodes, heads, kv_heads, dim, most):
+    """Pieces of a row's items: one and `target` more in all, four times as many where rows are not few; a record has 2 more
+    numbers than values. Two rows of 63 nodes of 7 heads: 16-bit, 9 nodes, 64 columns, (2 + 192) x 4 records of 64 x 130 numbers."""
+    assert ops.tree_attention_workspace(rows, nodes, heads, kv_heads, dim) <= most
+
+
 def test_arguments_that_are_something_else_are_refused():
     import types
 
