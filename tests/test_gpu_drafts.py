@@ -574,6 +574,67 @@ def test_draws_of_logits_of_any_size(dtype):
         check_draws(logits, draws, temperature, draw_one_each(logits, draws, temperature))
 
 
+@pytest.mark.parametrize("dtype,offset", [(F32, 1), (F32, 3), (BF16, 1), (F16, 3), (BF16, 7)])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 9, 1009, 40003])
+def test_draws_of_logits_that_lie_anywhere(dtype, offset, vocab):
+    """Tokens before the first 16 bytes and behind the last ones, near whole numbers and far from them."""
+    say("draws of logits that lie anywhere", dtype, offset, vocab)
+    g, n = seeded(26), 24
+    for temperature, base in ((0.7, 0.0), (1e-5, 40.0)):
+        temperature = float(torch.tensor(temperature))
+        wide = (torch.randn((n, 1, vocab + offset + 2), generator=g) + base).to(dtype)
+        logits = on_gpu(wide)[:, :, offset: offset + vocab]
+        logits[::4, :, : vocab // 2] = -math.inf
+        logits[1::4, :, vocab // 2 + 1:] = -math.inf
+        draws = torch.rand(n, generator=g)
+        draws[:4], draws[4:8], draws[8:12] = 0.0, 1.0, 1 - 2.0 ** -24
+        path, counts, following = (torch.full(s, 99, dtype=torch.int32, device="cuda") for s in ((n, 1), (n,), (n,)))
+        w = ops.Workspace(ops.tree_accept_workspace(n, 1, vocab))
+        ops.tree_accept(logits, int32([[0]] * n).cuda(), int32([[-1]] * n).cuda(), path, counts, following, w,
+                        draws=draws[:, None].cuda(), temperature=temperature)
+        assert (counts == 1).all() and (path == 0).all()
+        check_draws(logits[:, 0], draws, temperature, following.long())
+
+
+def test_drawn_answers_in_a_graph():
+    """Captured once; replayed over other logits, draws and trees: likely tokens, masks, logits of many temperatures, trees
+    that are bad or not there in between."""
+    say("drawn answers in a graph")
+    g, rows, nodes, vocab, temperature = seeded(27), 6, 9, 33000, float(torch.tensor(0.8))
+    logits = torch.zeros((rows, nodes, vocab), device="cuda")
+    tokens, parents = (torch.zeros((rows, nodes), dtype=torch.int32, device="cuda") for _ in range(2))
+    draws = torch.zeros((rows, nodes), device="cuda")
+    path, counts, following = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in ((rows, nodes), (rows,), (rows,)))
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    w = ops.Workspace(ops.tree_accept_workspace(rows, nodes, vocab))
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        ops.tree_accept(logits, tokens, parents, path, counts, following, w, draws=draws, temperature=temperature, errors=error,
+                        stream=torch.cuda.current_stream().cuda_stream)
+    for step in range(8):
+        x = torch.randn((rows, nodes, vocab), generator=g)
+        x[:, :, ::500] += 9.0
+        if step % 4 == 1:
+            x[:, :, : vocab - 700] = -math.inf
+        elif step % 4 == 2:
+            x += 3e6
+        some = some_trees(g, rows, nodes)
+        middle = torch.stack([middles(g, y, temperature)[0] for y in x])
+        wanted = answer(g, x, some, middle, temperature)
+        logits.copy_(x), tokens.copy_(wanted), parents.copy_(some), draws.copy_(middle)
+        if step % 4 == 3:
+            parents[0, 3] = 7
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(error) == (ops.BAD_PARENT if step % 4 == 3 else 0)
+        error.zero_()
+        first = 1 if step % 4 == 3 else 0
+        want = oracle.accept(x[first:], wanted[first:], some[first:], middle[first:], temperature)
+        for got, y in zip((path, counts, following), want):
+            assert torch.equal(got[first:].cpu(), y), step
+
+
 @pytest.mark.parametrize("sampled", [False, True])
 def test_accept_of_masked_and_infinite_logits(sampled):
     vocab = 9001
