@@ -278,7 +278,8 @@ QD_API qd_status qd_beam_select_workspace(uint32_t groups, uint32_t beams, uint3
 /* qd_paged_append with a place of its own for each token: token t is rotated for
  * positions[t] and written to position slots[t] of its row (both plus position_bias;
  * slots NULL: qd_paged_append). A drafted token is rotated for its depth in the tree and
- * stands at its node's place. A token is skipped if either is negative. */
+ * stands at its node's place. A token is skipped if either is negative; a (row, slot) given
+ * twice is as a (row, position) there. */
 QD_API qd_status qd_paged_append_at(const qd_paged_cache *cache, const qd_append_args *args, const int32_t *slots,
                                     void *stream);
 
@@ -404,8 +405,8 @@ QD_API qd_status qd_tree_commit(const qd_commit_args *args, void *stream);
 
 /* The bounds of every page that holds one of a row's last `recent` positions, over all of
  * the row's positions in it. NaN counts as neither; a page of NaN alone gets +inf and -inf.
- * Rows that share a page write the same bounds if they hold equally much of it, else one of
- * them does. A row with a bad length or page sets an error bit; its other pages are done. */
+ * Rows that share a page write the same bounds if they hold equally much of it, else each
+ * value is one of theirs. A row with a bad length or page sets an error bit; its other pages are done. */
 QD_API qd_status qd_page_bounds(const qd_paged_cache *cache, void *bounds, uint32_t recent, void *stream);
 
 /* qd_paged_attention over up to `budget` pages of each row and KV head. Of a row of n

@@ -918,12 +918,12 @@ TreePlan tree_plan(uint32_t rows, uint32_t nodes, uint32_t heads, uint32_t kv_he
 
 // ---- accept ------------------------------------------------------------------------
 // A workgroup takes a share of one node's logits, a quarter of it each wave: the largest, or
-// (draws) each wave's sum of exp(x / T) in 64 bits, relative to a power of two. Greedy, the last
+// (draws) each wave's sum of exp(x / T) in 64 bits, relative to a power of two above its largest. Greedy, the last
 // share of a row to arrive finds each node's largest and walks the tree; with draws the last
 // share of a node finds the quarter in which the running sum passes the draw, reads that one
 // again and picks the token, and the last node of a row walks. Bound by memory for large
-// batches (16 drawn trees of 16 over 151,936 tokens in FP32, 130 MB, 38 us; arithmetic left out
-// changed nothing), by the chain of hand-overs for small ones (a tree of 8 6.5 us).
+// batches (16 drawn trees of 16 over 151,936 tokens in FP32, 130 MB, 37 us; arithmetic left out
+// changed nothing; in BF16 28 us), by the chain of hand-overs for small ones (a tree of 8 6.5 us).
 constexpr int kAcceptT = 256, kAcceptWaves = kAcceptT / kWave;
 constexpr uint32_t kAcceptShares = 64;    // of a node at most: a lane each
 // (1,024: 16 drawn trees of 16 41 us instead of 38, 4,096 44)
