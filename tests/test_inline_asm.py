@@ -29,3 +29,20 @@ def test_clobbers_are_declared():
             seen += 1
             assert '"memory"' in clobbers, where
     assert seen >= 8
+
+
+def test_transfers_wait_for_what_they_read():
+    """One wait state between the write of m0 and the transfer that reads it, in every form; five where its address is
+    in scalar registers too, which a vector instruction may have written right before."""
+    seen = 0
+    for where, body in statements():
+        code, operands = re.split(r'"\s*:', body, maxsplit=1)
+        if "global_load_lds" not in code:
+            continue
+        m = re.search(r"s_mov_b32 m0, %\d\\n\\ts_nop (\d+)\\n\\tglobal_load_lds_dwordx4 %\d, (off|%\d)", code)
+        assert m, where
+        scalars = re.findall(r'"s"\s*\(', operands)
+        assert len(scalars) == (1 if m.group(2) == "off" else 2), where
+        assert int(m.group(1)) >= (0 if m.group(2) == "off" else 4), where
+        seen += 1
+    assert seen >= 5
